@@ -431,6 +431,110 @@ RKV_API int rkv_decode_split(const rkv_summary* summary, const void* query, int 
                              unsigned stage, void* stream);
 
 /*
+ * Rotary positions (no reference counterpart: the reference attaches after
+ * its model has rotated queries and keys).  Of each row's head_dim channels
+ * the first rotary_dim are rotated in rotary_dim / 2 pairs, the rest copied:
+ *   y_a = x_a cos - x_b sin, y_b = x_b cos + x_a sin,
+ * with pair i = channels (i, i + rotary_dim / 2), or (2i, 2i + 1) when
+ * `interleaved`.  cos_sin is a fp32 (table_rows, rotary_dim) table, rows
+ * table_stride elements apart: per position the pairs' cosines, then their
+ * sines, with whatever scaling of frequencies or amplitude the model uses.
+ * `inverse` negates the sines: the backward pass of the rotation.
+ *   query / key: (batch, tokens, heads, head_dim) of `dtype` by element
+ *     strides [batch, token, head], innermost stride 1; key may be null with
+ *     key_heads 0.  Outputs likewise, of the same dtype; an output may be its
+ *     own input.  positions: (batch, tokens) int32, or int64 with
+ *     positions_i64.  A position outside [0, table_rows) reads nothing and
+ *     gives NaN in its row's rotary channels.
+ *   head_dim even up to 1024, rotary_dim even in [2, head_dim].
+ * Arithmetic is fp32, each product and sum rounded by itself, so a rotation
+ * has the same bits in every layout and in rkv_paged_append.
+ */
+typedef struct rkv_rotary_args {
+  const void* query;
+  const void* key;
+  void* query_out;
+  void* key_out;
+  const void* positions;
+  const float* cos_sin;
+  int64_t query_strides[3];
+  int64_t key_strides[3];
+  int64_t query_out_strides[3];
+  int64_t key_out_strides[3];
+  int64_t position_strides[2];
+  int64_t positions_i64;
+  int64_t table_rows;
+  int64_t table_stride;
+  int64_t batch;
+  int64_t tokens;
+  int64_t query_heads;
+  int64_t key_heads;
+  int64_t head_dim;
+  int64_t rotary_dim;
+  int64_t dtype; /* RKV_DTYPE_BF16 or RKV_DTYPE_F32 */
+  int64_t interleaved;
+  int64_t inverse;
+} rkv_rotary_args;
+RKV_API int rkv_rotary(const rkv_rotary_args* args, void* stream);
+
+/*
+ * Append new tokens to a page pool, rotating keys (and queries) on the way
+ * (no reference counterpart: the reference keeps one contiguous cache).
+ * Token t belongs to sequence s = sequence_ids[t] (t itself when null) at
+ * position p = positions[t]; its key and value rows go to row p % block_size
+ * of physical page page_table[s * page_table_stride + p / block_size], each
+ * rounded once to the pool's bf16.  With cos_sin the key is rotated first as
+ * rkv_rotary does; without it keys are copied.  `query`, optional, is rotated
+ * (or copied) into query_out, (tokens, query_heads, head_dim).
+ *   key / value / query: (tokens, heads, head_dim) of `dtype` by element
+ *     strides [token, head]; pools: element strides [page, head, row], rows
+ *     of head_dim contiguous bf16 (HND and NHD pools are both expressible).
+ *   A negative position is padding (a captured step with idle slots): nothing
+ *   is written to the pools and the query row is zero.  A position past the
+ *   rotation table or the sequence's table row, a sequence id outside
+ *   [0, sequences) or a page outside [0, pool_pages) sets
+ *   RKV_DEVICE_BAD_INPUT in *status (when given) and writes nothing to the
+ *   pools; past the rotation table the query row's rotary channels are NaN.
+ *   Two tokens of one call must not name the same row of the pool.
+ *   head_dim and block_size as everywhere in this header.
+ */
+typedef struct rkv_append_args {
+  const void* key;
+  const void* value;
+  const void* query;
+  void* query_out;
+  void* key_pool;
+  void* value_pool;
+  const int32_t* page_table;
+  const int32_t* sequence_ids;
+  const void* positions;
+  const float* cos_sin;
+  int32_t* status;
+  int64_t key_strides[2];
+  int64_t value_strides[2];
+  int64_t query_strides[2];
+  int64_t query_out_strides[2];
+  int64_t key_pool_strides[3];
+  int64_t value_pool_strides[3];
+  int64_t page_table_stride;
+  int64_t sequences;
+  int64_t table_blocks; /* entries of each sequence's table row */
+  int64_t pool_pages;
+  int64_t block_size;
+  int64_t tokens;
+  int64_t query_heads;
+  int64_t kv_heads;
+  int64_t head_dim;
+  int64_t rotary_dim; /* ignored without cos_sin */
+  int64_t table_rows;
+  int64_t table_stride;
+  int64_t dtype;
+  int64_t positions_i64;
+  int64_t interleaved;
+} rkv_append_args;
+RKV_API int rkv_paged_append(const rkv_append_args* args, void* stream);
+
+/*
  * Diagnostic: one bounded device wait on an mbarrier that nothing completes,
  * with a limit of `limit_ns` (0 < limit_ns <= 1e9) instead of the kernels'
  * 1 s; it ORs RKV_DEVICE_TIMEOUT into the device int32 *status and returns,

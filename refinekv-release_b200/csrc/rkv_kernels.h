@@ -264,6 +264,38 @@ cudaError_t launch_fused(const FusedMaps& maps, const FusedParams& p, int dim, i
                          size_t smem, cudaStream_t stream, bool pdl);
 cudaError_t launch_merge(const MergeParams& p, int dim, cudaStream_t stream, bool pdl);
 
+// One stream of rows of rows_kernel: element strides per batch, token and
+// head.  A pool's output strides are those of a page, a row and a head.
+struct RowStream {
+  const void* in;
+  void* out;
+  int64_t in_b, in_t, in_h;
+  int64_t out_b, out_t, out_h;
+  int heads;
+};
+
+struct RowsParams {
+  RowStream query, key, value;  // heads 0: absent; value only when appending
+  int dim, rotary;              // rotary 0: rows are copied
+  float sign;                   // of the sines: -1 for the inverse rotation
+  const float* cos_sin;
+  int64_t table_rows, table_stride;
+  const void* positions;
+  int64_t pos_b, pos_t;
+  int pos_i64;
+  int64_t batch, tokens;
+  // appending only
+  const int32_t* page_table;
+  int64_t page_table_stride;
+  const int32_t* sequence_ids;
+  int64_t sequences, table_blocks, pool_pages;
+  int block_shift;
+  int* status;
+};
+
+cudaError_t launch_rows(const RowsParams& p, bool f32, bool vector, bool interleaved, bool append,
+                        cudaStream_t stream);
+
 // Raise `func`'s dynamic shared-memory limit to at least `bytes` on the
 // current device.  Done once per (kernel, device): later calls, including
 // those made while a CUDA graph is being captured, only read a cache.

@@ -10,7 +10,9 @@ lockstep, stacked on the head axis), ``build_summary_into`` (the prefill's
 cache write and the summary in one pass), ``attach_page_pool`` (decode from a
 vLLM-style K/V page pool through a page table), ``page_view`` and
 ``dense_attention`` (dense decode of the full-attention layers on the same
-kernel) and ``refinekv_b200.parallel`` (KV-head sharding and sequence split
+kernel), ``rotary_table`` / ``apply_rotary`` (rotary positions),
+``paged_append`` (new tokens into the page pool, rotated on the way) and
+``refinekv_b200.parallel`` (KV-head sharding and sequence split
 over GPUs).
 
 All compute runs in the CUDA library ``librefinekv_b200.so`` built from
@@ -34,6 +36,9 @@ __all__ = [
     "dense_attention",
     "select_blocks",
     "sparse_attention",
+    "rotary_table",
+    "apply_rotary",
+    "paged_append",
     "RefineKV",
     "make_visible_static_cache",
 ]
@@ -49,6 +54,14 @@ def __getattr__(name):
         from . import summary
 
         return getattr(summary, name)
+    if name in ("rotary_table", "apply_rotary"):
+        from . import rotary
+
+        return getattr(rotary, name)
+    if name in ("paged_append",):
+        from . import paged
+
+        return getattr(paged, name)
     if name in ("RefineKV", "make_visible_static_cache"):
         from .integrations import transformers as adapter
 

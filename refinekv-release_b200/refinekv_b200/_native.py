@@ -8,7 +8,10 @@ from __future__ import annotations
 
 import ctypes
 import pathlib
+import struct
 import threading
+
+import torch
 
 LIB_PATH = pathlib.Path(__file__).resolve().parent / "_lib" / "librefinekv_b200.so"
 ABI_VERSION = 2
@@ -58,6 +61,8 @@ EXPORTS = (
     "rkv_select_split",
     "rkv_split_exchange_slabs",
     "rkv_decode_split",
+    "rkv_rotary",
+    "rkv_paged_append",
     "rkv_selftest_wait_timeout",
     "rkv_last_error",
     "rkv_status_string",
@@ -98,6 +103,12 @@ class Summary(ctypes.Structure):
         ("value_token_stride", c_i64),
     ]
 
+
+#: ``struct rkv_rotary_args`` and ``struct rkv_append_args``: 8-byte fields only, packed in the
+#: header's order (pointers as integers, 0 for null).  Packing costs a tenth of filling a
+#: ``ctypes.Structure``, which counts in calls whose kernel takes a few microseconds.
+ROTARY_ARGS = struct.Struct("=32q")
+APPEND_ARGS = struct.Struct("=40q")
 
 _SIGNATURES = {
     "rkv_summarize": (ctypes.c_int, [c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64,
@@ -143,6 +154,9 @@ _SIGNATURES = {
                                         c_i64, c_ptr, ctypes.c_float, ctypes.c_int, c_ptr, c_ptr,
                                         c_ptr, ctypes.c_size_t, c_i64, c_i64, c_i64, c_ptr,
                                         ctypes.c_size_t, ctypes.c_uint, c_ptr]),
+    # The argument structs of the paged operators are packed bytes (ROTARY_ARGS, APPEND_ARGS).
+    "rkv_rotary": (ctypes.c_int, [ctypes.c_char_p, c_ptr]),
+    "rkv_paged_append": (ctypes.c_int, [ctypes.c_char_p, c_ptr]),
     "rkv_selftest_wait_timeout": (ctypes.c_int, [c_ptr, c_i64, c_ptr]),
     "rkv_last_error": (ctypes.c_char_p, []),
     "rkv_status_string": (ctypes.c_char_p, [ctypes.c_int]),
@@ -188,3 +202,28 @@ def check(rc: int) -> None:
     if rc in (RKV_ERR_INVALID_ARGUMENT, RKV_ERR_UNSUPPORTED, RKV_ERR_ALIGNMENT):
         raise ValueError(message)
     raise RuntimeError(message)
+
+
+_b200_devices = set()
+
+
+def launch(function, packed: bytes, device: torch.device) -> None:
+    """Call an entry point that takes packed arguments on the device's current stream.
+
+    The calling thread's current device is switched only when it is another
+    one, and the capability is looked up once per device: both matter for
+    kernels of a few microseconds.
+    """
+    index = device.index
+    if index not in _b200_devices:
+        if torch.cuda.get_device_capability(device)[0] != 10:
+            raise RuntimeError("librefinekv_b200 is built for sm_100a (B200) only")
+        _b200_devices.add(index)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch.cuda.current_device() == index:
+        rc = function(packed, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = function(packed, stream)
+    if rc != RKV_OK:
+        check(rc)

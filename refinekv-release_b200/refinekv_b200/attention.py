@@ -84,11 +84,20 @@ def _scratch(workspace, name, nbytes, device):
 
 
 def device_status(workspace: dict) -> int:
-    """Sticky device status word of the decode workspace (synchronises); 0 means healthy."""
-    scratch = workspace.get("rkv_decode_scratch") if workspace else None
-    if scratch is None:
-        return 0
-    return int(scratch[:4].view(torch.int32).item())
+    """Sticky device status of a workspace's calls (synchronises); 0 means healthy.
+
+    The union of the status words of ``sparse_attention``, ``paged_attention``
+    and ``paged_append`` calls that were given this workspace.
+    """
+    status = 0
+    for name in ("rkv_decode_scratch", "rkv_paged_scratch"):
+        scratch = workspace.get(name) if workspace else None
+        if scratch is not None:
+            status |= int(scratch[:4].view(torch.int32).item())
+    appended = workspace.get("rkv_append_status") if workspace else None
+    if appended is not None:
+        status |= int(appended[0].item())
+    return status
 
 
 def _query_code(query):

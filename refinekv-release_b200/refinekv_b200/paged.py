@@ -1,0 +1,160 @@
+"""Serving from a page pool: appending new tokens, and dense attention of one new token.
+
+No counterpart in the reference, which keeps one contiguous cache per layer
+and decodes one sequence.  A server keeps the keys and values of many
+sequences of different lengths in a pool of fixed-size pages; a page table
+gives each sequence's pages.  ``attach_page_pool`` lets the refined layers
+decode from such a pool; here is what fills it (``paged_append``) and what
+the dense layers decode with (``paged_attention``).
+
+Pools are bf16, ``(pages, kv_heads, block, dim)`` (``layout="HND"``) or
+``(pages, block, kv_heads, dim)`` (``"NHD"``); page tables are int32
+``(sequences, blocks)``.  Everything that changes from step to step
+(positions, lengths, page tables) is read on the device, so a captured CUDA
+graph serves growing sequences.  Results carry no gradient.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _native
+from .attention import _buffer, _scratch
+from .rotary import _DTYPES, check_table
+from .summary import SUPPORTED_HEAD_DIMS, require_cuda_tensor
+
+_BLOCKS = (16, 32, 64)
+
+
+def _pools(key_pool, value_pool, layout):
+    """(pages, kv_heads, block, dim) and both pools' (page, head, row) strides, checked."""
+    if layout not in ("HND", "NHD"):
+        raise ValueError("layout must be 'HND' or 'NHD'")
+    shape = key_pool.shape
+    if len(shape) != 4 or value_pool.shape != shape:
+        raise ValueError("key and value pools must have the same 4-D shape")
+    require_cuda_tensor(key_pool, "key_pool")
+    if key_pool.dtype != torch.bfloat16 or value_pool.dtype != torch.bfloat16:
+        raise TypeError("page pools must be bf16")
+    if value_pool.device != key_pool.device:
+        raise ValueError("key and value pools must be on the same device")
+    ks, vs = key_pool.stride(), value_pool.stride()
+    if ks[3] != 1 or vs[3] != 1:
+        raise ValueError("pool rows must be contiguous in head_dim")
+    if layout == "HND":
+        pages, heads, block, dim = shape
+        ks, vs = ks[:3], vs[:3]
+    else:
+        pages, block, heads, dim = shape
+        ks, vs = (ks[0], ks[2], ks[1]), (vs[0], vs[2], vs[1])
+    if block not in _BLOCKS:
+        raise ValueError("pool blocks must hold 16, 32 or 64 tokens")
+    if dim not in SUPPORTED_HEAD_DIMS:
+        raise ValueError(f"head_dim must be one of {SUPPORTED_HEAD_DIMS}")
+    return pages, heads, block, dim, ks, vs
+
+
+def _table(page_table, device):
+    """(sequences, blocks, stride) of an int32 page table (1-D: one sequence)."""
+    shape, stride = page_table.shape, page_table.stride()
+    if len(shape) == 1:
+        shape, stride = (1, shape[0]), (shape[0], stride[0])
+    if len(shape) != 2 or stride[1] != 1 or page_table.device != device:
+        raise ValueError("page_table must be (sequences, blocks) with contiguous rows on the "
+                         "pools' device")
+    if page_table.dtype != torch.int32:
+        raise TypeError("page_table must be int32")
+    return shape[0], shape[1], stride[0]
+
+
+def paged_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Tensor,
+                 value_pool: torch.Tensor, page_table: torch.Tensor, positions: torch.Tensor, *,
+                 layout: str = "HND", sequence_ids: torch.Tensor | None = None,
+                 query: torch.Tensor | None = None, cos_sin: torch.Tensor | None = None,
+                 interleaved: bool = False, workspace: dict | None = None) -> torch.Tensor | None:
+    """Write new tokens' keys and values into the pool's pages, rotated on the way.
+
+    ``key``/``value``: (tokens, kv_heads, head_dim) bf16 or fp32, any strides
+    with contiguous rows (slices of a fused projection, say).  Token t is
+    token ``positions[t]`` (int32 or int64) of sequence ``sequence_ids[t]``
+    (int32; without it token t belongs to sequence t: one new token each) and
+    goes to page ``page_table[sequence, position // block]``, row
+    ``position % block``, rounded once to bf16.  With ``cos_sin`` (see
+    ``apply_rotary``) keys are rotated by their positions first, and so is
+    ``query`` ((tokens, q_heads, head_dim), the keys' dtype) when given.
+
+    Returns the rotated queries (backed by ``workspace``, reused by the next
+    call of the same shape), or None without ``query``.  The pools are
+    written in place.  Any mix of prompts, chunks and single tokens goes in
+    one call; no two tokens of a call may name the same sequence and position.
+
+    A negative position is padding (an idle slot of a captured step): nothing
+    is written and its query row is zero.  A position past the page table's
+    row or the rotation table, a sequence id outside the page table or a page
+    outside the pool writes nothing and sets bit 1 of the status word
+    (``attention.device_status(workspace)``).
+    """
+    pages, heads, block, dim, ks, vs = _pools(key_pool, value_pool, layout)
+    device = key_pool.device
+    sequences, blocks, table_stride = _table(page_table, device)
+    shape, dtype = key.shape, key.dtype
+    if len(shape) != 3 or value.shape != shape or shape[1] != heads or shape[2] != dim:
+        raise ValueError("key and value must be (tokens, kv_heads, head_dim) matching the pools")
+    if key.device != device or value.device != device:
+        raise ValueError("key and value must be on the pools' device")
+    if dtype not in _DTYPES or value.dtype != dtype:
+        raise TypeError("key and value must both be BF16 or both FP32")
+    tokens = shape[0]
+    if positions.shape != (tokens,) or positions.device != device:
+        raise ValueError("positions must be (tokens,) on the pools' device")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError("positions must be int32 or int64")
+    if sequence_ids is None:
+        if tokens > sequences:
+            raise ValueError("more tokens than sequences: pass sequence_ids")
+        ids = 0
+    else:
+        if sequence_ids.shape != (tokens,) or sequence_ids.device != device:
+            raise ValueError("sequence_ids must be (tokens,) on the pools' device")
+        if sequence_ids.dtype != torch.int32:
+            raise TypeError("sequence_ids must be int32")
+        sequence_ids = sequence_ids.contiguous()
+        ids = sequence_ids.data_ptr()
+    table = rotary = rows = row_stride = 0
+    if cos_sin is not None:
+        check_table(cos_sin, dim, device)
+        table, rotary = cos_sin.data_ptr(), cos_sin.shape[1]
+        rows, row_stride = cos_sin.shape[0], cos_sin.stride(0)
+    if key.stride(2) != 1:
+        key = key.contiguous()
+    if value.stride(2) != 1:
+        value = value.contiguous()
+    positions = positions.contiguous()
+    out = None
+    query_ptr = out_ptr = query_heads = 0
+    query_strides = out_strides = (0, 0)
+    if query is not None:
+        if (query.ndim != 3 or query.shape[0] != tokens or query.shape[2] != dim
+                or query.device != device):
+            raise ValueError("query must be (tokens, q_heads, head_dim) on the pools' device")
+        if query.dtype != dtype:
+            raise TypeError("query must have the keys' dtype")
+        if query.stride(2) != 1:
+            query = query.contiguous()
+        out = _buffer(workspace, "append_query", query.shape, device, dtype)
+        query_ptr, out_ptr, query_heads = query.data_ptr(), out.data_ptr(), query.shape[1]
+        query_strides, out_strides = query.stride()[:2], out.stride()[:2]
+    status = 0
+    if workspace is not None:
+        status = _buffer(workspace, "rkv_append_status", (64,), device, torch.int32,
+                         zero=True).data_ptr()
+    _native.launch(
+        _native.load().rkv_paged_append,
+        _native.APPEND_ARGS.pack(
+            key.data_ptr(), value.data_ptr(), query_ptr, out_ptr, key_pool.data_ptr(),
+            value_pool.data_ptr(), page_table.data_ptr(), ids, positions.data_ptr(), table, status,
+            *key.stride()[:2], *value.stride()[:2], *query_strides, *out_strides, *ks, *vs,
+            table_stride, sequences, blocks, pages, block, tokens, query_heads, heads, dim, rotary,
+            rows, row_stride, _DTYPES[dtype], positions.dtype == torch.int64, interleaved),
+        device)
+    return out

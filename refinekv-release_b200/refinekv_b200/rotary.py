@@ -1,0 +1,230 @@
+"""Rotary positions of queries and keys.
+
+No counterpart in the reference, which attaches behind a model that has
+rotated its own queries and keys; a server that fills a page pool
+(``paged_append``) and decodes from it needs the rotation itself.  The angles
+come from a table (``rotary_table``, or any fp32 table of the same layout), so
+every frequency scaling for long contexts is the table's, not the kernel's.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _native
+from .summary import require_cuda_tensor
+
+_DTYPES = {torch.bfloat16: _native.DTYPE_BF16, torch.float32: _native.DTYPE_F32}
+
+
+def _frequencies(rotary_dim: int, base: float, scaling: dict | None):
+    """fp64 angular frequencies of the pairs and the amplitude of the table."""
+    exponent = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
+    plain = base ** -exponent
+    scaling = dict(scaling or {})
+    kind = scaling.pop("rope_type", scaling.pop("type", "default"))
+    if kind in ("default", "none"):
+        return plain, 1.0
+    try:
+        factor = float(scaling["factor"])
+    except KeyError:
+        raise ValueError(f"scaling {kind!r} needs a 'factor'") from None
+    if not math.isfinite(factor) or factor < 1:
+        raise ValueError("scaling factor must be at least 1")
+    if kind == "linear":
+        return plain / factor, 1.0
+    if kind == "ntk":  # the base stretched so that the slowest pair slows by `factor`
+        if rotary_dim == 2:
+            return plain, 1.0
+        return (base * factor ** (rotary_dim / (rotary_dim - 2))) ** -exponent, 1.0
+    if kind not in ("yarn", "llama3"):
+        raise ValueError("scaling type must be 'linear', 'ntk', 'yarn' or 'llama3'")
+    original = scaling.get("original_max_position_embeddings")
+    if original is None:
+        raise ValueError(f"scaling {kind!r} needs 'original_max_position_embeddings'")
+    if kind == "llama3":
+        # Pairs that turn more than high_freq_factor times within the original
+        # context are kept, fewer than low_freq_factor times slowed by
+        # `factor`, and blended linearly in between.
+        low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        turns = original * plain / (2 * math.pi)
+        keep = ((turns - low) / (high - low)).clamp(0, 1)
+        return plain * keep + plain / factor * (1 - keep), 1.0
+
+    # YaRN: the same idea, blended linearly over the channel index between the
+    # (rounded) channels that turn beta_fast and beta_slow times.
+    def channel(turns):
+        return rotary_dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+    first, last = channel(scaling.get("beta_fast") or 32), channel(scaling.get("beta_slow") or 1)
+    if scaling.get("truncate", True):
+        first, last = math.floor(first), math.ceil(last)
+    first, last = max(first, 0), min(last, rotary_dim - 1)
+    if first == last:
+        last += 0.001
+    index = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    slow = ((index - first) / (last - first)).clamp(0, 1)
+    amplitude = scaling.get("attention_factor")
+    if amplitude is None:
+        amplitude = 0.1 * math.log(factor) + 1 if factor > 1 else 1.0
+    return plain / factor * slow + plain * (1 - slow), float(amplitude)
+
+
+def rotary_table(rotary_dim: int, positions: int, *, base: float = 10000.0,
+                 scaling: dict | None = None, device="cuda") -> torch.Tensor:
+    """The fp32 (positions, rotary_dim) table ``apply_rotary`` and ``paged_append`` read.
+
+    Row p holds the cosines of p * frequency of the rotary_dim / 2 pairs, then
+    their sines, computed in fp64 and rounded once (an fp32 product of a
+    position near 10^5 with a frequency is off by up to 4e-3 rad).
+    ``scaling`` is a model configuration's rope scaling: ``{"rope_type":
+    "linear" | "ntk" | "yarn" | "llama3", "factor": ...}`` with that type's
+    further keys.  Built once and kept by the caller.
+    """
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be even and positive")
+    if positions < 1:
+        raise ValueError("positions must be positive")
+    if not math.isfinite(base) or base <= 1:
+        raise ValueError("base must be finite and above 1")
+    frequency, amplitude = _frequencies(rotary_dim, float(base), scaling)
+    frequency = frequency.to(device)
+    table = torch.empty(positions, rotary_dim, device=device, dtype=torch.float32)
+    step = max(1, (1 << 24) // rotary_dim)  # bounds the fp64 temporaries
+    for low in range(0, positions, step):
+        high = min(positions, low + step)
+        angle = torch.arange(low, high, device=device, dtype=torch.float64)[:, None] * frequency
+        table[low:high, : rotary_dim // 2] = angle.cos() * amplitude
+        table[low:high, rotary_dim // 2:] = angle.sin() * amplitude
+    return table
+
+
+def check_table(cos_sin: torch.Tensor, dim: int, device: torch.device) -> None:
+    """The argument checks of a cos/sin table shared with ``paged_append``."""
+    if cos_sin.ndim != 2 or cos_sin.stride(1) != 1 or cos_sin.shape[0] < 1:
+        raise ValueError("cos_sin must be a (positions, rotary_dim) table with contiguous rows")
+    if cos_sin.dtype != torch.float32:
+        raise TypeError("cos_sin must be fp32")
+    if cos_sin.device != device:
+        raise ValueError("cos_sin must be on the rows' device")
+    rotary = cos_sin.shape[1]
+    if rotary < 2 or rotary % 2 or rotary > dim:
+        raise ValueError("rotary_dim (cos_sin's width) must be even and at most head_dim")
+
+
+def _rows(tensor: torch.Tensor, what: str, in_place: bool) -> torch.Tensor:
+    if tensor.stride(-1) == 1:
+        return tensor
+    if in_place:
+        raise ValueError(f"{what} must be contiguous in head_dim to be rotated in place")
+    return tensor.contiguous()
+
+
+def _strides(tensor: torch.Tensor) -> tuple:
+    """(batch, token, head) element strides of a 3-D or 4-D tensor of rows."""
+    stride = tensor.stride()
+    return stride[:3] if len(stride) == 4 else (0, stride[0], stride[1])
+
+
+_NO_STRIDES = (0, 0, 0)
+
+
+def _launch(query, key, positions, cos_sin, interleaved, inverse, in_place):
+    query = _rows(query, "query", in_place)
+    query_out = query if in_place else torch.empty_like(query)
+    key_out = None
+    key_ptr = key_out_ptr = key_heads = 0
+    key_strides = key_out_strides = _NO_STRIDES
+    if key is not None:
+        key = _rows(key, "key", in_place)
+        key_out = key if in_place else torch.empty_like(key)
+        key_ptr, key_out_ptr, key_heads = key.data_ptr(), key_out.data_ptr(), key.shape[-2]
+        key_strides, key_out_strides = _strides(key), _strides(key_out)
+    shape = query.shape
+    at = positions.stride()
+    _native.launch(
+        _native.load().rkv_rotary,
+        _native.ROTARY_ARGS.pack(
+            query.data_ptr(), key_ptr, query_out.data_ptr(), key_out_ptr, positions.data_ptr(),
+            cos_sin.data_ptr(), *_strides(query), *key_strides, *_strides(query_out),
+            *key_out_strides, *(at if len(at) == 2 else (0, at[0])),
+            positions.dtype == torch.int64, cos_sin.shape[0], cos_sin.stride(0),
+            shape[0] if len(shape) == 4 else 1, shape[-3], shape[-2], key_heads, shape[-1],
+            cos_sin.shape[1], _DTYPES[query.dtype], interleaved, inverse),
+        query.device)
+    return query_out, key_out
+
+
+class _Rotary(torch.autograd.Function):
+    """The rotation is linear in its rows: its backward pass is the inverse rotation."""
+
+    @staticmethod
+    def forward(ctx, query, key, positions, cos_sin, interleaved, inverse):
+        ctx.save_for_backward(positions, cos_sin)
+        ctx.flags = interleaved, inverse, key is not None
+        out = _launch(query, key, positions, cos_sin, interleaved, inverse, False)
+        return out if key is not None else out[0]
+
+    @staticmethod
+    def backward(ctx, query_grad, key_grad=None):
+        positions, cos_sin = ctx.saved_tensors
+        interleaved, inverse, both = ctx.flags
+        query_grad, key_grad = apply_rotary(query_grad, key_grad if both else None, positions,
+                                            cos_sin, interleaved=interleaved,
+                                            inverse=not inverse)
+        return query_grad, key_grad, None, None, None, None
+
+
+def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor,
+                 cos_sin: torch.Tensor, *, interleaved: bool = False, inverse: bool = False,
+                 in_place: bool = False) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Rotate queries and keys by their positions in one launch.
+
+    ``query``: (tokens, heads, head_dim) or (batch, tokens, heads, head_dim)
+    bf16 or fp32, any strides with contiguous rows (a model's (batch, heads,
+    tokens, dim) tensor goes in as ``x.transpose(1, 2)``); ``key`` the same
+    with its own head count, or None.  ``positions``: int32 or int64, the
+    leading shape (tokens,) or (batch, tokens).  ``cos_sin``: an fp32
+    (positions, rotary_dim) table (``rotary_table``); its width rotary_dim may
+    be less than head_dim: the channels after it are copied.  Pair i of the
+    rotary channels is (i, i + rotary_dim / 2), or (2i, 2i + 1) with
+    ``interleaved``.  ``inverse`` turns back.  A position outside the table
+    gives NaN in the rotary channels.
+
+    Returns (query, key) in new tensors, or the arguments themselves when
+    ``in_place`` (rows must then not overlap).  Differentiable in query and
+    key; the backward pass is one launch of the inverse rotation.
+    """
+    shape = query.shape
+    if query.ndim not in (3, 4):
+        raise ValueError("query must have shape ([batch,] tokens, heads, head_dim)")
+    require_cuda_tensor(query, "query")
+    if query.dtype not in _DTYPES:
+        raise TypeError("apply_rotary takes BF16 or FP32 queries and keys")
+    if shape[-1] % 2 or not 2 <= shape[-1] <= 1024:
+        raise ValueError("head_dim must be even and at most 1024")
+    if key is not None:
+        if (key.ndim != query.ndim or key.shape[:-2] != shape[:-2] or key.shape[-1] != shape[-1]
+                or key.device != query.device):
+            raise ValueError("key must match the query but for its heads")
+        if key.dtype != query.dtype:
+            raise TypeError("query and key must have the same dtype")
+    if positions.shape != shape[:-2] or positions.device != query.device:
+        raise ValueError("positions must be ([batch,] tokens) on the query's device")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError("positions must be int32 or int64")
+    check_table(cos_sin, shape[-1], query.device)
+    if torch.is_grad_enabled() and (query.requires_grad
+                                    or (key is not None and key.requires_grad)):
+        if in_place:
+            raise ValueError("rows that require a gradient cannot be rotated in place")
+        out = _Rotary.apply(query, key, positions, cos_sin, interleaved, inverse)
+        return out if key is not None else (out, None)
+    if in_place:
+        for rows in (query, key):
+            if rows is not None and any(s == 0 and n > 1
+                                        for s, n in zip(rows.stride(), rows.shape)):
+                raise ValueError("overlapping rows cannot be rotated in place")
+    return _launch(query, key, positions, cos_sin, interleaved, inverse, in_place)
