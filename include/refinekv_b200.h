@@ -535,6 +535,57 @@ typedef struct rkv_append_args {
 RKV_API int rkv_paged_append(const rkv_append_args* args, void* stream);
 
 /*
+ * Dense attention of one new token per sequence over a page pool (no
+ * reference counterpart; the dense layers of a server's decode step).  With
+ * length L = lengths[s], each query row of KV head h attends to the rows
+ * j in [max(0, L - window), L) of its sequence (window 0: all of them):
+ *   output = sum_j exp(x_j) v_j / sum_j exp(x_j), x_j = scale q.k_j,
+ *   lse = log sum_j exp(x_j)   (natural log; optional),
+ * read from row j % block_size of page page_table[s * page_table_stride +
+ * j / block_size].  A sequence of length 0 gives a zero row and lse -inf.
+ * Nothing outside the visible rows enters the result, whatever it holds.
+ *   query: (sequences, kv_heads * group, head_dim) of query_dtype by element
+ *     strides [sequence, head], 16-byte aligned rows; rounded to bf16 before
+ *     use, as every query of this library.  Query row r belongs to KV head
+ *     r / group.  output: the same shape, contiguous, in query_dtype; lse:
+ *     (sequences, kv_heads * group) fp32 or null.
+ *   pools: bf16, element strides [page, head, row], all multiples of 16 bytes.
+ *   lengths: (sequences,) int32 on the device.
+ * A length outside [0, table_blocks * block_size] or a page outside
+ * [0, pool_pages) sets RKV_DEVICE_BAD_INPUT in the workspace's status word;
+ * the kernel then takes the nearest length, and page 0.
+ * The workspace follows the rules at the top of this header; its size does
+ * not depend on the lengths.  Calls that share one must be ordered.
+ */
+typedef struct rkv_paged_args {
+  const void* query;
+  void* output;
+  float* lse;
+  const void* key_pool;
+  const void* value_pool;
+  const int32_t* page_table;
+  const int32_t* lengths;
+  void* workspace;
+  int64_t workspace_size;
+  int64_t query_strides[2];
+  int64_t key_pool_strides[3];
+  int64_t value_pool_strides[3];
+  int64_t page_table_stride;
+  int64_t sequences;
+  int64_t table_blocks;
+  int64_t pool_pages;
+  int64_t block_size;
+  int64_t kv_heads;
+  int64_t group;
+  int64_t head_dim;
+  int64_t query_dtype;
+  int64_t window;
+  double scale;
+} rkv_paged_args;
+RKV_API size_t rkv_paged_workspace_size(int64_t group, int64_t head_dim);
+RKV_API int rkv_paged_attention(const rkv_paged_args* args, void* stream);
+
+/*
  * Diagnostic: one bounded device wait on an mbarrier that nothing completes,
  * with a limit of `limit_ns` (0 < limit_ns <= 1e9) instead of the kernels'
  * 1 s; it ORs RKV_DEVICE_TIMEOUT into the device int32 *status and returns,

@@ -3,6 +3,7 @@
 #pragma once
 
 #include <cuda.h>
+#include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -295,6 +296,28 @@ struct RowsParams {
 
 cudaError_t launch_rows(const RowsParams& p, bool f32, bool vector, bool interleaved, bool append,
                         cudaStream_t stream);
+
+struct PagedParams {
+  const void* query;
+  int64_t q_seq, q_head;  // element strides
+  int query_f32;
+  void* out;
+  float* lse;  // or null
+  const __nv_bfloat16* keys;
+  const __nv_bfloat16* values;
+  int64_t k_page, k_head, k_row, v_page, v_head, v_row;
+  const int32_t* page_table;
+  int64_t page_table_stride;
+  const int32_t* lengths;
+  int sequences, heads, group, dim;
+  int block_shift;
+  int64_t table_blocks, pool_pages;
+  int64_t window;  // 0: none
+  float scale;
+  int* status;
+};
+
+cudaError_t launch_paged(const PagedParams& p, cudaStream_t stream);
 
 // Raise `func`'s dynamic shared-memory limit to at least `bytes` on the
 // current device.  Done once per (kernel, device): later calls, including

@@ -11,8 +11,9 @@ cache write and the summary in one pass), ``attach_page_pool`` (decode from a
 vLLM-style K/V page pool through a page table), ``page_view`` and
 ``dense_attention`` (dense decode of the full-attention layers on the same
 kernel), ``rotary_table`` / ``apply_rotary`` (rotary positions),
-``paged_append`` (new tokens into the page pool, rotated on the way) and
-``refinekv_b200.parallel`` (KV-head sharding and sequence split
+``paged_append`` (new tokens into the page pool, rotated on the way),
+``paged_attention`` (dense attention of one new token per sequence, each over
+its own length of the pool) and ``refinekv_b200.parallel`` (KV-head sharding and sequence split
 over GPUs).
 
 All compute runs in the CUDA library ``librefinekv_b200.so`` built from
@@ -39,6 +40,7 @@ __all__ = [
     "rotary_table",
     "apply_rotary",
     "paged_append",
+    "paged_attention",
     "RefineKV",
     "make_visible_static_cache",
 ]
@@ -58,7 +60,7 @@ def __getattr__(name):
         from . import rotary
 
         return getattr(rotary, name)
-    if name in ("paged_append",):
+    if name in ("paged_append", "paged_attention"):
         from . import paged
 
         return getattr(paged, name)

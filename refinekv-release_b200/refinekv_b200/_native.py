@@ -63,6 +63,8 @@ EXPORTS = (
     "rkv_decode_split",
     "rkv_rotary",
     "rkv_paged_append",
+    "rkv_paged_workspace_size",
+    "rkv_paged_attention",
     "rkv_selftest_wait_timeout",
     "rkv_last_error",
     "rkv_status_string",
@@ -104,11 +106,12 @@ class Summary(ctypes.Structure):
     ]
 
 
-#: ``struct rkv_rotary_args`` and ``struct rkv_append_args``: 8-byte fields only, packed in the
-#: header's order (pointers as integers, 0 for null).  Packing costs a tenth of filling a
+#: ``struct rkv_rotary_args``, ``rkv_append_args`` and ``rkv_paged_args``: 8-byte fields only,
+#: packed in the header's order (pointers as integers, 0 for null).  Packing costs a tenth of filling a
 #: ``ctypes.Structure``, which counts in calls whose kernel takes a few microseconds.
 ROTARY_ARGS = struct.Struct("=32q")
 APPEND_ARGS = struct.Struct("=40q")
+PAGED_ARGS = struct.Struct("=27qd")
 
 _SIGNATURES = {
     "rkv_summarize": (ctypes.c_int, [c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64,
@@ -154,9 +157,11 @@ _SIGNATURES = {
                                         c_i64, c_ptr, ctypes.c_float, ctypes.c_int, c_ptr, c_ptr,
                                         c_ptr, ctypes.c_size_t, c_i64, c_i64, c_i64, c_ptr,
                                         ctypes.c_size_t, ctypes.c_uint, c_ptr]),
-    # The argument structs of the paged operators are packed bytes (ROTARY_ARGS, APPEND_ARGS).
+    # The argument structs of the paged operators are packed bytes (ROTARY_ARGS and so on).
     "rkv_rotary": (ctypes.c_int, [ctypes.c_char_p, c_ptr]),
     "rkv_paged_append": (ctypes.c_int, [ctypes.c_char_p, c_ptr]),
+    "rkv_paged_workspace_size": (ctypes.c_size_t, [c_i64, c_i64]),
+    "rkv_paged_attention": (ctypes.c_int, [ctypes.c_char_p, c_ptr]),
     "rkv_selftest_wait_timeout": (ctypes.c_int, [c_ptr, c_i64, c_ptr]),
     "rkv_last_error": (ctypes.c_char_p, []),
     "rkv_status_string": (ctypes.c_char_p, [ctypes.c_int]),

@@ -19,11 +19,18 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from .attention import _buffer, _scratch
+from .attention import MAX_GROUP, _buffer, _scratch
 from .rotary import _DTYPES, check_table
 from .summary import SUPPORTED_HEAD_DIMS, require_cuda_tensor
 
 _BLOCKS = (16, 32, 64)
+
+
+def _paged_scratch(lib, workspace, group, dim, device):
+    """``paged_attention``'s zero-filled scratch; its size follows from the head shape alone."""
+    with torch.cuda.device(device):
+        return _scratch(workspace, "rkv_paged_scratch", lib.rkv_paged_workspace_size(group, dim),
+                        device)
 
 
 def _pools(key_pool, value_pool, layout):
@@ -158,3 +165,70 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Tensor,
             rows, row_stride, _DTYPES[dtype], positions.dtype == torch.int64, interleaved),
         device)
     return out
+
+
+def paged_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor,
+                    page_table: torch.Tensor, lengths: torch.Tensor, *, layout: str = "HND",
+                    scale: float | None = None, window: int | None = None,
+                    return_lse: bool = False, workspace: dict | None = None):
+    """Exact attention of one new token per sequence over its own length of the pool.
+
+    ``query``: (sequences, q_heads, head_dim) bf16 or fp32, any strides; query
+    head r reads KV head r // (q_heads // kv_heads), at most 16 to a KV head.
+    ``lengths``: (sequences,) int32, the tokens of each sequence now in the
+    pool (the new one included, once ``paged_append`` has written it); a
+    sequence of length 0 (an idle slot) gives a zero row.  ``scale`` defaults
+    to head_dim ** -0.5; ``window`` limits each query to the last ``window``
+    tokens.  Rows of a page past a sequence's length, pages past it and pages
+    before its window are never used, whatever they hold.  An fp32 query is
+    rounded to bf16 first, like every query of this package; its
+    probabilities, sums and output stay fp32.
+
+    Returns the (sequences, q_heads, head_dim) output in the query's dtype or,
+    with ``return_lse``, (output, lse) with the fp32 natural-log sum of the
+    exponentials (-inf for an empty row): outputs over parts of a sequence join
+    as sum_i exp(lse_i - lse) output_i.  Backed by ``workspace``, reused by the
+    next call of the same shape.  A length past the page table's row or a page
+    outside the pool sets bit 1 of ``attention.device_status(workspace)``.
+    One launch; its results repeat bit for bit.
+    """
+    pages, heads, block, dim, ks, vs = _pools(key_pool, value_pool, layout)
+    device = key_pool.device
+    sequences, blocks, table_stride = _table(page_table, device)
+    shape, dtype = query.shape, query.dtype
+    if len(shape) != 3 or shape[0] != sequences or shape[2] != dim:
+        raise ValueError("query must be (sequences, q_heads, head_dim) matching the page table "
+                         "and the pools")
+    if query.device != device:
+        raise ValueError("query must be on the pools' device")
+    if dtype not in _DTYPES:
+        raise TypeError("the CUDA backend requires BF16 or FP32 queries")
+    group = shape[1] // heads
+    if group * heads != shape[1] or not 1 <= group <= MAX_GROUP:
+        raise ValueError("q_heads must be 1 to 16 times the pools' KV heads")
+    if lengths.shape != (sequences,) or lengths.device != device:
+        raise ValueError("lengths must be (sequences,) on the pools' device")
+    if lengths.dtype != torch.int32:
+        raise TypeError("lengths must be int32")
+    if window is not None and window < 1:
+        raise ValueError("window must be at least 1")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    qs = query.stride()
+    width = 2 if dtype == torch.bfloat16 else 4
+    if qs[2] != 1 or (query.data_ptr() | qs[0] * width | qs[1] * width) & 15:
+        query = query.clone(memory_format=torch.contiguous_format)
+        qs = query.stride()
+    lengths = lengths.contiguous()
+    lib = _native.load()
+    out = _buffer(workspace, "paged_output", shape, device, dtype)
+    lse = _buffer(workspace, "paged_lse", shape[:2], device, torch.float32) if return_lse else None
+    scratch = _paged_scratch(lib, workspace, group, dim, device)
+    _native.launch(
+        lib.rkv_paged_attention,
+        _native.PAGED_ARGS.pack(
+            query.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
+            key_pool.data_ptr(), value_pool.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
+            scratch.data_ptr(), scratch.numel(), qs[0], qs[1], *ks, *vs, table_stride, sequences,
+            blocks, pages, block, heads, group, dim, _DTYPES[dtype], window or 0, scale),
+        device)
+    return (out, lse) if return_lse else out

@@ -102,6 +102,12 @@ APPEND_FIELDS = ("key", "value", "query", "query_out", "key_pool", "value_pool",
                  "positions_i64", "interleaved")
 
 
+PAGED_FIELDS = ("query", "output", "lse", "key_pool", "value_pool", "page_table", "lengths",
+                "workspace", "workspace_size", *["qs"] * 2, *["kps"] * 3, *["vps"] * 3,
+                "page_table_stride", "sequences", "table_blocks", "pool_pages", "block_size",
+                "kv_heads", "group", "head_dim", "query_dtype", "window", "scale")
+
+
 def test_packed_arguments_have_the_headers_fields():
     """The packed structs count every 8-byte field of the header's declarations, in its order."""
     import pathlib
@@ -109,7 +115,8 @@ def test_packed_arguments_have_the_headers_fields():
 
     header = (pathlib.Path(__file__).parents[1] / "include" / "refinekv_b200.h").read_text()
     for name, packer, fields in (("rotary", _native.ROTARY_ARGS, ROTARY_FIELDS),
-                                 ("append", _native.APPEND_ARGS, APPEND_FIELDS)):
+                                 ("append", _native.APPEND_ARGS, APPEND_FIELDS),
+                                 ("paged", _native.PAGED_ARGS, PAGED_FIELDS)):
         body = re.search(r"typedef struct rkv_%s_args \{(.*?)\}" % name, header, re.S).group(1)
         body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
         names = []
@@ -177,3 +184,37 @@ def _append(lib, **change):
 def test_append_entry_point_refuses_before_touching_a_device(lib, change, code):
     assert _append(lib, **change) == code
     assert lib.rkv_paged_append(None, None) == _native.RKV_ERR_INVALID_ARGUMENT
+
+
+def _attend(lib, **change):
+    values = dict(query=16, output=16, key_pool=16, value_pool=16, page_table=16, lengths=16,
+                  workspace=256, workspace_size=1 << 30, qs=128, kps=4096, vps=4096,
+                  page_table_stride=2, sequences=2, table_blocks=2, pool_pages=4, block_size=32,
+                  kv_heads=2, group=4, head_dim=64, scale=0.125)
+    values.update(change)
+    return lib.rkv_paged_attention(
+        _native.PAGED_ARGS.pack(*[values.get(f, 0) for f in PAGED_FIELDS]), None)
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(query=0), _native.RKV_ERR_INVALID_ARGUMENT),
+    (dict(lengths=0), _native.RKV_ERR_INVALID_ARGUMENT),
+    (dict(key_pool=0), _native.RKV_ERR_INVALID_ARGUMENT),
+    (dict(pool_pages=0), _native.RKV_ERR_INVALID_ARGUMENT),
+    (dict(window=-1), _native.RKV_ERR_INVALID_ARGUMENT),
+    (dict(table_blocks=1 << 31), _native.RKV_ERR_INVALID_ARGUMENT),
+    (dict(query_dtype=2), _native.RKV_ERR_INVALID_ARGUMENT),
+    (dict(group=17), _native.RKV_ERR_UNSUPPORTED),
+    (dict(group=0), _native.RKV_ERR_UNSUPPORTED),
+    (dict(head_dim=288), _native.RKV_ERR_UNSUPPORTED),
+    (dict(block_size=8), _native.RKV_ERR_UNSUPPORTED),
+    (dict(sequences=8193), _native.RKV_ERR_UNSUPPORTED),
+    (dict(workspace=0), _native.RKV_ERR_WORKSPACE),
+    (dict(workspace_size=16), _native.RKV_ERR_WORKSPACE),
+    (dict(query=24), _native.RKV_ERR_ALIGNMENT),
+    (dict(kps=100), _native.RKV_ERR_ALIGNMENT),
+    (dict(sequences=0), _native.RKV_OK),
+])
+def test_attention_entry_point_refuses_before_touching_a_device(lib, change, code):
+    assert _attend(lib, **change) == code
+    assert lib.rkv_paged_attention(None, None) == _native.RKV_ERR_INVALID_ARGUMENT
