@@ -433,12 +433,12 @@ int rows_map(CUtensorMap* map, const void* base, int64_t dim, int64_t rows, int6
 }
 
 // 4-D bf16 map of K/V pages (dim, row in page, head, page), read one
-// [block x 64] box per page and column half (the same shared-memory tile as
-// rows_map's boxes).  Contiguous pages and HND / NHD page pools are the
+// [block x 64] box per page and column half, or in boxes of `box_rows` rows
+// (the same shared-memory tile as rows_map's boxes).  Contiguous pages and HND / NHD page pools are the
 // same map with different strides.
 int pages_map(CUtensorMap* map, const void* base, int64_t dim, int64_t block, int64_t heads,
               int64_t pages, int64_t token_stride, int64_t head_stride, int64_t page_stride,
-              const char* what) {
+              const char* what, int box_rows = 0) {
   EncodeTiled encode = encoder();
   if (encode == nullptr) return fail(RKV_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   if (!aligned16(base) || (token_stride * 2) % 16 != 0 || (head_stride * 2) % 16 != 0 ||
@@ -453,7 +453,7 @@ int pages_map(CUtensorMap* map, const void* base, int64_t dim, int64_t block, in
   cuuint64_t gstride[3] = {static_cast<cuuint64_t>(token_stride * 2),
                            static_cast<cuuint64_t>((heads > 1 ? head_stride : block * token_stride) * 2),
                            static_cast<cuuint64_t>((pages > 1 ? page_stride : heads * block * token_stride) * 2)};
-  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(block), 1, 1};
+  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows > 0 ? box_rows : block), 1, 1};
   cuuint32_t estride[4] = {1, 1, 1, 1};
   const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), gdim,
                             gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -739,6 +739,20 @@ int run_selector(const Plan& pl, const rkv_summary* s, const void* q, int qdtype
 }  // namespace
 
 void set_last_error(const std::string& message) { g_last_error = message; }
+
+int device_sms(int* sms) {
+  DeviceInfo info;
+  const int rc = device_info(&info);
+  if (rc == RKV_OK) *sms = info.sms;
+  return rc;
+}
+
+int pool_map(CUtensorMap* map, const void* base, int64_t dim, int64_t block, int box_rows,
+             int64_t heads, int64_t pages, int64_t token_stride, int64_t head_stride,
+             int64_t page_stride, const char* what) {
+  return pages_map(map, base, dim, block, heads, pages, token_stride, head_stride, page_stride,
+                   what, box_rows);
+}
 
 cudaError_t ensure_smem_limit(const void* func, size_t bytes) {
   int dev = 0;

@@ -3,7 +3,6 @@
 #pragma once
 
 #include <cuda.h>
-#include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -297,27 +296,41 @@ struct RowsParams {
 cudaError_t launch_rows(const RowsParams& p, bool f32, bool vector, bool interleaved, bool append,
                         cudaStream_t stream);
 
+constexpr int64_t kMostSequences = 8192;      // the kernel's table of lengths in shared memory
+constexpr int64_t kMostPagedHeads = 4096;
+constexpr int64_t kMostPagedTokens = 1 << 30;  // of one sequence
+
+struct PagedMaps {
+  CUtensorMap keys;  // pages_map's map of the pool, read in boxes of a tile's rows at most
+  CUtensorMap values;
+};
+
 struct PagedParams {
   const void* query;
   int64_t q_seq, q_head;  // element strides
   int query_f32;
   void* out;
   float* lse;  // or null
-  const __nv_bfloat16* keys;
-  const __nv_bfloat16* values;
-  int64_t k_page, k_head, k_row, v_page, v_head, v_row;
   const int32_t* page_table;
   int64_t page_table_stride;
   const int32_t* lengths;
   int sequences, heads, group, dim;
-  int block_shift;
-  int64_t table_blocks, pool_pages;
-  int64_t window;  // 0: none
+  int block_shift, capacity, pool_pages;
+  int window;  // 0: none
   float scale;
   int* status;
+  int* counters;          // three per CTA, zero between calls
+  float* warp_partials;   // one per warp
+  float* cta_partials;    // two per CTA
+  float* group_partials;  // two per CTA
 };
 
-cudaError_t launch_paged(const PagedParams& p, cudaStream_t stream);
+// Host helpers of rkv_capi.cu for entry points in other files: the current
+// device's SM count, and the 4-D map of a page pool with boxes of `box_rows`.
+int device_sms(int* sms);
+int pool_map(CUtensorMap* map, const void* base, int64_t dim, int64_t block, int box_rows,
+             int64_t heads, int64_t pages, int64_t token_stride, int64_t head_stride,
+             int64_t page_stride, const char* what);
 
 // Raise `func`'s dynamic shared-memory limit to at least `bytes` on the
 // current device.  Done once per (kernel, device): later calls, including

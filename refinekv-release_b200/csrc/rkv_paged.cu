@@ -1,8 +1,30 @@
-// Dense attention of one new token per sequence over a page pool.
+// Dense attention of one new token per sequence over a page pool, in one launch.
 //
-// One CTA per (query head, sequence), four warps: warp w takes the visible
-// rows w, w + 4, ... with an online softmax (a lane holds dim / 32 channels),
-// and the warps' partials are merged in shared memory.
+// Mathematics.  Per sequence s and KV head h a row of `group` queries attends
+// to the visible tokens of its sequence: an online softmax over tiles of R
+// tokens keeps (m, l, o) per query, and partial results over parts of the
+// tokens join exactly as l = sum l_i e^(m_i - m), o = sum o_i e^(m_i - m).
+//
+// Bound: HBM.  Each visible K and V row is read once (4 D bytes for 4 G D
+// flop, G <= 16).  mma.sync with the tokens on M and the group on N leaves
+// the tensor pipe nearly idle at the streaming rate, so tcgen05 (M = 64 at
+// least, operands from shared memory descriptors) would not move the bound.
+//
+// Split.  The tiles of all rows, sequence-major then head, form one list that
+// is cut into equal contiguous ranges, one per CTA, and each CTA's range into
+// equal contiguous ranges, one per warp: every warp streams the same number
+// of tiles whatever the lengths are.  A warp streams through its own
+// shared-memory stage by TMA with one barrier each for K and V (K of the next
+// tile is requested as soon as this one's scores are done).  Rows that lie
+// within one warp's range are written from registers; a row cut by a range
+// end leaves a partial, at most two per warp; the CTA joins its warps'
+// partials, and a row cut by CTA ranges is joined by whichever of its CTAs
+// arrives last at a counter -- nobody waits.  All joins run in token order, so
+// results repeat bit for bit.
+//
+// The lengths and the page table are read on the device (graphs replay with
+// growing sequences): every CTA scans the lengths itself.
+#include <algorithm>
 #include <string>
 
 #include "refinekv_b200.h"
@@ -14,77 +36,619 @@ void set_last_error(const std::string& message);
 
 namespace {
 
-constexpr int kWarps = 4;
+// Tokens per tile: 64 for head dims up to 64, else 32, so that a K and V tile
+// is 16 KB at D 64 and 128.
+constexpr int tile_rows(int D) { return D <= 64 ? 64 : 32; }
+// One stage (a K and a V tile) per warp, up to eight warps.
+constexpr int paged_warps(int D) { return D <= 192 ? 8 : 6; }
+constexpr int stage_bytes(int D) { return 2 * tile_rows(D) * D * 2; }
 
-template <int C>
-__global__ void __launch_bounds__(kWarps * 32) paged_kernel(const __grid_constant__ PagedParams p) {
-  __shared__ float sm_m[kWarps], sm_l[kWarps], sm_o[kWarps][C * 32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row = blockIdx.x, seq = blockIdx.y, head = row / p.group;
-  int64_t length = p.lengths[seq];
-  const int64_t most = p.table_blocks << p.block_shift;
-  if (length < 0 || length > most) {
-    if (threadIdx.x == 0) atomicOr(p.status, kStatusBadInput);
-    length = length < 0 ? 0 : most;
-  }
-  const int64_t low = p.window > 0 && length > p.window ? length - p.window : 0;
-  float q[C], o[C];
-#pragma unroll
-  for (int i = 0; i < C; ++i) {
-    const int64_t at = seq * p.q_seq + row * p.q_head + lane * C + i;
-    q[i] = p.query_f32 ? bf16_round(static_cast<const float*>(p.query)[at])
-                       : __bfloat162float(static_cast<const __nv_bfloat16*>(p.query)[at]);
-    o[i] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  for (int64_t j = low + warp; j < length; j += kWarps) {
-    int64_t page = p.page_table[seq * p.page_table_stride + (j >> p.block_shift)];
-    if (page < 0 || page >= p.pool_pages) {
-      if (lane == 0) atomicOr(p.status, kStatusBadInput);
-      page = 0;
-    }
-    const int64_t in = j & ((1 << p.block_shift) - 1);
-    const __nv_bfloat16* k = p.keys + page * p.k_page + head * p.k_head + in * p.k_row + lane * C;
-    const __nv_bfloat16* v = p.values + page * p.v_page + head * p.v_head + in * p.v_row + lane * C;
-    float x = 0.f;
-#pragma unroll
-    for (int i = 0; i < C; ++i) x += q[i] * __bfloat162float(k[i]);
-    for (int s = 16; s > 0; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
-    x *= p.scale;
-    const float top = fmaxf(m, x), ref = top == -INFINITY ? 0.f : top;
-    const float keep = __expf(m - ref), w = __expf(x - ref);
-    m = top;
-    l = l * keep + w;
-#pragma unroll
-    for (int i = 0; i < C; ++i) o[i] = o[i] * keep + w * __bfloat162float(v[i]);
-  }
-  if (lane == 0) {
-    sm_m[warp] = m;
-    sm_l[warp] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < C; ++i) sm_o[warp][lane * C + i] = o[i];
-  __syncthreads();
-  float top = -INFINITY, sum = 0.f;
-  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_m[w]);
-  const float ref = top == -INFINITY ? 0.f : top;
-  for (int w = 0; w < kWarps; ++w) sum += sm_l[w] * __expf(sm_m[w] - ref);
-  const int64_t out_row = static_cast<int64_t>(seq) * p.heads * p.group + row;
-  for (int d = threadIdx.x; d < p.dim; d += blockDim.x) {
-    float acc = 0.f;
-    for (int w = 0; w < kWarps; ++w) acc += sm_o[w][d] * __expf(sm_m[w] - ref);
-    // An empty row is zero; a row whose every logit is -inf is 0 / 0 as the formula has it.
-    const float y = length > low ? acc / sum : 0.f;
-    if (p.query_f32) static_cast<float*>(p.out)[out_row * p.dim + d] = y;
-    else static_cast<__nv_bfloat16*>(p.out)[out_row * p.dim + d] = __float2bfloat16_rn(y);
-  }
-  if (p.lse != nullptr && threadIdx.x == 0) p.lse[out_row] = ref + logf(sum);
+// A row's CTAs are joined in one level up to this many, else in groups.
+constexpr int kFlatJoin = 16;
+
+// Workspace: status word, counters (at the same place for every geometry;
+// they are zero between calls), then the partials.
+constexpr size_t kCounterBytes = 256;
+constexpr int kMostCtas = 512;
+constexpr size_t kHeader = 8192;
+
+// A partial: m[G8], l[G8], o[G8][D].
+constexpr int partial_floats(int D, int NT) { return NT * 8 * (D + 2); }
+
+struct Cursor {
+  int seq, head, tile, tiles;  // tile of `tiles` of the row
+  int first;                   // the row's first tile, in tiles from the sequence's start
+  int low, length;             // visible tokens [low, length)
+};
+
+template <int D, int NT>
+struct Paged {
+  static constexpr int R = tile_rows(D);
+  static constexpr int W = paged_warps(D);
+  static constexpr int G8 = NT * 8;
+  static constexpr int kTile = R * D * 2;
+  static constexpr int kPartial = partial_floats(D, NT);
+};
+
+__device__ __forceinline__ int clamp_length(const PagedParams& p, int seq) {
+  const int length = p.lengths[seq];
+  return max(0, min(length, p.capacity));
 }
 
-template <int C>
-cudaError_t launch_c(const PagedParams& p, cudaStream_t stream) {
-  paged_kernel<C><<<dim3(p.heads * p.group, p.sequences), kWarps * 32, 0, stream>>>(p);
-  return cudaGetLastError();
+__device__ __forceinline__ int first_visible(const PagedParams& p, int length) {
+  return p.window > 0 && length > p.window ? length - p.window : 0;
+}
+
+// Tiles of a sequence: those that hold its visible tokens.
+template <int R>
+__device__ __forceinline__ int tiles_of(const PagedParams& p, int seq) {
+  const int length = clamp_length(p, seq);
+  return (length + R - 1) / R - first_visible(p, length) / R;
+}
+
+template <int R>
+__device__ __forceinline__ void enter_row(const PagedParams& p, const int* start, Cursor& c) {
+  c.tiles = start[c.seq + 1] - start[c.seq];
+  c.length = clamp_length(p, c.seq);
+  c.low = first_visible(p, c.length);
+  c.first = c.low / R;
+}
+
+// The cursor at global tile x.
+template <int R>
+__device__ __forceinline__ Cursor seek(const PagedParams& p, const int* start, long long x) {
+  int a = 0, b = p.sequences;  // start[a] * heads <= x < start[b] * heads
+  while (b - a > 1) {
+    const int mid = (a + b) >> 1;
+    if (static_cast<long long>(start[mid]) * p.heads <= x) a = mid; else b = mid;
+  }
+  Cursor c;
+  c.seq = a;
+  enter_row<R>(p, start, c);
+  const long long y = x - static_cast<long long>(start[a]) * p.heads;
+  c.head = static_cast<int>(y / c.tiles);
+  c.tile = static_cast<int>(y - static_cast<long long>(c.head) * c.tiles);
+  return c;
+}
+
+// The next tile of the list (there must be one).
+template <int R>
+__device__ __forceinline__ void advance(const PagedParams& p, const int* start, Cursor& c) {
+  if (++c.tile < c.tiles) return;
+  c.tile = 0;
+  if (++c.head < p.heads) return;
+  c.head = 0;
+  do ++c.seq; while (start[c.seq + 1] == start[c.seq]);
+  enter_row<R>(p, start, c);
+}
+
+// Query B fragments: rows at `q`, p.q_head elements apart.
+template <int D, int NT>
+__device__ __forceinline__ void load_queries(uint32_t (&qb)[D / 16][NT][2], const PagedParams& p,
+                                             int seq, int head, int lane) {
+  const int64_t base = seq * p.q_seq + static_cast<int64_t>(head) * p.group * p.q_head;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int g = nt * 8 + (lane >> 2);
+    const int64_t row = base + min(g, p.group - 1) * p.q_head;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int d = ks * 16 + half * 8 + 2 * (lane & 3);
+        const int64_t at = row + min(d, p.dim - 2);
+        uint32_t bits;
+        if (p.query_f32) {
+          const float2 x = *reinterpret_cast<const float2*>(static_cast<const float*>(p.query) + at);
+          bits = pack_bf16(x.x, x.y);
+        } else {
+          bits = *reinterpret_cast<const uint32_t*>(
+              static_cast<const __nv_bfloat16*>(p.query) + at);
+        }
+        qb[ks][nt][half] = g < p.group && d < p.dim ? bits : 0u;
+      }
+  }
+}
+
+// o += V^T p for a tile's weights p (C layout), held in `Terms` bf16 terms:
+// one for bf16 queries (rounded, 2^-8 at most, within the output's own
+// rounding), three for fp32 queries, which hold all 24 bits of p.  The further
+// terms may be negative or zero, so they meet V with its infinities clamped:
+// an infinite value times p is infinite, whatever p's bits are.
+template <int R, int D, int NT, int Terms>
+__device__ __forceinline__ void weigh_values(uint32_t tile, float (&p)[R / 16][NT][4],
+                                             float (&o)[D / 16][NT][4], int lane) {
+  uint32_t frag[Terms][R / 16][NT][2];
+#pragma unroll
+  for (int term = 0; term < Terms; ++term)
+#pragma unroll
+    for (int mt = 0; mt < R / 16; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float& a = p[mt][nt][2 * half];
+          float& b = p[mt][nt][2 * half + 1];
+          const __nv_bfloat162 part = __floats2bfloat162_rn(a, b);
+          a -= __low2float(part);
+          b -= __high2float(part);
+          frag[term][mt][nt][half] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&part));
+        }
+  const int trow = (lane & 7) + ((lane >> 4) & 1) * 8;
+  const int cadd = (lane >> 3) & 1;
+#pragma unroll
+  for (int dt = 0; dt < D / 16; ++dt) {
+#pragma unroll
+    for (int kt = 0; kt < R / 16; ++kt) {
+      uint32_t a[4];
+      ldsm_x4_trans(tile + swz(kt * 16 + trow, dt * 2 + cadd, R), a);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) mma_bf16(o[dt][nt], a, frag[0][kt][nt][0], frag[0][kt][nt][1]);
+      if constexpr (Terms > 1) {
+        const __nv_bfloat162 most = __halves2bfloat162(__ushort_as_bfloat16(0x7f7f),
+                                                       __ushort_as_bfloat16(0x7f7f));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          __nv_bfloat162& v = *reinterpret_cast<__nv_bfloat162*>(&a[i]);
+          v = __hmax2(__hmin2(v, most), __hneg2(most));
+        }
+#pragma unroll
+        for (int term = 1; term < Terms; ++term)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mma_bf16(o[dt][nt], a, frag[term][kt][nt][0], frag[term][kt][nt][1]);
+      }
+    }
+  }
+}
+
+// One normalised output value; an all -inf row is 0 / 0, as the formula has it.
+__device__ __forceinline__ void put(const PagedParams& p, int64_t at, float x) {
+  if (p.query_f32) static_cast<float*>(p.out)[at] = x;
+  else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(x);
+}
+
+// Joins `count` partials of one row (part(k) points at the k-th's m, l, o):
+// channels d, d + 1 of query g.  Remote: other CTAs wrote them.
+template <int D, int G8, bool Remote, typename Part>
+__device__ __forceinline__ void join(int count, Part part, int g, int d, float& m, float& l,
+                                     float2& o) {
+  constexpr int kBatch = 8;
+  m = -INFINITY;
+  l = 0.f;
+  o = make_float2(0.f, 0.f);
+  for (int k0 = 0; k0 < count; k0 += kBatch) {
+    float mk[kBatch], lk[kBatch];
+    float2 ok[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (k0 + u < count) {
+        const float* at = part(k0 + u);
+        const float2* row = reinterpret_cast<const float2*>(at + 2 * G8 + g * D + d);
+        mk[u] = Remote ? __ldcg(at + g) : at[g];
+        lk[u] = Remote ? __ldcg(at + G8 + g) : at[G8 + g];
+        ok[u] = Remote ? __ldcg(row) : *row;
+      } else {
+        mk[u] = -INFINITY;
+        lk[u] = 0.f;
+        ok[u] = make_float2(0.f, 0.f);
+      }
+    }
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) top = fmaxf(top, mk[u]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    const float keep = __expf(m - ref);
+    l *= keep;
+    o.x *= keep;
+    o.y *= keep;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (k0 + u < count) {
+        const float w = __expf(mk[u] - ref);
+        l += w * lk[u];
+        o.x += w * ok[u].x;
+        o.y += w * ok[u].y;
+      }
+    }
+    m = top;
+  }
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(paged_warps(D) * 32, 1)
+    paged_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant__ PagedParams p) {
+  using K = Paged<D, NT>;
+  constexpr int R = K::R, W = K::W, G8 = K::G8, kTile = K::kTile, kPartial = K::kPartial;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = align_smem(smem_raw);  // [warp][K | V]
+  __shared__ __align__(8) uint64_t bars[W][2];
+  __shared__ int warp_sum[W];
+  __shared__ int seg_row[2 * W];  // the row of each of the CTA's partials, or -1
+  __shared__ int last_arrival;
+  int* start = reinterpret_cast<int*>(ring + W * 2 * kTile);  // tiles before each sequence
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) {
+    mbar_init(&bars[warp][0], 1);
+    mbar_init(&bars[warp][1], 1);
+    mbar_fence_init();
+    seg_row[2 * warp] = seg_row[2 * warp + 1] = -1;
+  }
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&maps.keys);
+    tma_prefetch_desc(&maps.values);
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // start[s] = tiles of the sequences before s, by a scan over the CTA.
+  {
+    const int per = (p.sequences + W * 32 - 1) / (W * 32);
+    const int s0 = min(p.sequences, static_cast<int>(threadIdx.x) * per);
+    const int s1 = min(p.sequences, s0 + per);
+    int sum = 0;
+    for (int s = s0; s < s1; ++s) {
+      if (blockIdx.x == 0 && (p.lengths[s] < 0 || p.lengths[s] > p.capacity)) {
+        atomicOr(p.status, kStatusBadInput);
+      }
+      sum += tiles_of<R>(p, s);
+    }
+    int scan = sum;
+#pragma unroll
+    for (int step = 1; step < 32; step <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, scan, step);
+      if (lane >= step) scan += other;
+    }
+    if (lane == 31) warp_sum[warp] = scan;
+    __syncthreads();
+    int before = scan - sum;
+    for (int w = 0; w < warp; ++w) before += warp_sum[w];
+    for (int s = s0; s < s1; ++s) {
+      start[s] = before;
+      before += tiles_of<R>(p, s);
+    }
+    if (s1 == p.sequences && s0 < s1) start[p.sequences] = before;
+    __syncthreads();
+  }
+  const long long T = static_cast<long long>(start[p.sequences]) * p.heads;
+  // Idle slots: zero rows.
+  for (int s = blockIdx.x; s < p.sequences; s += gridDim.x) {
+    if (start[s + 1] != start[s]) continue;
+    const int queries = p.heads * p.group;
+    const int64_t row = static_cast<int64_t>(s) * queries;
+    for (int i = threadIdx.x; i < queries * p.dim; i += blockDim.x) put(p, row * p.dim + i, 0.f);
+    if (p.lse != nullptr) {
+      for (int i = threadIdx.x; i < queries; i += blockDim.x) p.lse[row + i] = -INFINITY;
+    }
+  }
+  const long long C = min(static_cast<long long>(gridDim.x), (T + W - 1) / W);
+  const long long cta = blockIdx.x;
+  if (cta >= C) return;
+  const long long lo = T * cta / C, hi = T * (cta + 1) / C;
+  const long long wlo = lo + (hi - lo) * warp / W, whi = lo + (hi - lo) * (warp + 1) / W;
+
+  uint8_t* stage = ring + warp * 2 * kTile;
+  const uint32_t k_tile = smem_addr(stage), v_tile = k_tile + kTile;
+  float* warp_partial = p.warp_partials + (cta * W + warp) * kPartial;
+  float* stash = reinterpret_cast<float*>(stage);
+  const uint64_t policy = l2_evict_first_policy();
+  const int page_rows = 1 << p.block_shift;
+  const int box_rows = min(R, page_rows), boxes = R / box_rows;
+
+  // Lane i of the first `boxes` lanes looks up the page of the tile's i-th
+  // box, or -1 where the box holds no visible token.
+  auto page_of = [&](const Cursor& c) {
+    if (lane >= boxes) return -1;
+    const int token = (c.first + c.tile) * R + lane * box_rows;
+    if (token >= c.length || token + box_rows <= c.low) return -1;
+    const int page = p.page_table[c.seq * p.page_table_stride + (token >> p.block_shift)];
+    if (page >= 0 && page < p.pool_pages) return page;
+    atomicOr(p.status, kStatusBadInput);  // flag the call; read page 0 instead
+    return 0;
+  };
+  auto issue = [&](int which, const Cursor& c, int page) {
+    uint64_t* bar = &bars[warp][which];
+    const unsigned used = __ballot_sync(0xffffffffu, page >= 0);
+    if (lane == 0) mbar_expect_tx(bar, __popc(used) * box_rows * D * 2);
+    fence_proxy_async();
+    __syncwarp();
+    if (page >= 0) {
+      const int token = (c.first + c.tile) * R + lane * box_rows;
+      uint8_t* to = stage + which * kTile + lane * box_rows * 128;
+      const CUtensorMap* map = which ? &maps.values : &maps.keys;
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) {
+        tma_load_4d_hint(to + i * R * 128, map, bar, i * 64, token & (page_rows - 1), c.head, page,
+                         policy);
+      }
+    }
+  };
+
+  if (wlo < whi) {
+    uint32_t qb[D / 16][NT][2];
+    float m[NT][2], l[NT][2], o[D / 16][NT][4];
+    Cursor cur = seek<R>(p, start, wlo), next = cur;
+    int page = page_of(cur);
+    issue(0, cur, page);
+    issue(1, cur, page);
+    const int count = static_cast<int>(whi - wlo);
+    int seg_first = cur.tile;  // the segment's first tile of its row
+    bool fresh = true, aborted = false;
+    if (count > 1) {
+      advance<R>(p, start, next);
+      page = page_of(next);
+    }
+    for (int j = 0; j < count; ++j) {
+      if (fresh) {
+        load_queries<D, NT>(qb, p, cur.seq, cur.head, lane);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          m[nt][0] = m[nt][1] = -INFINITY;
+          l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+          for (int dt = 0; dt < D / 16; ++dt)
+            o[dt][nt][0] = o[dt][nt][1] = o[dt][nt][2] = o[dt][nt][3] = 0.f;
+        }
+        fresh = false;
+      }
+      const bool more = j + 1 < count;
+      const int token = (cur.first + cur.tile) * R;
+      const int row_lo = max(0, cur.low - token), row_hi = min(R, cur.length - token);
+      // A wait that runs out leaves the rest of the warp's range out (the
+      // status word says so); nothing is in flight after its drain.
+      if (!aborted && !warp_wait(&bars[warp][0], j & 1)) {
+        if (lane == 0) atomicOr(p.status, kStatusTimeout);
+        warp_wait(&bars[warp][1], j & 1);
+        aborted = true;
+      }
+      if (!aborted) {
+        float logit[R / 16][NT][4];
+        score_tile<R, D, NT>(k_tile, qb, logit, lane);
+#pragma unroll
+        for (int mt = 0; mt < R / 16; ++mt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int r = mt * 16 + (lane >> 2) + (c >> 1) * 8;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              logit[mt][nt][c] =
+                  r >= row_lo && r < row_hi ? logit[mt][nt][c] * p.scale : -INFINITY;
+          }
+        __syncwarp();
+        if (more) issue(0, next, page);
+        softmax_update<R, D, NT>(logit, m, l, o);
+        if (!warp_wait(&bars[warp][1], j & 1)) {
+          if (lane == 0) atomicOr(p.status, kStatusTimeout);
+          warp_wait(&bars[warp][1], j & 1);
+          if (more) warp_wait(&bars[warp][0], (j + 1) & 1);
+          aborted = true;
+        } else {
+          if (row_lo > 0 || row_hi < R) {
+            // Rows that are not visible may hold anything: a weight of zero
+            // would not silence a NaN, so they are zeroed.
+            for (int i = lane; i < R * (D / 8); i += 32) {
+              const int r = i / (D / 8), c16 = i - r * (D / 8);
+              if (r < row_lo || r >= row_hi) {
+                *reinterpret_cast<uint4*>(stage + kTile + swz(r, c16, R)) = make_uint4(0, 0, 0, 0);
+              }
+            }
+            fence_proxy_async();
+            __syncwarp();
+          }
+          if (p.query_f32) {
+            weigh_values<R, D, NT, 3>(v_tile, logit, o, lane);
+          } else {
+            weigh_values<R, D, NT, 1>(v_tile, logit, o, lane);
+          }
+          __syncwarp();
+          if (more) issue(1, next, page);
+        }
+      }
+      const bool row_done = cur.tile + 1 == cur.tiles;
+      if (row_done || !more) {
+        reduce_l<NT>(l);
+        const int row = cur.seq * p.heads + cur.head;
+        const bool whole = row_done && seg_first == 0;
+        if (whole) {
+          const int64_t out_row = static_cast<int64_t>(row) * p.group;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int g = nt * 8 + 2 * (lane & 3) + c;
+              if (g >= p.group) continue;
+              const float inv = 1.f / l[nt][c];
+#pragma unroll
+              for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                  const int d = dt * 16 + half * 8 + (lane >> 2);
+                  if (d < p.dim) put(p, (out_row + g) * p.dim + d, o[dt][nt][2 * half + c] * inv);
+                }
+              if (p.lse != nullptr && lane < 4) {
+                const float ref = m[nt][c] == -INFINITY ? 0.f : m[nt][c];
+                p.lse[out_row + g] = ref + logf(l[nt][c]);
+              }
+            }
+        } else {
+          // The range's last row waits in the warp's own idle stage, an
+          // earlier one (which began before the range) in the workspace.
+          float* to = more ? warp_partial : stash;
+          if (lane == 0) seg_row[2 * warp + (more ? 0 : 1)] = row;
+          stash_warp_partial<D, NT>(to, to + G8, to + 2 * G8, 0, lane, m, l, o);
+        }
+        seg_first = 0;
+        fresh = true;
+      }
+      if (more) {
+        cur = next;
+        if (j + 2 < count) {
+          advance<R>(p, start, next);
+          page = page_of(next);
+        }
+      }
+    }
+  }
+  __syncthreads();
+
+  // Join the CTA's partials row by row (they lie in token order).  A row that
+  // began and ended within the CTA is written; one that began before it goes
+  // to the CTA's slot 0, one that only goes on after it to slot 1.
+  auto segment = [&](int i) -> const float* {
+    const int w = i >> 1;
+    return i & 1 ? reinterpret_cast<const float*>(ring + w * 2 * kTile)
+                 : p.warp_partials + (cta * W + w) * kPartial;
+  };
+  constexpr int kChunks = D / 64;  // 64 channels, two per lane
+  int cut[2] = {-1, -1};  // the rows in slots 0 and 1
+  int turn = 0;
+  for (int i = 0; i < 2 * W;) {
+    const int row = seg_row[i];
+    if (row < 0) {
+      ++i;
+      continue;
+    }
+    int list[2 * W], count = 0;  // compile-time bound; indices in local order
+    for (; i < 2 * W && (seg_row[i] == row || seg_row[i] < 0); ++i) {
+      if (seg_row[i] == row) list[count++] = i;
+    }
+    const int seq = row / p.heads, head = row - seq * p.heads;
+    const int tiles = start[seq + 1] - start[seq];
+    const long long begin = static_cast<long long>(start[seq]) * p.heads +
+                            static_cast<long long>(head) * tiles;
+    const bool before = begin < lo, after = begin + tiles > hi;
+    const int slot = before ? 0 : 1;
+    if (before || after) cut[slot] = row;
+    float* to = p.cta_partials + (cta * 2 + slot) * kPartial;
+    for (int c = 0; c < p.group * kChunks; ++c, ++turn) {
+      if (turn % W != warp) continue;
+      const int g = c / kChunks, d = (c - g * kChunks) * 64 + 2 * lane;
+      float m, l;
+      float2 o;
+      join<D, G8, false>(count, [&](int k) { return segment(list[k]); }, g, d, m, l, o);
+      if (before || after) {
+        *reinterpret_cast<float2*>(to + 2 * G8 + g * D + d) = o;
+        if (d == 0) {
+          to[g] = m;
+          to[G8 + g] = l;
+        }
+      } else {
+        const int64_t out_row = static_cast<int64_t>(row) * p.group + g;
+        if (d < p.dim) {
+          put(p, out_row * p.dim + d, o.x / l);
+          put(p, out_row * p.dim + d + 1, o.y / l);
+        }
+        if (d == 0 && p.lse != nullptr) {
+          p.lse[out_row] = (m == -INFINITY ? 0.f : m) + logf(l);
+        }
+      }
+    }
+  }
+
+  // Rows cut by CTA ranges: the last of a row's CTAs to arrive joins them; a
+  // row over many CTAs is joined in groups first, so that no CTA reads more
+  // than a few partials.
+  for (int slot = 0; slot < 2; ++slot) {
+    const int row = cut[slot];
+    if (row < 0) continue;
+    const int seq = row / p.heads, head = row - seq * p.heads;
+    const int tiles = start[seq + 1] - start[seq];
+    const long long begin = static_cast<long long>(start[seq]) * p.heads +
+                            static_cast<long long>(head) * tiles;
+    // The CTA that holds tile x.
+    const auto owner = [&](long long x) { return static_cast<int>(((x + 1) * C + T - 1) / T - 1); };
+    const int c1 = owner(begin), parts = owner(begin + tiles - 1) - c1 + 1;
+    int fan = parts;
+    if (parts > kFlatJoin) {
+      fan = 1;
+      while (fan * fan < parts) ++fan;
+    }
+    const int groups = (parts + fan - 1) / fan;
+    const int mine = (static_cast<int>(cta) - c1) / fan;
+    const int first = c1 + mine * fan;
+    // Partials of the row's CTA c, and of the group that begins at it.  A CTA
+    // can end one row (slot 0) and begin another (slot 1).
+    const auto slot_of = [&](int c) {
+      return p.cta_partials + (static_cast<int64_t>(c) * 2 + (c == c1 ? 1 : 0)) * kPartial;
+    };
+    const auto group_slot = [&](int c) {
+      return p.group_partials + (static_cast<int64_t>(c) * 2 + (c == c1 ? 1 : 0)) * kPartial;
+    };
+    const auto arrive = [&](int* counter, int expected) {
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        __threadfence();
+        const int seen = atomicAdd(counter, 1);
+        last_arrival = seen == expected - 1;
+        if (last_arrival) *counter = 0;
+        __threadfence();
+      }
+      __syncthreads();
+      return last_arrival != 0;
+    };
+    const int members = min(fan, parts - mine * fan);
+    if (!arrive(p.counters + first * 3 + (first == c1 ? 1 : 0), members)) continue;
+    const auto combine = [&](int count, auto part, bool final) {
+      for (int c = warp; c < p.group * kChunks; c += W) {
+        const int g = c / kChunks, d = (c - g * kChunks) * 64 + 2 * lane;
+        float m, l;
+        float2 o;
+        join<D, G8, true>(count, part, g, d, m, l, o);
+        if (final) {
+          const int64_t out_row = static_cast<int64_t>(row) * p.group + g;
+          if (d < p.dim) {
+            put(p, out_row * p.dim + d, o.x / l);
+            put(p, out_row * p.dim + d + 1, o.y / l);
+          }
+          if (d == 0 && p.lse != nullptr) {
+            p.lse[out_row] = (m == -INFINITY ? 0.f : m) + logf(l);
+          }
+        } else {
+          float* to = group_slot(first);
+          *reinterpret_cast<float2*>(to + 2 * G8 + g * D + d) = o;
+          if (d == 0) {
+            to[g] = m;
+            to[G8 + g] = l;
+          }
+        }
+      }
+    };
+    combine(members, [&](int k) { return static_cast<const float*>(slot_of(first + k)); },
+            groups == 1);
+    if (groups == 1) continue;
+    if (!arrive(p.counters + c1 * 3 + 2, groups)) continue;
+    combine(groups,
+            [&](int k) { return static_cast<const float*>(group_slot(c1 + k * fan)); }, true);
+  }
+}
+
+template <int D, int NT>
+cudaError_t launch_t(const PagedMaps& maps, const PagedParams& p, int ctas, cudaStream_t stream) {
+  const size_t smem = kSmemSlack + static_cast<size_t>(paged_warps(D)) * stage_bytes(D) +
+                      static_cast<size_t>(p.sequences + 1) * 4;
+  // One limit for every batch: the largest this kernel takes.
+  const size_t most = kSmemSlack + static_cast<size_t>(paged_warps(D)) * stage_bytes(D) +
+                      static_cast<size_t>(kMostSequences + 1) * 4;
+  cudaError_t err =
+      ensure_smem_limit(reinterpret_cast<const void*>(&paged_kernel<D, NT>), most);
+  if (err != cudaSuccess) return err;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(paged_warps(D) * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_kernel<D, NT>, maps, p);
+}
+
+template <int D>
+cudaError_t launch_d(const PagedMaps& maps, const PagedParams& p, int ctas, cudaStream_t stream) {
+  return p.group <= 8 ? launch_t<D, 1>(maps, p, ctas, stream)
+                      : launch_t<D, 2>(maps, p, ctas, stream);
 }
 
 int reject(int code, const char* message) {
@@ -92,30 +656,38 @@ int reject(int code, const char* message) {
   return code;
 }
 
-}  // namespace
+int padded(int64_t dim) { return static_cast<int>((dim + 63) / 64 * 64); }
 
-cudaError_t launch_paged(const PagedParams& p, cudaStream_t stream) {
-  switch (p.dim / 32) {
-    case 1: return launch_c<1>(p, stream);
-    case 2: return launch_c<2>(p, stream);
-    case 3: return launch_c<3>(p, stream);
-    case 4: return launch_c<4>(p, stream);
-    case 5: return launch_c<5>(p, stream);
-    case 6: return launch_c<6>(p, stream);
-    case 7: return launch_c<7>(p, stream);
-    default: return launch_c<8>(p, stream);
+struct Layout {
+  size_t warp_partials, cta_partials, group_partials, bytes;
+  Layout(int64_t group, int64_t dim, int sms) {
+    const int D = padded(dim), NT = group <= 8 ? 1 : 2;
+    const size_t one = static_cast<size_t>(partial_floats(D, NT)) * 4;
+    size_t off = kHeader;
+    warp_partials = off;
+    off += one * sms * paged_warps(D);
+    cta_partials = off;
+    off += one * sms * 2;
+    group_partials = off;
+    off += one * sms * 2;
+    bytes = (off + 255) & ~static_cast<size_t>(255);
   }
-}
+};
+
+}  // namespace
 
 }  // namespace rkv
 
 extern "C" {
 
 size_t rkv_paged_workspace_size(int64_t group, int64_t head_dim) {
-  if (group < 1 || group > rkv::kMaxGroup || head_dim < 32 || head_dim > 256 || head_dim % 32) {
+  using namespace rkv;
+  int sms = 0;
+  if (group < 1 || group > kMaxGroup || head_dim < 32 || head_dim > 256 || head_dim % 32 ||
+      device_sms(&sms) != RKV_OK || sms > kMostCtas) {
     return 0;
   }
-  return 256;
+  return Layout(group, head_dim, sms).bytes;
 }
 
 int rkv_paged_attention(const rkv_paged_args* a, void* stream) {
@@ -131,39 +703,59 @@ int rkv_paged_attention(const rkv_paged_args* a, void* stream) {
   if (a->group < 1 || a->group > kMaxGroup) {
     return reject(RKV_ERR_UNSUPPORTED, "group must be 1..16");
   }
-  if (a->sequences < 0 || a->sequences > 8192 || a->kv_heads < 1 || a->kv_heads > 4096) {
+  if (a->sequences < 0 || a->sequences > kMostSequences || a->kv_heads < 1 ||
+      a->kv_heads > kMostPagedHeads) {
     return reject(RKV_ERR_UNSUPPORTED, "at most 8192 sequences and 4096 KV heads");
   }
   if (a->query_dtype != RKV_DTYPE_BF16 && a->query_dtype != RKV_DTYPE_F32) {
     return reject(RKV_ERR_INVALID_ARGUMENT, "query dtype must be bf16 or fp32");
   }
-  if (a->window < 0 || a->table_blocks < 0 || a->table_blocks > (1LL << 31) / a->block_size - 1 ||
-      a->page_table_stride < 0 || a->pool_pages < 0 || a->pool_pages > (1LL << 31) - 1) {
+  if (a->window < 0 || a->table_blocks < 0 ||
+      a->table_blocks > kMostPagedTokens / a->block_size || a->page_table_stride < 0 ||
+      a->pool_pages < 0 || a->pool_pages > (1LL << 31) - 1) {
     return reject(RKV_ERR_INVALID_ARGUMENT, "window, page table or pool sizes are out of range");
   }
+  if (a->sequences * a->table_blocks * (a->block_size / 16) > (1LL << 31) - 1) {
+    return reject(RKV_ERR_UNSUPPORTED, "the page table covers more tokens than are counted");
+  }
   if (a->sequences == 0) return RKV_OK;
-  if (!a->query || !a->output || !a->lengths ||
-      (a->table_blocks > 0 && (!a->page_table || !a->key_pool || !a->value_pool))) {
+  if (!a->query || !a->output || !a->lengths || !a->key_pool || !a->value_pool ||
+      !a->page_table) {
     return reject(RKV_ERR_INVALID_ARGUMENT,
                   "query, output, pools, page_table and lengths must be non-null");
   }
-  if (a->table_blocks > 0 && a->pool_pages < 1) {
-    return reject(RKV_ERR_INVALID_ARGUMENT, "the pool has no pages");
-  }
-  const size_t need = rkv_paged_workspace_size(a->group, a->head_dim);
-  if (a->workspace == nullptr || a->workspace_size < static_cast<int64_t>(need)) {
+  if (a->pool_pages < 1) return reject(RKV_ERR_INVALID_ARGUMENT, "the pool has no pages");
+  if (a->workspace == nullptr || a->workspace_size < static_cast<int64_t>(kHeader)) {
     return reject(RKV_ERR_WORKSPACE, "workspace is missing or too small");
   }
   const int width = a->query_dtype == RKV_DTYPE_F32 ? 4 : 2;
-  uintptr_t bits = reinterpret_cast<uintptr_t>(a->query) | reinterpret_cast<uintptr_t>(a->output) |
-                   reinterpret_cast<uintptr_t>(a->key_pool) |
-                   reinterpret_cast<uintptr_t>(a->value_pool);
+  uintptr_t bits = reinterpret_cast<uintptr_t>(a->query) | reinterpret_cast<uintptr_t>(a->output);
+  bits |= reinterpret_cast<uintptr_t>(a->key_pool) | reinterpret_cast<uintptr_t>(a->value_pool);
   for (int64_t s : a->query_strides) bits |= static_cast<uintptr_t>(s * width);
   for (int64_t s : a->key_pool_strides) bits |= static_cast<uintptr_t>(s * 2);
   for (int64_t s : a->value_pool_strides) bits |= static_cast<uintptr_t>(s * 2);
   if (bits & 15u) {
     return reject(RKV_ERR_ALIGNMENT, "pointers and strides must be 16-byte aligned");
   }
+  int rc = RKV_OK, sms = 0;
+  PagedMaps maps;
+  const int D = padded(a->head_dim), R = tile_rows(D);
+  const int box_rows = static_cast<int>(std::min<int64_t>(R, a->block_size));
+  const int64_t *ks = a->key_pool_strides, *vs = a->value_pool_strides;
+  if ((rc = pool_map(&maps.keys, a->key_pool, a->head_dim, a->block_size, box_rows, a->kv_heads,
+                     a->pool_pages, ks[2], ks[1], ks[0], "key_pool")) != RKV_OK ||
+      (rc = pool_map(&maps.values, a->value_pool, a->head_dim, a->block_size, box_rows,
+                     a->kv_heads, a->pool_pages, vs[2], vs[1], vs[0], "value_pool")) != RKV_OK ||
+      (rc = device_sms(&sms)) != RKV_OK) {
+    return rc;
+  }
+  if (sms > kMostCtas) return reject(RKV_ERR_UNSUPPORTED, "more SMs than the workspace counts");
+  const Layout layout(a->group, a->head_dim, sms);
+  if (a->workspace_size < static_cast<int64_t>(layout.bytes) ||
+      (reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0) {
+    return reject(RKV_ERR_WORKSPACE, "workspace is too small or not 256-byte aligned");
+  }
+  char* ws = static_cast<char*>(a->workspace);
   PagedParams p = {};
   p.query = a->query;
   p.q_seq = a->query_strides[0];
@@ -171,14 +763,6 @@ int rkv_paged_attention(const rkv_paged_args* a, void* stream) {
   p.query_f32 = a->query_dtype == RKV_DTYPE_F32;
   p.out = a->output;
   p.lse = a->lse;
-  p.keys = static_cast<const __nv_bfloat16*>(a->key_pool);
-  p.values = static_cast<const __nv_bfloat16*>(a->value_pool);
-  p.k_page = a->key_pool_strides[0];
-  p.k_head = a->key_pool_strides[1];
-  p.k_row = a->key_pool_strides[2];
-  p.v_page = a->value_pool_strides[0];
-  p.v_head = a->value_pool_strides[1];
-  p.v_row = a->value_pool_strides[2];
   p.page_table = a->page_table;
   p.page_table_stride = a->page_table_stride;
   p.lengths = a->lengths;
@@ -187,12 +771,25 @@ int rkv_paged_attention(const rkv_paged_args* a, void* stream) {
   p.group = static_cast<int>(a->group);
   p.dim = static_cast<int>(a->head_dim);
   p.block_shift = a->block_size == 16 ? 4 : a->block_size == 32 ? 5 : 6;
-  p.table_blocks = a->table_blocks;
-  p.pool_pages = a->pool_pages;
-  p.window = a->window;
+  p.capacity = static_cast<int>(a->table_blocks * a->block_size);
+  p.pool_pages = static_cast<int>(a->pool_pages);
+  p.window = static_cast<int>(std::min<int64_t>(a->window, kMostPagedTokens));
   p.scale = static_cast<float>(a->scale);
-  p.status = static_cast<int*>(a->workspace);
-  const cudaError_t err = launch_paged(p, static_cast<cudaStream_t>(stream));
+  p.status = reinterpret_cast<int*>(ws);
+  p.counters = reinterpret_cast<int*>(ws + kCounterBytes);
+  p.warp_partials = reinterpret_cast<float*>(ws + layout.warp_partials);
+  p.cta_partials = reinterpret_cast<float*>(ws + layout.cta_partials);
+  p.group_partials = reinterpret_cast<float*>(ws + layout.group_partials);
+  const int64_t tiles = a->sequences * a->kv_heads * ((p.capacity + R - 1) / R);
+  const int ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms, tiles)));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t err = cudaErrorInvalidValue;
+  switch (D) {
+    case 64: err = launch_d<64>(maps, p, ctas, st); break;
+    case 128: err = launch_d<128>(maps, p, ctas, st); break;
+    case 192: err = launch_d<192>(maps, p, ctas, st); break;
+    case 256: err = launch_d<256>(maps, p, ctas, st); break;
+  }
   if (err != cudaSuccess) {
     set_last_error(std::string("paged attention launch: ") + cudaGetErrorString(err));
     return RKV_ERR_CUDA;
