@@ -296,7 +296,7 @@ struct RowsParams {
 cudaError_t launch_rows(const RowsParams& p, bool f32, bool vector, bool interleaved, bool append,
                         cudaStream_t stream);
 
-constexpr int64_t kMostSequences = 8192;      // the kernel's table of lengths in shared memory
+constexpr int64_t kMostSequences = 4096;      // the kernel's table of lengths in shared memory
 constexpr int64_t kMostPagedHeads = 4096;
 constexpr int64_t kMostPagedTokens = 1 << 30;  // of one sequence
 

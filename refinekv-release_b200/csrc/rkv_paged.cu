@@ -44,7 +44,9 @@ constexpr int paged_warps(int D) { return D <= 192 ? 8 : 6; }
 constexpr int stage_bytes(int D) { return 2 * tile_rows(D) * D * 2; }
 
 // A row's CTAs are joined in one level up to this many, else in groups.
-constexpr int kFlatJoin = 16;
+constexpr int kFlatJoin = 32;
+// A row shorter than this many tiles a CTA is not spread over more CTAs.
+constexpr unsigned kPartTiles = 32;
 
 // Workspace: status word, counters (at the same place for every geometry;
 // they are zero between calls), then the partials.
@@ -52,7 +54,11 @@ constexpr size_t kCounterBytes = 256;
 constexpr int kMostCtas = 512;
 constexpr size_t kHeader = 8192;
 
-// A partial: m[G8], l[G8], o[G8][D].
+// A warp's partial is o[G8][D + 4] (the pad spreads the fragments' rows over
+// the shared-memory banks), its m and l wait in shared memory; a CTA's is
+// m[G8], l[G8], o[G8][D].
+constexpr int kPad = 4;
+constexpr int warp_partial_floats(int D, int NT) { return NT * 8 * (D + kPad); }
 constexpr int partial_floats(int D, int NT) { return NT * 8 * (D + 2); }
 
 struct Cursor {
@@ -67,7 +73,9 @@ struct Paged {
   static constexpr int W = paged_warps(D);
   static constexpr int G8 = NT * 8;
   static constexpr int kTile = R * D * 2;
+  static constexpr int kThreads = W * 32;
   static constexpr int kPartial = partial_floats(D, NT);
+  static constexpr int kWarpPartial = warp_partial_floats(D, NT);
 };
 
 __device__ __forceinline__ int clamp_length(const PagedParams& p, int seq) {
@@ -96,19 +104,39 @@ __device__ __forceinline__ void enter_row(const PagedParams& p, const int* start
 
 // The cursor at global tile x.
 template <int R>
-__device__ __forceinline__ Cursor seek(const PagedParams& p, const int* start, long long x) {
+__device__ __forceinline__ Cursor seek(const PagedParams& p, const int* start, unsigned x) {
   int a = 0, b = p.sequences;  // start[a] * heads <= x < start[b] * heads
   while (b - a > 1) {
     const int mid = (a + b) >> 1;
-    if (static_cast<long long>(start[mid]) * p.heads <= x) a = mid; else b = mid;
+    if (static_cast<unsigned>(start[mid]) * p.heads <= x) a = mid; else b = mid;
   }
   Cursor c;
   c.seq = a;
   enter_row<R>(p, start, c);
-  const long long y = x - static_cast<long long>(start[a]) * p.heads;
+  const unsigned y = x - static_cast<unsigned>(start[a]) * p.heads;
   c.head = static_cast<int>(y / c.tiles);
-  c.tile = static_cast<int>(y - static_cast<long long>(c.head) * c.tiles);
+  c.tile = static_cast<int>(y - static_cast<unsigned>(c.head) * c.tiles);
   return c;
+}
+
+// `total` things in `parts` equal contiguous ranges: the k-th begins at
+// bound(k), and x lies in range owner(x).
+struct Ranges {
+  unsigned each, rest, parts;
+  __device__ Ranges(unsigned total, unsigned n) : each(total / n), rest(total % n), parts(n) {}
+  // rest < parts <= 512, so the product stays small.
+  __device__ unsigned bound(unsigned k) const { return each * k + rest * k / parts; }
+  __device__ unsigned owner(unsigned x) const {
+    unsigned k = min(parts - 1, x / max(1u, each));  // at or past the owner
+    while (bound(k) > x) --k;
+    return k;
+  }
+};
+
+__device__ __forceinline__ int arrive_add(int* counter) {
+  int seen;
+  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(seen) : "l"(counter) : "memory");
+  return seen;
 }
 
 // The next tile of the list (there must be one).
@@ -208,50 +236,119 @@ __device__ __forceinline__ void put(const PagedParams& p, int64_t at, float x) {
   else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(x);
 }
 
-// Joins `count` partials of one row (part(k) points at the k-th's m, l, o):
-// channels d, d + 1 of query g.  Remote: other CTAs wrote them.
-template <int D, int G8, bool Remote, typename Part>
-__device__ __forceinline__ void join(int count, Part part, int g, int d, float& m, float& l,
-                                     float2& o) {
-  constexpr int kBatch = 8;
-  m = -INFINITY;
-  l = 0.f;
-  o = make_float2(0.f, 0.f);
-  for (int k0 = 0; k0 < count; k0 += kBatch) {
-    float mk[kBatch], lk[kBatch];
-    float2 ok[kBatch];
+__device__ __forceinline__ void put4(const PagedParams& p, int64_t at, float4 x) {
+  if (p.query_f32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = x;
+  } else {
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + at) =
+        make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
+  }
+}
+
+__device__ __forceinline__ void fma4(float4& acc, float w, const float4& x) {
+  acc.x += w * x.x;
+  acc.y += w * x.y;
+  acc.z += w * x.z;
+  acc.w += w * x.w;
+}
+
+__device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
+
+// Four finished channels of query g of a row.
+__device__ __forceinline__ void put_joined(const PagedParams& p, int row, int g, int d, float m,
+                                           float l, float4 o) {
+  const int64_t at = static_cast<int64_t>(row) * p.group + g;
+  if (d < p.dim) put4(p, at * p.dim + d, make_float4(o.x / l, o.y / l, o.z / l, o.w / l));
+  if (d == 0 && p.lse != nullptr) p.lse[at] = finite_or_zero(m) + logf(l);
+}
+
+// Four channels of query g of a partial (m, l, o as partial_floats lays out).
+template <int D, int G8>
+__device__ __forceinline__ void put_partial(float* to, int g, int d, float m, float l, float4 o) {
+  *reinterpret_cast<float4*>(to + 2 * G8 + g * D + d) = o;
+  if (d == 0) {
+    to[g] = m;
+    to[G8 + g] = l;
+  }
+}
+
+// The whole CTA joins the `count` <= kFlatJoin partials part(0), part(1), ...
+// of one row, which other CTAs wrote, and writes the row, or the partial `to`
+// when that is given.  Every load of the join is in flight at once (up to
+// kBatch parts a thread): a warp per query turns the partials' m and l, a lane
+// each, into weights while their o arrive.  `scratch`: idle shared memory.
+template <int D, int NT, typename Part>
+__device__ __forceinline__ void join_remote(const PagedParams& p, int count, Part part, int row,
+                                            float* to, float* scratch) {
+  constexpr int G8 = NT * 8, kThreads = Paged<D, NT>::kThreads, kBatch = 16;
+  const int G = p.group, columns = G * (D / 4), tid = threadIdx.x;
+  float* sm_weight = scratch;                   // [kFlatJoin][G8]
+  float* sm_top = sm_weight + kFlatJoin * G8;   // [G8]
+  float* sm_sum = sm_top + G8;                  // [G8]
+  float4* sm_o = reinterpret_cast<float4*>(sm_sum + G8);  // [kThreads]
+  // Few columns: teams of threads share the parts of a column.
+  const int teams = max(1, kThreads / columns);
+  const int team = tid / columns, first_column = tid - team * columns;
+  const bool active = team < teams;
+  const auto load = [&](int k, int column) {
+    const int g = column / (D / 4), d = (column - g * (D / 4)) * 4;
+    return __ldcg(reinterpret_cast<const float4*>(part(k) + 2 * G8 + g * D + d));
+  };
+  float4 batch[kBatch];
+  const auto fetch = [&](int k0, int column) {
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      if (k0 + u < count) {
-        const float* at = part(k0 + u);
-        const float2* row = reinterpret_cast<const float2*>(at + 2 * G8 + g * D + d);
-        mk[u] = Remote ? __ldcg(at + g) : at[g];
-        lk[u] = Remote ? __ldcg(at + G8 + g) : at[G8 + g];
-        ok[u] = Remote ? __ldcg(row) : *row;
-      } else {
-        mk[u] = -INFINITY;
-        lk[u] = 0.f;
-        ok[u] = make_float2(0.f, 0.f);
-      }
+      const int k = k0 + u * teams;
+      if (k < count) batch[u] = load(k, column);
     }
+  };
+  if (active) fetch(team, first_column);
+  static_assert(kFlatJoin <= 32, "a lane per part");
+  const int lane = tid & 31;
+  for (int g = tid >> 5; g < G; g += kThreads / 32) {
+    const float m = lane < count ? __ldcg(part(lane) + g) : -INFINITY;
+    const float l = lane < count ? __ldcg(part(lane) + G8 + g) : 0.f;
     float top = m;
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) top = fmaxf(top, mk[u]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    const float keep = __expf(m - ref);
-    l *= keep;
-    o.x *= keep;
-    o.y *= keep;
+    for (int step = 16; step > 0; step >>= 1) {
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
+    }
+    const float w = __expf(m - finite_or_zero(top));
+    float sum = lane < count ? w * l : 0.f;
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      if (k0 + u < count) {
-        const float w = __expf(mk[u] - ref);
-        l += w * lk[u];
-        o.x += w * ok[u].x;
-        o.y += w * ok[u].y;
+    for (int step = 16; step > 0; step >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, step);
+    sm_weight[lane * G8 + g] = w;
+    if (lane == 0) {
+      sm_top[g] = top;
+      sm_sum[g] = sum;
+    }
+  }
+  __syncthreads();
+  // Threads left over by one whole team have no column.
+  for (int column = active || teams > 1 ? first_column : columns; column < columns;
+       column += kThreads) {
+    const int g = column / (D / 4), d = (column - g * (D / 4)) * 4;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (active) {
+      for (int k0 = team; k0 < count; k0 += kBatch * teams) {
+        if (k0 != team || column != first_column) fetch(k0, column);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int k = k0 + u * teams;
+          if (k < count) fma4(acc, sm_weight[k * G8 + g], batch[u]);
+        }
       }
     }
-    m = top;
+    if (teams > 1) {  // then every thread has at most one column
+      sm_o[tid] = acc;
+      __syncthreads();
+      if (team != 0) break;
+      for (int other = 1; other < teams; ++other) {
+        fma4(acc, 1.f, sm_o[other * columns + column]);
+      }
+    }
+    if (to == nullptr) put_joined(p, row, g, d, sm_top[g], sm_sum[g], acc);
+    else put_partial<D, G8>(to, g, d, sm_top[g], sm_sum[g], acc);
   }
 }
 
@@ -259,13 +356,21 @@ template <int D, int NT>
 __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
     paged_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant__ PagedParams p) {
   using K = Paged<D, NT>;
-  constexpr int R = K::R, W = K::W, G8 = K::G8, kTile = K::kTile, kPartial = K::kPartial;
+  constexpr int R = K::R, W = K::W, G8 = K::G8, kTile = K::kTile;
+  constexpr int kThreads = K::kThreads, kPartial = K::kPartial, kWarpPartial = K::kWarpPartial;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = align_smem(smem_raw);  // [warp][K | V]
   __shared__ __align__(8) uint64_t bars[W][2];
   __shared__ int warp_sum[W];
-  __shared__ int seg_row[2 * W];  // the row of each of the CTA's partials, or -1
+  // The CTA's partials, two per warp, in token order: the row (or -1), each
+  // query's m and l, then its weight within the CTA and the CTA's m and l of
+  // the row (kept at the row's first partial).
+  __shared__ int seg_row[2 * W], seg_slot[2 * W];
+  __shared__ float seg_m[2 * W][G8], seg_l[2 * W][G8];
+  __shared__ float seg_weight[2 * W][G8], row_m[2 * W][G8], row_l[2 * W][G8];
+  __shared__ int cut[2];  // the rows in the CTA's two slots, or -1
   __shared__ int last_arrival;
+  __shared__ int busy;  // sequences that are not empty
   int* start = reinterpret_cast<int*>(ring + W * 2 * kTile);  // tiles before each sequence
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (lane == 0) {
@@ -275,6 +380,8 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
     seg_row[2 * warp] = seg_row[2 * warp + 1] = -1;
   }
   if (threadIdx.x == 0) {
+    busy = 0;
+    cut[0] = cut[1] = -1;
     tma_prefetch_desc(&maps.keys);
     tma_prefetch_desc(&maps.values);
   }
@@ -286,12 +393,14 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
     const int per = (p.sequences + W * 32 - 1) / (W * 32);
     const int s0 = min(p.sequences, static_cast<int>(threadIdx.x) * per);
     const int s1 = min(p.sequences, s0 + per);
-    int sum = 0;
+    int sum = 0, some = 0;
     for (int s = s0; s < s1; ++s) {
       if (blockIdx.x == 0 && (p.lengths[s] < 0 || p.lengths[s] > p.capacity)) {
         atomicOr(p.status, kStatusBadInput);
       }
-      sum += tiles_of<R>(p, s);
+      const int tiles = tiles_of<R>(p, s);
+      sum += tiles;
+      some += tiles > 0;
     }
     int scan = sum;
 #pragma unroll
@@ -303,6 +412,8 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
     __syncthreads();
     int before = scan - sum;
     for (int w = 0; w < warp; ++w) before += warp_sum[w];
+    some = __reduce_add_sync(0xffffffffu, some);
+    if (lane == 0 && some > 0) atomicAdd(&busy, some);
     for (int s = s0; s < s1; ++s) {
       start[s] = before;
       before += tiles_of<R>(p, s);
@@ -310,7 +421,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
     if (s1 == p.sequences && s0 < s1) start[p.sequences] = before;
     __syncthreads();
   }
-  const long long T = static_cast<long long>(start[p.sequences]) * p.heads;
+  const unsigned T = static_cast<unsigned>(start[p.sequences]) * p.heads;
   // Idle slots: zero rows.
   for (int s = blockIdx.x; s < p.sequences; s += gridDim.x) {
     if (start[s + 1] != start[s]) continue;
@@ -321,16 +432,34 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
       for (int i = threadIdx.x; i < queries; i += blockDim.x) p.lse[row + i] = -INFINITY;
     }
   }
-  const long long C = min(static_cast<long long>(gridDim.x), (T + W - 1) / W);
-  const long long cta = blockIdx.x;
+  // How many CTAs share the tiles.  Few rows: whole CTAs per row where that
+  // leaves few SMs idle, since a CTA of one row has one join less; no more of
+  // them than the rows' lengths are worth.  Many rows: every SM, but a tile a
+  // warp at least.
+  const unsigned rows = static_cast<unsigned>(busy) * p.heads, grid = gridDim.x;
+  unsigned C = min(grid, (T + W - 1) / W);
+  if (rows > 0 && rows <= grid) {
+    const unsigned fit = grid / rows, worth = (T / rows + kPartTiles - 1) / kPartTiles;
+    if (worth < fit) C = rows * max(1u, worth);
+    else if (fit * rows * 16 >= grid * 15) C = fit * rows;
+    C = min(C, T);
+  }
+  const unsigned cta = blockIdx.x;
   if (cta >= C) return;
-  const long long lo = T * cta / C, hi = T * (cta + 1) / C;
-  const long long wlo = lo + (hi - lo) * warp / W, whi = lo + (hi - lo) * (warp + 1) / W;
+  const Ranges ranges(T, C);
+  const unsigned lo = ranges.bound(cta), hi = ranges.bound(cta + 1);
+  const Ranges shares(hi - lo, W);
+  const unsigned wlo = lo + shares.bound(warp), whi = lo + shares.bound(warp + 1);
 
   uint8_t* stage = ring + warp * 2 * kTile;
   const uint32_t k_tile = smem_addr(stage), v_tile = k_tile + kTile;
-  float* warp_partial = p.warp_partials + (cta * W + warp) * kPartial;
-  float* stash = reinterpret_cast<float*>(stage);
+  // Where partial i of the CTA keeps its o: a warp's last row waits in the
+  // warp's own idle stage, an earlier one (cut by the range's start) in the
+  // workspace.
+  const auto segment = [&](int i) {
+    return i & 1 ? reinterpret_cast<float*>(ring + (i >> 1) * 2 * kTile)
+                 : p.warp_partials + (static_cast<size_t>(cta) * W + (i >> 1)) * kWarpPartial;
+  };
   const uint64_t policy = l2_evict_first_policy();
   const int page_rows = 1 << p.block_shift;
   const int box_rows = min(R, page_rows), boxes = R / box_rows;
@@ -471,11 +600,25 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
               }
             }
         } else {
-          // The range's last row waits in the warp's own idle stage, an
-          // earlier one (which began before the range) in the workspace.
-          float* to = more ? warp_partial : stash;
-          if (lane == 0) seg_row[2 * warp + (more ? 0 : 1)] = row;
-          stash_warp_partial<D, NT>(to, to + G8, to + 2 * G8, 0, lane, m, l, o);
+          const int i = 2 * warp + (more ? 0 : 1);
+          float* to = segment(i);
+          if (lane == 0) seg_row[i] = row;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int g = nt * 8 + 2 * (lane & 3) + c;
+              if (g >= p.group) continue;
+              if (lane < 4) {
+                seg_m[i][g] = m[nt][c];
+                seg_l[i][g] = l[nt][c];
+              }
+#pragma unroll
+              for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+                  to[g * (D + kPad) + dt * 16 + half * 8 + (lane >> 2)] = o[dt][nt][2 * half + c];
+            }
         }
         seg_first = 0;
         fresh = true;
@@ -491,56 +634,70 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   }
   __syncthreads();
 
-  // Join the CTA's partials row by row (they lie in token order).  A row that
-  // began and ended within the CTA is written; one that began before it goes
-  // to the CTA's slot 0, one that only goes on after it to slot 1.
-  auto segment = [&](int i) -> const float* {
-    const int w = i >> 1;
-    return i & 1 ? reinterpret_cast<const float*>(ring + w * 2 * kTile)
-                 : p.warp_partials + (cta * W + w) * kPartial;
-  };
-  constexpr int kChunks = D / 64;  // 64 channels, two per lane
-  int cut[2] = {-1, -1};  // the rows in slots 0 and 1
-  int turn = 0;
-  for (int i = 0; i < 2 * W;) {
-    const int row = seg_row[i];
-    if (row < 0) {
-      ++i;
-      continue;
-    }
-    int list[2 * W], count = 0;  // compile-time bound; indices in local order
-    for (; i < 2 * W && (seg_row[i] == row || seg_row[i] < 0); ++i) {
-      if (seg_row[i] == row) list[count++] = i;
-    }
-    const int seq = row / p.heads, head = row - seq * p.heads;
-    const int tiles = start[seq + 1] - start[seq];
-    const long long begin = static_cast<long long>(start[seq]) * p.heads +
-                            static_cast<long long>(head) * tiles;
-    const bool before = begin < lo, after = begin + tiles > hi;
-    const int slot = before ? 0 : 1;
-    if (before || after) cut[slot] = row;
-    float* to = p.cta_partials + (cta * 2 + slot) * kPartial;
-    for (int c = 0; c < p.group * kChunks; ++c, ++turn) {
-      if (turn % W != warp) continue;
-      const int g = c / kChunks, d = (c - g * kChunks) * 64 + 2 * lane;
-      float m, l;
-      float2 o;
-      join<D, G8, false>(count, [&](int k) { return segment(list[k]); }, g, d, m, l, o);
-      if (before || after) {
-        *reinterpret_cast<float2*>(to + 2 * G8 + g * D + d) = o;
-        if (d == 0) {
-          to[g] = m;
-          to[G8 + g] = l;
+  // Join the CTA's partials.  A row that began and ended within the CTA is
+  // written; one that began before it goes to the CTA's slot 0, one that only
+  // goes on after it to slot 1.
+  {
+    const int mine = lane < 2 * W ? seg_row[lane] : -1;
+    const unsigned used = __ballot_sync(0xffffffffu, mine >= 0);
+    const unsigned below = used & ((1u << lane) - 1);
+    const int previous = __shfl_sync(0xffffffffu, mine, below ? 31 - __clz(below) : 0);
+    // The first partial of each row.
+    const unsigned heads =
+        __ballot_sync(0xffffffffu, mine >= 0 && (below == 0 || previous != mine));
+    // Partials of the row whose first one is i.
+    const auto members = [&](int i) {
+      const unsigned later = heads & ~((2u << i) - 1);
+      return used & ~((1u << i) - 1) & (later ? (later & -later) - 1 : 0xffffffffu);
+    };
+    const int i = threadIdx.x / G8, g = threadIdx.x % G8;  // 2 W G8 threads at most
+    if (i < 2 * W && (used >> i & 1) && g < p.group) {
+      const int head = 31 - __clz(heads & ((2u << i) - 1));
+      float top = -INFINITY;
+      for (unsigned set = members(head); set; set &= set - 1) {
+        top = fmaxf(top, seg_m[__ffs(set) - 1][g]);
+      }
+      const float ref = finite_or_zero(top);
+      seg_weight[i][g] = __expf(seg_m[i][g] - ref);
+      if (i == head) {
+        float sum = 0.f;
+        for (unsigned set = members(head); set; set &= set - 1) {
+          const int j = __ffs(set) - 1;
+          sum += __expf(seg_m[j][g] - ref) * seg_l[j][g];
         }
+        row_m[i][g] = top;
+        row_l[i][g] = sum;
+        if (g == 0) {
+          const int row = seg_row[i], seq = row / p.heads;
+          const unsigned tiles = start[seq + 1] - start[seq];
+          const unsigned begin =
+              static_cast<unsigned>(start[seq]) * p.heads + (row - seq * p.heads) * tiles;
+          const int slot = begin < lo ? 0 : begin + tiles > hi ? 1 : -1;
+          seg_slot[i] = slot;
+          if (slot >= 0) cut[slot] = row;
+        }
+      }
+    }
+    __syncthreads();
+    const int columns = p.group * (D / 4), total = __popc(heads) * columns;
+    for (int x = threadIdx.x; x < total; x += kThreads) {
+      const int k = x / columns, column = x - k * columns;
+      unsigned set = heads;
+      for (int skip = 0; skip < k; ++skip) set &= set - 1;
+      const int head = __ffs(set) - 1;
+      const int q = column / (D / 4), d = (column - q * (D / 4)) * 4;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (set = members(head); set; set &= set - 1) {
+        const int j = __ffs(set) - 1;
+        fma4(acc, seg_weight[j][q],
+             *reinterpret_cast<const float4*>(segment(j) + q * (D + kPad) + d));
+      }
+      const int slot = seg_slot[head];
+      if (slot < 0) {
+        put_joined(p, seg_row[head], q, d, row_m[head][q], row_l[head][q], acc);
       } else {
-        const int64_t out_row = static_cast<int64_t>(row) * p.group + g;
-        if (d < p.dim) {
-          put(p, out_row * p.dim + d, o.x / l);
-          put(p, out_row * p.dim + d + 1, o.y / l);
-        }
-        if (d == 0 && p.lse != nullptr) {
-          p.lse[out_row] = (m == -INFINITY ? 0.f : m) + logf(l);
-        }
+        put_partial<D, G8>(p.cta_partials + (static_cast<size_t>(cta) * 2 + slot) * kPartial, q, d,
+                           row_m[head][q], row_l[head][q], acc);
       }
     }
   }
@@ -553,11 +710,8 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
     if (row < 0) continue;
     const int seq = row / p.heads, head = row - seq * p.heads;
     const int tiles = start[seq + 1] - start[seq];
-    const long long begin = static_cast<long long>(start[seq]) * p.heads +
-                            static_cast<long long>(head) * tiles;
-    // The CTA that holds tile x.
-    const auto owner = [&](long long x) { return static_cast<int>(((x + 1) * C + T - 1) / T - 1); };
-    const int c1 = owner(begin), parts = owner(begin + tiles - 1) - c1 + 1;
+    const unsigned begin = static_cast<unsigned>(start[seq]) * p.heads + head * tiles;
+    const int c1 = ranges.owner(begin), parts = ranges.owner(begin + tiles - 1) - c1 + 1;
     int fan = parts;
     if (parts > kFlatJoin) {
       fan = 1;
@@ -577,48 +731,21 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
     const auto arrive = [&](int* counter, int expected) {
       __syncthreads();
       if (threadIdx.x == 0) {
-        __threadfence();
-        const int seen = atomicAdd(counter, 1);
-        last_arrival = seen == expected - 1;
+        last_arrival = arrive_add(counter) == expected - 1;
         if (last_arrival) *counter = 0;
-        __threadfence();
       }
       __syncthreads();
       return last_arrival != 0;
     };
     const int members = min(fan, parts - mine * fan);
     if (!arrive(p.counters + first * 3 + (first == c1 ? 1 : 0), members)) continue;
-    const auto combine = [&](int count, auto part, bool final) {
-      for (int c = warp; c < p.group * kChunks; c += W) {
-        const int g = c / kChunks, d = (c - g * kChunks) * 64 + 2 * lane;
-        float m, l;
-        float2 o;
-        join<D, G8, true>(count, part, g, d, m, l, o);
-        if (final) {
-          const int64_t out_row = static_cast<int64_t>(row) * p.group + g;
-          if (d < p.dim) {
-            put(p, out_row * p.dim + d, o.x / l);
-            put(p, out_row * p.dim + d + 1, o.y / l);
-          }
-          if (d == 0 && p.lse != nullptr) {
-            p.lse[out_row] = (m == -INFINITY ? 0.f : m) + logf(l);
-          }
-        } else {
-          float* to = group_slot(first);
-          *reinterpret_cast<float2*>(to + 2 * G8 + g * D + d) = o;
-          if (d == 0) {
-            to[g] = m;
-            to[G8 + g] = l;
-          }
-        }
-      }
-    };
-    combine(members, [&](int k) { return static_cast<const float*>(slot_of(first + k)); },
-            groups == 1);
+    float* scratch = reinterpret_cast<float*>(ring);
+    join_remote<D, NT>(p, members, [&](int k) { return slot_of(first + k); }, row,
+                       groups == 1 ? nullptr : group_slot(first), scratch);
     if (groups == 1) continue;
     if (!arrive(p.counters + c1 * 3 + 2, groups)) continue;
-    combine(groups,
-            [&](int k) { return static_cast<const float*>(group_slot(c1 + k * fan)); }, true);
+    join_remote<D, NT>(p, groups, [&](int k) { return group_slot(c1 + k * fan); }, row, nullptr,
+                       scratch);
   }
 }
 
@@ -665,7 +792,7 @@ struct Layout {
     const size_t one = static_cast<size_t>(partial_floats(D, NT)) * 4;
     size_t off = kHeader;
     warp_partials = off;
-    off += one * sms * paged_warps(D);
+    off += static_cast<size_t>(warp_partial_floats(D, NT)) * 4 * sms * paged_warps(D);
     cta_partials = off;
     off += one * sms * 2;
     group_partials = off;
@@ -705,7 +832,7 @@ int rkv_paged_attention(const rkv_paged_args* a, void* stream) {
   }
   if (a->sequences < 0 || a->sequences > kMostSequences || a->kv_heads < 1 ||
       a->kv_heads > kMostPagedHeads) {
-    return reject(RKV_ERR_UNSUPPORTED, "at most 8192 sequences and 4096 KV heads");
+    return reject(RKV_ERR_UNSUPPORTED, "at most 4096 sequences and 4096 KV heads");
   }
   if (a->query_dtype != RKV_DTYPE_BF16 && a->query_dtype != RKV_DTYPE_F32) {
     return reject(RKV_ERR_INVALID_ARGUMENT, "query dtype must be bf16 or fp32");
@@ -715,8 +842,10 @@ int rkv_paged_attention(const rkv_paged_args* a, void* stream) {
       a->pool_pages < 0 || a->pool_pages > (1LL << 31) - 1) {
     return reject(RKV_ERR_INVALID_ARGUMENT, "window, page table or pool sizes are out of range");
   }
-  if (a->sequences * a->table_blocks * (a->block_size / 16) > (1LL << 31) - 1) {
-    return reject(RKV_ERR_UNSUPPORTED, "the page table covers more tokens than are counted");
+  const int D = padded(a->head_dim), R = tile_rows(D);
+  const int64_t tiles = a->sequences * a->kv_heads * ((a->table_blocks * a->block_size + R - 1) / R);
+  if (tiles > (1LL << 31) - 1) {  // a product below 2^13 * 2^12 * 2^25
+    return reject(RKV_ERR_UNSUPPORTED, "the page table covers more rows than are counted");
   }
   if (a->sequences == 0) return RKV_OK;
   if (!a->query || !a->output || !a->lengths || !a->key_pool || !a->value_pool ||
@@ -739,7 +868,6 @@ int rkv_paged_attention(const rkv_paged_args* a, void* stream) {
   }
   int rc = RKV_OK, sms = 0;
   PagedMaps maps;
-  const int D = padded(a->head_dim), R = tile_rows(D);
   const int box_rows = static_cast<int>(std::min<int64_t>(R, a->block_size));
   const int64_t *ks = a->key_pool_strides, *vs = a->value_pool_strides;
   if ((rc = pool_map(&maps.keys, a->key_pool, a->head_dim, a->block_size, box_rows, a->kv_heads,
@@ -780,7 +908,6 @@ int rkv_paged_attention(const rkv_paged_args* a, void* stream) {
   p.warp_partials = reinterpret_cast<float*>(ws + layout.warp_partials);
   p.cta_partials = reinterpret_cast<float*>(ws + layout.cta_partials);
   p.group_partials = reinterpret_cast<float*>(ws + layout.group_partials);
-  const int64_t tiles = a->sequences * a->kv_heads * ((p.capacity + R - 1) / R);
   const int ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms, tiles)));
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t err = cudaErrorInvalidValue;
