@@ -319,7 +319,7 @@ struct PagedParams {
   int window;  // 0: none
   float scale;
   int* status;
-  int* counters;          // three per CTA, zero between calls
+  int* counters;          // zero between calls
   float* warp_partials;   // one per warp
   float* cta_partials;    // two per CTA
   float* group_partials;  // two per CTA

@@ -51,7 +51,7 @@ constexpr unsigned kPartTiles = 32;
 // Workspace: status word, counters (at the same place for every geometry;
 // they are zero between calls), then the partials.
 constexpr size_t kCounterBytes = 256;
-constexpr int kMostCtas = 512;
+constexpr int kMostCtas = 512;  // two counters per CTA and one per row that begins in it
 constexpr size_t kHeader = 8192;
 
 // A warp's partial is o[G8][D + 4] (the pad spreads the fragments' rows over
@@ -132,6 +132,28 @@ struct Ranges {
     return k;
   }
 };
+
+// A row cut by the CTA's range: slot 0 began before it, slot 1 within it.  Its
+// parts are the partials of CTAs first_cta, first_cta + 1, ..., joined `fan`
+// at a time.
+struct Cut {
+  int row;  // -1: none
+  int first_cta, parts, fan;
+};
+
+__device__ __forceinline__ Cut cut_row(const Ranges& ranges, int row, unsigned begin,
+                                       unsigned tiles) {
+  Cut c;
+  c.row = row;
+  c.first_cta = ranges.owner(begin);
+  c.parts = ranges.owner(begin + tiles - 1) - c.first_cta + 1;
+  c.fan = c.parts;
+  if (c.parts > kFlatJoin) {
+    c.fan = 1;
+    while (c.fan * c.fan < c.parts) ++c.fan;
+  }
+  return c;
+}
 
 __device__ __forceinline__ int arrive_add(int* counter) {
   int seen;
@@ -365,11 +387,11 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   // The CTA's partials, two per warp, in token order: the row (or -1), each
   // query's m and l, then its weight within the CTA and the CTA's m and l of
   // the row (kept at the row's first partial).
-  __shared__ int seg_row[2 * W], seg_slot[2 * W];
+  __shared__ int seg_row[2 * W];
   __shared__ float seg_m[2 * W][G8], seg_l[2 * W][G8];
   __shared__ float seg_weight[2 * W][G8], row_m[2 * W][G8], row_l[2 * W][G8];
-  __shared__ int cut[2];  // the rows in the CTA's two slots, or -1
-  __shared__ int last_arrival;
+  __shared__ Cut cuts[2];
+  __shared__ int last_arrival[2];
   __shared__ int busy;  // sequences that are not empty
   int* start = reinterpret_cast<int*>(ring + W * 2 * kTile);  // tiles before each sequence
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -381,7 +403,6 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   }
   if (threadIdx.x == 0) {
     busy = 0;
-    cut[0] = cut[1] = -1;
     tma_prefetch_desc(&maps.keys);
     tma_prefetch_desc(&maps.values);
   }
@@ -493,6 +514,19 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
     }
   };
 
+  // The rows that the range's two ends cut: known from the start, so worked out
+  // while the first tiles are on their way.
+  const auto find_cuts = [&] {
+    if (warp >= 2) return;
+    const Cursor c = seek<R>(p, start, warp == 0 ? lo : hi - 1);
+    const unsigned begin = (warp == 0 ? lo : hi - 1) - c.tile;
+    const bool cut = warp == 0 ? begin < lo : begin >= lo && begin + c.tiles > hi;
+    Cut found;
+    found.row = -1;
+    if (cut) found = cut_row(ranges, c.seq * p.heads + c.head, begin, c.tiles);
+    if (lane == 0) cuts[warp] = found;
+  };
+  if (wlo >= whi) find_cuts();
   if (wlo < whi) {
     uint32_t qb[D / 16][NT][2];
     float m[NT][2], l[NT][2], o[D / 16][NT][4];
@@ -500,6 +534,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
     int page = page_of(cur);
     issue(0, cur, page);
     issue(1, cur, page);
+    find_cuts();
     const int count = static_cast<int>(whi - wlo);
     int seg_first = cur.tile;  // the segment's first tile of its row
     bool fresh = true, aborted = false;
@@ -667,15 +702,6 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
         }
         row_m[i][g] = top;
         row_l[i][g] = sum;
-        if (g == 0) {
-          const int row = seg_row[i], seq = row / p.heads;
-          const unsigned tiles = start[seq + 1] - start[seq];
-          const unsigned begin =
-              static_cast<unsigned>(start[seq]) * p.heads + (row - seq * p.heads) * tiles;
-          const int slot = begin < lo ? 0 : begin + tiles > hi ? 1 : -1;
-          seg_slot[i] = slot;
-          if (slot >= 0) cut[slot] = row;
-        }
       }
     }
     __syncthreads();
@@ -687,14 +713,18 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
       const int head = __ffs(set) - 1;
       const int q = column / (D / 4), d = (column - q * (D / 4)) * 4;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (set = members(head); set; set &= set - 1) {
-        const int j = __ffs(set) - 1;
-        fma4(acc, seg_weight[j][q],
-             *reinterpret_cast<const float4*>(segment(j) + q * (D + kPad) + d));
+      set = members(head);
+#pragma unroll
+      for (int j = 0; j < 2 * W; ++j) {
+        if (set >> j & 1) {
+          fma4(acc, seg_weight[j][q],
+               *reinterpret_cast<const float4*>(segment(j) + q * (D + kPad) + d));
+        }
       }
-      const int slot = seg_slot[head];
+      const int row = seg_row[head];
+      const int slot = row == cuts[0].row ? 0 : row == cuts[1].row ? 1 : -1;
       if (slot < 0) {
-        put_joined(p, seg_row[head], q, d, row_m[head][q], row_l[head][q], acc);
+        put_joined(p, row, q, d, row_m[head][q], row_l[head][q], acc);
       } else {
         put_partial<D, G8>(p.cta_partials + (static_cast<size_t>(cta) * 2 + slot) * kPartial, q, d,
                            row_m[head][q], row_l[head][q], acc);
@@ -705,47 +735,50 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   // Rows cut by CTA ranges: the last of a row's CTAs to arrive joins them; a
   // row over many CTAs is joined in groups first, so that no CTA reads more
   // than a few partials.
+  // Partials of a row's CTA c, and of the group that begins at it, with the
+  // counter of the group: a CTA can end one row (slot 0) and begin another.
+  const auto at_cta = [&](const Cut& cut, int c) { return 2 * c + (c == cut.first_cta ? 1 : 0); };
+  const auto part_of = [&](const Cut& cut, int c) {
+    return p.cta_partials + static_cast<int64_t>(at_cta(cut, c)) * kPartial;
+  };
+  const auto group_of = [&](const Cut& cut, int c) {
+    return p.group_partials + static_cast<int64_t>(at_cta(cut, c)) * kPartial;
+  };
+  // Whether this arrival is the last of `expected`; the counter is then zero again.
+  const auto arrive = [](int* counter, int expected) {
+    const bool last = arrive_add(counter) == expected - 1;
+    if (last) *counter = 0;
+    return last;
+  };
+  const auto group_first = [&](const Cut& cut) {
+    return cut.first_cta + (static_cast<int>(cta) - cut.first_cta) / cut.fan * cut.fan;
+  };
+  const auto group_members = [&](const Cut& cut) {
+    return min(cut.fan, cut.first_cta + cut.parts - group_first(cut));
+  };
+  __syncthreads();
+  if (lane == 0 && warp < 2 && cuts[warp].row >= 0) {  // both slots at once
+    const Cut cut = cuts[warp];
+    last_arrival[warp] = arrive(p.counters + at_cta(cut, group_first(cut)), group_members(cut));
+  }
+  __syncthreads();
+  float* scratch = reinterpret_cast<float*>(ring);
   for (int slot = 0; slot < 2; ++slot) {
-    const int row = cut[slot];
-    if (row < 0) continue;
-    const int seq = row / p.heads, head = row - seq * p.heads;
-    const int tiles = start[seq + 1] - start[seq];
-    const unsigned begin = static_cast<unsigned>(start[seq]) * p.heads + head * tiles;
-    const int c1 = ranges.owner(begin), parts = ranges.owner(begin + tiles - 1) - c1 + 1;
-    int fan = parts;
-    if (parts > kFlatJoin) {
-      fan = 1;
-      while (fan * fan < parts) ++fan;
-    }
-    const int groups = (parts + fan - 1) / fan;
-    const int mine = (static_cast<int>(cta) - c1) / fan;
-    const int first = c1 + mine * fan;
-    // Partials of the row's CTA c, and of the group that begins at it.  A CTA
-    // can end one row (slot 0) and begin another (slot 1).
-    const auto slot_of = [&](int c) {
-      return p.cta_partials + (static_cast<int64_t>(c) * 2 + (c == c1 ? 1 : 0)) * kPartial;
-    };
-    const auto group_slot = [&](int c) {
-      return p.group_partials + (static_cast<int64_t>(c) * 2 + (c == c1 ? 1 : 0)) * kPartial;
-    };
-    const auto arrive = [&](int* counter, int expected) {
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        last_arrival = arrive_add(counter) == expected - 1;
-        if (last_arrival) *counter = 0;
-      }
-      __syncthreads();
-      return last_arrival != 0;
-    };
-    const int members = min(fan, parts - mine * fan);
-    if (!arrive(p.counters + first * 3 + (first == c1 ? 1 : 0), members)) continue;
-    float* scratch = reinterpret_cast<float*>(ring);
-    join_remote<D, NT>(p, members, [&](int k) { return slot_of(first + k); }, row,
-                       groups == 1 ? nullptr : group_slot(first), scratch);
+    const Cut cut = cuts[slot];
+    if (cut.row < 0 || !last_arrival[slot]) continue;
+    const int first = group_first(cut), groups = (cut.parts + cut.fan - 1) / cut.fan;
+    join_remote<D, NT>(p, group_members(cut), [&](int k) { return part_of(cut, first + k); },
+                       cut.row, groups == 1 ? nullptr : group_of(cut, first), scratch);
+    __syncthreads();  // the scratch is used again
     if (groups == 1) continue;
-    if (!arrive(p.counters + c1 * 3 + 2, groups)) continue;
-    join_remote<D, NT>(p, groups, [&](int k) { return group_slot(c1 + k * fan); }, row, nullptr,
-                       scratch);
+    if (threadIdx.x == 0) {
+      last_arrival[slot] = arrive(p.counters + 2 * kMostCtas + cut.first_cta, groups);
+    }
+    __syncthreads();
+    if (!last_arrival[slot]) continue;
+    join_remote<D, NT>(p, groups, [&](int k) { return group_of(cut, cut.first_cta + k * cut.fan); },
+                       cut.row, nullptr, scratch);
+    __syncthreads();
   }
 }
 
