@@ -320,7 +320,7 @@ struct PagedParams {
   float scale;
   int* status;
   int* counters;          // zero between calls
-  float* warp_partials;   // one per warp
+  float* warp_partials;   // one per warp, for wide heads
   float* cta_partials;    // two per CTA
   float* group_partials;  // two per CTA
 };

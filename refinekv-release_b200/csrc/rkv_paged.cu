@@ -57,9 +57,21 @@ constexpr size_t kHeader = 8192;
 // A warp's partial is o[G8][D + 4] (the pad spreads the fragments' rows over
 // the shared-memory banks), its m and l wait in shared memory; a CTA's is
 // m[G8], l[G8], o[G8][D].
+// A warp's first partial, left while its stage is in use, has its own place in
+// shared memory where that fits, else in the workspace.
 constexpr int kPad = 4;
+constexpr bool first_in_smem(int D) { return D <= 128; }
 constexpr int warp_partial_floats(int D, int NT) { return NT * 8 * (D + kPad); }
 constexpr int partial_floats(int D, int NT) { return NT * 8 * (D + 2); }
+// Dynamic shared memory: the stages, the warps' first partials, then the
+// table of the sequences' first tiles.
+constexpr size_t table_offset(int D, int NT) {
+  return static_cast<size_t>(paged_warps(D)) *
+         (stage_bytes(D) + (first_in_smem(D) ? warp_partial_floats(D, NT) * 4 : 0));
+}
+constexpr size_t paged_smem(int D, int NT, int64_t sequences) {
+  return kSmemSlack + table_offset(D, NT) + static_cast<size_t>(sequences + 1) * 4;
+}
 
 struct Cursor {
   int seq, head, tile, tiles;  // tile of `tiles` of the row
@@ -276,101 +288,28 @@ __device__ __forceinline__ void fma4(float4& acc, float w, const float4& x) {
 
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
 
-// Four finished channels of query g of a row.
-__device__ __forceinline__ void put_joined(const PagedParams& p, int row, int g, int d, float m,
-                                           float l, float4 o) {
-  const int64_t at = static_cast<int64_t>(row) * p.group + g;
-  if (d < p.dim) put4(p, at * p.dim + d, make_float4(o.x / l, o.y / l, o.z / l, o.w / l));
-  if (d == 0 && p.lse != nullptr) p.lse[at] = finite_or_zero(m) + logf(l);
+// Four joined channels of query g of a row: finished, or into the partial `to`.
+template <int D, int G8>
+__device__ __forceinline__ void put_joined(const PagedParams& p, int row, int g, int d, float* to,
+                                           float inverse, const float4& o) {
+  if (to != nullptr) {
+    *reinterpret_cast<float4*>(to + 2 * G8 + g * D + d) = o;
+  } else if (d < p.dim) {
+    const int64_t at = static_cast<int64_t>(row) * p.group + g;
+    put4(p, at * p.dim + d,
+         make_float4(o.x * inverse, o.y * inverse, o.z * inverse, o.w * inverse));
+  }
 }
 
-// Four channels of query g of a partial (m, l, o as partial_floats lays out).
-template <int D, int G8>
-__device__ __forceinline__ void put_partial(float* to, int g, int d, float m, float l, float4 o) {
-  *reinterpret_cast<float4*>(to + 2 * G8 + g * D + d) = o;
-  if (d == 0) {
+// The m and l of query g of a joined row: into the partial, or the row's lse.
+template <int G8>
+__device__ __forceinline__ void put_sums(const PagedParams& p, int row, int g, float* to, float m,
+                                         float l) {
+  if (to != nullptr) {
     to[g] = m;
     to[G8 + g] = l;
-  }
-}
-
-// The whole CTA joins the `count` <= kFlatJoin partials part(0), part(1), ...
-// of one row, which other CTAs wrote, and writes the row, or the partial `to`
-// when that is given.  Every load of the join is in flight at once (up to
-// kBatch parts a thread): a warp per query turns the partials' m and l, a lane
-// each, into weights while their o arrive.  `scratch`: idle shared memory.
-template <int D, int NT, typename Part>
-__device__ __forceinline__ void join_remote(const PagedParams& p, int count, Part part, int row,
-                                            float* to, float* scratch) {
-  constexpr int G8 = NT * 8, kThreads = Paged<D, NT>::kThreads, kBatch = 16;
-  const int G = p.group, columns = G * (D / 4), tid = threadIdx.x;
-  float* sm_weight = scratch;                   // [kFlatJoin][G8]
-  float* sm_top = sm_weight + kFlatJoin * G8;   // [G8]
-  float* sm_sum = sm_top + G8;                  // [G8]
-  float4* sm_o = reinterpret_cast<float4*>(sm_sum + G8);  // [kThreads]
-  // Few columns: teams of threads share the parts of a column.
-  const int teams = max(1, kThreads / columns);
-  const int team = tid / columns, first_column = tid - team * columns;
-  const bool active = team < teams;
-  const auto load = [&](int k, int column) {
-    const int g = column / (D / 4), d = (column - g * (D / 4)) * 4;
-    return __ldcg(reinterpret_cast<const float4*>(part(k) + 2 * G8 + g * D + d));
-  };
-  float4 batch[kBatch];
-  const auto fetch = [&](int k0, int column) {
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int k = k0 + u * teams;
-      if (k < count) batch[u] = load(k, column);
-    }
-  };
-  if (active) fetch(team, first_column);
-  static_assert(kFlatJoin <= 32, "a lane per part");
-  const int lane = tid & 31;
-  for (int g = tid >> 5; g < G; g += kThreads / 32) {
-    const float m = lane < count ? __ldcg(part(lane) + g) : -INFINITY;
-    const float l = lane < count ? __ldcg(part(lane) + G8 + g) : 0.f;
-    float top = m;
-#pragma unroll
-    for (int step = 16; step > 0; step >>= 1) {
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
-    }
-    const float w = __expf(m - finite_or_zero(top));
-    float sum = lane < count ? w * l : 0.f;
-#pragma unroll
-    for (int step = 16; step > 0; step >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, step);
-    sm_weight[lane * G8 + g] = w;
-    if (lane == 0) {
-      sm_top[g] = top;
-      sm_sum[g] = sum;
-    }
-  }
-  __syncthreads();
-  // Threads left over by one whole team have no column.
-  for (int column = active || teams > 1 ? first_column : columns; column < columns;
-       column += kThreads) {
-    const int g = column / (D / 4), d = (column - g * (D / 4)) * 4;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (active) {
-      for (int k0 = team; k0 < count; k0 += kBatch * teams) {
-        if (k0 != team || column != first_column) fetch(k0, column);
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-          const int k = k0 + u * teams;
-          if (k < count) fma4(acc, sm_weight[k * G8 + g], batch[u]);
-        }
-      }
-    }
-    if (teams > 1) {  // then every thread has at most one column
-      sm_o[tid] = acc;
-      __syncthreads();
-      if (team != 0) break;
-      for (int other = 1; other < teams; ++other) {
-        fma4(acc, 1.f, sm_o[other * columns + column]);
-      }
-    }
-    if (to == nullptr) put_joined(p, row, g, d, sm_top[g], sm_sum[g], acc);
-    else put_partial<D, G8>(to, g, d, sm_top[g], sm_sum[g], acc);
+  } else if (p.lse != nullptr) {
+    p.lse[static_cast<int64_t>(row) * p.group + g] = finite_or_zero(m) + logf(l);
   }
 }
 
@@ -384,16 +323,18 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   uint8_t* ring = align_smem(smem_raw);  // [warp][K | V]
   __shared__ __align__(8) uint64_t bars[W][2];
   __shared__ int warp_sum[W];
-  // The CTA's partials, two per warp, in token order: the row (or -1), each
-  // query's m and l, then its weight within the CTA and the CTA's m and l of
-  // the row (kept at the row's first partial).
+  // The CTA's partials, two per warp, in token order: the row (or -1), and each
+  // query's m and l.
   __shared__ int seg_row[2 * W];
   __shared__ float seg_m[2 * W][G8], seg_l[2 * W][G8];
-  __shared__ float seg_weight[2 * W][G8], row_m[2 * W][G8], row_l[2 * W][G8];
+  // Joins: the rows of the CTA's partials, first and last partial of each, and
+  // the parts' weights and the rows' inverse sums.
+  __shared__ int join_rows, join_first[2 * W], join_last[2 * W];
+  __shared__ float weight[2 * kFlatJoin][G8], inverse[2 * W][G8];
   __shared__ Cut cuts[2];
   __shared__ int last_arrival[2];
   __shared__ int busy;  // sequences that are not empty
-  int* start = reinterpret_cast<int*>(ring + W * 2 * kTile);  // tiles before each sequence
+  int* start = reinterpret_cast<int*>(ring + table_offset(D, NT));  // tiles before each sequence
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (lane == 0) {
     mbar_init(&bars[warp][0], 1);
@@ -475,11 +416,13 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   uint8_t* stage = ring + warp * 2 * kTile;
   const uint32_t k_tile = smem_addr(stage), v_tile = k_tile + kTile;
   // Where partial i of the CTA keeps its o: a warp's last row waits in the
-  // warp's own idle stage, an earlier one (cut by the range's start) in the
-  // workspace.
+  // warp's own idle stage, an earlier one (cut by the range's start) apart.
+  float* firsts = first_in_smem(D)
+                      ? reinterpret_cast<float*>(ring + W * 2 * kTile)
+                      : p.warp_partials + static_cast<size_t>(cta) * W * kWarpPartial;
   const auto segment = [&](int i) {
     return i & 1 ? reinterpret_cast<float*>(ring + (i >> 1) * 2 * kTile)
-                 : p.warp_partials + (static_cast<size_t>(cta) * W + (i >> 1)) * kWarpPartial;
+                 : firsts + (i >> 1) * kWarpPartial;
   };
   const uint64_t policy = l2_evict_first_policy();
   const int page_rows = 1 << p.block_shift;
@@ -672,63 +615,72 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   // Join the CTA's partials.  A row that began and ended within the CTA is
   // written; one that began before it goes to the CTA's slot 0, one that only
   // goes on after it to slot 1.
+  //
+  // First the weights, half a warp per query and a lane per partial (partials
+  // that are not there weigh nothing), by scans over the lanes of each row;
+  // then every four channels of a row by a thread.
+  const auto slot_of = [&](int row) {
+    return row == cuts[0].row ? 0 : row == cuts[1].row ? 1 : -1;
+  };
+  const auto partial_of = [&](int slot) {
+    return slot < 0 ? nullptr : p.cta_partials + (static_cast<size_t>(cta) * 2 + slot) * kPartial;
+  };
   {
-    const int mine = lane < 2 * W ? seg_row[lane] : -1;
-    const unsigned used = __ballot_sync(0xffffffffu, mine >= 0);
-    const unsigned below = used & ((1u << lane) - 1);
-    const int previous = __shfl_sync(0xffffffffu, mine, below ? 31 - __clz(below) : 0);
-    // The first partial of each row.
+    const int i = lane & 15;
+    const int row = i < 2 * W ? seg_row[i] : -1;
+    const unsigned used = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
+    const unsigned below = used & ((1u << i) - 1);
+    const int previous = __shfl_sync(0xffffffffu, row, below ? 31 - __clz(below) : 0);
     const unsigned heads =
-        __ballot_sync(0xffffffffu, mine >= 0 && (below == 0 || previous != mine));
-    // Partials of the row whose first one is i.
-    const auto members = [&](int i) {
-      const unsigned later = heads & ~((2u << i) - 1);
-      return used & ~((1u << i) - 1) & (later ? (later & -later) - 1 : 0xffffffffu);
-    };
-    const int i = threadIdx.x / G8, g = threadIdx.x % G8;  // 2 W G8 threads at most
-    if (i < 2 * W && (used >> i & 1) && g < p.group) {
-      const int head = 31 - __clz(heads & ((2u << i) - 1));
-      float top = -INFINITY;
-      for (unsigned set = members(head); set; set &= set - 1) {
-        top = fmaxf(top, seg_m[__ffs(set) - 1][g]);
+        __ballot_sync(0xffffffffu, row >= 0 && (below == 0 || previous != row)) & 0xffffu;
+    const unsigned from = heads & ((2u << i) - 1), beyond = heads & ~((2u << i) - 1);
+    const int first = from ? 31 - __clz(from) : 0, last = beyond ? __ffs(beyond) - 2 : 15;
+    if (threadIdx.x < 16) {
+      if (i == 0) join_rows = __popc(heads);
+      if (heads >> i & 1) {
+        const int k = __popc(heads & ((1u << i) - 1));
+        join_first[k] = first;
+        join_last[k] = min(last, 2 * W - 1);
       }
-      const float ref = finite_or_zero(top);
-      seg_weight[i][g] = __expf(seg_m[i][g] - ref);
-      if (i == head) {
-        float sum = 0.f;
-        for (unsigned set = members(head); set; set &= set - 1) {
-          const int j = __ffs(set) - 1;
-          sum += __expf(seg_m[j][g] - ref) * seg_l[j][g];
-        }
-        row_m[i][g] = top;
-        row_l[i][g] = sum;
+    }
+    for (int g = 2 * warp + (lane >> 4); g < G8; g += 2 * W) {
+      const float m = row >= 0 ? seg_m[i][g] : -INFINITY;
+      float top = m;
+#pragma unroll
+      for (int step = 1; step < 16; step <<= 1) {
+        const float other = __shfl_up_sync(0xffffffffu, top, step, 16);
+        if (i - step >= first) top = fmaxf(top, other);
+      }
+      top = __shfl_sync(0xffffffffu, top, last, 16);
+      const float w = row >= 0 ? __expf(m - finite_or_zero(top)) : 0.f;
+      float sum = row >= 0 ? w * seg_l[i][g] : 0.f;
+#pragma unroll
+      for (int step = 1; step < 16; step <<= 1) {
+        const float other = __shfl_up_sync(0xffffffffu, sum, step, 16);
+        if (i - step >= first) sum += other;
+      }
+      sum = __shfl_sync(0xffffffffu, sum, last, 16);
+      if (i < 2 * W) weight[i][g] = w;
+      if ((heads >> i & 1) && g < p.group) {
+        inverse[i][g] = 1.f / sum;
+        put_sums<G8>(p, row, g, partial_of(slot_of(row)), top, sum);
       }
     }
     __syncthreads();
-    const int columns = p.group * (D / 4), total = __popc(heads) * columns;
-    for (int x = threadIdx.x; x < total; x += kThreads) {
+    const int columns = p.group * (D / 4);
+    for (int x = threadIdx.x; x < join_rows * columns; x += kThreads) {
       const int k = x / columns, column = x - k * columns;
-      unsigned set = heads;
-      for (int skip = 0; skip < k; ++skip) set &= set - 1;
-      const int head = __ffs(set) - 1;
       const int q = column / (D / 4), d = (column - q * (D / 4)) * 4;
+      const int a = join_first[k], z = join_last[k], r = seg_row[a];
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      set = members(head);
-#pragma unroll
-      for (int j = 0; j < 2 * W; ++j) {
-        if (set >> j & 1) {
-          fma4(acc, seg_weight[j][q],
+#pragma unroll 4
+      for (int j = a; j <= z; ++j) {
+        if (used >> j & 1) {
+          fma4(acc, weight[j][q],
                *reinterpret_cast<const float4*>(segment(j) + q * (D + kPad) + d));
         }
       }
-      const int row = seg_row[head];
-      const int slot = row == cuts[0].row ? 0 : row == cuts[1].row ? 1 : -1;
-      if (slot < 0) {
-        put_joined(p, row, q, d, row_m[head][q], row_l[head][q], acc);
-      } else {
-        put_partial<D, G8>(p.cta_partials + (static_cast<size_t>(cta) * 2 + slot) * kPartial, q, d,
-                           row_m[head][q], row_l[head][q], acc);
-      }
+      put_joined<D, G8>(p, r, q, d, partial_of(slot_of(r)), inverse[a][q], acc);
     }
   }
 
@@ -757,40 +709,111 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
     return min(cut.fan, cut.first_cta + cut.parts - group_first(cut));
   };
   __syncthreads();
-  if (lane == 0 && warp < 2 && cuts[warp].row >= 0) {  // both slots at once
+  if (lane == 0 && warp < 2) {  // both slots at once
     const Cut cut = cuts[warp];
-    last_arrival[warp] = arrive(p.counters + at_cta(cut, group_first(cut)), group_members(cut));
+    last_arrival[warp] = cut.row >= 0 && arrive(p.counters + at_cta(cut, group_first(cut)),
+                                                group_members(cut));
   }
   __syncthreads();
-  float* scratch = reinterpret_cast<float*>(ring);
-  for (int slot = 0; slot < 2; ++slot) {
-    const Cut cut = cuts[slot];
-    if (cut.row < 0 || !last_arrival[slot]) continue;
-    const int first = group_first(cut), groups = (cut.parts + cut.fan - 1) / cut.fan;
-    join_remote<D, NT>(p, group_members(cut), [&](int k) { return part_of(cut, first + k); },
-                       cut.row, groups == 1 ? nullptr : group_of(cut, first), scratch);
-    __syncthreads();  // the scratch is used again
-    if (groups == 1) continue;
-    if (threadIdx.x == 0) {
-      last_arrival[slot] = arrive(p.counters + 2 * kMostCtas + cut.first_cta, groups);
+  // Joins the parts of the rows whose last arrival was this CTA's: count_of the
+  // parts, at(cut, k) the k-th, to_of the destination.  Like the join above,
+  // but a whole warp finds a query's weights, a lane per part, while the first
+  // parts' channels are on their way to the threads that will add them.
+  const auto join_arrived = [&](auto count_of, auto at, auto to_of) {
+    constexpr int kBatch = 16;
+    const bool both = last_arrival[0] && last_arrival[1];
+    const int only = last_arrival[0] ? 0 : 1;
+    if (!last_arrival[only]) return;
+    const int columns = p.group * (D / 4), total = both ? 2 * columns : columns;
+    float4 batch[kBatch];
+    const auto place = [&](int x, int& slot, int& q, int& d) {
+      slot = both ? (x >= columns ? 1 : 0) : only;
+      const int column = both && slot ? x - columns : x;
+      q = column / (D / 4);
+      d = (column - q * (D / 4)) * 4;
+    };
+    const auto fetch = [&](int x, int base) {
+      int slot, q, d;
+      place(x, slot, q, d);
+      const Cut& cut = cuts[slot];
+      const int count = count_of(cut);
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        if (base + u < count) {
+          batch[u] = __ldcg(
+              reinterpret_cast<const float4*>(at(cut, base + u) + 2 * G8 + q * D + d));
+        }
+      }
+    };
+    if (static_cast<int>(threadIdx.x) < total) fetch(threadIdx.x, 0);
+    for (int task = warp; task < (both ? 2 * p.group : p.group); task += W) {
+      const int slot = both ? (task >= p.group ? 1 : 0) : only;
+      const int g = both && slot ? task - p.group : task;
+      const Cut& cut = cuts[slot];
+      const int count = count_of(cut);
+      const float* mine = at(cut, min(lane, count - 1));
+      const float m = lane < count ? __ldcg(mine + g) : -INFINITY;
+      const float l = lane < count ? __ldcg(mine + G8 + g) : 0.f;
+      float top = m;
+#pragma unroll
+      for (int step = 16; step > 0; step >>= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
+      }
+      const float w = __expf(m - finite_or_zero(top));
+      float sum = lane < count ? w * l : 0.f;
+#pragma unroll
+      for (int step = 16; step > 0; step >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, step);
+      weight[slot * kFlatJoin + lane][g] = w;
+      if (lane == 0) {
+        inverse[slot][g] = 1.f / sum;
+        put_sums<G8>(p, cut.row, g, to_of(cut), top, sum);
+      }
     }
     __syncthreads();
-    if (!last_arrival[slot]) continue;
-    join_remote<D, NT>(p, groups, [&](int k) { return group_of(cut, cut.first_cta + k * cut.fan); },
-                       cut.row, nullptr, scratch);
-    __syncthreads();
+    for (int x = threadIdx.x; x < total; x += kThreads) {
+      int slot, q, d;
+      place(x, slot, q, d);
+      const Cut& cut = cuts[slot];
+      const int count = count_of(cut);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int base = 0; base < count; base += kBatch) {
+        if (base > 0 || x >= kThreads) fetch(x, base);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          if (base + u < count) fma4(acc, weight[slot * kFlatJoin + base + u][q], batch[u]);
+        }
+      }
+      put_joined<D, G8>(p, cut.row, q, d, to_of(cut), inverse[slot][q], acc);
+    }
+  };
+  join_arrived(group_members, [&](const Cut& cut, int k) { return part_of(cut, group_first(cut) + k); },
+            [&](const Cut& cut) {
+              return cut.fan < cut.parts ? group_of(cut, group_first(cut)) : nullptr;
+            });
+  // The joined groups of rows over more CTAs than kFlatJoin.
+  if ((cuts[0].row < 0 || cuts[0].fan == cuts[0].parts) &&
+      (cuts[1].row < 0 || cuts[1].fan == cuts[1].parts)) {
+    return;
   }
+  const auto groups_of = [](const Cut& cut) { return (cut.parts + cut.fan - 1) / cut.fan; };
+  __syncthreads();
+  if (lane == 0 && warp < 2) {
+    const Cut cut = cuts[warp];
+    last_arrival[warp] = last_arrival[warp] && cut.fan < cut.parts &&
+                         arrive(p.counters + 2 * kMostCtas + cut.first_cta, groups_of(cut));
+  }
+  __syncthreads();
+  join_arrived(groups_of,
+            [&](const Cut& cut, int k) { return group_of(cut, cut.first_cta + k * cut.fan); },
+            [](const Cut&) -> float* { return nullptr; });
 }
 
 template <int D, int NT>
 cudaError_t launch_t(const PagedMaps& maps, const PagedParams& p, int ctas, cudaStream_t stream) {
-  const size_t smem = kSmemSlack + static_cast<size_t>(paged_warps(D)) * stage_bytes(D) +
-                      static_cast<size_t>(p.sequences + 1) * 4;
+  const size_t smem = paged_smem(D, NT, p.sequences);
   // One limit for every batch: the largest this kernel takes.
-  const size_t most = kSmemSlack + static_cast<size_t>(paged_warps(D)) * stage_bytes(D) +
-                      static_cast<size_t>(kMostSequences + 1) * 4;
-  cudaError_t err =
-      ensure_smem_limit(reinterpret_cast<const void*>(&paged_kernel<D, NT>), most);
+  cudaError_t err = ensure_smem_limit(reinterpret_cast<const void*>(&paged_kernel<D, NT>),
+                                      paged_smem(D, NT, kMostSequences));
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
@@ -825,7 +848,9 @@ struct Layout {
     const size_t one = static_cast<size_t>(partial_floats(D, NT)) * 4;
     size_t off = kHeader;
     warp_partials = off;
-    off += static_cast<size_t>(warp_partial_floats(D, NT)) * 4 * sms * paged_warps(D);
+    if (!first_in_smem(D)) {
+      off += static_cast<size_t>(warp_partial_floats(D, NT)) * 4 * sms * paged_warps(D);
+    }
     cta_partials = off;
     off += one * sms * 2;
     group_partials = off;
