@@ -146,24 +146,32 @@ struct Ranges {
 };
 
 // A row cut by the CTA's range: slot 0 began before it, slot 1 within it.  Its
-// parts are the partials of CTAs first_cta, first_cta + 1, ..., joined `fan`
-// at a time.
+// parts are the partials of the CTAs from first_cta on, each CTA's in slot 1 if
+// the row begins there and slot 0 otherwise.  `members` of them from CTA
+// `first` on, this CTA's among them, are joined by the last of those to
+// arrive; where they are not all of the row's, the `groups` results, `fan` CTAs
+// apart, are joined in turn.
 struct Cut {
   int row;  // -1: none
-  int first_cta, parts, fan;
+  int first_cta, first, members, groups, fan;
+  __device__ int slot_at(int cta) const { return 2 * cta + (cta == first_cta ? 1 : 0); }
 };
 
-__device__ __forceinline__ Cut cut_row(const Ranges& ranges, int row, unsigned begin,
+__device__ __forceinline__ Cut cut_row(const Ranges& ranges, int cta, int row, unsigned begin,
                                        unsigned tiles) {
   Cut c;
   c.row = row;
   c.first_cta = ranges.owner(begin);
-  c.parts = ranges.owner(begin + tiles - 1) - c.first_cta + 1;
-  c.fan = c.parts;
-  if (c.parts > kFlatJoin) {
+  const int parts = ranges.owner(begin + tiles - 1) - c.first_cta + 1;
+  c.fan = parts;
+  if (parts > kFlatJoin) {
     c.fan = 1;
-    while (c.fan * c.fan < c.parts) ++c.fan;
+    while (c.fan * c.fan < parts) ++c.fan;
   }
+  const int group = (cta - c.first_cta) / c.fan;
+  c.first = c.first_cta + group * c.fan;
+  c.members = min(c.fan, parts - group * c.fan);
+  c.groups = (parts + c.fan - 1) / c.fan;
   return c;
 }
 
@@ -466,7 +474,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
     const bool cut = warp == 0 ? begin < lo : begin >= lo && begin + c.tiles > hi;
     Cut found;
     found.row = -1;
-    if (cut) found = cut_row(ranges, c.seq * p.heads + c.head, begin, c.tiles);
+    if (cut) found = cut_row(ranges, cta, c.seq * p.heads + c.head, begin, c.tiles);
     if (lane == 0) cuts[warp] = found;
   };
   if (wlo >= whi) find_cuts();
@@ -687,40 +695,25 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   // Rows cut by CTA ranges: the last of a row's CTAs to arrive joins them; a
   // row over many CTAs is joined in groups first, so that no CTA reads more
   // than a few partials.
-  // Partials of a row's CTA c, and of the group that begins at it, with the
-  // counter of the group: a CTA can end one row (slot 0) and begin another.
-  const auto at_cta = [&](const Cut& cut, int c) { return 2 * c + (c == cut.first_cta ? 1 : 0); };
-  const auto part_of = [&](const Cut& cut, int c) {
-    return p.cta_partials + static_cast<int64_t>(at_cta(cut, c)) * kPartial;
-  };
-  const auto group_of = [&](const Cut& cut, int c) {
-    return p.group_partials + static_cast<int64_t>(at_cta(cut, c)) * kPartial;
-  };
   // Whether this arrival is the last of `expected`; the counter is then zero again.
   const auto arrive = [](int* counter, int expected) {
     const bool last = arrive_add(counter) == expected - 1;
     if (last) *counter = 0;
     return last;
   };
-  const auto group_first = [&](const Cut& cut) {
-    return cut.first_cta + (static_cast<int>(cta) - cut.first_cta) / cut.fan * cut.fan;
-  };
-  const auto group_members = [&](const Cut& cut) {
-    return min(cut.fan, cut.first_cta + cut.parts - group_first(cut));
-  };
   __syncthreads();
   if (lane == 0 && warp < 2) {  // both slots at once
     const Cut cut = cuts[warp];
-    last_arrival[warp] = cut.row >= 0 && arrive(p.counters + at_cta(cut, group_first(cut)),
-                                                group_members(cut));
+    last_arrival[warp] =
+        cut.row >= 0 && arrive(p.counters + cut.slot_at(cut.first), cut.members);
   }
   __syncthreads();
-  // Joins the parts of the rows whose last arrival was this CTA's: count_of the
-  // parts, at(cut, k) the k-th, to_of the destination.  Like the join above,
-  // but a whole warp finds a query's weights, a lane per part, while the first
-  // parts' channels are on their way to the threads that will add them.
-  const auto join_arrived = [&](auto count_of, auto at, auto to_of) {
-    constexpr int kBatch = 16;
+  // Joins the rows whose last arrival was this CTA's: its members' partials
+  // or, once those are joined, the groups'.  Like the join above, but a whole
+  // warp finds a query's weights, a lane per part, while the first parts'
+  // channels are on their way to the threads that will add them.
+  const auto join_arrived = [&](const bool grouped) {
+    constexpr int kBatch = 20;  // 18 or 19 parts: eight rows over the whole GPU
     const bool both = last_arrival[0] && last_arrival[1];
     const int only = last_arrival[0] ? 0 : 1;
     if (!last_arrival[only]) return;
@@ -732,16 +725,28 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
       q = column / (D / 4);
       d = (column - q * (D / 4)) * 4;
     };
+    // The k-th part of the join of `cut` is part(cut, k).
+    const auto count_of = [&](const Cut& cut) { return grouped ? cut.groups : cut.members; };
+    const auto part = [&](const Cut& cut, int k) -> const float* {
+      return grouped ? p.group_partials +
+                           static_cast<size_t>(cut.slot_at(cut.first_cta + k * cut.fan)) * kPartial
+                     : p.cta_partials + static_cast<size_t>(cut.slot_at(cut.first + k)) * kPartial;
+    };
+    const auto to_of = [&](const Cut& cut) {
+      return grouped || cut.groups == 1
+                 ? nullptr
+                 : p.group_partials + static_cast<size_t>(cut.slot_at(cut.first)) * kPartial;
+    };
     const auto fetch = [&](int x, int base) {
       int slot, q, d;
       place(x, slot, q, d);
-      const Cut& cut = cuts[slot];
+      const Cut cut = cuts[slot];
       const int count = count_of(cut);
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
         if (base + u < count) {
           batch[u] = __ldcg(
-              reinterpret_cast<const float4*>(at(cut, base + u) + 2 * G8 + q * D + d));
+              reinterpret_cast<const float4*>(part(cut, base + u) + 2 * G8 + q * D + d));
         }
       }
     };
@@ -749,9 +754,9 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
     for (int task = warp; task < (both ? 2 * p.group : p.group); task += W) {
       const int slot = both ? (task >= p.group ? 1 : 0) : only;
       const int g = both && slot ? task - p.group : task;
-      const Cut& cut = cuts[slot];
+      const Cut cut = cuts[slot];
       const int count = count_of(cut);
-      const float* mine = at(cut, min(lane, count - 1));
+      const float* mine = part(cut, min(lane, count - 1));
       const float m = lane < count ? __ldcg(mine + g) : -INFINITY;
       const float l = lane < count ? __ldcg(mine + G8 + g) : 0.f;
       float top = m;
@@ -773,7 +778,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
     for (int x = threadIdx.x; x < total; x += kThreads) {
       int slot, q, d;
       place(x, slot, q, d);
-      const Cut& cut = cuts[slot];
+      const Cut cut = cuts[slot];
       const int count = count_of(cut);
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int base = 0; base < count; base += kBatch) {
@@ -786,26 +791,18 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
       put_joined<D, G8>(p, cut.row, q, d, to_of(cut), inverse[slot][q], acc);
     }
   };
-  join_arrived(group_members, [&](const Cut& cut, int k) { return part_of(cut, group_first(cut) + k); },
-            [&](const Cut& cut) {
-              return cut.fan < cut.parts ? group_of(cut, group_first(cut)) : nullptr;
-            });
-  // The joined groups of rows over more CTAs than kFlatJoin.
-  if ((cuts[0].row < 0 || cuts[0].fan == cuts[0].parts) &&
-      (cuts[1].row < 0 || cuts[1].fan == cuts[1].parts)) {
+  join_arrived(false);
+  if (!(cuts[0].row >= 0 && cuts[0].groups > 1) && !(cuts[1].row >= 0 && cuts[1].groups > 1)) {
     return;
   }
-  const auto groups_of = [](const Cut& cut) { return (cut.parts + cut.fan - 1) / cut.fan; };
   __syncthreads();
   if (lane == 0 && warp < 2) {
     const Cut cut = cuts[warp];
-    last_arrival[warp] = last_arrival[warp] && cut.fan < cut.parts &&
-                         arrive(p.counters + 2 * kMostCtas + cut.first_cta, groups_of(cut));
+    last_arrival[warp] = last_arrival[warp] && cut.groups > 1 &&
+                         arrive(p.counters + 2 * kMostCtas + cut.first_cta, cut.groups);
   }
   __syncthreads();
-  join_arrived(groups_of,
-            [&](const Cut& cut, int k) { return group_of(cut, cut.first_cta + k * cut.fan); },
-            [](const Cut&) -> float* { return nullptr; });
+  join_arrived(true);
 }
 
 template <int D, int NT>
