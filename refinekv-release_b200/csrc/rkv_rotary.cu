@@ -23,36 +23,53 @@ void set_last_error(const std::string& message);
 
 namespace {
 
+// V consecutive elements as they lie in memory.
 template <typename T, int V>
-struct alignas(V * sizeof(T)) Pack {
-  T at[V];
+struct Piece {
+  uint32_t word[4];  // 16 bytes
+  __device__ void load(const T* from) {
+    const uint4 x = *reinterpret_cast<const uint4*>(from);
+    word[0] = x.x, word[1] = x.y, word[2] = x.z, word[3] = x.w;
+  }
+  __device__ void store(T* to) const {
+    *reinterpret_cast<uint4*>(to) = make_uint4(word[0], word[1], word[2], word[3]);
+  }
 };
 
+template <typename T>
+struct Piece<T, 1> {
+  T one;
+  __device__ void load(const T* from) { one = *from; }
+  __device__ void store(T* to) const { *to = one; }
+};
+
+__device__ __forceinline__ float low(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 __device__ __forceinline__ float widen(float x) { return x; }
 __device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void narrow(float& to, float x) { to = x; }
+__device__ __forceinline__ void narrow(__nv_bfloat16& to, float x) { to = __float2bfloat16_rn(x); }
+
+// The piece rounded to bf16 (as it is when it holds bf16).
+__device__ __forceinline__ void store_bf16(const Piece<__nv_bfloat16, 8>& x, __nv_bfloat16* to) {
+  x.store(to);
+}
+__device__ __forceinline__ void store_bf16(const Piece<float, 4>& x, __nv_bfloat16* to) {
+  *reinterpret_cast<uint2*>(to) =
+      make_uint2(pack_bf16(__uint_as_float(x.word[0]), __uint_as_float(x.word[1])),
+                 pack_bf16(__uint_as_float(x.word[2]), __uint_as_float(x.word[3])));
+}
 template <typename T>
-__device__ __forceinline__ T narrow(float x);
-template <>
-__device__ __forceinline__ float narrow<float>(float x) { return x; }
-template <>
-__device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float x) {
-  return __float2bfloat16_rn(x);
+__device__ __forceinline__ void store_bf16(const Piece<T, 1>& x, __nv_bfloat16* to) {
+  narrow(*to, widen(x.one));
 }
 
 template <typename T, int V>
-__device__ __forceinline__ void load_pack(const T* from, float (&x)[V]) {
-  const Pack<T, V> p = *reinterpret_cast<const Pack<T, V>*>(from);
-#pragma unroll
-  for (int i = 0; i < V; ++i) x[i] = widen(p.at[i]);
+__device__ __forceinline__ void clear(Piece<T, V>& x) {
+  x.word[0] = x.word[1] = x.word[2] = x.word[3] = 0;
 }
-
-template <typename T, int V>
-__device__ __forceinline__ void store_pack(T* to, const float (&x)[V]) {
-  Pack<T, V> p;
-#pragma unroll
-  for (int i = 0; i < V; ++i) p.at[i] = narrow<T>(x[i]);
-  *reinterpret_cast<Pack<T, V>*>(to) = p;
-}
+template <typename T>
+__device__ __forceinline__ void clear(Piece<T, 1>& x) { narrow(x.one, 0.f); }
 
 // V cosines or sines: at most 16 bytes a load.
 template <int V>
@@ -60,45 +77,153 @@ __device__ __forceinline__ void load_table(const float* from, float (&x)[V]) {
   constexpr int W = V < 4 ? V : 4;
 #pragma unroll
   for (int i = 0; i < V; i += W) {
-    const Pack<float, W> p = *reinterpret_cast<const Pack<float, W>*>(from + i);
-#pragma unroll
-    for (int j = 0; j < W; ++j) x[i + j] = p.at[j];
+    if constexpr (W == 4) {
+      const float4 four = *reinterpret_cast<const float4*>(from + i);
+      x[i] = four.x, x[i + 1] = four.y, x[i + 2] = four.z, x[i + 3] = four.w;
+    } else {
+      x[i] = from[i];
+    }
   }
 }
 
-// One product pair of the rotation.  Products and sums are rounded one by one
-// (no fused multiply-add): the result then depends on nothing but its
-// operands, so rotating alone, rotating while appending and the formula in
-// fp32 agree bit for bit.
-__device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
-  const float y = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
-  const float z = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
+// Two pairs (a, b) turned.  Products and sums are rounded one by one (no fused
+// multiply-add): the result then depends on nothing but its operands, so
+// rotating alone, rotating while appending and the formula in fp32 agree bit
+// for bit.
+__device__ __forceinline__ void turn2(float2& a, float2& b, float2 c, float2 s) {
+  const float2 y = __fadd2_rn(__fmul2_rn(a, c), __fmul2_rn(b, make_float2(-s.x, -s.y)));
+  b = __fadd2_rn(__fmul2_rn(b, c), __fmul2_rn(a, s));
   a = y;
-  b = z;
 }
 
+// The V pairs of a unit's two pieces turned: (p_i, q_i), or interleaved the
+// neighbours of p and then those of q.
+template <bool Interleaved>
+__device__ __forceinline__ void turn(Piece<__nv_bfloat16, 8>& p, Piece<__nv_bfloat16, 8>& q,
+                                     const float (&c)[8], const float (&s)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {  // pairs 2 i and 2 i + 1
+    const float2 c2 = make_float2(c[2 * i], c[2 * i + 1]);
+    const float2 s2 = make_float2(s[2 * i], s[2 * i + 1]);
+    if constexpr (Interleaved) {
+      uint32_t& w0 = i < 2 ? p.word[2 * i] : q.word[2 * i - 4];
+      uint32_t& w1 = i < 2 ? p.word[2 * i + 1] : q.word[2 * i - 3];
+      float2 a = make_float2(low(w0), low(w1)), b = make_float2(high(w0), high(w1));
+      turn2(a, b, c2, s2);
+      w0 = pack_bf16(a.x, b.x);
+      w1 = pack_bf16(a.y, b.y);
+    } else {
+      float2 a = make_float2(low(p.word[i]), high(p.word[i]));
+      float2 b = make_float2(low(q.word[i]), high(q.word[i]));
+      turn2(a, b, c2, s2);
+      p.word[i] = pack_bf16(a.x, a.y);
+      q.word[i] = pack_bf16(b.x, b.y);
+    }
+  }
+}
+
+template <bool Interleaved>
+__device__ __forceinline__ void turn(Piece<float, 4>& p, Piece<float, 4>& q, const float (&c)[4],
+                                     const float (&s)[4]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t& a0 = Interleaved ? (i ? q : p).word[0] : p.word[2 * i];
+    uint32_t& b0 = Interleaved ? (i ? q : p).word[1] : q.word[2 * i];
+    uint32_t& a1 = Interleaved ? (i ? q : p).word[2] : p.word[2 * i + 1];
+    uint32_t& b1 = Interleaved ? (i ? q : p).word[3] : q.word[2 * i + 1];
+    float2 a = make_float2(__uint_as_float(a0), __uint_as_float(a1));
+    float2 b = make_float2(__uint_as_float(b0), __uint_as_float(b1));
+    turn2(a, b, make_float2(c[2 * i], c[2 * i + 1]), make_float2(s[2 * i], s[2 * i + 1]));
+    a0 = __float_as_uint(a.x), a1 = __float_as_uint(a.y);
+    b0 = __float_as_uint(b.x), b1 = __float_as_uint(b.y);
+  }
+}
+
+template <bool Interleaved, typename T>
+__device__ __forceinline__ void turn(Piece<T, 1>& p, Piece<T, 1>& q, const float (&c)[1],
+                                     const float (&s)[1]) {
+  float2 a = make_float2(widen(p.one), 0.f), b = make_float2(widen(q.one), 0.f);
+  turn2(a, b, make_float2(c[0], 0.f), make_float2(s[0], 0.f));
+  narrow(p.one, a.x);
+  narrow(q.one, b.x);
+}
+
+// A CTA takes the heads of one blockIdx.y and every gridDim.x-th token; the
+// next token's position is requested ahead.  A thread keeps its channels (unit
+// c) of kHeads heads, so their cosines and sines are loaded once a token and
+// the heads' addresses worked out once.
+constexpr int kHeads = 2;
+// Vector units: CTAs of up to 256 threads, four to an SM or more (64 registers).
+constexpr int row_threads(int V) { return V == 1 ? 512 : 256; }
+constexpr int row_ctas(int V) { return V == 1 ? 2 : 4; }
+
 template <typename T, int V, bool Interleaved, bool Append>
-__global__ void __launch_bounds__(512) rows_kernel(const __grid_constant__ RowsParams p) {
-  const int per_head = p.dim / (2 * V), turned = p.rotary / (2 * V);
-  const int q_units = p.query.heads * per_head, k_units = p.key.heads * per_head;
-  const int units = q_units + k_units + (Append ? p.value.heads * per_head : 0);
+__global__ void __launch_bounds__(row_threads(V), row_ctas(V))
+    rows_kernel(const __grid_constant__ RowsParams p) {
+  const int per_head = p.dim / (2 * V);
+  const int stride = blockDim.x / per_head, c = threadIdx.x % per_head;
+  const int k_from = p.query.heads, v_from = k_from + p.key.heads;
+  const int heads = v_from + (Append ? p.value.heads : 0);
+  const bool rotary = c < p.rotary / (2 * V);
+  // The unit's two pieces; unrotated rows are copied in the same pieces.
+  const bool halves = !Interleaved && rotary;
+  const int first = halves ? c * V : c * 2 * V;
+  const int gap = halves ? p.rotary / 2 : V;
+  int kind[kHeads];  // 0 query, 1 key, 2 value, -1 nothing
+  int64_t in_at[kHeads], out_at[kHeads];
+#pragma unroll
+  for (int u = 0; u < kHeads; ++u) {
+    const int lane_head = threadIdx.x / per_head;
+    const int head = (blockIdx.y * kHeads + u) * stride + lane_head;
+    kind[u] = lane_head >= stride || head >= heads ? -1 : head < k_from ? 0 : head < v_from ? 1 : 2;
+    const RowStream& s = kind[u] <= 0 ? p.query : kind[u] == 1 ? p.key : p.value;
+    const int own = head - (kind[u] <= 0 ? 0 : kind[u] == 1 ? k_from : v_from);
+    in_at[u] = own * s.in_h + first;
+    out_at[u] = own * s.out_h + first;
+  }
   pdl_wait();
   pdl_launch_dependents();
-  for (int64_t n = blockIdx.x; n < p.batch * p.tokens; n += gridDim.x) {
+  const int64_t count = p.batch * p.tokens;
+  const auto position = [&](int64_t n) -> int64_t {
+    const int64_t b = p.batch > 1 ? n / p.tokens : 0;
+    const int64_t at = b * p.pos_b + (n - b * p.tokens) * p.pos_t;
+    return p.pos_i64 ? static_cast<const int64_t*>(p.positions)[at]
+                     : static_cast<const int32_t*>(p.positions)[at];
+  };
+  int64_t upcoming = position(blockIdx.x);
+  for (int64_t n = blockIdx.x; n < count; n += gridDim.x) {
     const int64_t b = p.batch > 1 ? n / p.tokens : 0, t = n - b * p.tokens;
-    const int64_t at = b * p.pos_b + t * p.pos_t;
-    const int64_t pos = p.pos_i64 ? static_cast<const int64_t*>(p.positions)[at]
-                                  : static_cast<const int32_t*>(p.positions)[at];
+    const int64_t pos = upcoming;
+    Piece<T, V> in[kHeads][2];
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u) {
+      if (kind[u] < 0) continue;
+      const RowStream& s = kind[u] == 0 ? p.query : !Append || kind[u] == 1 ? p.key : p.value;
+      const T* from = static_cast<const T*>(s.in) + (b * s.in_b + t * s.in_t) + in_at[u];
+      in[u][0].load(from);
+      in[u][1].load(from + gap);
+    }
+    if (n + gridDim.x < count) upcoming = position(n + gridDim.x);
     const bool known = p.rotary == 0 || (pos >= 0 && pos < p.table_rows);
-    const float* table = p.cos_sin + (known ? pos : 0) * p.table_stride;
+    float cs[V], sn[V];
+    if (rotary && known) {
+      const float* table = p.cos_sin + pos * p.table_stride + c * V;
+      load_table<V>(table, cs);
+      load_table<V>(table + p.rotary / 2, sn);
+#pragma unroll
+      for (int i = 0; i < V; ++i) sn[i] *= p.sign;
+    } else {  // a position outside the table: NaN
+#pragma unroll
+      for (int i = 0; i < V; ++i) cs[i] = sn[i] = __int_as_float(0x7fc00000);
+    }
     bool keep = true;  // the token's rows go to the pool
-    int64_t page = 0, row = 0;
+    int64_t page = 0, page_row = 0;
     if (Append) {
       keep = pos >= 0;
       if (keep) {
         const int64_t seq = p.sequence_ids != nullptr ? p.sequence_ids[n] : n;
         const int64_t block = pos >> p.block_shift;
-        row = pos - (block << p.block_shift);
+        page_row = pos - (block << p.block_shift);
         bool ok = known && seq >= 0 && seq < p.sequences && block < p.table_blocks;
         if (ok) {
           page = p.page_table[seq * p.page_table_stride + block];
@@ -106,59 +231,32 @@ __global__ void __launch_bounds__(512) rows_kernel(const __grid_constant__ RowsP
         }
         if (!ok) {
           keep = false;
-          if (threadIdx.x == 0 && p.status != nullptr) atomicOr(p.status, kStatusBadInput);
+          if (threadIdx.x == 0 && blockIdx.y == 0 && p.status != nullptr) {
+            atomicOr(p.status, kStatusBadInput);
+          }
         }
       }
     }
-    for (int u = threadIdx.x; u < units; u += blockDim.x) {
-      const int kind = u < q_units ? 0 : u < q_units + k_units ? 1 : 2;
-      const RowStream& s = kind == 0 ? p.query : kind == 1 ? p.key : p.value;
-      const int v = u - (kind == 0 ? 0 : kind == 1 ? q_units : q_units + k_units);
-      const int h = v / per_head, c = v - h * per_head;
-      const bool rotate = c < turned && kind < 2;
-      const int first = rotate && !Interleaved ? c * V : c * 2 * V;
-      const int second = rotate && !Interleaved ? p.rotary / 2 + c * V : c * 2 * V + V;
-      if (Append && kind > 0 && !keep) continue;
-      const T* in = static_cast<const T*>(s.in) + b * s.in_b + t * s.in_t + h * s.in_h;
-      float x[V], y[V];
-      load_pack<T, V>(in + first, x);
-      load_pack<T, V>(in + second, y);
-      if (rotate) {
-        float cs[V], sn[V];
-        load_table<V>(table + c * V, cs);
-        load_table<V>(table + p.rotary / 2 + c * V, sn);
-        if (Interleaved) {
-          if constexpr (V == 1) {
-            turn(x[0], y[0], cs[0], p.sign * sn[0]);
-          } else {
 #pragma unroll
-            for (int i = 0; i < V / 2; ++i) {
-              turn(x[2 * i], x[2 * i + 1], cs[i], p.sign * sn[i]);
-              turn(y[2 * i], y[2 * i + 1], cs[V / 2 + i], p.sign * sn[V / 2 + i]);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) turn(x[i], y[i], cs[i], p.sign * sn[i]);
-        }
-        if (!known) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) x[i] = y[i] = __int_as_float(0x7fc00000);
-        }
-      }
-      if (Append && kind > 0) {
-        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(s.out) + page * s.out_b + row * s.out_t +
-                             h * s.out_h;
-        store_pack<__nv_bfloat16, V>(out + first, x);
-        store_pack<__nv_bfloat16, V>(out + second, y);
+    for (int u = 0; u < kHeads; ++u) {
+      if (kind[u] < 0) continue;
+      if (rotary && (!Append || kind[u] < 2)) turn<Interleaved>(in[u][0], in[u][1], cs, sn);
+      if (Append && kind[u] > 0) {
+        const RowStream& s = kind[u] == 1 ? p.key : p.value;
+        if (!keep) continue;
+        __nv_bfloat16* to = static_cast<__nv_bfloat16*>(s.out) +
+                            (page * s.out_b + page_row * s.out_t) + out_at[u];
+        store_bf16(in[u][0], to);
+        store_bf16(in[u][1], to + gap);
       } else {
         if (Append && pos < 0) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) x[i] = y[i] = 0.f;
+          clear(in[u][0]);
+          clear(in[u][1]);
         }
-        T* out = static_cast<T*>(s.out) + b * s.out_b + t * s.out_t + h * s.out_h;
-        store_pack<T, V>(out + first, x);
-        store_pack<T, V>(out + second, y);
+        const RowStream& s = kind[u] == 0 ? p.query : p.key;
+        T* to = static_cast<T*>(s.out) + (b * s.out_b + t * s.out_t) + out_at[u];
+        in[u][0].store(to);
+        in[u][1].store(to + gap);
       }
     }
   }
@@ -167,11 +265,17 @@ __global__ void __launch_bounds__(512) rows_kernel(const __grid_constant__ RowsP
 template <typename T, int V, bool Interleaved, bool Append>
 cudaError_t launch_rows_t(const RowsParams& p, cudaStream_t stream) {
   const int heads = p.query.heads + p.key.heads + (Append ? p.value.heads : 0);
-  const int units = heads * (p.dim / (2 * V));
-  const int threads = std::min(512, (units + 31) / 32 * 32);
-  const int64_t rows = p.batch * p.tokens;
+  const int per_head = p.dim / (2 * V);
+  // kHeads heads a thread, as many as the CTA holds; the rest in blockIdx.y.
+  const int wanted = std::min(row_threads(V), per_head * ((heads + kHeads - 1) / kHeads));
+  const int threads = (wanted + 31) / 32 * 32;
+  const int each = threads / per_head * kHeads, slices = (heads + each - 1) / each;
+  int sms = 0;
+  if (device_sms(&sms) != RKV_OK) return cudaErrorInvalidDevice;
+  const int64_t resident =
+      std::max<int64_t>(1, static_cast<int64_t>(sms) * std::min(32, 1024 / threads) / slices);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(rows));
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min(p.batch * p.tokens, resident)), slices);
   cfg.blockDim = dim3(threads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -212,7 +316,7 @@ bool aligned_stream(const RowStream& s, int in_width, int out_width, int in_byte
 }
 
 constexpr int64_t kMostTokens = (1LL << 31) - 1;  // the grid's x extent
-constexpr int64_t kMostHeads = 1 << 16;
+constexpr int64_t kMostHeads = 4096;
 
 // The rotation's arguments, shared by the two entry points.
 int check_rotation(const float* cos_sin, int64_t rotary, int64_t dim, int64_t rows,
