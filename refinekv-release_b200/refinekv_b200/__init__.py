@@ -46,26 +46,21 @@ __all__ = [
 ]
 
 
+_HOMES = {
+    "attention": ("AttentionResult", "select_blocks", "sparse_attention", "dense_attention"),
+    "summary": ("BlockSummary", "build_summary", "build_summary_batch", "build_summary_into",
+                "attach_page_pool", "page_view", "PageView"),
+    "rotary": ("rotary_table", "apply_rotary"),
+    "paged": ("paged_append", "paged_attention"),
+    "integrations.transformers": ("RefineKV", "make_visible_static_cache"),
+}
+
+
 def __getattr__(name):
-    if name in ("AttentionResult", "select_blocks", "sparse_attention", "dense_attention"):
-        from . import attention
+    from importlib import import_module
 
-        return getattr(attention, name)
-    if name in ("BlockSummary", "build_summary", "build_summary_batch", "build_summary_into",
-                "attach_page_pool", "page_view", "PageView"):
-        from . import summary
-
-        return getattr(summary, name)
-    if name in ("rotary_table", "apply_rotary"):
-        from . import rotary
-
-        return getattr(rotary, name)
-    if name in ("paged_append", "paged_attention"):
-        from . import paged
-
-        return getattr(paged, name)
-    if name in ("RefineKV", "make_visible_static_cache"):
-        from .integrations import transformers as adapter
-
-        return getattr(adapter, name)
+    for home, names in _HOMES.items():
+        if name in names:
+            value = globals()[name] = getattr(import_module(f".{home}", __name__), name)
+            return value
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -225,7 +225,7 @@ def launch(function, packed: bytes, device: torch.device) -> None:
             raise RuntimeError("librefinekv_b200 is built for sm_100a (B200) only")
         _b200_devices.add(index)
     stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         rc = function(packed, stream)
     else:
         with torch.cuda.device(index):

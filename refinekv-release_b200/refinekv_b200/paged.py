@@ -16,6 +16,8 @@ graph serves growing sequences.  Results carry no gradient.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _native
@@ -26,11 +28,11 @@ from .summary import SUPPORTED_HEAD_DIMS, require_cuda_tensor
 _BLOCKS = (16, 32, 64)
 
 
-def _paged_scratch(lib, workspace, group, dim, device):
-    """``paged_attention``'s zero-filled scratch; its size follows from the head shape alone."""
-    with torch.cuda.device(device):
-        return _scratch(workspace, "rkv_paged_scratch", lib.rkv_paged_workspace_size(group, dim),
-                        device)
+@functools.lru_cache(maxsize=None)
+def _scratch_bytes(index: int, group: int, dim: int) -> int:
+    """``paged_attention``'s workspace size on a device: it follows from the head shape alone."""
+    with torch.cuda.device(index):
+        return _native.load().rkv_paged_workspace_size(group, dim)
 
 
 def _pools(key_pool, value_pool, layout):
@@ -219,12 +221,12 @@ def paged_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: tor
         query = query.clone(memory_format=torch.contiguous_format)
         qs = query.stride()
     lengths = lengths.contiguous()
-    lib = _native.load()
     out = _buffer(workspace, "paged_output", shape, device, dtype)
     lse = _buffer(workspace, "paged_lse", shape[:2], device, torch.float32) if return_lse else None
-    scratch = _paged_scratch(lib, workspace, group, dim, device)
+    scratch = _scratch(workspace, "rkv_paged_scratch", _scratch_bytes(device.index, group, dim),
+                       device)
     _native.launch(
-        lib.rkv_paged_attention,
+        _native.load().rkv_paged_attention,
         _native.PAGED_ARGS.pack(
             query.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
             key_pool.data_ptr(), value_pool.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
