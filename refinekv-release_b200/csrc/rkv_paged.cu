@@ -224,7 +224,9 @@ __device__ __forceinline__ void load_queries(uint32_t (&qb)[D / 16][NT][2], cons
 // one for bf16 queries (rounded, 2^-8 at most, within the output's own
 // rounding), three for fp32 queries, which hold all 24 bits of p.  The further
 // terms may be negative or zero, so they meet V with its infinities clamped:
-// an infinite value times p is infinite, whatever p's bits are.
+// an infinite value times p is infinite, whatever p's bits are.  And a tile's
+// products are summed apart and added to o by a rounded addition: the tensor
+// cores cut their sums off, which over a long row would cost fp32 digits.
 template <int R, int D, int NT, int Terms>
 __device__ __forceinline__ void weigh_values(uint32_t tile, float (&p)[R / 16][NT][4],
                                              float (&o)[D / 16][NT][4], int lane) {
@@ -248,12 +250,16 @@ __device__ __forceinline__ void weigh_values(uint32_t tile, float (&p)[R / 16][N
   const int cadd = (lane >> 3) & 1;
 #pragma unroll
   for (int dt = 0; dt < D / 16; ++dt) {
+    float sum[NT][4];  // of the tile
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) sum[nt][0] = sum[nt][1] = sum[nt][2] = sum[nt][3] = 0.f;
+    float(&to)[NT][4] = Terms > 1 ? sum : o[dt];
 #pragma unroll
     for (int kt = 0; kt < R / 16; ++kt) {
       uint32_t a[4];
       ldsm_x4_trans(tile + swz(kt * 16 + trow, dt * 2 + cadd, R), a);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mma_bf16(o[dt][nt], a, frag[0][kt][nt][0], frag[0][kt][nt][1]);
+      for (int nt = 0; nt < NT; ++nt) mma_bf16(to[nt], a, frag[0][kt][nt][0], frag[0][kt][nt][1]);
       if constexpr (Terms > 1) {
         const __nv_bfloat162 most = __halves2bfloat162(__ushort_as_bfloat16(0x7f7f),
                                                        __ushort_as_bfloat16(0x7f7f));
@@ -266,8 +272,14 @@ __device__ __forceinline__ void weigh_values(uint32_t tile, float (&p)[R / 16][N
         for (int term = 1; term < Terms; ++term)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
-            mma_bf16(o[dt][nt], a, frag[term][kt][nt][0], frag[term][kt][nt][1]);
+            mma_bf16(to[nt], a, frag[term][kt][nt][0], frag[term][kt][nt][1]);
       }
+    }
+    if constexpr (Terms > 1) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[dt][nt][c] += sum[nt][c];
     }
   }
 }
