@@ -45,8 +45,6 @@ constexpr int stage_bytes(int D) { return 2 * tile_rows(D) * D * 2; }
 
 // A row's CTAs are joined in one level up to this many, else in groups.
 constexpr int kFlatJoin = 32;
-// A row shorter than this many tiles a CTA is not spread over more CTAs.
-constexpr unsigned kPartTiles = 32;
 
 // Workspace: status word, counters (at the same place for every geometry;
 // they are zero between calls), then the partials.
@@ -414,15 +412,18 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
       for (int i = threadIdx.x; i < queries; i += blockDim.x) p.lse[row + i] = -INFINITY;
     }
   }
-  // How many CTAs share the tiles.  Few rows: whole CTAs per row where that
-  // leaves few SMs idle, since a CTA of one row has one join less; no more of
-  // them than the rows' lengths are worth.  Many rows: every SM, but a tile a
-  // warp at least.
+  // How many CTAs share the tiles.  Many rows: every SM, but a tile a warp at
+  // least.  Few rows: whole CTAs per row where that leaves few SMs idle, since a
+  // CTA with one row has one join less (three D 256 sequences 43.3 against 47.3
+  // us, two of 60K tokens 79.5 against 80.5, one of 128K 88.0 against 87.3), and
+  // no more of them than give every warp a tile (2K tokens, 8 heads: 10.3 us,
+  // with four tiles a warp 14.1), one for a row of up to two tiles a warp (333
+  // tokens: 8.3 us, with a tile a warp and the join across CTAs 9.8).
   const unsigned rows = static_cast<unsigned>(busy) * p.heads, grid = gridDim.x;
   unsigned C = min(grid, (T + W - 1) / W);
   if (rows > 0 && rows <= grid) {
-    const unsigned fit = grid / rows, worth = (T / rows + kPartTiles - 1) / kPartTiles;
-    if (worth < fit) C = rows * max(1u, worth);
+    const unsigned fit = grid / rows, worth = T <= 2 * W * rows ? 1 : (T / rows + W - 1) / W;
+    if (worth < fit) C = rows * worth;
     else if (fit * rows * 16 >= grid * 15) C = fit * rows;
     C = min(C, T);
   }

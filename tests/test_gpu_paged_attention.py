@@ -116,6 +116,10 @@ CASES = [
     ([65], 10, 2, 224, 64, "HND", None),
     ([20000, 3], 8, 1, 128, 32, "HND", None),
     ([1 + 7 * (i % 41) for i in range(300)], 8, 2, 64, 16, "HND", None),
+    # rows over so many CTAs that their parts are joined in groups
+    ([70000, 3], 8, 1, 128, 32, "HND", None),
+    ([150000], 16, 1, 64, 16, "NHD", None),
+    ([66000, 68000], 4, 1, 256, 64, "HND", None),
     ([1000, 5, 64, 0, 33], 32, 8, 128, 32, "HND", 1),
     ([1000, 5, 64, 0, 33, 130], 28, 4, 128, 16, "NHD", 20),
     ([1000, 555, 64, 63], 8, 8, 64, 64, "HND", 64),
