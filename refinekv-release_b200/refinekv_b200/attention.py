@@ -64,7 +64,7 @@ def _buffer(workspace, name, shape, device, dtype, zero=False):
     """Reuse a workspace tensor keyed by name/shape/dtype/device, like ``runtime.py:26-37``."""
     tensor = workspace.get(name) if workspace is not None else None
     if (tensor is None or tensor.dtype != dtype or tensor.device != device
-            or tensor.shape != torch.Size(shape)):
+            or tensor.shape != shape):
         tensor = (torch.zeros if zero else torch.empty)(shape, device=device, dtype=dtype)
         if workspace is not None:
             workspace[name] = tensor

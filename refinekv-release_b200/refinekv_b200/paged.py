@@ -22,7 +22,7 @@ import torch
 
 from . import _native
 from .attention import MAX_GROUP, _buffer, _scratch
-from .rotary import _DTYPES, check_table
+from .rotary import _DTYPES, _POSITIONS, check_table
 from .summary import SUPPORTED_HEAD_DIMS, require_cuda_tensor
 
 _BLOCKS = (16, 32, 64)
@@ -42,8 +42,9 @@ def _pools(key_pool, value_pool, layout):
     shape = key_pool.shape
     if len(shape) != 4 or value_pool.shape != shape:
         raise ValueError("key and value pools must have the same 4-D shape")
-    require_cuda_tensor(key_pool, "key_pool")
-    if key_pool.dtype != torch.bfloat16 or value_pool.dtype != torch.bfloat16:
+    if not key_pool.is_cuda:
+        require_cuda_tensor(key_pool, "key_pool")
+    if key_pool.dtype is not torch.bfloat16 or value_pool.dtype is not torch.bfloat16:
         raise TypeError("page pools must be bf16")
     if value_pool.device != key_pool.device:
         raise ValueError("key and value pools must be on the same device")
@@ -116,7 +117,7 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Tensor,
     tokens = shape[0]
     if positions.shape != (tokens,) or positions.device != device:
         raise ValueError("positions must be (tokens,) on the pools' device")
-    if positions.dtype not in (torch.int32, torch.int64):
+    if positions.dtype not in _POSITIONS:
         raise TypeError("positions must be int32 or int64")
     if sequence_ids is None:
         if tokens > sequences:
@@ -127,32 +128,40 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Tensor,
             raise ValueError("sequence_ids must be (tokens,) on the pools' device")
         if sequence_ids.dtype != torch.int32:
             raise TypeError("sequence_ids must be int32")
-        sequence_ids = sequence_ids.contiguous()
+        if not sequence_ids.is_contiguous():
+            sequence_ids = sequence_ids.contiguous()
         ids = sequence_ids.data_ptr()
     table = rotary = rows = row_stride = 0
     if cos_sin is not None:
         check_table(cos_sin, dim, device)
         table, rotary = cos_sin.data_ptr(), cos_sin.shape[1]
         rows, row_stride = cos_sin.shape[0], cos_sin.stride(0)
-    if key.stride(2) != 1:
+    key_strides, value_strides = key.stride(), value.stride()
+    if key_strides[2] != 1:
         key = key.contiguous()
-    if value.stride(2) != 1:
+        key_strides = key.stride()
+    if value_strides[2] != 1:
         value = value.contiguous()
-    positions = positions.contiguous()
+        value_strides = value.stride()
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
     out = None
     query_ptr = out_ptr = query_heads = 0
     query_strides = out_strides = (0, 0)
     if query is not None:
-        if (query.ndim != 3 or query.shape[0] != tokens or query.shape[2] != dim
-                or query.device != device):
+        like = query.shape
+        if len(like) != 3 or like[0] != tokens or like[2] != dim or query.device != device:
             raise ValueError("query must be (tokens, q_heads, head_dim) on the pools' device")
         if query.dtype != dtype:
             raise TypeError("query must have the keys' dtype")
-        if query.stride(2) != 1:
+        query_strides = query.stride()
+        if query_strides[2] != 1:
             query = query.contiguous()
-        out = _buffer(workspace, "append_query", query.shape, device, dtype)
-        query_ptr, out_ptr, query_heads = query.data_ptr(), out.data_ptr(), query.shape[1]
-        query_strides, out_strides = query.stride()[:2], out.stride()[:2]
+            query_strides = query.stride()
+        query_strides = query_strides[:2]
+        out = _buffer(workspace, "append_query", like, device, dtype)
+        query_ptr, out_ptr, query_heads = query.data_ptr(), out.data_ptr(), like[1]
+        out_strides = (query_heads * dim, dim)
     status = 0
     if workspace is not None:
         status = _buffer(workspace, "rkv_append_status", (64,), device, torch.int32,
@@ -162,9 +171,10 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Tensor,
         _native.APPEND_ARGS.pack(
             key.data_ptr(), value.data_ptr(), query_ptr, out_ptr, key_pool.data_ptr(),
             value_pool.data_ptr(), page_table.data_ptr(), ids, positions.data_ptr(), table, status,
-            *key.stride()[:2], *value.stride()[:2], *query_strides, *out_strides, *ks, *vs,
+            key_strides[0], key_strides[1], value_strides[0], value_strides[1], *query_strides,
+            *out_strides, *ks, *vs,
             table_stride, sequences, blocks, pages, block, tokens, query_heads, heads, dim, rotary,
-            rows, row_stride, _DTYPES[dtype], positions.dtype == torch.int64, interleaved),
+            rows, row_stride, _DTYPES[dtype], positions.dtype is torch.int64, interleaved),
         device)
     return out
 
@@ -220,7 +230,8 @@ def paged_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: tor
     if qs[2] != 1 or (query.data_ptr() | qs[0] * width | qs[1] * width) & 15:
         query = query.clone(memory_format=torch.contiguous_format)
         qs = query.stride()
-    lengths = lengths.contiguous()
+    if not lengths.is_contiguous():
+        lengths = lengths.contiguous()
     out = _buffer(workspace, "paged_output", shape, device, dtype)
     lse = _buffer(workspace, "paged_lse", shape[:2], device, torch.float32) if return_lse else None
     scratch = _scratch(workspace, "rkv_paged_scratch", _scratch_bytes(device.index, group, dim),

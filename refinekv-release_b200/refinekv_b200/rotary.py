@@ -16,6 +16,7 @@ import torch
 from . import _native
 from .summary import require_cuda_tensor
 
+_POSITIONS = (torch.int32, torch.int64)
 _DTYPES = {torch.bfloat16: _native.DTYPE_BF16, torch.float32: _native.DTYPE_F32}
 
 
@@ -103,23 +104,19 @@ def rotary_table(rotary_dim: int, positions: int, *, base: float = 10000.0,
 
 def check_table(cos_sin: torch.Tensor, dim: int, device: torch.device) -> None:
     """The argument checks of a cos/sin table shared with ``paged_append``."""
-    if cos_sin.ndim != 2 or cos_sin.stride(1) != 1 or cos_sin.shape[0] < 1:
+    shape = cos_sin.shape
+    if len(shape) != 2 or cos_sin.stride(1) != 1 or shape[0] < 1:
         raise ValueError("cos_sin must be a (positions, rotary_dim) table with contiguous rows")
-    if cos_sin.dtype != torch.float32:
+    if cos_sin.dtype is not torch.float32:
         raise TypeError("cos_sin must be fp32")
     if cos_sin.device != device:
         raise ValueError("cos_sin must be on the rows' device")
-    rotary = cos_sin.shape[1]
+    rotary = shape[1]
     if rotary < 2 or rotary % 2 or rotary > dim:
         raise ValueError("rotary_dim (cos_sin's width) must be even and at most head_dim")
 
 
-def _rows(tensor: torch.Tensor, what: str, in_place: bool) -> torch.Tensor:
-    if tensor.stride(-1) == 1:
-        return tensor
-    if in_place:
-        raise ValueError(f"{what} must be contiguous in head_dim to be rotated in place")
-    return tensor.contiguous()
+_NO_STRIDES = (0, 0, 0)
 
 
 def _strides(tensor: torch.Tensor) -> tuple:
@@ -128,31 +125,43 @@ def _strides(tensor: torch.Tensor) -> tuple:
     return stride[:3] if len(stride) == 4 else (0, stride[0], stride[1])
 
 
-_NO_STRIDES = (0, 0, 0)
-
-
 def _launch(query, key, positions, cos_sin, interleaved, inverse, in_place):
-    query = _rows(query, "query", in_place)
-    query_out = query if in_place else torch.empty_like(query)
-    key_out = None
-    key_ptr = key_out_ptr = key_heads = 0
+    if query.stride(-1) != 1:
+        if in_place:
+            raise ValueError("query must be contiguous in head_dim to be rotated in place")
+        query = query.contiguous()
+    strides = out_strides = _strides(query)
+    query_out = query
+    if not in_place:
+        query_out = torch.empty_like(query)
+        out_strides = _strides(query_out)
+    key_out, key_ptr, key_out_ptr, key_heads = None, 0, 0, 0
     key_strides = key_out_strides = _NO_STRIDES
     if key is not None:
-        key = _rows(key, "key", in_place)
-        key_out = key if in_place else torch.empty_like(key)
-        key_ptr, key_out_ptr, key_heads = key.data_ptr(), key_out.data_ptr(), key.shape[-2]
-        key_strides, key_out_strides = _strides(key), _strides(key_out)
-    shape = query.shape
+        if key.stride(-1) != 1:
+            if in_place:
+                raise ValueError("key must be contiguous in head_dim to be rotated in place")
+            key = key.contiguous()
+        key_strides = key_out_strides = _strides(key)
+        key_out, key_ptr = key, key.data_ptr()
+        key_out_ptr, key_heads = key_ptr, key.shape[-2]
+        if not in_place:
+            key_out = torch.empty_like(key)
+            key_out_ptr, key_out_strides = key_out.data_ptr(), _strides(key_out)
+    batch, (tokens, heads, dim) = 1, query.shape[-3:]
     at = positions.stride()
+    if len(at) == 2:
+        batch = query.shape[0]
+    else:
+        at = (0, at[0])
+    rows, rotary = cos_sin.shape
     _native.launch(
         _native.load().rkv_rotary,
         _native.ROTARY_ARGS.pack(
             query.data_ptr(), key_ptr, query_out.data_ptr(), key_out_ptr, positions.data_ptr(),
-            cos_sin.data_ptr(), *_strides(query), *key_strides, *_strides(query_out),
-            *key_out_strides, *(at if len(at) == 2 else (0, at[0])),
-            positions.dtype == torch.int64, cos_sin.shape[0], cos_sin.stride(0),
-            shape[0] if len(shape) == 4 else 1, shape[-3], shape[-2], key_heads, shape[-1],
-            cos_sin.shape[1], _DTYPES[query.dtype], interleaved, inverse),
+            cos_sin.data_ptr(), *strides, *key_strides, *out_strides, *key_out_strides, *at,
+            positions.dtype is torch.int64, rows, cos_sin.stride(0), batch, tokens, heads,
+            key_heads, dim, rotary, _DTYPES[query.dtype], interleaved, inverse),
         query.device)
     return query_out, key_out
 
@@ -197,25 +206,27 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch
     ``in_place`` (rows must then not overlap).  Differentiable in query and
     key; the backward pass is one launch of the inverse rotation.
     """
-    shape = query.shape
-    if query.ndim not in (3, 4):
+    shape, dtype, device = query.shape, query.dtype, query.device
+    lead, dim = shape[:-2], shape[-1]
+    if len(shape) not in (3, 4):
         raise ValueError("query must have shape ([batch,] tokens, heads, head_dim)")
-    require_cuda_tensor(query, "query")
-    if query.dtype not in _DTYPES:
+    if not query.is_cuda:
+        require_cuda_tensor(query, "query")
+    if dtype not in _DTYPES:
         raise TypeError("apply_rotary takes BF16 or FP32 queries and keys")
-    if shape[-1] % 2 or not 2 <= shape[-1] <= 1024:
+    if dim % 2 or not 2 <= dim <= 1024:
         raise ValueError("head_dim must be even and at most 1024")
     if key is not None:
-        if (key.ndim != query.ndim or key.shape[:-2] != shape[:-2] or key.shape[-1] != shape[-1]
-                or key.device != query.device):
+        other = key.shape
+        if other[:-2] != lead or other[-1] != dim or key.device != device:
             raise ValueError("key must match the query but for its heads")
-        if key.dtype != query.dtype:
+        if key.dtype != dtype:
             raise TypeError("query and key must have the same dtype")
-    if positions.shape != shape[:-2] or positions.device != query.device:
+    if positions.shape != lead or positions.device != device:
         raise ValueError("positions must be ([batch,] tokens) on the query's device")
-    if positions.dtype not in (torch.int32, torch.int64):
+    if positions.dtype not in _POSITIONS:
         raise TypeError("positions must be int32 or int64")
-    check_table(cos_sin, shape[-1], query.device)
+    check_table(cos_sin, dim, device)
     if torch.is_grad_enabled() and (query.requires_grad
                                     or (key is not None and key.requires_grad)):
         if in_place:
