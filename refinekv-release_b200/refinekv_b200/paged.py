@@ -186,7 +186,7 @@ def paged_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: tor
     """Exact attention of one new token per sequence over its own length of the pool.
 
     ``query``: (sequences, q_heads, head_dim) bf16 or fp32, any strides; query
-    head r reads KV head r // (q_heads // kv_heads), at most 16 to a KV head.
+    head r reads KV head r // (q_heads // kv_heads), at most 16 to a KV head; at most 4096 sequences.
     ``lengths``: (sequences,) int32, the tokens of each sequence now in the
     pool (the new one included, once ``paged_append`` has written it); a
     sequence of length 0 (an idle slot) gives a zero row.  ``scale`` defaults

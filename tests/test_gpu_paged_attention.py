@@ -324,6 +324,29 @@ def test_other_stream_after_an_append():
     assert device_status(ws) == 0
 
 
+@pytest.mark.parametrize("dim,hq,hk", [(192, 16, 1), (128, 2, 2)])
+def test_as_many_sequences_as_the_kernel_takes(dim, hq, hk):
+    lengths = [(7 * i) % 5 for i in range(4095)] + [900]
+    s = Served(lengths, hq, hk, dim, 16, seed=dim)
+    out, lse = s.call()
+    some = [0, 1, 2, 3, 4, 2047, 4094, 4095]
+    for i in some:
+        one = paged_attention(s.q[i:i + 1], s.kp, s.vp, s.table[i:i + 1], s.n[i:i + 1],
+                              return_lse=True)
+        part = Served.__new__(Served)
+        part.__dict__.update(s.__dict__)
+        part.keys, part.values, part.q = s.keys[i:i + 1], s.values[i:i + 1], s.q[i:i + 1]
+        part.check(*one)
+        part.check(out[i:i + 1], lse[i:i + 1])
+    empty = s.n == 0
+    assert not bool(out[empty].any()) and bool((lse[empty] == -math.inf).all())
+    assert bool(out[~empty].isfinite().all())
+    more = torch.zeros(1, dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError, match="4096 sequences"):
+        paged_attention(torch.cat([s.q, s.q[:1]]), s.kp, s.vp, torch.cat([s.table, s.table[:1]]),
+                        torch.cat([s.n, more]))
+
+
 def test_no_sequences():
     s = Served([5], 4, 2, 64, 16)
     out, lse = paged_attention(s.q[:0], s.kp, s.vp, s.table[:0], s.n[:0], return_lse=True)

@@ -208,7 +208,7 @@ def _attend(lib, **change):
     (dict(group=0), _native.RKV_ERR_UNSUPPORTED),
     (dict(head_dim=288), _native.RKV_ERR_UNSUPPORTED),
     (dict(block_size=8), _native.RKV_ERR_UNSUPPORTED),
-    (dict(sequences=8193), _native.RKV_ERR_UNSUPPORTED),
+    (dict(sequences=4097), _native.RKV_ERR_UNSUPPORTED),
     (dict(workspace=0), _native.RKV_ERR_WORKSPACE),
     (dict(workspace_size=16), _native.RKV_ERR_WORKSPACE),
     (dict(query=24), _native.RKV_ERR_ALIGNMENT),
