@@ -5,10 +5,17 @@
 // tokens keeps (m, l, o) per query, and partial results over parts of the
 // tokens join exactly as l = sum l_i e^(m_i - m), o = sum o_i e^(m_i - m).
 //
-// Bound: HBM.  Each visible K and V row is read once (4 D bytes for 4 G D
-// flop, G <= 16).  mma.sync with the tokens on M and the group on N leaves
-// the tensor pipe nearly idle at the streaming rate, so tcgen05 (M = 64 at
-// least, operands from shared memory descriptors) would not move the bound.
+// Bound: HBM on long sequences.  Each visible K and V row is read once (4 D
+// bytes for 4 G D flop, G <= 16).  mma.sync with the tokens on M and the group
+// on N keeps the tensor pipe 10 % active at the streaming rate, so tcgen05
+// (M = 64 at least, operands from shared-memory descriptors) would not move
+// the bound.  Measured on B200 (graph replay): 16 sequences of 32K tokens, 8 KV
+// heads, D 128: 324 us for 2.15 GB, 6.6 TB/s, what a plain copy reaches; one of
+// 128K: 88 us for 537 MB (6.1 TB/s; the SMs that stream slowest, about a fifth
+// of them, end 10 us after the mean, and equal shares cannot follow that); a
+// ragged batch of 43, 270 MB: 52 us.  About 5 us before the stream is up and 6
+// for the joins at its end are what short calls consist of: one sequence of
+// 333 tokens takes 8.3 us.
 //
 // Split.  The tiles of all rows, sequence-major then head, form one list that
 // is cut into equal contiguous ranges, one per CTA, and each CTA's range into
@@ -39,7 +46,10 @@ namespace {
 // Tokens per tile: 64 for head dims up to 64, else 32, so that a K and V tile
 // is 16 KB at D 64 and 128.
 constexpr int tile_rows(int D) { return D <= 64 ? 64 : 32; }
-// One stage (a K and a V tile) per warp, up to eight warps.
+// One stage (a K and a V tile) per warp, up to eight warps.  Six warps take 86 us
+// for one sequence of 128K tokens against 88, but 47.6 against 46.5 for a
+// ragged batch of 32 and 26 against 24 at D 64; two CTAs of four warps per SM
+// cost 2 to 4 us on every batch (more parts to join).
 constexpr int paged_warps(int D) { return D <= 192 ? 8 : 6; }
 constexpr int stage_bytes(int D) { return 2 * tile_rows(D) * D * 2; }
 
@@ -379,6 +389,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
         atomicOr(p.status, kStatusBadInput);
       }
       const int tiles = tiles_of<R>(p, s);
+      start[s] = tiles;
       sum += tiles;
       some += tiles > 0;
     }
@@ -395,8 +406,9 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
     some = __reduce_add_sync(0xffffffffu, some);
     if (lane == 0 && some > 0) atomicAdd(&busy, some);
     for (int s = s0; s < s1; ++s) {
+      const int tiles = start[s];
       start[s] = before;
-      before += tiles_of<R>(p, s);
+      before += tiles;
     }
     if (s1 == p.sequences && s0 < s1) start[p.sequences] = before;
     __syncthreads();

@@ -4,13 +4,22 @@
 // rotary channels by the position's row of the cos/sin table, write it to a
 // tensor or to the pool's page.  Bound: HBM on long inputs (every element
 // read once and written once, a few flops per pair), latency on single
-// tokens.
+// tokens.  Measured on B200 (graph replay): 8192 tokens of 40 bf16 heads, D
+// 128: 30 us, 172 MB, 0.88 of the measured copy rate; 24.5K prompt tokens into the
+// pool, 48 heads each: 114 us, 653 MB, 0.87; one token: 2.1 us (2.5 appended).
+//
+// What it took: CTAs that stay and take token after token (one CTA a token
+// launched too slowly: 45 us for the 8192), the pieces of a row kept as they
+// lie in memory and turned in place (as arrays of floats they went to local
+// memory: 44 us), two pairs per arithmetic instruction, two heads in flight per
+// thread (one: 35 us, three: 33), 1024 resident threads an SM (768: 34 us).
 //
 // A unit of work is 2V channels of one head: for a rotated half-layout unit
 // the V channels at c and the V at c + rotary/2 (the two halves of V pairs),
 // for an interleaved or copied one 2V consecutive channels.  V is 16 bytes of
 // elements, or 1 where strides, alignment or a rotary width that is no
-// multiple of 2V forbid 16-byte accesses.
+// multiple of 2V forbid 16-byte accesses (the 8192 tokens
+// then take 111 us).
 #include <algorithm>
 #include <string>
 
