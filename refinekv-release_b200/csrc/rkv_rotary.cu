@@ -5,21 +5,21 @@
 // tensor or to the pool's page.  Bound: HBM on long inputs (every element
 // read once and written once, a few flops per pair), latency on single
 // tokens.  Measured on B200 (graph replay): 8192 tokens of 40 bf16 heads, D
-// 128: 30 us, 172 MB, 0.88 of the measured copy rate; 24.5K prompt tokens into the
-// pool, 48 heads each: 114 us, 653 MB, 0.87; one token: 2.1 us (2.5 appended).
+// 128: 30 us, 172 MB, 0.88 of the measured copy rate; 24.5K prompt tokens into
+// the pool, 48 heads each: 117 us, 653 MB, 0.85; one token: 2.1 us (eight
+// appended: 2.5).
 //
 // What it took: CTAs that stay and take token after token (one CTA a token
 // launched too slowly: 45 us for the 8192), the pieces of a row kept as they
 // lie in memory and turned in place (as arrays of floats they went to local
-// memory: 44 us), two pairs per arithmetic instruction, two heads in flight per
-// thread (one: 35 us, three: 33), 1024 resident threads an SM (768: 34 us).
+// memory: 44 us), two heads in flight per thread (one: 35 us, three: 33), 1024
+// resident threads an SM (768: 34 us).
 //
 // A unit of work is 2V channels of one head: for a rotated half-layout unit
 // the V channels at c and the V at c + rotary/2 (the two halves of V pairs),
 // for an interleaved or copied one 2V consecutive channels.  V is 16 bytes of
 // elements, or 1 where strides, alignment or a rotary width that is no
-// multiple of 2V forbid 16-byte accesses (the 8192 tokens
-// then take 111 us).
+// multiple of 2V forbid 16-byte accesses (the 8192 tokens then take 111 us).
 #include <algorithm>
 #include <string>
 
@@ -95,14 +95,21 @@ __device__ __forceinline__ void load_table(const float* from, float (&x)[V]) {
   }
 }
 
-// Two pairs (a, b) turned.  Products and sums are rounded one by one (no fused
+// One pair (a, b) turned.  Products and sums are rounded one by one (no fused
 // multiply-add): the result then depends on nothing but its operands, so
 // rotating alone, rotating while appending and the formula in fp32 agree bit
-// for bit.
-__device__ __forceinline__ void turn2(float2& a, float2& b, float2 c, float2 s) {
-  const float2 y = __fadd2_rn(__fmul2_rn(a, c), __fmul2_rn(b, make_float2(-s.x, -s.y)));
-  b = __fadd2_rn(__fmul2_rn(b, c), __fmul2_rn(a, s));
+// for bit.  (The two-wide fp32 instructions would halve the arithmetic, but
+// their products and sums are fused by the assembler.)
+__device__ __forceinline__ void turn1(float& a, float& b, float c, float s) {
+  const float y = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
+  b = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
   a = y;
+}
+
+// Two pairs.
+__device__ __forceinline__ void turn2(float2& a, float2& b, float2 c, float2 s) {
+  turn1(a.x, b.x, c.x, s.x);
+  turn1(a.y, b.y, c.y, s.y);
 }
 
 // The V pairs of a unit's two pieces turned: (p_i, q_i), or interleaved the
@@ -151,10 +158,10 @@ __device__ __forceinline__ void turn(Piece<float, 4>& p, Piece<float, 4>& q, con
 template <bool Interleaved, typename T>
 __device__ __forceinline__ void turn(Piece<T, 1>& p, Piece<T, 1>& q, const float (&c)[1],
                                      const float (&s)[1]) {
-  float2 a = make_float2(widen(p.one), 0.f), b = make_float2(widen(q.one), 0.f);
-  turn2(a, b, make_float2(c[0], 0.f), make_float2(s[0], 0.f));
-  narrow(p.one, a.x);
-  narrow(q.one, b.x);
+  float a = widen(p.one), b = widen(q.one);
+  turn1(a, b, c[0], s[0]);
+  narrow(p.one, a);
+  narrow(q.one, b);
 }
 
 // A CTA takes the heads of one blockIdx.y and every gridDim.x-th token; the

@@ -82,6 +82,30 @@ def test_rotation_matches_the_formula(lead, hq, hk, dim, rotary, dtype, interlea
     assert torch.equal(mine, got_q) and (k is None or torch.equal(mine_k, got_k))
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype,rotary", [(torch.bfloat16, 96), (torch.bfloat16, 20),
+                                          (torch.float32, 96), (torch.float32, 20)])
+def test_rotation_has_the_bits_of_the_fp32_formula(dtype, rotary, interleaved):
+    """Each product and sum is rounded by itself: the elementwise formula, bit for bit."""
+    gen = torch.Generator(device=DEV).manual_seed(rotary)
+    table = rotary_table(rotary, 5000, scaling={"type": "yarn", "factor": 4.0,
+                                                "original_max_position_embeddings": 1024})
+    q = _normal(gen, 200, 6, 128, dtype=dtype)
+    at = torch.randint(0, 5000, (200,), generator=gen, device=DEV)
+    row = table[at][:, None]
+    c, s = row[..., : rotary // 2], row[..., rotary // 2:]
+    x = q.float()
+    first = slice(0, rotary, 2) if interleaved else slice(0, rotary // 2)
+    second = slice(1, rotary, 2) if interleaved else slice(rotary // 2, rotary)
+    for sign in (1.0, -1.0):
+        want = x.clone()
+        a, b = x[..., first], x[..., second]
+        want[..., first] = a * c - b * (s * sign)
+        want[..., second] = b * c + a * (s * sign)
+        got, _ = apply_rotary(q, None, at, table, interleaved=interleaved, inverse=sign < 0)
+        assert torch.equal(got, want.to(dtype))
+
+
 def test_strides_of_models_and_servers():
     gen = torch.Generator(device=DEV).manual_seed(1)
     table = rotary_table(64, 500)
@@ -172,7 +196,7 @@ def test_gradient_is_the_inverse_rotation(interleaved, dtype):
     amplitude = float((table[0, 0]).double()) ** 2
     scale = torch.ones(64, device=DEV, dtype=torch.float64)
     scale[:48] = amplitude
-    assert float((first.double() - 2 * scale * only.double()).abs().max()) <= 1e-4
+    assert float((first.detach().double() - 2 * scale * only.detach().double()).abs().max()) <= 1e-4
     assert float((second.double() - 2 * scale).abs().max()) <= 1e-4
 
 
