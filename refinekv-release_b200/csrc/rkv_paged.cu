@@ -10,12 +10,12 @@
 // on N keeps the tensor pipe 10 % active at the streaming rate, so tcgen05
 // (M = 64 at least, operands from shared-memory descriptors) would not move
 // the bound.  Measured on B200 (graph replay): 16 sequences of 32K tokens, 8 KV
-// heads, D 128: 324 us for 2.15 GB, 6.6 TB/s, what a plain copy reaches; one of
-// 128K: 88 us for 537 MB (6.1 TB/s; the SMs that stream slowest, about a fifth
-// of them, end 10 us after the mean, and equal shares cannot follow that); a
-// ragged batch of 43, 270 MB: 52 us.  About 5 us before the stream is up and 6
-// for the joins at its end are what short calls consist of: one sequence of
-// 333 tokens takes 8.3 us.
+// heads, D 128: 317-324 us for 2.15 GB, 6.7 TB/s, more than a plain copy reaches;
+// one of 128K: 86 us for 537 MB (6.2 TB/s; the SMs that stream slowest, about a
+// fifth of them, end 10 us after the mean, and equal shares cannot follow that);
+// a ragged batch of 43, 270 MB: 51 us.  About 5 us before the stream is up and 4
+// to 6 for the joins at its end are what short calls consist of: one sequence of
+// 333 tokens takes 7.8 us.
 //
 // Split.  The tiles of all rows, sequence-major then head, form one list that
 // is cut into equal contiguous ranges, one per CTA, and each CTA's range into
@@ -316,28 +316,87 @@ __device__ __forceinline__ void fma4(float4& acc, float w, const float4& x) {
 
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
 
-// Four joined channels of query g of a row: finished, or into the partial `to`.
-template <int D, int G8>
-__device__ __forceinline__ void put_joined(const PagedParams& p, int row, int g, int d, float* to,
-                                           float inverse, const float4& o) {
-  if (to != nullptr) {
-    *reinterpret_cast<float4*>(to + 2 * G8 + g * D + d) = o;
-  } else if (d < p.dim) {
-    const int64_t at = static_cast<int64_t>(row) * p.group + g;
-    put4(p, at * p.dim + d,
-         make_float4(o.x * inverse, o.y * inverse, o.z * inverse, o.w * inverse));
+// Joins the parts k of the bit set `members` for one query: m_of(k) and l_of(k)
+// give part k's m and l, o_of(k, d) its channels d .. d + 3, and put(d, m, l, o)
+// takes the joined ones of d = 4 lane, 4 (lane + kLanes), ...  Every load of
+// kBatch parts is in flight at once.  Each thread finds the weights for
+// itself: an exponential a part instead of a barrier for the CTA.  The batches
+// are short because this code runs once and cold: twenty parts unrolled cost a
+// batch of two or three 0.8 us.
+template <int D, int kLanes, int kBatch, typename M, typename L, typename O, typename Put>
+__device__ __forceinline__ void join(unsigned members, int lane, M m_of, L l_of, O o_of, Put put) {
+  constexpr int kCols = (D / 4 + kLanes - 1) / kLanes;
+  float top = -INFINITY, sum = 0.f;
+  float4 acc[kCols];
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int base = 0; base < 32; base += kBatch) {
+    const unsigned set = members >> base;
+    if (set == 0) break;
+    float m[kBatch], l[kBatch];
+    float4 o[kCols][kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      m[u] = -INFINITY;
+      if (set >> u & 1) {
+        m[u] = m_of(base + u);
+        l[u] = l_of(base + u);
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+          const int d = 4 * (lane + c * kLanes);
+          if (d < D) o[c][u] = o_of(base + u, d);
+        }
+      }
+    }
+    float next = top;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) next = fmaxf(next, m[u]);
+    const float ref = finite_or_zero(next);
+    if (base > 0) {
+      const float keep = __expf(top - ref);
+      sum *= keep;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) {
+        acc[c] = make_float4(acc[c].x * keep, acc[c].y * keep, acc[c].z * keep, acc[c].w * keep);
+      }
+    }
+    top = next;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (set >> u & 1) {
+        const float w = __expf(m[u] - ref);
+        sum += w * l[u];
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+          if (4 * (lane + c * kLanes) < D) fma4(acc[c], w, o[c][u]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) {
+    const int d = 4 * (lane + c * kLanes);
+    if (d < D) put(d, top, sum, acc[c]);
   }
 }
 
-// The m and l of query g of a joined row: into the partial, or the row's lse.
-template <int G8>
-__device__ __forceinline__ void put_sums(const PagedParams& p, int row, int g, float* to, float m,
-                                         float l) {
+// Four joined channels of query g of a row and, with the first of them, its m
+// and l: finished, or into the partial `to`.
+template <int D, int G8>
+__device__ __forceinline__ void put_joined(const PagedParams& p, int row, int g, int d, float* to,
+                                           float m, float l, const float4& o) {
   if (to != nullptr) {
-    to[g] = m;
-    to[G8 + g] = l;
-  } else if (p.lse != nullptr) {
-    p.lse[static_cast<int64_t>(row) * p.group + g] = finite_or_zero(m) + logf(l);
+    *reinterpret_cast<float4*>(to + 2 * G8 + g * D + d) = o;
+    if (d == 0) {
+      to[g] = m;
+      to[G8 + g] = l;
+    }
+  } else if (d < p.dim) {
+    const int64_t at = static_cast<int64_t>(row) * p.group + g;
+    const float inverse = 1.f / l;
+    put4(p, at * p.dim + d,
+         make_float4(o.x * inverse, o.y * inverse, o.z * inverse, o.w * inverse));
+    if (d == 0 && p.lse != nullptr) p.lse[at] = finite_or_zero(m) + logf(l);
   }
 }
 
@@ -355,10 +414,6 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   // query's m and l.
   __shared__ int seg_row[2 * W];
   __shared__ float seg_m[2 * W][G8], seg_l[2 * W][G8];
-  // Joins: the rows of the CTA's partials, first and last partial of each, and
-  // the parts' weights and the rows' inverse sums.
-  __shared__ int join_rows, join_first[2 * W], join_last[2 * W];
-  __shared__ float weight[2 * kFlatJoin][G8], inverse[2 * W][G8];
   __shared__ Cut cuts[2];
   __shared__ int last_arrival[2];
   __shared__ int busy;  // sequences that are not empty
@@ -374,6 +429,17 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
     busy = 0;
     tma_prefetch_desc(&maps.keys);
     tma_prefetch_desc(&maps.values);
+  }
+  // The lengths and the page table's lines come to L2 before the dependency wait
+  // (hints: they return no data, so what the previous kernel still writes is
+  // read correctly after it): 6.9 -> 6.6 us for 128 tokens, whose table was last
+  // read a layer's worth of traffic ago.
+  {
+    const int64_t bytes =
+        ((p.sequences - 1) * p.page_table_stride + (p.capacity >> p.block_shift)) * 4;
+    const int64_t at = (blockIdx.x + static_cast<int64_t>(lane) * gridDim.x) * 128;
+    if (warp == 0 && at < bytes) prefetch_l2(reinterpret_cast<const char*>(p.page_table) + at);
+    if (warp == 1 && lane * 32 < p.sequences) prefetch_l2(p.lengths + lane * 32);
   }
   pdl_wait();
   pdl_launch_dependents();
@@ -426,11 +492,12 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   }
   // How many CTAs share the tiles.  Many rows: every SM, but a tile a warp at
   // least.  Few rows: whole CTAs per row where that leaves few SMs idle, since a
-  // CTA with one row has one join less (three D 256 sequences 43.3 against 47.3
-  // us, two of 60K tokens 79.5 against 80.5, one of 128K 88.0 against 87.3), and
-  // no more of them than give every warp a tile (2K tokens, 8 heads: 10.3 us,
-  // with four tiles a warp 14.1), one for a row of up to two tiles a warp (333
-  // tokens: 8.3 us, with a tile a warp and the join across CTAs 9.8).
+  // CTA with one row has one join less (when the rule was made: three D 256
+  // sequences 43.3 against 47.3 us, two of 60K tokens 79.5 against 80.5, one of
+  // 128K 88.0 against 87.3), and no more of them than give every warp a tile (2K
+  // tokens, 8 heads: 10.3 us, with four tiles a warp 14.1), one for a row of up to
+  // two tiles a warp (333 tokens: 8.3 us, with a tile a warp and the join across
+  // CTAs 9.8).
   const unsigned rows = static_cast<unsigned>(busy) * p.heads, grid = gridDim.x;
   unsigned C = min(grid, (T + W - 1) / W);
   if (rows > 0 && rows <= grid) {
@@ -648,72 +715,38 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   // Join the CTA's partials.  A row that began and ended within the CTA is
   // written; one that began before it goes to the CTA's slot 0, one that only
   // goes on after it to slot 1.
-  //
-  // First the weights, half a warp per query and a lane per partial (partials
-  // that are not there weigh nothing), by scans over the lanes of each row;
-  // then every four channels of a row by a thread.
-  const auto slot_of = [&](int row) {
-    return row == cuts[0].row ? 0 : row == cuts[1].row ? 1 : -1;
-  };
-  const auto partial_of = [&](int slot) {
-    return slot < 0 ? nullptr : p.cta_partials + (static_cast<size_t>(cta) * 2 + slot) * kPartial;
-  };
+  // kLanes threads share the channels of a query.
+  constexpr int kLanes = D / 4 < kThreads / G8 ? D / 4 : kThreads / G8;
+  constexpr int kBatch = D > 192 && NT > 1 ? 4 : 8;
   {
-    const int i = lane & 15;
-    const int row = i < 2 * W ? seg_row[i] : -1;
-    const unsigned used = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
-    const unsigned below = used & ((1u << i) - 1);
-    const int previous = __shfl_sync(0xffffffffu, row, below ? 31 - __clz(below) : 0);
+    const int mine = lane < 2 * W ? seg_row[lane] : -1;
+    const unsigned used = __ballot_sync(0xffffffffu, mine >= 0);
+    const unsigned below = used & ((1u << lane) - 1);
+    const int previous = __shfl_sync(0xffffffffu, mine, below ? 31 - __clz(below) : 0);
+    // The first partial of each row.
     const unsigned heads =
-        __ballot_sync(0xffffffffu, row >= 0 && (below == 0 || previous != row)) & 0xffffu;
-    const unsigned from = heads & ((2u << i) - 1), beyond = heads & ~((2u << i) - 1);
-    const int first = from ? 31 - __clz(from) : 0, last = beyond ? __ffs(beyond) - 2 : 15;
-    if (threadIdx.x < 16) {
-      if (i == 0) join_rows = __popc(heads);
-      if (heads >> i & 1) {
-        const int k = __popc(heads & ((1u << i) - 1));
-        join_first[k] = first;
-        join_last[k] = min(last, 2 * W - 1);
-      }
-    }
-    for (int g = 2 * warp + (lane >> 4); g < G8; g += 2 * W) {
-      const float m = row >= 0 ? seg_m[i][g] : -INFINITY;
-      float top = m;
-#pragma unroll
-      for (int step = 1; step < 16; step <<= 1) {
-        const float other = __shfl_up_sync(0xffffffffu, top, step, 16);
-        if (i - step >= first) top = fmaxf(top, other);
-      }
-      top = __shfl_sync(0xffffffffu, top, last, 16);
-      const float w = row >= 0 ? __expf(m - finite_or_zero(top)) : 0.f;
-      float sum = row >= 0 ? w * seg_l[i][g] : 0.f;
-#pragma unroll
-      for (int step = 1; step < 16; step <<= 1) {
-        const float other = __shfl_up_sync(0xffffffffu, sum, step, 16);
-        if (i - step >= first) sum += other;
-      }
-      sum = __shfl_sync(0xffffffffu, sum, last, 16);
-      if (i < 2 * W) weight[i][g] = w;
-      if ((heads >> i & 1) && g < p.group) {
-        inverse[i][g] = 1.f / sum;
-        put_sums<G8>(p, row, g, partial_of(slot_of(row)), top, sum);
-      }
-    }
-    __syncthreads();
-    const int columns = p.group * (D / 4);
-    for (int x = threadIdx.x; x < join_rows * columns; x += kThreads) {
-      const int k = x / columns, column = x - k * columns;
-      const int q = column / (D / 4), d = (column - q * (D / 4)) * 4;
-      const int a = join_first[k], z = join_last[k], r = seg_row[a];
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int j = a; j <= z; ++j) {
-        if (used >> j & 1) {
-          fma4(acc, weight[j][q],
-               *reinterpret_cast<const float4*>(segment(j) + q * (D + kPad) + d));
-        }
-      }
-      put_joined<D, G8>(p, r, q, d, partial_of(slot_of(r)), inverse[a][q], acc);
+        __ballot_sync(0xffffffffu, mine >= 0 && (below == 0 || previous != mine));
+    for (int x = threadIdx.x; x < __popc(heads) * p.group * kLanes; x += kThreads) {
+      const int k = x / kLanes / p.group, g = x / kLanes - k * p.group;
+      unsigned rest = heads;
+      for (int skip = 0; skip < k; ++skip) rest &= rest - 1;
+      const int head = __ffs(rest) - 1, row = seg_row[head];
+      rest &= rest - 1;
+      // The row's partials: from its first to the next row's first.
+      const unsigned members =
+          used & ~((1u << head) - 1) & (rest ? (rest & -rest) - 1 : 0xffffffffu);
+      const int slot = row == cuts[0].row ? 0 : row == cuts[1].row ? 1 : -1;
+      float* to = slot < 0 ? nullptr
+                           : p.cta_partials + (static_cast<size_t>(cta) * 2 + slot) * kPartial;
+      join<D, kLanes, kBatch>(
+          members, x % kLanes, [&](int j) { return seg_m[j][g]; },
+          [&](int j) { return seg_l[j][g]; },
+          [&](int j, int d) {
+            return *reinterpret_cast<const float4*>(segment(j) + g * (D + kPad) + d);
+          },
+          [&](int d, float m, float l, const float4& o) {
+            put_joined<D, G8>(p, row, g, d, to, m, l, o);
+          });
     }
   }
 
@@ -734,86 +767,37 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   }
   __syncthreads();
   // Joins the rows whose last arrival was this CTA's: its members' partials
-  // or, once those are joined, the groups'.  Like the join above, but a whole
-  // warp finds a query's weights, a lane per part, while the first parts'
-  // channels are on their way to the threads that will add them.
+  // or, once those are joined, the groups'.
   const auto join_arrived = [&](const bool grouped) {
-    constexpr int kBatch = 20;  // 18 or 19 parts: eight rows over the whole GPU
-    const bool both = last_arrival[0] && last_arrival[1];
-    const int only = last_arrival[0] ? 0 : 1;
-    if (!last_arrival[only]) return;
-    const int columns = p.group * (D / 4), total = both ? 2 * columns : columns;
-    float4 batch[kBatch];
-    const auto place = [&](int x, int& slot, int& q, int& d) {
-      slot = both ? (x >= columns ? 1 : 0) : only;
-      const int column = both && slot ? x - columns : x;
-      q = column / (D / 4);
-      d = (column - q * (D / 4)) * 4;
-    };
-    // The k-th part of the join of `cut` is part(cut, k).
-    const auto count_of = [&](const Cut& cut) { return grouped ? cut.groups : cut.members; };
-    const auto part = [&](const Cut& cut, int k) -> const float* {
-      return grouped ? p.group_partials +
-                           static_cast<size_t>(cut.slot_at(cut.first_cta + k * cut.fan)) * kPartial
-                     : p.cta_partials + static_cast<size_t>(cut.slot_at(cut.first + k)) * kPartial;
-    };
-    const auto to_of = [&](const Cut& cut) {
-      return grouped || cut.groups == 1
-                 ? nullptr
-                 : p.group_partials + static_cast<size_t>(cut.slot_at(cut.first)) * kPartial;
-    };
-    const auto fetch = [&](int x, int base) {
-      int slot, q, d;
-      place(x, slot, q, d);
+    const int all = p.group * kLanes;
+    const int from = last_arrival[0] ? 0 : all, to = last_arrival[1] ? 2 * all : all;
+    for (int x = from + threadIdx.x; x < to; x += kThreads) {
+      const int slot = x >= all ? 1 : 0, g = x / kLanes - slot * p.group;
       const Cut cut = cuts[slot];
-      const int count = count_of(cut);
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        if (base + u < count) {
-          batch[u] = __ldcg(
-              reinterpret_cast<const float4*>(part(cut, base + u) + 2 * G8 + q * D + d));
-        }
+      const auto part = [&](int k) -> const float* {
+        return grouped
+                   ? p.group_partials +
+                         static_cast<size_t>(cut.slot_at(cut.first_cta + k * cut.fan)) * kPartial
+                   : p.cta_partials + static_cast<size_t>(cut.slot_at(cut.first + k)) * kPartial;
+      };
+      float* target = grouped || cut.groups == 1
+                          ? nullptr
+                          : p.group_partials + static_cast<size_t>(cut.slot_at(cut.first)) * kPartial;
+      const unsigned members = 0xffffffffu >> (32 - (grouped ? cut.groups : cut.members));
+      const auto m_of = [&](int k) { return __ldcg(part(k) + g); };
+      const auto l_of = [&](int k) { return __ldcg(part(k) + G8 + g); };
+      const auto o_of = [&](int k, int d) {
+        return __ldcg(reinterpret_cast<const float4*>(part(k) + 2 * G8 + g * D + d));
+      };
+      const auto put = [&](int d, float m, float l, const float4& o) {
+        put_joined<D, G8>(p, cut.row, g, d, target, m, l, o);
+      };
+      // Eight rows over the whole GPU are 18 or 19 parts each: in one batch.
+      if (kLanes == D / 4 && members >> kBatch) {
+        join<D, kLanes, 20>(members, x % kLanes, m_of, l_of, o_of, put);
+      } else {
+        join<D, kLanes, kBatch>(members, x % kLanes, m_of, l_of, o_of, put);
       }
-    };
-    if (static_cast<int>(threadIdx.x) < total) fetch(threadIdx.x, 0);
-    for (int task = warp; task < (both ? 2 * p.group : p.group); task += W) {
-      const int slot = both ? (task >= p.group ? 1 : 0) : only;
-      const int g = both && slot ? task - p.group : task;
-      const Cut cut = cuts[slot];
-      const int count = count_of(cut);
-      const float* mine = part(cut, min(lane, count - 1));
-      const float m = lane < count ? __ldcg(mine + g) : -INFINITY;
-      const float l = lane < count ? __ldcg(mine + G8 + g) : 0.f;
-      float top = m;
-#pragma unroll
-      for (int step = 16; step > 0; step >>= 1) {
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
-      }
-      const float w = __expf(m - finite_or_zero(top));
-      float sum = lane < count ? w * l : 0.f;
-#pragma unroll
-      for (int step = 16; step > 0; step >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, step);
-      weight[slot * kFlatJoin + lane][g] = w;
-      if (lane == 0) {
-        inverse[slot][g] = 1.f / sum;
-        put_sums<G8>(p, cut.row, g, to_of(cut), top, sum);
-      }
-    }
-    __syncthreads();
-    for (int x = threadIdx.x; x < total; x += kThreads) {
-      int slot, q, d;
-      place(x, slot, q, d);
-      const Cut cut = cuts[slot];
-      const int count = count_of(cut);
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int base = 0; base < count; base += kBatch) {
-        if (base > 0 || x >= kThreads) fetch(x, base);
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-          if (base + u < count) fma4(acc, weight[slot * kFlatJoin + base + u][q], batch[u]);
-        }
-      }
-      put_joined<D, G8>(p, cut.row, q, d, to_of(cut), inverse[slot][q], acc);
     }
   };
   join_arrived(false);
