@@ -554,8 +554,11 @@ RKV_API int rkv_paged_append(const rkv_append_args* args, void* stream);
  * A length outside [0, table_blocks * block_size] or a page outside
  * [0, pool_pages) sets RKV_DEVICE_BAD_INPUT in the workspace's status word;
  * the kernel then takes the nearest length, and page 0.
+ * At most 4096 sequences and 4096 KV heads, and 2^31 - 1 tiles (64 tokens of a
+ * KV head for head_dim up to 64, else 32) that the page table can cover.
  * The workspace follows the rules at the top of this header; its size does
- * not depend on the lengths.  Calls that share one must be ordered.
+ * not depend on the lengths.  Calls that share one must be ordered; no CTA
+ * waits for another, so calls with workspaces of their own may overlap.
  */
 typedef struct rkv_paged_args {
   const void* query;

@@ -714,8 +714,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
 
   // Join the CTA's partials.  A row that began and ended within the CTA is
   // written; one that began before it goes to the CTA's slot 0, one that only
-  // goes on after it to slot 1.
-  // kLanes threads share the channels of a query.
+  // goes on after it to slot 1.  kLanes threads share the channels of a query.
   constexpr int kLanes = D / 4 < kThreads / G8 ? D / 4 : kThreads / G8;
   constexpr int kBatch = D > 192 && NT > 1 ? 4 : 8;
   {
@@ -752,8 +751,8 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
 
   // Rows cut by CTA ranges: the last of a row's CTAs to arrive joins them; a
   // row over many CTAs is joined in groups first, so that no CTA reads more
-  // than a few partials.
-  // Whether this arrival is the last of `expected`; the counter is then zero again.
+  // than a few partials.  arrive() says whether this is the last of `expected`
+  // arrivals, and then leaves the counter at zero.
   const auto arrive = [](int* counter, int expected) {
     const bool last = arrive_add(counter) == expected - 1;
     if (last) *counter = 0;
