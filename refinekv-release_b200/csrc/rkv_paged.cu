@@ -53,8 +53,11 @@ constexpr int tile_rows(int D) { return D <= 64 ? 64 : 32; }
 constexpr int paged_warps(int D) { return D <= 192 ? 8 : 6; }
 constexpr int stage_bytes(int D) { return 2 * tile_rows(D) * D * 2; }
 
-// A row's CTAs are joined in one level up to this many, else in groups.
-constexpr int kFlatJoin = 32;
+// A row's CTAs are joined in one level up to this many, else in groups of about
+// the square root.  24 against 32: three ragged D 256 sequences (24 to 39 parts)
+// 36.9 against 43 us, 8K tokens of one head 13.4 against 14.8; 16: 128K tokens
+// of eight heads (18 parts) 87.6 against 87.0; 80 and 160: up to 18 us more.
+constexpr int kFlatJoin = 24;
 
 // Workspace: status word, counters (at the same place for every geometry;
 // they are zero between calls), then the partials.
@@ -230,7 +233,9 @@ __device__ __forceinline__ void load_queries(uint32_t (&qb)[D / 16][NT][2], cons
 
 // o += V^T p for a tile's weights p (C layout), held in `Terms` bf16 terms:
 // one for bf16 queries (rounded, 2^-8 at most, within the output's own
-// rounding), three for fp32 queries, which hold all 24 bits of p.  The further
+// rounding; a second term would bring the error against 64 bits from 2.2e-3 to
+// the output's 1.7e-3 for up to 5 % more time), three for fp32 queries, which
+// hold all 24 bits of p.  The further
 // terms may be negative or zero, so they meet V with its infinities clamped:
 // an infinite value times p is infinite, whatever p's bits are.  And a tile's
 // products are summed apart and added to o by a rounded addition: the tensor
