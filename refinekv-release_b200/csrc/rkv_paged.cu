@@ -497,12 +497,11 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   }
   // How many CTAs share the tiles.  Many rows: every SM, but a tile a warp at
   // least.  Few rows: whole CTAs per row where that leaves few SMs idle, since a
-  // CTA with one row has one join less (when the rule was made: three D 256
-  // sequences 43.3 against 47.3 us, two of 60K tokens 79.5 against 80.5, one of
-  // 128K 88.0 against 87.3), and no more of them than give every warp a tile (2K
-  // tokens, 8 heads: 10.3 us, with four tiles a warp 14.1), one for a row of up to
-  // two tiles a warp (333 tokens: 8.3 us, with a tile a warp and the join across
-  // CTAs 9.8).
+  // CTA with one row has one join less (three D 256 sequences 36.7 us against 39.7
+  // with every SM, two of 60K tokens 79.1 against 80.1, one of 128K 86.8 against
+  // 86.6), and no more of them than give every warp a tile (2K tokens, 8 heads: 9.3
+  // us against 10.4 with two tiles a warp), one for a row of up to two tiles a warp
+  // (333 tokens: 7.9 us against 8.3 with a tile a warp and a join across CTAs).
   const unsigned rows = static_cast<unsigned>(busy) * p.heads, grid = gridDim.x;
   unsigned C = min(grid, (T + W - 1) / W);
   if (rows > 0 && rows <= grid) {
