@@ -446,7 +446,8 @@ RKV_API int rkv_decode_split(const rkv_summary* summary, const void* query, int 
  *     own input.  positions: (batch, tokens) int32, or int64 with
  *     positions_i64.  A position outside [0, table_rows) reads nothing and
  *     gives NaN in its row's rotary channels.
- *   head_dim even up to 1024, rotary_dim even in [2, head_dim].
+ *   head_dim even up to 1024, rotary_dim even in [2, head_dim]; at most 4096
+ *   heads each and 2^31 - 1 tokens in all.
  * Arithmetic is fp32, each product and sum rounded by itself, so a rotation
  * has the same bits in every layout and in rkv_paged_append.
  */

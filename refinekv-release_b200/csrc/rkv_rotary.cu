@@ -199,16 +199,19 @@ __global__ void __launch_bounds__(row_threads(V), row_ctas(V))
   }
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t count = p.batch * p.tokens;
-  const auto position = [&](int64_t n) -> int64_t {
-    const int64_t b = p.batch > 1 ? n / p.tokens : 0;
-    const int64_t at = b * p.pos_b + (n - b * p.tokens) * p.pos_t;
+  // Tokens are counted in 32 bits (below 2^31): their divisions are cheap.
+  const unsigned tokens = static_cast<unsigned>(p.tokens);
+  const unsigned count = static_cast<unsigned>(p.batch) * tokens;
+  const auto position = [&](unsigned n) -> int64_t {
+    const unsigned b = p.batch > 1 ? n / tokens : 0;
+    const int64_t at = b * p.pos_b + (n - b * tokens) * p.pos_t;
     return p.pos_i64 ? static_cast<const int64_t*>(p.positions)[at]
                      : static_cast<const int32_t*>(p.positions)[at];
   };
   int64_t upcoming = position(blockIdx.x);
-  for (int64_t n = blockIdx.x; n < count; n += gridDim.x) {
-    const int64_t b = p.batch > 1 ? n / p.tokens : 0, t = n - b * p.tokens;
+  for (unsigned n = blockIdx.x; n < count; n += gridDim.x) {
+    const unsigned at_b = p.batch > 1 ? n / tokens : 0;
+    const int64_t b = at_b, t = n - at_b * tokens;
     const int64_t pos = upcoming;
     Piece<T, V> in[kHeads][2];
 #pragma unroll
@@ -237,7 +240,7 @@ __global__ void __launch_bounds__(row_threads(V), row_ctas(V))
     if (Append) {
       keep = pos >= 0;
       if (keep) {
-        const int64_t seq = p.sequence_ids != nullptr ? p.sequence_ids[n] : n;
+        const int64_t seq = p.sequence_ids != nullptr ? p.sequence_ids[n] : static_cast<int64_t>(n);
         const int64_t block = pos >> p.block_shift;
         page_row = pos - (block << p.block_shift);
         bool ok = known && seq >= 0 && seq < p.sequences && block < p.table_blocks;

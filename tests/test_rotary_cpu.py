@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from refinekv_b200 import _native, apply_rotary, paged_append, rotary_table
+from refinekv_b200 import _native, apply_rotary, paged_append, paged_attention, rotary_table
 
 
 @pytest.fixture(scope="module")
@@ -86,6 +86,8 @@ def test_cpu_tensors_are_refused():
     pool = torch.zeros(5, 2, 16, 64, dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match="CUDA"):
         paged_append(x, x, pool, pool, torch.zeros(3, 2, dtype=torch.int32), at)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        paged_attention(x, pool, pool, torch.zeros(3, 2, dtype=torch.int32), at)
     with pytest.raises(ValueError, match="layout"):
         paged_append(x, x, pool, pool, torch.zeros(3, 2, dtype=torch.int32), at, layout="HDN")
 
