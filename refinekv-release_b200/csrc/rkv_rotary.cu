@@ -5,9 +5,9 @@
 // tensor or to the pool's page.  Bound: HBM on long inputs (every element
 // read once and written once, a few flops per pair), latency on single
 // tokens.  Measured on B200 (graph replay): 8192 tokens of 40 bf16 heads, D
-// 128: 30 us, 172 MB, 0.88 of the measured copy rate; 24.5K prompt tokens into
-// the pool, 48 heads each: 117 us, 653 MB, 0.85; one token: 2.1 us (eight
-// appended: 2.5).
+// 128: 29 us, 172 MB, 0.90 of the measured copy rate; 24.5K prompt tokens into
+// the pool, 48 heads each: 116 us, 653 MB, 0.86; one token: 2.1 to 2.4 us (eight
+// appended: 2.5 to 2.8).
 //
 // What it took: CTAs that stay and take token after token (one CTA a token
 // launched too slowly: 45 us for the 8192), the pieces of a row kept as they
