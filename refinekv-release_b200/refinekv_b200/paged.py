@@ -12,6 +12,11 @@ Pools are bf16, ``(pages, kv_heads, block, dim)`` (``layout="HND"``) or
 ``(sequences, blocks)``.  Everything that changes from step to step
 (positions, lengths, page tables) is read on the device, so a captured CUDA
 graph serves growing sequences.  Results carry no gradient.
+
+Pass the ``workspace`` dict of a layer or a server to every call: without one,
+each call allocates its outputs and zero-fills its scratch anew.  A captured
+graph keeps using the buffers it was captured with, so it wants a dict of its
+own: a call of another shape replaces them in the dict.
 """
 
 from __future__ import annotations
