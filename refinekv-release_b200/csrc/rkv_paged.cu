@@ -231,15 +231,18 @@ __device__ __forceinline__ void load_queries(uint32_t (&qb)[D / 16][NT][2], cons
   }
 }
 
-// o += V^T p for a tile's weights p (C layout), held in `Terms` bf16 terms:
-// one for bf16 queries (rounded, 2^-8 at most, within the output's own
-// rounding; a second term would bring the error against 64 bits from 2.2e-3 to
-// the output's 1.7e-3 for up to 5 % more time), three for fp32 queries, which
-// hold all 24 bits of p.  The further
+// o += V^T p for a tile's weights p (C layout), held in `Terms` bf16 terms: two
+// for bf16 queries (2^-16 at most, far within the output's own rounding: the
+// error against 64 bits is the output's 1.66e-3; one term, 2^-8, made it 2.0 to
+// 2.3e-3 and took 7.9 instead of 8.3 us for 333 tokens, 319 instead of 322 for 16
+// sequences of 32K, 46 instead of 50 for D 256 with 16 queries a KV head), three
+// for fp32 queries, which hold all 24 bits of p.  The further
 // terms may be negative or zero, so they meet V with its infinities clamped:
-// an infinite value times p is infinite, whatever p's bits are.  And a tile's
-// products are summed apart and added to o by a rounded addition: the tensor
-// cores cut their sums off, which over a long row would cost fp32 digits.
+// an infinite value times p is infinite, whatever p's bits are.  For fp32 queries
+// a tile's products are summed apart and added to o by a rounded addition: the
+// tensor cores cut their sums off, which over a long row would cost fp32 digits.
+// A bf16 output does not see them (the same error with both), and the second
+// set of sums would spill: 68 us instead of 50 for that D 256 batch.
 template <int R, int D, int NT, int Terms>
 __device__ __forceinline__ void weigh_values(uint32_t tile, float (&p)[R / 16][NT][4],
                                              float (&o)[D / 16][NT][4], int lane) {
@@ -266,7 +269,7 @@ __device__ __forceinline__ void weigh_values(uint32_t tile, float (&p)[R / 16][N
     float sum[NT][4];  // of the tile
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) sum[nt][0] = sum[nt][1] = sum[nt][2] = sum[nt][3] = 0.f;
-    float(&to)[NT][4] = Terms > 1 ? sum : o[dt];
+    float(&to)[NT][4] = Terms > 2 ? sum : o[dt];
 #pragma unroll
     for (int kt = 0; kt < R / 16; ++kt) {
       uint32_t a[4];
@@ -288,7 +291,7 @@ __device__ __forceinline__ void weigh_values(uint32_t tile, float (&p)[R / 16][N
             mma_bf16(to[nt], a, frag[term][kt][nt][0], frag[term][kt][nt][1]);
       }
     }
-    if constexpr (Terms > 1) {
+    if constexpr (Terms > 2) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -649,7 +652,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
           if (p.query_f32) {
             weigh_values<R, D, NT, 3>(v_tile, logit, o, lane);
           } else {
-            weigh_values<R, D, NT, 1>(v_tile, logit, o, lane);
+            weigh_values<R, D, NT, 2>(v_tile, logit, o, lane);
           }
           __syncwarp();
           if (more) issue(1, next, page);
