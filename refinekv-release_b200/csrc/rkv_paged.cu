@@ -36,6 +36,7 @@
 
 #include "refinekv_b200.h"
 #include "rkv_device.cuh"
+#include "rkv_drain.h"
 #include "rkv_kernels.h"
 
 namespace rkv {
@@ -588,6 +589,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
     const int count = static_cast<int>(whi - wlo);
     int seg_first = cur.tile;  // the segment's first tile of its row
     bool fresh = true, aborted = false;
+    const auto again = [&](int which, int parity) { warp_wait(&bars[warp][which], parity); };
     if (count > 1) {
       advance<R>(p, start, next);
       page = page_of(next);
@@ -612,7 +614,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
       // status word says so); nothing is in flight after its drain.
       if (!aborted && !warp_wait(&bars[warp][0], j & 1)) {
         if (lane == 0) atomicOr(p.status, kStatusTimeout);
-        warp_wait(&bars[warp][1], j & 1);
+        drain_keys_and_values(j, again);
         aborted = true;
       }
       if (!aborted) {
@@ -633,8 +635,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
         softmax_update<R, D, NT>(logit, m, l, o);
         if (!warp_wait(&bars[warp][1], j & 1)) {
           if (lane == 0) atomicOr(p.status, kStatusTimeout);
-          warp_wait(&bars[warp][1], j & 1);
-          if (more) warp_wait(&bars[warp][0], (j + 1) & 1);
+          drain_values(j, more, again);
           aborted = true;
         } else {
           if (row_lo > 0 || row_hi < R) {
