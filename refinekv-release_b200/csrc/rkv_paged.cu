@@ -102,10 +102,14 @@ struct Paged {
   static constexpr int kWarpPartial = warp_partial_floats(D, NT);
 };
 
+// A length that the page table cannot hold counts as zero: nothing of its row
+// is read, and the row is NaN.
 __device__ __forceinline__ int clamp_length(const PagedParams& p, int seq) {
   const int length = p.lengths[seq];
-  return max(0, min(length, p.capacity));
+  return length > p.capacity ? 0 : max(0, length);
 }
+
+constexpr int kNoPage = -1, kBadPage = -2;  // of a box: nothing visible; not in the pool
 
 __device__ __forceinline__ int first_visible(const PagedParams& p, int length) {
   return p.window > 0 && length > p.window ? length - p.window : 0;
@@ -489,14 +493,19 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
     __syncthreads();
   }
   const unsigned T = static_cast<unsigned>(start[p.sequences]) * p.heads;
-  // Idle slots: zero rows.
+  // Idle slots: zero rows; lengths past the table: NaN.
   for (int s = blockIdx.x; s < p.sequences; s += gridDim.x) {
     if (start[s + 1] != start[s]) continue;
+    const bool past = p.lengths[s] > p.capacity;
     const int queries = p.heads * p.group;
     const int64_t row = static_cast<int64_t>(s) * queries;
-    for (int i = threadIdx.x; i < queries * p.dim; i += blockDim.x) put(p, row * p.dim + i, 0.f);
+    for (int i = threadIdx.x; i < queries * p.dim; i += blockDim.x) {
+      put(p, row * p.dim + i, past ? NAN : 0.f);
+    }
     if (p.lse != nullptr) {
-      for (int i = threadIdx.x; i < queries; i += blockDim.x) p.lse[row + i] = -INFINITY;
+      for (int i = threadIdx.x; i < queries; i += blockDim.x) {
+        p.lse[row + i] = past ? NAN : -INFINITY;
+      }
     }
   }
   // How many CTAs share the tiles.  Many rows: every SM, but a tile a warp at
@@ -536,17 +545,17 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   const int page_rows = 1 << p.block_shift;
   const int box_rows = min(R, page_rows), boxes = R / box_rows;
 
-  // Lane i of the first `boxes` lanes looks up the page of the tile's i-th
-  // box, or -1 where the box holds no visible token.
+  // Lane i of the first `boxes` lanes looks up the page of the tile's i-th box.
   auto page_of = [&](const Cursor& c) {
-    if (lane >= boxes) return -1;
+    if (lane >= boxes) return kNoPage;
     const int token = (c.first + c.tile) * R + lane * box_rows;
-    if (token >= c.length || token + box_rows <= c.low) return -1;
+    if (token >= c.length || token + box_rows <= c.low) return kNoPage;
     const int page = p.page_table[c.seq * p.page_table_stride + (token >> p.block_shift)];
     if (page >= 0 && page < p.pool_pages) return page;
-    atomicOr(p.status, kStatusBadInput);  // flag the call; read page 0 instead
-    return 0;
+    atomicOr(p.status, kStatusBadInput);
+    return kBadPage;
   };
+  // Requests the tile's boxes; a bad page's are left out, and its row is NaN.
   auto issue = [&](int which, const Cursor& c, int page) {
     uint64_t* bar = &bars[warp][which];
     const unsigned used = __ballot_sync(0xffffffffu, page >= 0);
@@ -585,6 +594,8 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
     int page = page_of(cur);
     issue(0, cur, page);
     issue(1, cur, page);
+    // Whether a tile lacks a page: this one, the next, any so far of the row.
+    bool bad = __any_sync(0xffffffffu, page == kBadPage), next_bad = false, spoilt = false;
     find_cuts();
     const int count = static_cast<int>(whi - wlo);
     int seg_first = cur.tile;  // the segment's first tile of its row
@@ -605,8 +616,9 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
           for (int dt = 0; dt < D / 16; ++dt)
             o[dt][nt][0] = o[dt][nt][1] = o[dt][nt][2] = o[dt][nt][3] = 0.f;
         }
-        fresh = false;
+        fresh = spoilt = false;
       }
+      spoilt = spoilt || bad;
       const bool more = j + 1 < count;
       const int token = (cur.first + cur.tile) * R;
       const int row_lo = max(0, cur.low - token), row_hi = min(R, cur.length - token);
@@ -631,7 +643,10 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
                   r >= row_lo && r < row_hi ? logit[mt][nt][c] * p.scale : -INFINITY;
           }
         __syncwarp();
-        if (more) issue(0, next, page);
+        if (more) {
+          issue(0, next, page);
+          next_bad = __any_sync(0xffffffffu, page == kBadPage);
+        }
         softmax_update<R, D, NT>(logit, m, l, o);
         if (!warp_wait(&bars[warp][1], j & 1)) {
           if (lane == 0) atomicOr(p.status, kStatusTimeout);
@@ -662,6 +677,10 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
       const bool row_done = cur.tile + 1 == cur.tiles;
       if (row_done || !more) {
         reduce_l<NT>(l);
+        if (spoilt) {  // a sum of NaN spreads through every join
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) l[nt][0] = l[nt][1] = NAN;
+        }
         const int row = cur.seq * p.heads + cur.head;
         const bool whole = row_done && seg_first == 0;
         if (whole) {
@@ -711,6 +730,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
       }
       if (more) {
         cur = next;
+        bad = next_bad;
         if (j + 2 < count) {
           advance<R>(p, start, next);
           page = page_of(next);

@@ -205,8 +205,10 @@ def paged_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: tor
     with ``return_lse``, (output, lse) with the fp32 natural-log sum of the
     exponentials (-inf for an empty row): outputs over parts of a sequence join
     as sum_i exp(lse_i - lse) output_i.  Backed by ``workspace``, reused by the
-    next call of the same shape.  A length past the page table's row or a page
-    outside the pool sets bit 1 of ``attention.device_status(workspace)``.
+    next call of the same shape.  A length past the page table's row or a
+    visible page outside the pool sets bit 1 of
+    ``attention.device_status(workspace)`` and makes that sequence's output (and
+    lse) NaN; a negative length sets it and counts as 0.
     One launch; its results repeat bit for bit.
     """
     pages, heads, block, dim, ks, vs = _pools(key_pool, value_pool, layout)
