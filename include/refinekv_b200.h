@@ -556,7 +556,8 @@ RKV_API int rkv_paged_append(const rkv_append_args* args, void* stream);
  * outside [0, pool_pages) sets RKV_DEVICE_BAD_INPUT in the workspace's status
  * word.  A negative length counts as 0; a length past the table makes its
  * sequence's output and lse NaN, nothing of it read; a bad page is not read
- * and makes the output and lse of its sequence NaN.
+ * and makes the output and lse of its sequence NaN.  So does a wait that runs out
+ * (RKV_DEVICE_TIMEOUT), for the rows that it leaves short.
  * At most 4096 sequences and 4096 KV heads, and 2^31 - 1 tiles (64 tokens of a
  * KV head for head_dim up to 64, else 32) that the page table can cover.
  * The workspace follows the rules at the top of this header; its size does

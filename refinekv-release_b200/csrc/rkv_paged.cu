@@ -623,7 +623,8 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
       const int token = (cur.first + cur.tile) * R;
       const int row_lo = max(0, cur.low - token), row_hi = min(R, cur.length - token);
       // A wait that runs out leaves the rest of the warp's range out (the
-      // status word says so); nothing is in flight after its drain.
+      // status word says so, and its rows are NaN); nothing is in flight after
+      // its drain.
       if (!aborted && !warp_wait(&bars[warp][0], j & 1)) {
         if (lane == 0) atomicOr(p.status, kStatusTimeout);
         drain_keys_and_values(j, again);
@@ -677,7 +678,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
       const bool row_done = cur.tile + 1 == cur.tiles;
       if (row_done || !more) {
         reduce_l<NT>(l);
-        if (spoilt) {  // a sum of NaN spreads through every join
+        if (spoilt || aborted) {  // a sum of NaN spreads through every join
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) l[nt][0] = l[nt][1] = NAN;
         }

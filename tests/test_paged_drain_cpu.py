@@ -83,3 +83,12 @@ def test_the_kernel_drains_by_that_schedule():
                         ("!warp_wait(&bars[warp][1], j & 1)", "drain_values(j, more,")):
         at = kernel.index(wait)
         assert drain in kernel[at:kernel.index("aborted = true", at)]
+
+
+def test_rows_left_short_by_a_timeout_are_nan():
+    """Where a row's or a part's sum is taken, an aborted warp's is NaN before any use of it."""
+    kernel = (native_build_module().CSRC / "rkv_paged.cu").read_text()
+    after = kernel[kernel.index("reduce_l<NT>(l);"):]
+    poison = after.index("l[nt][0] = l[nt][1] = NAN")
+    assert "aborted" in after[:poison]
+    assert poison < after.index("1.f / l[nt][c]") and poison < after.index("seg_l[i][g] = l[nt][c]")
