@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 namespace rkv {
 
 constexpr int kSelectTile = 32;  // summary blocks per selector tile
@@ -324,6 +326,13 @@ struct PagedParams {
   float* cta_partials;    // two per CTA
   float* group_partials;  // two per CTA
 };
+
+// Whether pointers (null or not) are aligned to elements of `bytes`.
+inline bool aligned_to(int bytes, std::initializer_list<const void*> pointers) {
+  uintptr_t bits = 0;
+  for (const void* p : pointers) bits |= reinterpret_cast<uintptr_t>(p);
+  return (bits & static_cast<uintptr_t>(bytes - 1)) == 0;
+}
 
 // Host helpers of rkv_capi.cu for entry points in other files: the current
 // device's SM count, and the 4-D map of a page pool with boxes of `box_rows`.

@@ -958,6 +958,10 @@ int rkv_paged_attention(const rkv_paged_args* a, void* stream) {
   if (bits & 15u) {
     return reject(RKV_ERR_ALIGNMENT, "pointers and strides must be 16-byte aligned");
   }
+  if (!aligned_to(4, {a->page_table, a->lengths, a->lse})) {
+    return reject(RKV_ERR_ALIGNMENT,
+                  "page_table, lengths and lse must be aligned to their elements");
+  }
   int rc = RKV_OK, sms = 0;
   PagedMaps maps;
   const int box_rows = static_cast<int>(std::min<int64_t>(R, a->block_size));

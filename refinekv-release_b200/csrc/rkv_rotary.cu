@@ -417,6 +417,9 @@ int rkv_rotary(const rkv_rotary_args* a, void* stream) {
        (a->key_heads > 0 && (!a->key || !a->key_out)))) {
     return reject(RKV_ERR_INVALID_ARGUMENT, "positions, rows and outputs must be non-null");
   }
+  if (!aligned_to(a->positions_i64 ? 8 : 4, {a->positions})) {
+    return reject(RKV_ERR_ALIGNMENT, "positions are not aligned to their elements");
+  }
   RowsParams p = {};
   const auto row_stream = [](const void* in, void* out, const int64_t* is, const int64_t* os,
                              int64_t heads) {
@@ -470,6 +473,11 @@ int rkv_paged_append(const rkv_append_args* a, void* stream) {
   }
   if (a->tokens > 0 && a->query_heads > 0 && (!a->query || !a->query_out)) {
     return reject(RKV_ERR_INVALID_ARGUMENT, "query and query_out must be non-null");
+  }
+  if (!aligned_to(a->positions_i64 ? 8 : 4, {a->positions}) ||
+      !aligned_to(4, {a->page_table, a->sequence_ids, a->status})) {
+    return reject(RKV_ERR_ALIGNMENT,
+                  "positions, page_table, sequence_ids and status must be aligned to their elements");
   }
   RowsParams p = {};
   p.query = RowStream{a->query, a->query_out, 0, a->query_strides[0], a->query_strides[1],
