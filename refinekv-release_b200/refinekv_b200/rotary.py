@@ -69,7 +69,11 @@ def _frequencies(rotary_dim: int, base: float, scaling: dict | None):
     slow = ((index - first) / (last - first)).clamp(0, 1)
     amplitude = scaling.get("attention_factor")
     if amplitude is None:
-        amplitude = 0.1 * math.log(factor) + 1 if factor > 1 else 1.0
+        def grown(by):
+            return 0.1 * by * math.log(factor) + 1
+
+        mscale, all_dim = scaling.get("mscale"), scaling.get("mscale_all_dim")
+        amplitude = grown(mscale) / grown(all_dim) if mscale and all_dim else grown(1.0)
     return plain / factor * slow + plain * (1 - slow), float(amplitude)
 
 

@@ -1,0 +1,33 @@
+"""Rotary tables from whole rope-scaling dictionaries, as model configurations keep them (no GPU)."""
+
+import pytest
+import torch
+
+from refinekv_b200 import rotary_table
+from refinekv_b200.rotary import _frequencies
+from test_rotary_cpu import _library_frequencies
+
+YARN = {"rope_type": "yarn", "factor": 40.0, "original_max_position_embeddings": 4096}
+
+
+@pytest.mark.parametrize("keys", [
+    {"mscale": 0.707, "mscale_all_dim": 0.707},
+    {"mscale": 1.0, "mscale_all_dim": 0.707},
+    {"mscale": 1.0, "mscale_all_dim": 1.0, "beta_fast": 32, "beta_slow": 1},
+    {"mscale": 0.707},            # one of the two alone has no effect
+    {"mscale_all_dim": 0.707},
+    {"mscale": 0.707, "mscale_all_dim": 0.0},
+    {"mscale": 0.707, "mscale_all_dim": 0.5, "attention_factor": 1.25},
+    {"attention_factor": 1.0},
+    {"beta_fast": 16, "beta_slow": 2},
+    {"truncate": False},
+])
+def test_yarn_amplitude_follows_the_configuration(keys):
+    scaling = {**YARN, **keys}
+    got, amplitude = _frequencies(64, 10000.0, scaling)
+    want, want_amplitude = _library_frequencies("yarn", 64, 10000.0, scaling)
+    # the library works in fp32: a power and a few products, 2^-23 each
+    torch.testing.assert_close(got, want.double(), rtol=2 ** -19, atol=0)
+    assert abs(amplitude - want_amplitude) <= 1e-6
+    row = rotary_table(64, 4, scaling=scaling, device="cpu")[0]  # cosines of 0, then sines
+    torch.testing.assert_close(row[:32], torch.full((32,), want_amplitude), rtol=1e-6, atol=0)
