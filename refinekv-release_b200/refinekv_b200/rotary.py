@@ -77,7 +77,7 @@ def _frequencies(rotary_dim: int, base: float, scaling: dict | None):
     return plain / factor * slow + plain * (1 - slow), float(amplitude)
 
 
-def rotary_table(rotary_dim: int, positions: int, *, base: float = 10000.0,
+def rotary_table(rotary_dim: int, positions: int, *, base: float | None = None,
                  scaling: dict | None = None, device="cuda") -> torch.Tensor:
     """The fp32 (positions, rotary_dim) table ``apply_rotary`` and ``paged_append`` read.
 
@@ -86,15 +86,21 @@ def rotary_table(rotary_dim: int, positions: int, *, base: float = 10000.0,
     position near 10^5 with a frequency is off by up to 4e-3 rad).
     ``scaling`` is a model configuration's rope scaling: ``{"rope_type":
     "linear" | "ntk" | "yarn" | "llama3", "factor": ...}`` with that type's
-    further keys.  Built once and kept by the caller.
+    further keys, and ``rope_theta``, the base, unless ``base`` is given (10000
+    without either).  Built once and kept by the caller.
     """
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError("rotary_dim must be even and positive")
     if positions < 1:
         raise ValueError("positions must be positive")
+    scaling = dict(scaling or {})
+    theta = scaling.pop("rope_theta", None)
+    if theta is not None and base is not None and float(theta) != float(base):
+        raise ValueError("base and the scaling's 'rope_theta' differ: give one of them")
+    base = float(base if base is not None else theta if theta is not None else 10000.0)
     if not math.isfinite(base) or base <= 1:
-        raise ValueError("base must be finite and above 1")
-    frequency, amplitude = _frequencies(rotary_dim, float(base), scaling)
+        raise ValueError("base (rope_theta) must be finite and above 1")
+    frequency, amplitude = _frequencies(rotary_dim, base, scaling)
     frequency = frequency.to(device)
     table = torch.empty(positions, rotary_dim, device=device, dtype=torch.float32)
     step = max(1, (1 << 24) // rotary_dim)  # bounds the fp64 temporaries

@@ -31,3 +31,25 @@ def test_yarn_amplitude_follows_the_configuration(keys):
     assert abs(amplitude - want_amplitude) <= 1e-6
     row = rotary_table(64, 4, scaling=scaling, device="cpu")[0]  # cosines of 0, then sines
     torch.testing.assert_close(row[:32], torch.full((32,), want_amplitude), rtol=1e-6, atol=0)
+
+
+LLAMA3 = {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+          "original_max_position_embeddings": 8192}
+
+
+@pytest.mark.parametrize("scaling", [{"rope_type": "default"}, {"rope_type": "linear", "factor": 4.0},
+                                     LLAMA3, YARN], ids=lambda s: s["rope_type"])
+def test_the_base_may_be_in_the_dictionary(scaling):
+    want = rotary_table(64, 50, base=500000.0, scaling=scaling, device="cpu")
+    whole = {**scaling, "rope_theta": 500000.0}
+    assert torch.equal(rotary_table(64, 50, scaling=whole, device="cpu"), want)
+    assert torch.equal(rotary_table(64, 50, base=500000, scaling=whole, device="cpu"), want)
+    assert torch.equal(rotary_table(64, 50, base=500000.0, device="cpu", scaling={
+        **scaling, "rope_theta": None}), want)
+    with pytest.raises(ValueError, match="rope_theta"):
+        rotary_table(64, 50, base=10000.0, scaling=whole, device="cpu")
+    with pytest.raises(ValueError, match="base"):
+        rotary_table(64, 50, scaling={**scaling, "rope_theta": 1.0}, device="cpu")
+    # without either: 10000
+    assert torch.equal(rotary_table(64, 50, scaling=scaling, device="cpu"),
+                       rotary_table(64, 50, base=10000.0, scaling=scaling, device="cpu"))
