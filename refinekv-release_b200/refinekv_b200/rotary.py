@@ -20,18 +20,40 @@ _POSITIONS = (torch.int32, torch.int64)
 _DTYPES = {torch.bfloat16: _native.DTYPE_BF16, torch.float32: _native.DTYPE_F32}
 
 
+#: The keys of a scaling dictionary that each type reads; the first ones it cannot do without.
+_SCALINGS = {
+    "default": ((), ()),
+    "none": ((), ()),
+    "linear": (("factor",), ()),
+    "ntk": (("factor",), ()),
+    "yarn": (("factor", "original_max_position_embeddings"),
+             ("attention_factor", "beta_fast", "beta_slow", "mscale", "mscale_all_dim",
+              "truncate")),
+    "llama3": (("factor", "original_max_position_embeddings", "low_freq_factor",
+                "high_freq_factor"), ()),
+}
+#: Keys that say nothing about the angles of a table of a given width.
+_NEUTRAL = ("partial_rotary_factor", "max_position_embeddings", "original_max_position_embeddings")
+
+
 def _frequencies(rotary_dim: int, base: float, scaling: dict | None):
     """fp64 angular frequencies of the pairs and the amplitude of the table."""
     exponent = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
     plain = base ** -exponent
-    scaling = dict(scaling or {})
+    scaling = {key: value for key, value in (scaling or {}).items() if value is not None}
     kind = scaling.pop("rope_type", scaling.pop("type", "default"))
-    if kind in ("default", "none"):
+    if kind not in _SCALINGS:
+        raise ValueError("scaling type must be 'linear', 'ntk', 'yarn' or 'llama3'")
+    needed, optional = _SCALINGS[kind]
+    for key in needed:
+        if key not in scaling:
+            raise ValueError(f"scaling {kind!r} needs {key!r}")
+    for key in scaling:
+        if key not in (*needed, *optional, *_NEUTRAL):
+            raise ValueError(f"scaling {kind!r} does not know {key!r}")
+    if not needed:
         return plain, 1.0
-    try:
-        factor = float(scaling["factor"])
-    except KeyError:
-        raise ValueError(f"scaling {kind!r} needs a 'factor'") from None
+    factor = float(scaling["factor"])
     if not math.isfinite(factor) or factor < 1:
         raise ValueError("scaling factor must be at least 1")
     if kind == "linear":
@@ -40,16 +62,16 @@ def _frequencies(rotary_dim: int, base: float, scaling: dict | None):
         if rotary_dim == 2:
             return plain, 1.0
         return (base * factor ** (rotary_dim / (rotary_dim - 2))) ** -exponent, 1.0
-    if kind not in ("yarn", "llama3"):
-        raise ValueError("scaling type must be 'linear', 'ntk', 'yarn' or 'llama3'")
-    original = scaling.get("original_max_position_embeddings")
-    if original is None:
-        raise ValueError(f"scaling {kind!r} needs 'original_max_position_embeddings'")
+    original = float(scaling["original_max_position_embeddings"])
+    if not math.isfinite(original) or original <= 0:
+        raise ValueError("original_max_position_embeddings must be positive")
     if kind == "llama3":
         # Pairs that turn more than high_freq_factor times within the original
         # context are kept, fewer than low_freq_factor times slowed by
         # `factor`, and blended linearly in between.
         low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        if not 0 <= low < high:
+            raise ValueError("high_freq_factor must be above low_freq_factor")
         turns = original * plain / (2 * math.pi)
         keep = ((turns - low) / (high - low)).clamp(0, 1)
         return plain * keep + plain / factor * (1 - keep), 1.0
@@ -86,7 +108,7 @@ def rotary_table(rotary_dim: int, positions: int, *, base: float | None = None,
     position near 10^5 with a frequency is off by up to 4e-3 rad).
     ``scaling`` is a model configuration's rope scaling: ``{"rope_type":
     "linear" | "ntk" | "yarn" | "llama3", "factor": ...}`` with that type's
-    further keys, and ``rope_theta``, the base, unless ``base`` is given (10000
+    further keys (one that the type does not know is refused), and ``rope_theta``, the base, unless ``base`` is given (10000
     without either).  Built once and kept by the caller.
     """
     if rotary_dim < 2 or rotary_dim % 2:

@@ -53,3 +53,34 @@ def test_the_base_may_be_in_the_dictionary(scaling):
     # without either: 10000
     assert torch.equal(rotary_table(64, 50, scaling=scaling, device="cpu"),
                        rotary_table(64, 50, base=10000.0, scaling=scaling, device="cpu"))
+
+
+@pytest.mark.parametrize("scaling,match", [
+    ({**YARN, "beta_fats": 16}, "beta_fats"),                      # misspelt
+    ({**YARN, "low_freq_factor": 1.0}, "low_freq_factor"),         # another type's
+    ({**LLAMA3, "mscale": 1.0}, "mscale"),
+    ({"rope_type": "linear", "factor": 2.0, "short_factor": [1.0]}, "short_factor"),
+    ({"factor": 8.0}, "factor"),                                   # a factor without a type
+    ({"full_attention": {"rope_type": "default"}}, "full_attention"),
+    ({k: v for k, v in LLAMA3.items() if k != "low_freq_factor"}, "low_freq_factor"),
+    ({k: v for k, v in LLAMA3.items() if k != "high_freq_factor"}, "high_freq_factor"),
+    ({**LLAMA3, "high_freq_factor": None}, "high_freq_factor"),
+    ({**LLAMA3, "high_freq_factor": 1.0}, "high_freq_factor"),     # no band between the two
+    ({**YARN, "factor": None}, "factor"),
+    ({**YARN, "original_max_position_embeddings": 0}, "original_max_position_embeddings"),
+])
+def test_keys_that_are_missing_or_not_understood_are_refused(scaling, match):
+    with pytest.raises(ValueError, match=match):
+        rotary_table(64, 4, scaling=scaling, device="cpu")
+
+
+def test_absent_keys_may_be_none_and_harmless_ones_are_accepted():
+    plain = rotary_table(64, 50, scaling=YARN, device="cpu")
+    more = dict(YARN, mscale=None, beta_fast=None, attention_factor=None, type="yarn",
+                partial_rotary_factor=0.5, max_position_embeddings=163840)
+    assert torch.equal(rotary_table(64, 50, scaling=more, device="cpu"), plain)
+    linear = {"type": "linear", "factor": 2.0}
+    assert torch.equal(
+        rotary_table(64, 50, device="cpu",
+                     scaling={**linear, "original_max_position_embeddings": 4096}),
+        rotary_table(64, 50, device="cpu", scaling=linear))
