@@ -71,15 +71,30 @@ def _buffer(workspace, name, shape, device, dtype, zero=False):
     return tensor
 
 
+#: Workspace entries whose first word is a sticky status that ``device_status`` reports.
+_STATUS_WORDS = ("rkv_decode_scratch", "rkv_paged_scratch", "rkv_append_status")
+
+
 def _scratch(workspace, name, nbytes, device):
-    """Zero-filled device scratch of at least ``nbytes`` (the C ABI's workspace)."""
+    """Zero-filled device scratch of at least ``nbytes`` (the C ABI's workspace).
+
+    A scratch that takes another's place takes over its status word.  While a
+    graph is captured a copy would be recorded instead of made (and zeros that
+    come after it, at every replay), so the old scratch is kept next to it.
+    """
     if nbytes == 0:
         raise RuntimeError("librefinekv_b200 rejected the workspace geometry")
-    tensor = workspace.get(name) if workspace is not None else None
-    if tensor is None or tensor.device != device or tensor.numel() < nbytes:
-        tensor = torch.zeros(nbytes, device=device, dtype=torch.uint8)
-        if workspace is not None:
-            workspace[name] = tensor
+    old = workspace.get(name) if workspace is not None else None
+    if old is not None and old.device == device and old.numel() >= nbytes:
+        return old
+    tensor = torch.zeros(nbytes, device=device, dtype=torch.uint8)
+    if old is not None and name in _STATUS_WORDS:
+        if torch.cuda.is_current_stream_capturing():
+            workspace.setdefault(name + "_replaced", []).append(old)
+        else:
+            tensor[:4].copy_(old[:4])
+    if workspace is not None:
+        workspace[name] = tensor
     return tensor
 
 
@@ -87,16 +102,16 @@ def device_status(workspace: dict) -> int:
     """Sticky device status of a workspace's calls (synchronises); 0 means healthy.
 
     The union of the status words of ``sparse_attention``, ``paged_attention``
-    and ``paged_append`` calls that were given this workspace.
+    and ``paged_append`` calls that were given this workspace.  A call that
+    allocates its scratch while a graph is captured (the first with this
+    workspace, or one of a wider shape) has the graph clear its word at every replay.
     """
+    workspace = workspace or {}
     status = 0
-    for name in ("rkv_decode_scratch", "rkv_paged_scratch"):
-        scratch = workspace.get(name) if workspace else None
-        if scratch is not None:
-            status |= int(scratch[:4].view(torch.int32).item())
-    appended = workspace.get("rkv_append_status") if workspace else None
-    if appended is not None:
-        status |= int(appended[0].item())
+    for name in _STATUS_WORDS:
+        for scratch in (workspace.get(name), *workspace.get(name + "_replaced", ())):
+            if scratch is not None:
+                status |= int(scratch[:4].view(torch.int32).item())
     return status
 
 

@@ -169,8 +169,7 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Tensor,
         out_strides = (query_heads * dim, dim)
     status = 0
     if workspace is not None:
-        status = _buffer(workspace, "rkv_append_status", (64,), device, torch.int32,
-                         zero=True).data_ptr()
+        status = _scratch(workspace, "rkv_append_status", 256, device).data_ptr()
     _native.launch(
         _native.load().rkv_paged_append,
         _native.APPEND_ARGS.pack(
