@@ -157,6 +157,14 @@ def _strides(tensor: torch.Tensor) -> tuple:
     return stride[:3] if len(stride) == 4 else (0, stride[0], stride[1])
 
 
+def _like(rows):
+    """An output for `rows`: their layout where they have one, each row contiguous in any case
+    (overlapping views may be given another innermost dimension)."""
+    out = torch.empty_like(rows)
+    return out if out.stride(-1) == 1 else torch.empty(rows.shape, device=rows.device,
+                                                       dtype=rows.dtype)
+
+
 def _launch(query, key, positions, cos_sin, interleaved, inverse, in_place):
     if query.stride(-1) != 1:
         if in_place:
@@ -165,7 +173,7 @@ def _launch(query, key, positions, cos_sin, interleaved, inverse, in_place):
     strides = out_strides = _strides(query)
     query_out = query
     if not in_place:
-        query_out = torch.empty_like(query)
+        query_out = _like(query)
         out_strides = _strides(query_out)
     key_out, key_ptr, key_out_ptr, key_heads = None, 0, 0, 0
     key_strides = key_out_strides = _NO_STRIDES
@@ -178,7 +186,7 @@ def _launch(query, key, positions, cos_sin, interleaved, inverse, in_place):
         key_out, key_ptr = key, key.data_ptr()
         key_out_ptr, key_heads = key_ptr, key.shape[-2]
         if not in_place:
-            key_out = torch.empty_like(key)
+            key_out = _like(key)
             key_out_ptr, key_out_strides = key_out.data_ptr(), _strides(key_out)
     batch, (tokens, heads, dim) = 1, query.shape[-3:]
     at = positions.stride()
