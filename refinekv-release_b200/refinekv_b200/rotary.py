@@ -12,6 +12,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from .summary import require_cuda_tensor
@@ -206,12 +207,21 @@ def _launch(query, key, positions, cos_sin, interleaved, inverse, in_place):
     return query_out, key_out
 
 
+def _is_dual(tensor) -> bool:
+    """Whether the tensor carries a tangent of forward-mode differentiation (outside of a dual
+    level, which is asked first because it is cheap, none does)."""
+    return (forward_ad._current_level >= 0 and tensor is not None
+            and forward_ad.unpack_dual(tensor).tangent is not None)
+
+
 class _Rotary(torch.autograd.Function):
-    """The rotation is linear in its rows: its backward pass is the inverse rotation."""
+    """The rotation is linear in its rows: its backward pass is the inverse rotation, and tangents
+    are rotated like the rows."""
 
     @staticmethod
     def forward(ctx, query, key, positions, cos_sin, interleaved, inverse):
         ctx.save_for_backward(positions, cos_sin)
+        ctx.save_for_forward(positions, cos_sin)
         ctx.flags = interleaved, inverse, key is not None
         out = _launch(query, key, positions, cos_sin, interleaved, inverse, False)
         return out if key is not None else out[0]
@@ -224,6 +234,14 @@ class _Rotary(torch.autograd.Function):
                                             cos_sin, interleaved=interleaved,
                                             inverse=not inverse)
         return query_grad, key_grad, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, query_tangent, key_tangent, *_):
+        positions, cos_sin = ctx.saved_tensors
+        interleaved, inverse, both = ctx.flags
+        out = apply_rotary(query_tangent, key_tangent if both else None, positions, cos_sin,
+                           interleaved=interleaved, inverse=inverse)
+        return out if both else out[0]
 
 
 def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor,
@@ -244,7 +262,7 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch
 
     Returns (query, key) in new tensors, or the arguments themselves when
     ``in_place`` (rows must then not overlap).  Differentiable in query and
-    key; the backward pass is one launch of the inverse rotation.
+    key, backward and forward; either is one more launch.
     """
     shape, dtype, device = query.shape, query.dtype, query.device
     lead, dim = shape[:-2], shape[-1]
@@ -267,10 +285,12 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch
     if positions.dtype not in _POSITIONS:
         raise TypeError("positions must be int32 or int64")
     check_table(cos_sin, dim, device)
-    if torch.is_grad_enabled() and (query.requires_grad
-                                    or (key is not None and key.requires_grad)):
+    if (torch.is_grad_enabled() and (query.requires_grad
+                                     or (key is not None and key.requires_grad))
+            or _is_dual(query) or _is_dual(key)):
         if in_place:
-            raise ValueError("rows that require a gradient cannot be rotated in place")
+            raise ValueError("rows that require a gradient or carry a tangent cannot be rotated "
+                             "in place")
         out = _Rotary.apply(query, key, positions, cos_sin, interleaved, inverse)
         return out if key is not None else (out, None)
     if in_place:
