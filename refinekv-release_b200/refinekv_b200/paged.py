@@ -27,7 +27,7 @@ import torch
 
 from . import _native
 from .attention import MAX_GROUP, _buffer, _scratch
-from .rotary import _DTYPES, _POSITIONS, check_table
+from .rotary import _DTYPES, _POSITIONS, check_table, mark_written
 from .summary import SUPPORTED_HEAD_DIMS, require_cuda_tensor
 
 _BLOCKS = (16, 32, 64)
@@ -180,6 +180,7 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Tensor,
             table_stride, sequences, blocks, pages, block, tokens, query_heads, heads, dim, rotary,
             rows, row_stride, _DTYPES[dtype], positions.dtype is torch.int64, interleaved),
         device)
+    mark_written(key_pool, value_pool)
     return out
 
 

@@ -214,6 +214,13 @@ def _is_dual(tensor) -> bool:
             and forward_ad.unpack_dual(tensor).tangent is not None)
 
 
+def mark_written(*tensors) -> None:
+    """Raise the version counters of tensors that a kernel wrote in place, so that autograd
+    refuses to use one that it saved before (inference tensors have no counter)."""
+    torch.autograd.graph.increment_version([t for t in tensors
+                                            if t is not None and not t.is_inference()])
+
+
 class _Rotary(torch.autograd.Function):
     """The rotation is linear in its rows: its backward pass is the inverse rotation, and tangents
     are rotated like the rows."""
@@ -298,4 +305,7 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch
             if rows is not None and any(s == 0 and n > 1
                                         for s, n in zip(rows.stride(), rows.shape)):
                 raise ValueError("overlapping rows cannot be rotated in place")
-    return _launch(query, key, positions, cos_sin, interleaved, inverse, in_place)
+    out = _launch(query, key, positions, cos_sin, interleaved, inverse, in_place)
+    if in_place:
+        mark_written(query, key)
+    return out

@@ -7,7 +7,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from refinekv_b200 import apply_rotary, rotary_table
+from refinekv_b200 import apply_rotary, paged_append, rotary_table
 from test_gpu_rotary import assert_rotated, rotate64
 
 pytestmark = pytest.mark.gpu
@@ -61,3 +61,42 @@ def test_tangents_are_not_rotated_in_place():
     with forward_ad.dual_level():
         with pytest.raises(ValueError, match="in place"):
             apply_rotary(forward_ad.make_dual(q, dq), None, at, table, in_place=True)
+
+
+def test_rows_rotated_in_place_cannot_be_what_autograd_saved():
+    q, k, _, _, at, table = _inputs()
+    for rows in (0, 1):
+        mine = [q.clone(), k.clone()]
+        weight = torch.ones_like(mine[rows], requires_grad=True)
+        loss = (weight * mine[rows]).sum()  # saves the rows for the weight's gradient
+        apply_rotary(mine[0], mine[1], at, table, in_place=True)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+
+def test_pools_written_by_an_append_cannot_be_what_autograd_saved():
+    pools = [torch.ones(2, 2, 16, 64, device=DEV, dtype=torch.bfloat16) for _ in "kv"]
+    k = torch.zeros(1, 2, 64, device=DEV, dtype=torch.bfloat16)
+    table = torch.zeros(1, 2, device=DEV, dtype=torch.int32)
+    at = torch.zeros(1, device=DEV, dtype=torch.int32)
+    for pool in pools:
+        weight = torch.ones_like(pool, requires_grad=True)
+        loss = (weight * pool).sum()
+        paged_append(k, k, *pools, table, at)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+
+def test_inference_tensors_are_written_all_the_same():
+    q, k, _, _, at, table = _inputs()
+    want = apply_rotary(q, k, at, table)
+    with torch.inference_mode():
+        mine = [q.clone(), k.clone()]
+        apply_rotary(*mine, at, table, in_place=True)
+        assert torch.equal(mine[0], want[0]) and torch.equal(mine[1], want[1])
+        pools = [torch.zeros(2, 2, 16, 64, device=DEV, dtype=torch.bfloat16) for _ in "kv"]
+        row = torch.ones(1, 2, 64, device=DEV, dtype=torch.bfloat16)
+        paged_append(row, row, *pools, torch.zeros(1, 2, device=DEV, dtype=torch.int32),
+                     torch.zeros(1, device=DEV, dtype=torch.int32))
+        assert float(pools[0].sum()) == 128.0 == float(pools[1].sum())
+    apply_rotary(*mine, at, table, inverse=True, in_place=True)  # and outside of the mode
