@@ -269,7 +269,8 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch
 
     Returns (query, key) in new tensors, or the arguments themselves when
     ``in_place`` (rows must then not overlap).  Differentiable in query and
-    key, backward and forward; either is one more launch.
+    key, backward and forward, either one more launch; a ``cos_sin`` that
+    requires a gradient is refused.
     """
     shape, dtype, device = query.shape, query.dtype, query.device
     lead, dim = shape[:-2], shape[-1]
@@ -292,6 +293,8 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch
     if positions.dtype not in _POSITIONS:
         raise TypeError("positions must be int32 or int64")
     check_table(cos_sin, dim, device)
+    if (cos_sin.requires_grad and torch.is_grad_enabled()) or _is_dual(cos_sin):
+        raise ValueError("apply_rotary has no gradient for cos_sin: detach it")
     if (torch.is_grad_enabled() and (query.requires_grad
                                      or (key is not None and key.requires_grad))
             or _is_dual(query) or _is_dual(key)):

@@ -63,6 +63,26 @@ def test_tangents_are_not_rotated_in_place():
             apply_rotary(forward_ad.make_dual(q, dq), None, at, table, in_place=True)
 
 
+def test_a_table_that_wants_a_gradient_is_refused():
+    q, k, _, _, at, table = _inputs()
+    learnt = table.clone().requires_grad_()
+    with pytest.raises(ValueError, match="cos_sin"):
+        apply_rotary(q, k, at, learnt)
+    with pytest.raises(ValueError, match="cos_sin"):
+        apply_rotary(q.clone().requires_grad_(), k, at, learnt)
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="cos_sin"):
+            apply_rotary(q, k, at, forward_ad.make_dual(table, table))
+    want = apply_rotary(q, k, at, table)
+    for got in (apply_rotary(q, k, at, learnt.detach()), _no_grad(q, k, at, learnt)):
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@torch.no_grad()
+def _no_grad(q, k, at, table):
+    return apply_rotary(q, k, at, table)
+
+
 def test_rows_rotated_in_place_cannot_be_what_autograd_saved():
     q, k, _, _, at, table = _inputs()
     for rows in (0, 1):
