@@ -60,11 +60,16 @@ class Decoder:
 
 
 class Server:
-    def __init__(self, model: Decoder, prompts, new_tokens: int, config=None, positions=4096):
+    """``positions``: rows of the rotation table, by default as many as the longest request has."""
+
+    def __init__(self, model: Decoder, prompts, new_tokens: int, config=None, positions=None):
         self.m, self.new, self.config = model, new_tokens, config or rkv.RefineKVConfig()
         dev = model.embed.device
         self.n = len(prompts)
-        self.cos_sin = rkv.rotary_table(model.dim, positions, device=dev)
+        longest = max(map(len, prompts)) + new_tokens
+        if positions is not None and positions < longest:
+            raise ValueError(f"positions: the longest request has {longest} tokens")
+        self.cos_sin = rkv.rotary_table(model.dim, positions or longest, device=dev)
         # Every request takes the pages of its prompt and its new tokens from the free list.
         need = [-(-(len(p) + new_tokens) // BLOCK) for p in prompts]
         free = torch.randperm(sum(need) + 1, device=dev).to(torch.int32)
