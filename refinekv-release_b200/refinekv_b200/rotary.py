@@ -264,7 +264,9 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch
     (positions, rotary_dim) table (``rotary_table``); its width rotary_dim may
     be less than head_dim: the channels after it are copied.  Pair i of the
     rotary channels is (i, i + rotary_dim / 2), or (2i, 2i + 1) with
-    ``interleaved``.  ``inverse`` turns back.  A position outside the table
+    ``interleaved``.  ``inverse`` negates the sines: the transposed map, which is the
+    backward pass, and which undoes a rotation where the table's amplitude is 1 (with
+    amplitude a the two give a^2 times the rows).  A position outside the table
     gives NaN in the rotary channels.
 
     Returns (query, key) in new tensors, or the arguments themselves when
