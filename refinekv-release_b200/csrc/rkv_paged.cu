@@ -7,15 +7,18 @@
 //
 // Bound: HBM on long sequences.  Each visible K and V row is read once (4 D
 // bytes for 4 G D flop, G <= 16).  mma.sync with the tokens on M and the group
-// on N keeps the tensor pipe 10 % active at the streaming rate, so tcgen05
+// on N keeps the tensor pipe 13 % active at the streaming rate, so tcgen05
 // (M = 64 at least, operands from shared-memory descriptors) would not move
 // the bound.  Measured on B200 (graph replay): 16 sequences of 32K tokens, 8 KV
-// heads, D 128: 317-324 us for 2.15 GB, 6.7 TB/s, more than a plain copy reaches;
-// one of 128K: 86 us for 537 MB (6.2 TB/s; the SMs that stream slowest, about a
-// fifth of them, end 10 us after the mean, and equal shares cannot follow that);
-// a ragged batch of 43, 270 MB: 51 us.  About 5 us before the stream is up and 4
-// to 6 for the joins at its end are what short calls consist of: one sequence of
-// 333 tokens takes 7.8 us.
+// heads, D 128: 320-326 us for 2.15 GB, 6.6-6.7 TB/s, what a plain copy reaches or
+// a little more; one of 128K: 87 us for 537 MB (6.2 TB/s; the SMs that stream
+// slowest, about a fifth of them, end 10 us after the mean, and equal shares
+// cannot follow that); a ragged batch of 43, 270 MB: 52 us.  About 5 us before
+// the stream is up and 4 to 6 for the joins at its end are what short calls
+// consist of: one sequence of 333 tokens takes 8.3 us.  Sixteen queries a KV head
+// of D 192 or 256 spill a little (200 and 292 bytes of stores a thread): 8
+// sequences of 32K tokens, 2 KV heads, D 256: 103 us for 537 MB, against 97 with
+// eight queries; D 192: 82 us for 403 MB, against 72 with four.
 //
 // Split.  The tiles of all rows, sequence-major then head, form one list that
 // is cut into equal contiguous ranges, one per CTA, and each CTA's range into
@@ -47,17 +50,19 @@ namespace {
 // Tokens per tile: 64 for head dims up to 64, else 32, so that a K and V tile
 // is 16 KB at D 64 and 128.
 constexpr int tile_rows(int D) { return D <= 64 ? 64 : 32; }
-// One stage (a K and a V tile) per warp, up to eight warps.  Six warps take 86 us
-// for one sequence of 128K tokens against 88, but 47.6 against 46.5 for a
-// ragged batch of 32 and 26 against 24 at D 64; two CTAs of four warps per SM
-// cost 2 to 4 us on every batch (more parts to join).
+// One stage (a K and a V tile) per warp, up to eight warps.  Eight against six:
+// one sequence of 2K tokens 9.4 us against 11.3, one of 128K 87.3 against 88.0, a
+// ragged batch of 43 51.0 against 53.5, D 64 23.4 against 25.1; only 16 sequences of
+// 32K are faster with six, 313 against 326.  Two CTAs of four warps per SM cost 2
+// to 4 us on every batch (more parts to join).
 constexpr int paged_warps(int D) { return D <= 192 ? 8 : 6; }
 constexpr int stage_bytes(int D) { return 2 * tile_rows(D) * D * 2; }
 
 // A row's CTAs are joined in one level up to this many, else in groups of about
 // the square root.  24 against 32: three ragged D 256 sequences (24 to 39 parts)
-// 36.9 against 43 us, 8K tokens of one head 13.4 against 14.8; 16: 128K tokens
-// of eight heads (18 parts) 87.6 against 87.0; 80 and 160: up to 18 us more.
+// 37.5 against 44.3 us, 8K tokens of one head (32 parts) 11.4 against 11.7; 16: 128K
+// tokens of eight heads (18 parts) 88.2 against 87.3, 21 and 24 parts the same;
+// 80 and 160: up to 18 us more.
 constexpr int kFlatJoin = 24;
 
 // Workspace: status word, counters (at the same place for every geometry;
@@ -510,11 +515,11 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   }
   // How many CTAs share the tiles.  Many rows: every SM, but a tile a warp at
   // least.  Few rows: whole CTAs per row where that leaves few SMs idle, since a
-  // CTA with one row has one join less (three D 256 sequences 36.7 us against 39.7
-  // with every SM, two of 60K tokens 79.1 against 80.1, one of 128K 86.8 against
-  // 86.6), and no more of them than give every warp a tile (2K tokens, 8 heads: 9.3
-  // us against 10.4 with two tiles a warp), one for a row of up to two tiles a warp
-  // (333 tokens: 7.9 us against 8.3 with a tile a warp and a join across CTAs).
+  // CTA with one row has one join less (three D 256 sequences 37.5 us against 40.5
+  // with every SM, two of 60K tokens 79.7 against 80.3, one of 128K 87.3 against
+  // 87.5), and no more of them than give every warp a tile (2K tokens, 8 heads: a
+  // microsecond less than with two tiles a warp), one for a row of up to two tiles a
+  // warp (333 tokens: 8.3 us against 8.9 with a tile a warp and a join across CTAs).
   const unsigned rows = static_cast<unsigned>(busy) * p.heads, grid = gridDim.x;
   unsigned C = min(grid, (T + W - 1) / W);
   if (rows > 0 && rows <= grid) {
@@ -820,7 +825,10 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
       const auto put = [&](int d, float m, float l, const float4& o) {
         put_joined<D, G8>(p, cut.row, g, d, target, m, l, o);
       };
-      // Eight rows over the whole GPU are 18 or 19 parts each: in one batch.
+      // More than one batch's parts, up to 24 (kFlatJoin) or a group's: in twenties.
+      // A row of 18 parts (128K tokens, eight heads) 87.3 us against 87.9 in eights,
+      // 21 and 24 parts (16K tokens, seven and six heads) 18.8 and 17.2 against 18.6
+      // and 17.0.
       if (kLanes == D / 4 && members >> kBatch) {
         join<D, kLanes, 20>(members, x % kLanes, m_of, l_of, o_of, put);
       } else {
