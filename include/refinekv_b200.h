@@ -66,6 +66,8 @@ typedef enum rkv_status {
 /* Query / output dtypes. */
 #define RKV_DTYPE_BF16 0
 #define RKV_DTYPE_F32 1
+/* Page pools of 4 bits (rkv_paged_append_fp4 says how they hold a row). */
+#define RKV_DTYPE_FP4 2
 
 /* Phases of rkv_decode (bit mask; RKV_PHASE_ALL for a normal call). */
 #define RKV_PHASE_STATS 1  /* selector phase A: scores, deltas, LSE partials */
@@ -534,6 +536,71 @@ typedef struct rkv_append_args {
   int64_t interleaved;
 } rkv_append_args;
 RKV_API int rkv_paged_append(const rkv_append_args* args, void* stream);
+
+/*
+ * Append new tokens to a page pool of 4 bits, rotating keys (and queries) on
+ * the way: rkv_paged_append with another pool.  Per 16 channels x of a row
+ * (divided by the KV head's factor, where there is one):
+ *   scale = e4m3(max |x| / 6), code = e2m1(x / scale),
+ * each to the nearest, ties to even, beyond 448 and 6 to those; the channel
+ * then stands for code * scale * factor.  16 channels whose greatest is below
+ * 2^-10 * 6 become zero; 16 channels with an infinity or a NaN become NaN.
+ *   pools: bytes.  The slab of a page's KV head is block_size * head_dim * 9 /
+ *   16 contiguous bytes: the codes of its rows, row after row (head_dim / 2
+ *   bytes each, channel 2i in the low half of byte i), then the scales of its
+ *   rows (head_dim / 16 bytes each).  rows.key_pool_strides and
+ *   rows.value_pool_strides hold the byte strides [page, head], multiples of 16
+ *   like the pools' addresses; their third entry is not used.
+ *   key_scale / value_scale: fp32 (kv_heads,) factors on the device, or null
+ *   for 1: what brings a head's channels into the scales' range.
+ */
+typedef struct rkv_append_fp4_args {
+  rkv_append_args rows;
+  const float* key_scale;
+  const float* value_scale;
+} rkv_append_fp4_args;
+RKV_API int rkv_paged_append_fp4(const rkv_append_fp4_args* args, void* stream);
+
+/*
+ * Rows of a page pool back as numbers: the counterpart of the appends.  Token t
+ * is token positions[t] of sequence sequence_ids[t] (t itself when null); its
+ * key and value rows go to row t of key_out and value_out, (tokens, kv_heads,
+ * head_dim) of `dtype` by element strides [token, head], rounded once.  A
+ * negative position gives zero rows; one past the sequence's table row, a
+ * sequence id outside [0, sequences) or a page outside [0, pool_pages) sets
+ * RKV_DEVICE_BAD_INPUT in *status (when given) and gives NaN rows.
+ *   pool_dtype RKV_DTYPE_BF16: strides in elements [page, head, row];
+ *   RKV_DTYPE_FP4: in bytes [page, head], with the appends' factors.
+ * Pools, outputs and their strides are multiples of 16 bytes.
+ */
+typedef struct rkv_read_args {
+  const void* key_pool;
+  const void* value_pool;
+  void* key_out;
+  void* value_out;
+  const int32_t* page_table;
+  const int32_t* sequence_ids;
+  const void* positions;
+  int32_t* status;
+  const float* key_scale;
+  const float* value_scale;
+  int64_t key_pool_strides[3];
+  int64_t value_pool_strides[3];
+  int64_t key_out_strides[2];
+  int64_t value_out_strides[2];
+  int64_t page_table_stride;
+  int64_t sequences;
+  int64_t table_blocks;
+  int64_t pool_pages;
+  int64_t block_size;
+  int64_t tokens;
+  int64_t kv_heads;
+  int64_t head_dim;
+  int64_t pool_dtype;
+  int64_t dtype;
+  int64_t positions_i64;
+} rkv_read_args;
+RKV_API int rkv_paged_read(const rkv_read_args* args, void* stream);
 
 /*
  * Dense attention of one new token per sequence over a page pool (no

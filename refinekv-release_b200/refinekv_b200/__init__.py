@@ -11,7 +11,8 @@ cache write and the summary in one pass), ``attach_page_pool`` (decode from a
 vLLM-style K/V page pool through a page table), ``page_view`` and
 ``dense_attention`` (dense decode of the full-attention layers on the same
 kernel), ``rotary_table`` / ``apply_rotary`` (rotary positions),
-``paged_append`` (new tokens into the page pool, rotated on the way),
+``paged_append`` (new tokens into the page pool, rotated on the way; ``fp4_pool`` for one
+of 4 bits), ``paged_read`` (its rows back),
 ``paged_attention`` (dense attention of one new token per sequence, each over
 its own length of the pool) and ``refinekv_b200.parallel`` (KV-head sharding and sequence split
 over GPUs).
@@ -39,7 +40,9 @@ __all__ = [
     "sparse_attention",
     "rotary_table",
     "apply_rotary",
+    "fp4_pool",
     "paged_append",
+    "paged_read",
     "paged_attention",
     "RefineKV",
     "make_visible_static_cache",
@@ -51,7 +54,7 @@ _HOMES = {
     "summary": ("BlockSummary", "build_summary", "build_summary_batch", "build_summary_into",
                 "attach_page_pool", "page_view", "PageView"),
     "rotary": ("rotary_table", "apply_rotary"),
-    "paged": ("paged_append", "paged_attention"),
+    "paged": ("fp4_pool", "paged_append", "paged_read", "paged_attention"),
     "integrations.transformers": ("RefineKV", "make_visible_static_cache"),
 }
 

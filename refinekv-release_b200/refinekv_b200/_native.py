@@ -29,6 +29,7 @@ DEVICE_BAD_INPUT = 2
 GQA_CODES = {"mean": 0, "max": 1, "any": 2}
 DTYPE_BF16 = 0
 DTYPE_F32 = 1
+DTYPE_FP4 = 2
 
 PHASE_STATS = 1
 PHASE_FINAL = 2
@@ -63,6 +64,8 @@ EXPORTS = (
     "rkv_decode_split",
     "rkv_rotary",
     "rkv_paged_append",
+    "rkv_paged_append_fp4",
+    "rkv_paged_read",
     "rkv_paged_workspace_size",
     "rkv_paged_attention",
     "rkv_selftest_wait_timeout",
@@ -106,11 +109,12 @@ class Summary(ctypes.Structure):
     ]
 
 
-#: ``struct rkv_rotary_args``, ``rkv_append_args`` and ``rkv_paged_args``: 8-byte fields only,
-#: packed in the header's order (pointers as integers, 0 for null).  Packing costs a tenth of filling a
+#: ``struct rkv_rotary_args``, ``rkv_append_args`` and so on: 8-byte fields only, packed in the header's order (pointers as integers, 0 for null).  Packing costs a tenth of filling a
 #: ``ctypes.Structure``, which counts in calls whose kernel takes a few microseconds.
 ROTARY_ARGS = struct.Struct("=32q")
 APPEND_ARGS = struct.Struct("=40q")
+APPEND_FP4_ARGS = struct.Struct("=42q")
+READ_ARGS = struct.Struct("=31q")
 PAGED_ARGS = struct.Struct("=27qd")
 
 _SIGNATURES = {
@@ -160,6 +164,8 @@ _SIGNATURES = {
     # The argument structs of the paged operators are packed bytes (ROTARY_ARGS and so on).
     "rkv_rotary": (ctypes.c_int, [ctypes.c_char_p, c_ptr]),
     "rkv_paged_append": (ctypes.c_int, [ctypes.c_char_p, c_ptr]),
+    "rkv_paged_append_fp4": (ctypes.c_int, [ctypes.c_char_p, c_ptr]),
+    "rkv_paged_read": (ctypes.c_int, [ctypes.c_char_p, c_ptr]),
     "rkv_paged_workspace_size": (ctypes.c_size_t, [c_i64, c_i64]),
     "rkv_paged_attention": (ctypes.c_int, [ctypes.c_char_p, c_ptr]),
     "rkv_selftest_wait_timeout": (ctypes.c_int, [c_ptr, c_i64, c_ptr]),

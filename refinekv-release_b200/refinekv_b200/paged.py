@@ -4,11 +4,13 @@ No counterpart in the reference, which keeps one contiguous cache per layer
 and decodes one sequence.  A server keeps the keys and values of many
 sequences of different lengths in a pool of fixed-size pages; a page table
 gives each sequence's pages.  ``attach_page_pool`` lets the refined layers
-decode from such a pool; here is what fills it (``paged_append``) and what
-the dense layers decode with (``paged_attention``).
+decode from such a pool; here is what fills it (``paged_append``), what reads
+rows back (``paged_read``) and what the dense layers decode with
+(``paged_attention``).
 
 Pools are bf16, ``(pages, kv_heads, block, dim)`` (``layout="HND"``) or
-``(pages, block, kv_heads, dim)`` (``"NHD"``); page tables are int32
+``(pages, block, kv_heads, dim)`` (``"NHD"``), or hold a row in 4 bits a
+channel (``fp4_pool``); page tables are int32
 ``(sequences, blocks)``.  Everything that changes from step to step
 (positions, lengths, page tables) is read on the device, so a captured CUDA
 graph serves growing sequences.  Results carry no gradient.
@@ -69,6 +71,69 @@ def _pools(key_pool, value_pool, layout):
     return pages, heads, block, dim, ks, vs
 
 
+def fp4_pool(pages: int, kv_heads: int, block: int, head_dim: int, *, device="cuda") -> torch.Tensor:
+    """A zeroed page pool of 4 bits a channel: (pages, kv_heads, block, head_dim * 9 / 16) bytes.
+
+    16 channels share an e4m3 scale (the greatest of them / 6), and a channel is
+    one of 0, 0.5, 1, 1.5, 2, 3, 4 or 6 times it, with a sign: 72 bytes for a row of
+    128 instead of 256.  The slab of a page's KV head, ``pool[page, head]``, holds
+    the codes of its rows, row after row (head_dim / 2 bytes each, channel 2i in
+    the low half of byte i), then their scales (head_dim / 16 bytes each).
+    ``paged_append``, ``paged_read`` and ``paged_attention`` take such pools where
+    they take bf16 ones, with an optional fp32 factor for each KV head
+    (``key_scale``, ``value_scale``: a row is divided by it before it is held, and
+    multiplied by it after): scales lie between 2^-9 and 448, so channels above
+    2688 times the factor are cut off and ones far below 0.01 times it lose digits.
+    """
+    if block not in _BLOCKS:
+        raise ValueError("pool blocks must hold 16, 32 or 64 tokens")
+    if head_dim not in SUPPORTED_HEAD_DIMS:
+        raise ValueError(f"head_dim must be one of {SUPPORTED_HEAD_DIMS}")
+    if pages < 0 or kv_heads < 1:
+        raise ValueError("a pool has pages of at least one KV head")
+    return torch.zeros(pages, kv_heads, block, head_dim * 9 // 16, device=device, dtype=torch.uint8)
+
+
+def _fp4_pools(key_pool, value_pool, layout):
+    """``_pools`` of two pools of 4 bits: strides in bytes, the third of them unused."""
+    if layout != "HND":
+        raise ValueError("a pool of 4 bits has layout 'HND'")
+    shape = key_pool.shape
+    if len(shape) != 4 or value_pool.shape != shape:
+        raise ValueError("key and value pools must have the same 4-D shape")
+    if not key_pool.is_cuda:
+        require_cuda_tensor(key_pool, "key_pool")
+    if value_pool.dtype is not torch.uint8:
+        raise TypeError("key and value pools must both be bf16 or both of 4 bits (uint8)")
+    if value_pool.device != key_pool.device:
+        raise ValueError("key and value pools must be on the same device")
+    pages, heads, block, row = shape
+    dim = row * 16 // 9
+    if dim not in SUPPORTED_HEAD_DIMS or dim * 9 != row * 16:
+        raise ValueError(f"a pool of 4 bits has rows of 9 / 16 of a head_dim in {SUPPORTED_HEAD_DIMS}")
+    if block not in _BLOCKS:
+        raise ValueError("pool blocks must hold 16, 32 or 64 tokens")
+    ks, vs = key_pool.stride(), value_pool.stride()
+    if ks[2:] != (row, 1) or vs[2:] != (row, 1):
+        raise ValueError("the slab of a page's KV head must be contiguous")
+    return pages, heads, block, dim, (*ks[:2], 0), (*vs[:2], 0)
+
+
+def _factors(key_scale, value_scale, heads, device):
+    """The addresses of the KV heads' factors of a pool of 4 bits (0: none)."""
+    at = [0, 0]
+    for i, factor in enumerate((key_scale, value_scale)):
+        if factor is None:
+            continue
+        if factor.shape != (heads,) or factor.device != device or factor.stride(0) != 1:
+            raise ValueError("key_scale and value_scale must be contiguous (kv_heads,) on the "
+                             "pools' device")
+        if factor.dtype is not torch.float32:
+            raise TypeError("key_scale and value_scale must be fp32")
+        at[i] = factor.data_ptr()
+    return at
+
+
 def _table(page_table, device):
     """(sequences, blocks, stride) of an int32 page table (1-D: one sequence)."""
     shape, stride = page_table.shape, page_table.stride()
@@ -86,7 +151,9 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Tensor,
                  value_pool: torch.Tensor, page_table: torch.Tensor, positions: torch.Tensor, *,
                  layout: str = "HND", sequence_ids: torch.Tensor | None = None,
                  query: torch.Tensor | None = None, cos_sin: torch.Tensor | None = None,
-                 interleaved: bool = False, workspace: dict | None = None) -> torch.Tensor | None:
+                 interleaved: bool = False, key_scale: torch.Tensor | None = None,
+                 value_scale: torch.Tensor | None = None,
+                 workspace: dict | None = None) -> torch.Tensor | None:
     """Write new tokens' keys and values into the pool's pages, rotated on the way.
 
     ``key``/``value``: (tokens, kv_heads, head_dim) bf16 or fp32, any strides
@@ -96,7 +163,10 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Tensor,
     goes to page ``page_table[sequence, position // block]``, row
     ``position % block``, rounded once to bf16.  With ``cos_sin`` (see
     ``apply_rotary``) keys are rotated by their positions first, and so is
-    ``query`` ((tokens, q_heads, head_dim), the keys' dtype) when given.
+    ``query`` ((tokens, q_heads, head_dim), the keys' dtype) when given.  Into
+    pools of 4 bits (``fp4_pool``) rows go from fp32 in one rounding too, divided by
+    ``key_scale`` and ``value_scale`` ((kv_heads,) fp32) where these are given; 16
+    channels that hold an infinity or a NaN become NaN.
 
     Returns the rotated queries (backed by ``workspace``, reused by the next
     call of the same shape), or None without ``query``.  The pools are
@@ -109,8 +179,14 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Tensor,
     outside the pool writes nothing and sets bit 1 of the status word
     (``attention.device_status(workspace)``).
     """
-    pages, heads, block, dim, ks, vs = _pools(key_pool, value_pool, layout)
+    fp4 = key_pool.dtype is torch.uint8
+    pages, heads, block, dim, ks, vs = (_fp4_pools if fp4 else _pools)(key_pool, value_pool, layout)
     device = key_pool.device
+    factors = ()
+    if fp4:
+        factors = _factors(key_scale, value_scale, heads, device)
+    elif key_scale is not None or value_scale is not None:
+        raise ValueError("key_scale and value_scale belong to pools of 4 bits")
     sequences, blocks, table_stride = _table(page_table, device)
     shape, dtype = key.shape, key.dtype
     if len(shape) != 3 or value.shape != shape or shape[1] != heads or shape[2] != dim:
@@ -165,23 +241,88 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Tensor,
             query_strides = query.stride()
         query_strides = query_strides[:2]
         out = _buffer(workspace, "append_query", like, device, dtype)
+        if fp4 and out.data_ptr() == query.data_ptr():  # partners are read by several threads
+            query = query.clone()
         query_ptr, out_ptr, query_heads = query.data_ptr(), out.data_ptr(), like[1]
         out_strides = (query_heads * dim, dim)
     status = 0
     if workspace is not None:
         status = _scratch(workspace, "rkv_append_status", 256, device).data_ptr()
+    lib = _native.load()
     _native.launch(
-        _native.load().rkv_paged_append,
-        _native.APPEND_ARGS.pack(
+        lib.rkv_paged_append_fp4 if fp4 else lib.rkv_paged_append,
+        (_native.APPEND_FP4_ARGS if fp4 else _native.APPEND_ARGS).pack(
             key.data_ptr(), value.data_ptr(), query_ptr, out_ptr, key_pool.data_ptr(),
             value_pool.data_ptr(), page_table.data_ptr(), ids, positions.data_ptr(), table, status,
             key_strides[0], key_strides[1], value_strides[0], value_strides[1], *query_strides,
             *out_strides, *ks, *vs,
             table_stride, sequences, blocks, pages, block, tokens, query_heads, heads, dim, rotary,
-            rows, row_stride, _DTYPES[dtype], positions.dtype is torch.int64, interleaved),
+            rows, row_stride, _DTYPES[dtype], positions.dtype is torch.int64, interleaved, *factors),
         device)
     mark_written(key_pool, value_pool)
     return out
+
+
+def paged_read(key_pool: torch.Tensor, value_pool: torch.Tensor, page_table: torch.Tensor,
+               positions: torch.Tensor, *, layout: str = "HND",
+               sequence_ids: torch.Tensor | None = None, key_scale: torch.Tensor | None = None,
+               value_scale: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16,
+               workspace: dict | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values that a pool's pages hold, as dense rows: ``paged_append`` read back.
+
+    Token t is token ``positions[t]`` (int32 or int64) of sequence
+    ``sequence_ids[t]`` (int32; without it token t is one of sequence t).
+    Returns new (tokens, kv_heads, head_dim) keys and values in ``dtype`` (bf16 or
+    fp32): what a chunk of a prompt needs of the tokens before it, or a summary
+    of a pool of 4 bits (its rows in bf16 are exact where there is no ``key_scale``
+    or ``value_scale``).  A negative position gives a zero row.  A position past
+    the page table's row, a sequence id outside the page table or a page outside
+    the pool gives a NaN row and sets bit 1 of the status word
+    (``attention.device_status(workspace)``).
+    """
+    fp4 = key_pool.dtype is torch.uint8
+    pages, heads, block, dim, ks, vs = (_fp4_pools if fp4 else _pools)(key_pool, value_pool, layout)
+    device = key_pool.device
+    if fp4:
+        factors = _factors(key_scale, value_scale, heads, device)
+    elif key_scale is not None or value_scale is not None:
+        raise ValueError("key_scale and value_scale belong to pools of 4 bits")
+    else:
+        factors = (0, 0)
+    sequences, blocks, table_stride = _table(page_table, device)
+    if positions.ndim != 1 or positions.device != device:
+        raise ValueError("positions must be (tokens,) on the pools' device")
+    if positions.dtype not in _POSITIONS:
+        raise TypeError("positions must be int32 or int64")
+    if dtype not in _DTYPES:
+        raise TypeError("rows are read as BF16 or FP32")
+    tokens = positions.shape[0]
+    ids = 0
+    if sequence_ids is None:
+        if tokens > sequences:
+            raise ValueError("more tokens than sequences: pass sequence_ids")
+    else:
+        if sequence_ids.shape != (tokens,) or sequence_ids.device != device:
+            raise ValueError("sequence_ids must be (tokens,) on the pools' device")
+        if sequence_ids.dtype != torch.int32:
+            raise TypeError("sequence_ids must be int32")
+        sequence_ids = sequence_ids.contiguous()
+        ids = sequence_ids.data_ptr()
+    positions = positions.contiguous()
+    keys, values = torch.empty(2, tokens, heads, dim, device=device, dtype=dtype)
+    status = 0
+    if workspace is not None:
+        status = _scratch(workspace, "rkv_append_status", 256, device).data_ptr()
+    _native.launch(
+        _native.load().rkv_paged_read,
+        _native.READ_ARGS.pack(
+            key_pool.data_ptr(), value_pool.data_ptr(), keys.data_ptr(), values.data_ptr(),
+            page_table.data_ptr(), ids, positions.data_ptr(), status, *factors, *ks, *vs,
+            heads * dim, dim, heads * dim, dim, table_stride, sequences, blocks, pages, block, tokens,
+            heads, dim, _native.DTYPE_FP4 if fp4 else _native.DTYPE_BF16, _DTYPES[dtype],
+            positions.dtype is torch.int64),
+        device)
+    return keys, values
 
 
 def paged_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor,
