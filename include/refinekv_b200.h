@@ -660,6 +660,44 @@ RKV_API size_t rkv_paged_workspace_size(int64_t group, int64_t head_dim);
 RKV_API int rkv_paged_attention(const rkv_paged_args* args, void* stream);
 
 /*
+ * rkv_paged_attention with more to it, over pools of bf16 or of 4 bits.  The
+ * logit of row j, of L visible up to the newest, for query row r:
+ *   x_j = c tanh(scale q.k_j / c) + slopes[r] (j - (L - 1)),
+ * c = softcap (0: no cap), slopes fp32 (kv_heads * group) or null; visible are
+ * the rows j in [max(0, L - window), L) and j < prefix (a prefix matters next to
+ * a window).  Everything else is as in rkv_paged_attention.
+ *   pool_dtype RKV_DTYPE_FP4: base's pool strides are bytes [page, head], the
+ *   third unused (rkv_paged_append_fp4 describes the pool); key_scale and
+ *   value_scale are its factors, fp32 (kv_heads) or null for 1.
+ *   weights: null, or fp32 rows of weight_width >= table_blocks * block_size
+ *   tokens, element strides [sequence, KV head]: to each visible row's is added
+ *     sum over the group of exp(x_j - lse),
+ *   what this step's queries gave it; a query whose lse is not finite adds
+ *   nothing.  base.lse must be given then, and `scores`: scores_size bytes of
+ *   scratch (16-byte aligned, of any content) for sequences * kv_heads * group *
+ *   table_blocks * block_size logits.  Takes a second launch.
+ * The workspace's size comes from rkv_paged_more_workspace_size; workspaces of
+ * rkv_paged_attention that are large enough serve here too, and the other way
+ * round.
+ */
+typedef struct rkv_paged_more_args {
+  rkv_paged_args base;
+  const float* slopes;
+  const float* key_scale;
+  const float* value_scale;
+  float* weights;
+  float* scores;
+  int64_t scores_size;
+  int64_t weight_strides[2];
+  int64_t weight_width;
+  int64_t pool_dtype;
+  int64_t prefix;
+  double softcap;
+} rkv_paged_more_args;
+RKV_API size_t rkv_paged_more_workspace_size(int64_t group, int64_t head_dim, int64_t pool_dtype);
+RKV_API int rkv_paged_attention_more(const rkv_paged_more_args* args, void* stream);
+
+/*
  * Diagnostic: one bounded device wait on an mbarrier that nothing completes,
  * with a limit of `limit_ns` (0 < limit_ns <= 1e9) instead of the kernels'
  * 1 s; it ORs RKV_DEVICE_TIMEOUT into the device int32 *status and returns,

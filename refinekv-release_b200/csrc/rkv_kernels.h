@@ -325,7 +325,41 @@ struct PagedParams {
   float* warp_partials;   // one per warp, for wide heads
   float* cta_partials;    // two per CTA
   float* group_partials;  // two per CTA
+  // rkv_paged_attention_more
+  int prefix;                // tokens that stay visible next to a window
+  float softcap;             // 0: none
+  const float* slopes;       // (heads * group) or null
+  const float* key_scale;    // (heads) or null: pools of 4 bits
+  const float* value_scale;
+  float* scores;             // logits, (sequences, heads * group, capacity), or null
 };
+
+struct PagedLayout {  // byte offsets into the workspace
+  size_t warp_partials, cta_partials, group_partials, bytes;
+};
+
+// Pools of 4 bits: byte strides of a page and a KV head's slab.
+struct Fp4Pages {
+  const uint8_t* keys;
+  const uint8_t* values;
+  int64_t key_page, key_head, value_page, value_head;
+};
+constexpr int kFp4Rows = 64;  // tokens of a tile
+
+struct WeightParams {
+  float* weights;  // rows of tokens, element strides of a sequence and a KV head
+  int64_t seq_stride, head_stride;
+};
+
+cudaError_t launch_paged_more(const PagedMaps& maps, const PagedParams& p, int D, int ctas,
+                              cudaStream_t stream);
+cudaError_t launch_paged_fp4(const Fp4Pages& pages, const PagedParams& p, int ctas,
+                             cudaStream_t stream);
+cudaError_t launch_paged_fp4_wide(const Fp4Pages& pages, const PagedParams& p, int ctas,
+                                  cudaStream_t stream);
+PagedLayout fp4_layout(int64_t group, int64_t dim, int sms);
+// Adds each visible token's weight, from the call's logits and sums.
+cudaError_t launch_weights(const WeightParams& w, const PagedParams& p, cudaStream_t stream);
 
 // Whether pointers (null or not) are aligned to elements of `bytes`.
 inline bool aligned_to(int bytes, std::initializer_list<const void*> pointers) {

@@ -1,4 +1,6 @@
-// Dense attention of one new token per sequence over a page pool, in one launch.
+// Dense attention of one new token per sequence over a page pool, in one launch:
+// the kernel, included by the files that instantiate it for pools of bf16
+// (rkv_paged_api.cu, rkv_paged_more.cu) and of 4 bits (rkv_paged_fp4.cu).
 //
 // Mathematics.  Per sequence s and KV head h a row of `group` queries attends
 // to the visible tokens of its sequence: an online softmax over tiles of R
@@ -34,8 +36,10 @@
 //
 // The lengths and the page table are read on the device (graphs replay with
 // growing sequences): every CTA scans the lengths itself.
+#ifndef RKV_PAGED_CU_
+#define RKV_PAGED_CU_
+
 #include <algorithm>
-#include <string>
 
 #include "refinekv_b200.h"
 #include "rkv_device.cuh"
@@ -43,20 +47,7 @@
 #include "rkv_kernels.h"
 
 namespace rkv {
-void set_last_error(const std::string& message);
-
 namespace {
-
-// Tokens per tile: 64 for head dims up to 64, else 32, so that a K and V tile
-// is 16 KB at D 64 and 128.
-constexpr int tile_rows(int D) { return D <= 64 ? 64 : 32; }
-// One stage (a K and a V tile) per warp, up to eight warps.  Eight against six:
-// one sequence of 2K tokens 9.4 us against 11.3, one of 128K 87.3 against 88.0, a
-// ragged batch of 43 51.0 against 53.5, D 64 23.4 against 25.1; only 16 sequences of
-// 32K are faster with six, 313 against 326.  Two CTAs of four warps per SM cost 2
-// to 4 us on every batch (more parts to join).
-constexpr int paged_warps(int D) { return D <= 192 ? 8 : 6; }
-constexpr int stage_bytes(int D) { return 2 * tile_rows(D) * D * 2; }
 
 // A row's CTAs are joined in one level up to this many, else in groups of about
 // the square root.  24 against 32: three ragged D 256 sequences (24 to 39 parts)
@@ -77,35 +68,27 @@ constexpr size_t kHeader = 8192;
 // A warp's first partial, left while its stage is in use, has its own place in
 // shared memory where that fits, else in the workspace.
 constexpr int kPad = 4;
-constexpr bool first_in_smem(int D) { return D <= 128; }
 constexpr int warp_partial_floats(int D, int NT) { return NT * 8 * (D + kPad); }
 constexpr int partial_floats(int D, int NT) { return NT * 8 * (D + 2); }
 // Dynamic shared memory: the stages, the warps' first partials, then the
 // table of the sequences' first tiles.
-constexpr size_t table_offset(int D, int NT) {
-  return static_cast<size_t>(paged_warps(D)) *
-         (stage_bytes(D) + (first_in_smem(D) ? warp_partial_floats(D, NT) * 4 : 0));
+template <typename Pool>
+constexpr size_t table_offset() {
+  return static_cast<size_t>(Pool::W) *
+         (2 * Pool::kTile + (Pool::kFirstInSmem ? warp_partial_floats(Pool::D, Pool::NT) * 4 : 0));
 }
-constexpr size_t paged_smem(int D, int NT, int64_t sequences) {
-  return kSmemSlack + table_offset(D, NT) + static_cast<size_t>(sequences + 1) * 4;
+template <typename Pool>
+constexpr size_t paged_smem(int64_t sequences) {
+  return kSmemSlack + table_offset<Pool>() + static_cast<size_t>(sequences + 1) * 4;
 }
 
 struct Cursor {
   int seq, head, tile, tiles;  // tile of `tiles` of the row
   int first;                   // the row's first tile, in tiles from the sequence's start
   int low, length;             // visible tokens [low, length)
+  int prefix, prefix_tiles;    // and [0, prefix), whose tiles come first
 };
 
-template <int D, int NT>
-struct Paged {
-  static constexpr int R = tile_rows(D);
-  static constexpr int W = paged_warps(D);
-  static constexpr int G8 = NT * 8;
-  static constexpr int kTile = R * D * 2;
-  static constexpr int kThreads = W * 32;
-  static constexpr int kPartial = partial_floats(D, NT);
-  static constexpr int kWarpPartial = warp_partial_floats(D, NT);
-};
 
 // A length that the page table cannot hold counts as zero: nothing of its row
 // is read, and the row is NaN.
@@ -120,23 +103,43 @@ __device__ __forceinline__ int first_visible(const PagedParams& p, int length) {
   return p.window > 0 && length > p.window ? length - p.window : 0;
 }
 
-// Tiles of a sequence: those that hold its visible tokens.
-template <int R>
-__device__ __forceinline__ int tiles_of(const PagedParams& p, int seq) {
-  const int length = clamp_length(p, seq);
-  return (length + R - 1) / R - first_visible(p, length) / R;
+// Tiles of a sequence: those that hold its visible tokens.  With a prefix
+// (`More`) these are the prefix's and, behind it, the window's.
+template <int R, bool More>
+__device__ __forceinline__ void enter_tokens(const PagedParams& p, int length, Cursor& c) {
+  c.length = length;
+  c.low = first_visible(p, length);
+  c.first = c.low / R;
+  c.prefix = c.prefix_tiles = 0;
+  if (More && p.prefix > 0) {
+    c.prefix = min(p.prefix, c.low);
+    c.prefix_tiles = (c.prefix + R - 1) / R;
+    // Tiles from here on are `first` behind their place in the row.
+    c.first = max(c.first, c.prefix_tiles) - c.prefix_tiles;
+  }
 }
 
-template <int R>
+template <int R, bool More>
+__device__ __forceinline__ int tiles_of(const PagedParams& p, int seq) {
+  Cursor c;
+  enter_tokens<R, More>(p, clamp_length(p, seq), c);
+  return (c.length + R - 1) / R - c.first;
+}
+
+template <int R, bool More>
 __device__ __forceinline__ void enter_row(const PagedParams& p, const int* start, Cursor& c) {
   c.tiles = start[c.seq + 1] - start[c.seq];
-  c.length = clamp_length(p, c.seq);
-  c.low = first_visible(p, c.length);
-  c.first = c.low / R;
+  enter_tokens<R, More>(p, clamp_length(p, c.seq), c);
+}
+
+// The first token of the cursor's tile.
+template <int R, bool More>
+__device__ __forceinline__ int tile_token(const Cursor& c) {
+  return (More && c.tile < c.prefix_tiles ? c.tile : c.first + c.tile) * R;
 }
 
 // The cursor at global tile x.
-template <int R>
+template <int R, bool More>
 __device__ __forceinline__ Cursor seek(const PagedParams& p, const int* start, unsigned x) {
   int a = 0, b = p.sequences;  // start[a] * heads <= x < start[b] * heads
   while (b - a > 1) {
@@ -145,7 +148,7 @@ __device__ __forceinline__ Cursor seek(const PagedParams& p, const int* start, u
   }
   Cursor c;
   c.seq = a;
-  enter_row<R>(p, start, c);
+  enter_row<R, More>(p, start, c);
   const unsigned y = x - static_cast<unsigned>(start[a]) * p.heads;
   c.head = static_cast<int>(y / c.tiles);
   c.tile = static_cast<int>(y - static_cast<unsigned>(c.head) * c.tiles);
@@ -203,111 +206,14 @@ __device__ __forceinline__ int arrive_add(int* counter) {
 }
 
 // The next tile of the list (there must be one).
-template <int R>
+template <int R, bool More>
 __device__ __forceinline__ void advance(const PagedParams& p, const int* start, Cursor& c) {
   if (++c.tile < c.tiles) return;
   c.tile = 0;
   if (++c.head < p.heads) return;
   c.head = 0;
   do ++c.seq; while (start[c.seq + 1] == start[c.seq]);
-  enter_row<R>(p, start, c);
-}
-
-// Query B fragments: rows at `q`, p.q_head elements apart.
-template <int D, int NT>
-__device__ __forceinline__ void load_queries(uint32_t (&qb)[D / 16][NT][2], const PagedParams& p,
-                                             int seq, int head, int lane) {
-  const int64_t base = seq * p.q_seq + static_cast<int64_t>(head) * p.group * p.q_head;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int g = nt * 8 + (lane >> 2);
-    const int64_t row = base + min(g, p.group - 1) * p.q_head;
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks)
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int d = ks * 16 + half * 8 + 2 * (lane & 3);
-        const int64_t at = row + min(d, p.dim - 2);
-        uint32_t bits;
-        if (p.query_f32) {
-          const float2 x = *reinterpret_cast<const float2*>(static_cast<const float*>(p.query) + at);
-          bits = pack_bf16(x.x, x.y);
-        } else {
-          bits = *reinterpret_cast<const uint32_t*>(
-              static_cast<const __nv_bfloat16*>(p.query) + at);
-        }
-        qb[ks][nt][half] = g < p.group && d < p.dim ? bits : 0u;
-      }
-  }
-}
-
-// o += V^T p for a tile's weights p (C layout), held in `Terms` bf16 terms: two
-// for bf16 queries (2^-16 at most, far within the output's own rounding: the
-// error against 64 bits is the output's 1.66e-3; one term, 2^-8, made it 2.0 to
-// 2.3e-3 and took 7.9 instead of 8.3 us for 333 tokens, 319 instead of 322 for 16
-// sequences of 32K, 46 instead of 50 for D 256 with 16 queries a KV head), three
-// for fp32 queries, which hold all 24 bits of p.  The further
-// terms may be negative or zero, so they meet V with its infinities clamped:
-// an infinite value times p is infinite, whatever p's bits are.  For fp32 queries
-// a tile's products are summed apart and added to o by a rounded addition: the
-// tensor cores cut their sums off, which over a long row would cost fp32 digits.
-// A bf16 output does not see them (the same error with both), and the second
-// set of sums would spill: 68 us instead of 50 for that D 256 batch.
-template <int R, int D, int NT, int Terms>
-__device__ __forceinline__ void weigh_values(uint32_t tile, float (&p)[R / 16][NT][4],
-                                             float (&o)[D / 16][NT][4], int lane) {
-  uint32_t frag[Terms][R / 16][NT][2];
-#pragma unroll
-  for (int term = 0; term < Terms; ++term)
-#pragma unroll
-    for (int mt = 0; mt < R / 16; ++mt)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float& a = p[mt][nt][2 * half];
-          float& b = p[mt][nt][2 * half + 1];
-          const __nv_bfloat162 part = __floats2bfloat162_rn(a, b);
-          a -= __low2float(part);
-          b -= __high2float(part);
-          frag[term][mt][nt][half] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&part));
-        }
-  const int trow = (lane & 7) + ((lane >> 4) & 1) * 8;
-  const int cadd = (lane >> 3) & 1;
-#pragma unroll
-  for (int dt = 0; dt < D / 16; ++dt) {
-    float sum[NT][4];  // of the tile
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) sum[nt][0] = sum[nt][1] = sum[nt][2] = sum[nt][3] = 0.f;
-    float(&to)[NT][4] = Terms > 2 ? sum : o[dt];
-#pragma unroll
-    for (int kt = 0; kt < R / 16; ++kt) {
-      uint32_t a[4];
-      ldsm_x4_trans(tile + swz(kt * 16 + trow, dt * 2 + cadd, R), a);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mma_bf16(to[nt], a, frag[0][kt][nt][0], frag[0][kt][nt][1]);
-      if constexpr (Terms > 1) {
-        const __nv_bfloat162 most = __halves2bfloat162(__ushort_as_bfloat16(0x7f7f),
-                                                       __ushort_as_bfloat16(0x7f7f));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          __nv_bfloat162& v = *reinterpret_cast<__nv_bfloat162*>(&a[i]);
-          v = __hmax2(__hmin2(v, most), __hneg2(most));
-        }
-#pragma unroll
-        for (int term = 1; term < Terms; ++term)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            mma_bf16(to[nt], a, frag[term][kt][nt][0], frag[term][kt][nt][1]);
-      }
-    }
-    if constexpr (Terms > 2) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) o[dt][nt][c] += sum[nt][c];
-    }
-  }
+  enter_row<R, More>(p, start, c);
 }
 
 // One normalised output value; an all -inf row is 0 / 0, as the formula has it.
@@ -330,6 +236,11 @@ __device__ __forceinline__ void fma4(float4& acc, float w, const float4& x) {
   acc.y += w * x.y;
   acc.z += w * x.z;
   acc.w += w * x.w;
+}
+
+// What a KV head's values are multiplied by (pools of 4 bits).
+__device__ __forceinline__ float value_factor(const PagedParams& p, int head) {
+  return p.value_scale != nullptr ? p.value_scale[head] : 1.f;
 }
 
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
@@ -400,7 +311,7 @@ __device__ __forceinline__ void join(unsigned members, int lane, M m_of, L l_of,
 
 // Four joined channels of query g of a row and, with the first of them, its m
 // and l: finished, or into the partial `to`.
-template <int D, int G8>
+template <int D, int G8, bool More>
 __device__ __forceinline__ void put_joined(const PagedParams& p, int row, int g, int d, float* to,
                                            float m, float l, const float4& o) {
   if (to != nullptr) {
@@ -411,19 +322,70 @@ __device__ __forceinline__ void put_joined(const PagedParams& p, int row, int g,
     }
   } else if (d < p.dim) {
     const int64_t at = static_cast<int64_t>(row) * p.group + g;
-    const float inverse = 1.f / l;
+    float inverse = 1.f / l;
+    if (More) inverse *= value_factor(p, row % p.heads);
     put4(p, at * p.dim + d,
          make_float4(o.x * inverse, o.y * inverse, o.z * inverse, o.w * inverse));
     if (d == 0 && p.lse != nullptr) p.lse[at] = finite_or_zero(m) + logf(l);
   }
 }
 
-template <int D, int NT>
-__global__ void __launch_bounds__(paged_warps(D) * 32, 1)
-    paged_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant__ PagedParams p) {
-  using K = Paged<D, NT>;
-  constexpr int R = K::R, W = K::W, G8 = K::G8, kTile = K::kTile;
-  constexpr int kThreads = K::kThreads, kPartial = K::kPartial, kWarpPartial = K::kWarpPartial;
+// The rows of a tile that are visible: [low, high) and [0, prefix).
+struct Seen {
+  int low, high, prefix;
+  __device__ bool row(int r) const { return r < high && (r >= low || r < prefix); }
+  __device__ bool all(int rows) const { return high == rows && (low == 0 || prefix >= rows); }
+};
+
+// A tile's products to logits: scaled, capped, biased by distance, -inf where the
+// row is not visible; and kept for the weights' sums where these are wanted.
+//   x = c tanh(scale q.k / c) + slope (j - (L - 1))
+template <typename Pool>
+__device__ __forceinline__ void shape_logits(float (&logit)[Pool::R / 16][Pool::NT][4],
+                                             const typename Pool::Query& query, const Seen& seen,
+                                             const Cursor& cur, int token, int lane,
+                                             const PagedParams& p) {
+  const float cap = p.softcap, inverse = 1.f / cap;
+  const int from = token - (cur.length - 1);
+#pragma unroll
+  for (int nt = 0; nt < Pool::NT; ++nt)
+#pragma unroll
+    for (int col = 0; col < 2; ++col) {
+      const int g = nt * 8 + 2 * (lane & 3) + col;
+      const float scale = Pool::column_scale(query, p, nt, col, lane);
+      const int head = cur.head * p.group + g;
+      const float slope = p.slopes != nullptr && g < p.group ? p.slopes[head] : 0.f;
+      float* keep = p.scores != nullptr && g < p.group
+                        ? p.scores + (static_cast<int64_t>(cur.seq) * p.heads * p.group + head) *
+                                         p.capacity + token
+                        : nullptr;
+#pragma unroll
+      for (int mt = 0; mt < Pool::R / 16; ++mt)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int r = Pool::token_of(mt, half, lane);
+          float& x = logit[mt][nt][2 * half + col];
+          x *= scale;
+          if (cap > 0.f) x = cap * tanhf(x * inverse);
+          if (p.slopes != nullptr) x += slope * static_cast<float>(from + r);
+          const bool visible = seen.row(r);
+          if (keep != nullptr && visible) keep[r] = x;
+          if (!visible) x = -INFINITY;
+        }
+    }
+}
+
+// The pool says how a tile is fetched, scored and weighed (Bf16Pool, Fp4Pool).
+// More: a cap, a bias, a prefix, factors and the logits for the weights' sums,
+// each looked up in the parameters; without it the kernel is as it was before
+// these (the same results, and the same time).
+template <typename Pool, bool More>
+__global__ void __launch_bounds__(Pool::W * 32, 1)
+    paged_kernel(const __grid_constant__ typename Pool::Source source,
+                 const __grid_constant__ PagedParams p) {
+  constexpr int D = Pool::D, NT = Pool::NT, R = Pool::R, W = Pool::W, kTile = Pool::kTile;
+  constexpr int G8 = NT * 8, kThreads = W * 32;
+  constexpr int kPartial = partial_floats(D, NT), kWarpPartial = warp_partial_floats(D, NT);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = align_smem(smem_raw);  // [warp][K | V]
   __shared__ __align__(8) uint64_t bars[W][2];
@@ -435,7 +397,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   __shared__ Cut cuts[2];
   __shared__ int last_arrival[2];
   __shared__ int busy;  // sequences that are not empty
-  int* start = reinterpret_cast<int*>(ring + table_offset(D, NT));  // tiles before each sequence
+  int* start = reinterpret_cast<int*>(ring + table_offset<Pool>());  // tiles before each sequence
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (lane == 0) {
     mbar_init(&bars[warp][0], 1);
@@ -445,8 +407,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   }
   if (threadIdx.x == 0) {
     busy = 0;
-    tma_prefetch_desc(&maps.keys);
-    tma_prefetch_desc(&maps.values);
+    Pool::prefetch(source);
   }
   // The lengths and the page table's lines come to L2 before the dependency wait
   // (hints: they return no data, so what the previous kernel still writes is
@@ -472,7 +433,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
       if (blockIdx.x == 0 && (p.lengths[s] < 0 || p.lengths[s] > p.capacity)) {
         atomicOr(p.status, kStatusBadInput);
       }
-      const int tiles = tiles_of<R>(p, s);
+      const int tiles = tiles_of<R, More>(p, s);
       start[s] = tiles;
       sum += tiles;
       some += tiles > 0;
@@ -539,7 +500,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   const uint32_t k_tile = smem_addr(stage), v_tile = k_tile + kTile;
   // Where partial i of the CTA keeps its o: a warp's last row waits in the
   // warp's own idle stage, an earlier one (cut by the range's start) apart.
-  float* firsts = first_in_smem(D)
+  float* firsts = Pool::kFirstInSmem
                       ? reinterpret_cast<float*>(ring + W * 2 * kTile)
                       : p.warp_partials + static_cast<size_t>(cta) * W * kWarpPartial;
   const auto segment = [&](int i) {
@@ -553,8 +514,9 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   // Lane i of the first `boxes` lanes looks up the page of the tile's i-th box.
   auto page_of = [&](const Cursor& c) {
     if (lane >= boxes) return kNoPage;
-    const int token = (c.first + c.tile) * R + lane * box_rows;
-    if (token >= c.length || token + box_rows <= c.low) return kNoPage;
+    const int token = tile_token<R, More>(c) + lane * box_rows;
+    if (token >= c.length) return kNoPage;
+    if (token + box_rows <= c.low && !(More && token < c.prefix)) return kNoPage;
     const int page = p.page_table[c.seq * p.page_table_stride + (token >> p.block_shift)];
     if (page >= 0 && page < p.pool_pages) return page;
     atomicOr(p.status, kStatusBadInput);
@@ -564,18 +526,13 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   auto issue = [&](int which, const Cursor& c, int page) {
     uint64_t* bar = &bars[warp][which];
     const unsigned used = __ballot_sync(0xffffffffu, page >= 0);
-    if (lane == 0) mbar_expect_tx(bar, __popc(used) * box_rows * D * 2);
+    if (lane == 0) mbar_expect_tx(bar, __popc(used) * Pool::box_bytes(box_rows));
     fence_proxy_async();
     __syncwarp();
     if (page >= 0) {
-      const int token = (c.first + c.tile) * R + lane * box_rows;
-      uint8_t* to = stage + which * kTile + lane * box_rows * 128;
-      const CUtensorMap* map = which ? &maps.values : &maps.keys;
-#pragma unroll
-      for (int i = 0; i < D / 64; ++i) {
-        tma_load_4d_hint(to + i * R * 128, map, bar, i * 64, token & (page_rows - 1), c.head, page,
-                         policy);
-      }
+      const int token = tile_token<R, More>(c) + lane * box_rows;
+      Pool::fetch(source, which, stage + which * kTile, lane, box_rows, bar,
+                  token & (page_rows - 1), c.head, page, policy);
     }
   };
 
@@ -583,7 +540,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   // while the first tiles are on their way.
   const auto find_cuts = [&] {
     if (warp >= 2) return;
-    const Cursor c = seek<R>(p, start, warp == 0 ? lo : hi - 1);
+    const Cursor c = seek<R, More>(p, start, warp == 0 ? lo : hi - 1);
     const unsigned begin = (warp == 0 ? lo : hi - 1) - c.tile;
     const bool cut = warp == 0 ? begin < lo : begin >= lo && begin + c.tiles > hi;
     Cut found;
@@ -593,9 +550,9 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   };
   if (wlo >= whi) find_cuts();
   if (wlo < whi) {
-    uint32_t qb[D / 16][NT][2];
+    typename Pool::Query query;
     float m[NT][2], l[NT][2], o[D / 16][NT][4];
-    Cursor cur = seek<R>(p, start, wlo), next = cur;
+    Cursor cur = seek<R, More>(p, start, wlo), next = cur;
     int page = page_of(cur);
     issue(0, cur, page);
     issue(1, cur, page);
@@ -607,12 +564,12 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
     bool fresh = true, aborted = false;
     const auto again = [&](int which, int parity) { warp_wait(&bars[warp][which], parity); };
     if (count > 1) {
-      advance<R>(p, start, next);
+      advance<R, More>(p, start, next);
       page = page_of(next);
     }
     for (int j = 0; j < count; ++j) {
       if (fresh) {
-        load_queries<D, NT>(qb, p, cur.seq, cur.head, lane);
+        Pool::load_queries(query, p, cur.seq, cur.head, lane);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           m[nt][0] = m[nt][1] = -INFINITY;
@@ -625,8 +582,11 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
       }
       spoilt = spoilt || bad;
       const bool more = j + 1 < count;
-      const int token = (cur.first + cur.tile) * R;
-      const int row_lo = max(0, cur.low - token), row_hi = min(R, cur.length - token);
+      const int token = tile_token<R, More>(cur);
+      Seen seen;
+      seen.low = max(0, cur.low - token);
+      seen.high = min(R, cur.length - token);
+      seen.prefix = More ? max(0, cur.prefix - token) : 0;
       // A wait that runs out leaves the rest of the warp's range out (the
       // status word says so, and its rows are NaN); nothing is in flight after
       // its drain.
@@ -637,45 +597,33 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
       }
       if (!aborted) {
         float logit[R / 16][NT][4];
-        score_tile<R, D, NT>(k_tile, qb, logit, lane);
+        Pool::score(k_tile, query, logit, lane, p);
+        if constexpr (More) {
+          shape_logits<Pool>(logit, query, seen, cur, token, lane, p);
+        } else {
 #pragma unroll
-        for (int mt = 0; mt < R / 16; ++mt)
+          for (int mt = 0; mt < R / 16; ++mt)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int r = mt * 16 + (lane >> 2) + (c >> 1) * 8;
+            for (int c = 0; c < 4; ++c) {
+              const int r = mt * 16 + (lane >> 2) + (c >> 1) * 8;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              logit[mt][nt][c] =
-                  r >= row_lo && r < row_hi ? logit[mt][nt][c] * p.scale : -INFINITY;
-          }
+              for (int nt = 0; nt < NT; ++nt)
+                logit[mt][nt][c] =
+                    r >= seen.low && r < seen.high ? logit[mt][nt][c] * p.scale : -INFINITY;
+            }
+        }
         __syncwarp();
         if (more) {
           issue(0, next, page);
           next_bad = __any_sync(0xffffffffu, page == kBadPage);
         }
-        softmax_update<R, D, NT>(logit, m, l, o);
+        Pool::softmax(logit, m, l, o);
         if (!warp_wait(&bars[warp][1], j & 1)) {
           if (lane == 0) atomicOr(p.status, kStatusTimeout);
           drain_values(j, more, again);
           aborted = true;
         } else {
-          if (row_lo > 0 || row_hi < R) {
-            // Rows that are not visible may hold anything: a weight of zero
-            // would not silence a NaN, so they are zeroed.
-            for (int i = lane; i < R * (D / 8); i += 32) {
-              const int r = i / (D / 8), c16 = i - r * (D / 8);
-              if (r < row_lo || r >= row_hi) {
-                *reinterpret_cast<uint4*>(stage + kTile + swz(r, c16, R)) = make_uint4(0, 0, 0, 0);
-              }
-            }
-            fence_proxy_async();
-            __syncwarp();
-          }
-          if (p.query_f32) {
-            weigh_values<R, D, NT, 3>(v_tile, logit, o, lane);
-          } else {
-            weigh_values<R, D, NT, 2>(v_tile, logit, o, lane);
-          }
+          Pool::weigh(stage + kTile, v_tile, logit, o, seen, lane, p);
           __syncwarp();
           if (more) issue(1, next, page);
         }
@@ -683,6 +631,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
       const bool row_done = cur.tile + 1 == cur.tiles;
       if (row_done || !more) {
         reduce_l<NT>(l);
+        Pool::settle(l, o);
         if (spoilt || aborted) {  // a sum of NaN spreads through every join
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) l[nt][0] = l[nt][1] = NAN;
@@ -697,12 +646,13 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
             for (int c = 0; c < 2; ++c) {
               const int g = nt * 8 + 2 * (lane & 3) + c;
               if (g >= p.group) continue;
-              const float inv = 1.f / l[nt][c];
+              float inv = 1.f / l[nt][c];
+              if (More) inv *= value_factor(p, cur.head);
 #pragma unroll
               for (int dt = 0; dt < D / 16; ++dt)
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                  const int d = dt * 16 + half * 8 + (lane >> 2);
+                  const int d = Pool::channel(dt, half, lane);
                   if (d < p.dim) put(p, (out_row + g) * p.dim + d, o[dt][nt][2 * half + c] * inv);
                 }
               if (p.lse != nullptr && lane < 4) {
@@ -728,7 +678,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
               for (int dt = 0; dt < D / 16; ++dt)
 #pragma unroll
                 for (int half = 0; half < 2; ++half)
-                  to[g * (D + kPad) + dt * 16 + half * 8 + (lane >> 2)] = o[dt][nt][2 * half + c];
+                  to[g * (D + kPad) + Pool::channel(dt, half, lane)] = o[dt][nt][2 * half + c];
             }
         }
         seg_first = 0;
@@ -738,7 +688,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
         cur = next;
         bad = next_bad;
         if (j + 2 < count) {
-          advance<R>(p, start, next);
+          advance<R, More>(p, start, next);
           page = page_of(next);
         }
       }
@@ -778,7 +728,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
             return *reinterpret_cast<const float4*>(segment(j) + g * (D + kPad) + d);
           },
           [&](int d, float m, float l, const float4& o) {
-            put_joined<D, G8>(p, row, g, d, to, m, l, o);
+            put_joined<D, G8, More>(p, row, g, d, to, m, l, o);
           });
     }
   }
@@ -823,7 +773,7 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
         return __ldcg(reinterpret_cast<const float4*>(part(k) + 2 * G8 + g * D + d));
       };
       const auto put = [&](int d, float m, float l, const float4& o) {
-        put_joined<D, G8>(p, cut.row, g, d, target, m, l, o);
+        put_joined<D, G8, More>(p, cut.row, g, d, target, m, l, o);
       };
       // More than one batch's parts, up to 24 (kFlatJoin) or a group's: in twenties.
       // A row of 18 parts (128K tokens, eight heads) 87.3 us against 87.9 in eights,
@@ -850,182 +800,45 @@ __global__ void __launch_bounds__(paged_warps(D) * 32, 1)
   join_arrived(true);
 }
 
-template <int D, int NT>
-cudaError_t launch_t(const PagedMaps& maps, const PagedParams& p, int ctas, cudaStream_t stream) {
-  const size_t smem = paged_smem(D, NT, p.sequences);
+template <typename Pool, bool More>
+cudaError_t launch_pool(const typename Pool::Source& source, const PagedParams& p, int ctas,
+                        cudaStream_t stream) {
   // One limit for every batch: the largest this kernel takes.
-  cudaError_t err = ensure_smem_limit(reinterpret_cast<const void*>(&paged_kernel<D, NT>),
-                                      paged_smem(D, NT, kMostSequences));
+  cudaError_t err = ensure_smem_limit(reinterpret_cast<const void*>(&paged_kernel<Pool, More>),
+                                      paged_smem<Pool>(kMostSequences));
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(paged_warps(D) * 32);
-  cfg.dynamicSmemBytes = smem;
+  cfg.blockDim = dim3(Pool::W * 32);
+  cfg.dynamicSmemBytes = paged_smem<Pool>(p.sequences);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_kernel<D, NT>, maps, p);
+  return cudaLaunchKernelEx(&cfg, paged_kernel<Pool, More>, source, p);
 }
 
-template <int D>
-cudaError_t launch_d(const PagedMaps& maps, const PagedParams& p, int ctas, cudaStream_t stream) {
-  return p.group <= 8 ? launch_t<D, 1>(maps, p, ctas, stream)
-                      : launch_t<D, 2>(maps, p, ctas, stream);
-}
-
-int reject(int code, const char* message) {
-  set_last_error(message);
-  return code;
-}
-
-int padded(int64_t dim) { return static_cast<int>((dim + 63) / 64 * 64); }
-
-struct Layout {
-  size_t warp_partials, cta_partials, group_partials, bytes;
-  Layout(int64_t group, int64_t dim, int sms) {
-    const int D = padded(dim), NT = group <= 8 ? 1 : 2;
-    const size_t one = static_cast<size_t>(partial_floats(D, NT)) * 4;
-    size_t off = kHeader;
-    warp_partials = off;
-    if (!first_in_smem(D)) {
-      off += static_cast<size_t>(warp_partial_floats(D, NT)) * 4 * sms * paged_warps(D);
-    }
-    cta_partials = off;
-    off += one * sms * 2;
-    group_partials = off;
-    off += one * sms * 2;
-    bytes = (off + 255) & ~static_cast<size_t>(255);
+// Where a workspace keeps an instance's partials.
+template <typename Pool>
+PagedLayout pool_layout(int sms) {
+  const size_t one = static_cast<size_t>(partial_floats(Pool::D, Pool::NT)) * 4;
+  PagedLayout l;
+  size_t off = kHeader;
+  l.warp_partials = off;
+  if (!Pool::kFirstInSmem) {
+    off += static_cast<size_t>(warp_partial_floats(Pool::D, Pool::NT)) * 4 * sms * Pool::W;
   }
-};
+  l.cta_partials = off;
+  off += one * sms * 2;
+  l.group_partials = off;
+  off += one * sms * 2;
+  l.bytes = (off + 255) & ~static_cast<size_t>(255);
+  return l;
+}
 
 }  // namespace
-
 }  // namespace rkv
 
-extern "C" {
-
-size_t rkv_paged_workspace_size(int64_t group, int64_t head_dim) {
-  using namespace rkv;
-  int sms = 0;
-  if (group < 1 || group > kMaxGroup || head_dim < 32 || head_dim > 256 || head_dim % 32 ||
-      device_sms(&sms) != RKV_OK || sms > kMostCtas) {
-    return 0;
-  }
-  return Layout(group, head_dim, sms).bytes;
-}
-
-int rkv_paged_attention(const rkv_paged_args* a, void* stream) {
-  using namespace rkv;
-  set_last_error("");
-  if (a == nullptr) return reject(RKV_ERR_INVALID_ARGUMENT, "args is null");
-  if (a->head_dim < 32 || a->head_dim > 256 || a->head_dim % 32 != 0) {
-    return reject(RKV_ERR_UNSUPPORTED, "head_dim must be a multiple of 32 in [32, 256]");
-  }
-  if (a->block_size != 16 && a->block_size != 32 && a->block_size != 64) {
-    return reject(RKV_ERR_UNSUPPORTED, "block_size must be 16, 32 or 64");
-  }
-  if (a->group < 1 || a->group > kMaxGroup) {
-    return reject(RKV_ERR_UNSUPPORTED, "group must be 1..16");
-  }
-  if (a->sequences < 0 || a->sequences > kMostSequences || a->kv_heads < 1 ||
-      a->kv_heads > kMostPagedHeads) {
-    return reject(RKV_ERR_UNSUPPORTED, "at most 4096 sequences and 4096 KV heads");
-  }
-  if (a->query_dtype != RKV_DTYPE_BF16 && a->query_dtype != RKV_DTYPE_F32) {
-    return reject(RKV_ERR_INVALID_ARGUMENT, "query dtype must be bf16 or fp32");
-  }
-  if (a->window < 0 || a->table_blocks < 0 ||
-      a->table_blocks > kMostPagedTokens / a->block_size || a->page_table_stride < 0 ||
-      a->pool_pages < 0 || a->pool_pages > (1LL << 31) - 1) {
-    return reject(RKV_ERR_INVALID_ARGUMENT, "window, page table or pool sizes are out of range");
-  }
-  const int D = padded(a->head_dim), R = tile_rows(D);
-  const int64_t tiles = a->sequences * a->kv_heads * ((a->table_blocks * a->block_size + R - 1) / R);
-  if (tiles > (1LL << 31) - 1) {  // a product below 2^13 * 2^12 * 2^25
-    return reject(RKV_ERR_UNSUPPORTED, "the page table covers more rows than are counted");
-  }
-  if (a->sequences == 0) return RKV_OK;
-  if (!a->query || !a->output || !a->lengths || !a->key_pool || !a->value_pool ||
-      !a->page_table) {
-    return reject(RKV_ERR_INVALID_ARGUMENT,
-                  "query, output, pools, page_table and lengths must be non-null");
-  }
-  if (a->pool_pages < 1) return reject(RKV_ERR_INVALID_ARGUMENT, "the pool has no pages");
-  if (a->workspace == nullptr || a->workspace_size < static_cast<int64_t>(kHeader)) {
-    return reject(RKV_ERR_WORKSPACE, "workspace is missing or too small");
-  }
-  const int width = a->query_dtype == RKV_DTYPE_F32 ? 4 : 2;
-  uintptr_t bits = reinterpret_cast<uintptr_t>(a->query) | reinterpret_cast<uintptr_t>(a->output);
-  bits |= reinterpret_cast<uintptr_t>(a->key_pool) | reinterpret_cast<uintptr_t>(a->value_pool);
-  for (int64_t s : a->query_strides) bits |= static_cast<uintptr_t>(s * width);
-  for (int64_t s : a->key_pool_strides) bits |= static_cast<uintptr_t>(s * 2);
-  for (int64_t s : a->value_pool_strides) bits |= static_cast<uintptr_t>(s * 2);
-  if (bits & 15u) {
-    return reject(RKV_ERR_ALIGNMENT, "pointers and strides must be 16-byte aligned");
-  }
-  if (!aligned_to(4, {a->page_table, a->lengths, a->lse})) {
-    return reject(RKV_ERR_ALIGNMENT,
-                  "page_table, lengths and lse must be aligned to their elements");
-  }
-  int rc = RKV_OK, sms = 0;
-  PagedMaps maps;
-  const int box_rows = static_cast<int>(std::min<int64_t>(R, a->block_size));
-  const int64_t *ks = a->key_pool_strides, *vs = a->value_pool_strides;
-  if ((rc = pool_map(&maps.keys, a->key_pool, a->head_dim, a->block_size, box_rows, a->kv_heads,
-                     a->pool_pages, ks[2], ks[1], ks[0], "key_pool")) != RKV_OK ||
-      (rc = pool_map(&maps.values, a->value_pool, a->head_dim, a->block_size, box_rows,
-                     a->kv_heads, a->pool_pages, vs[2], vs[1], vs[0], "value_pool")) != RKV_OK ||
-      (rc = device_sms(&sms)) != RKV_OK) {
-    return rc;
-  }
-  if (sms > kMostCtas) return reject(RKV_ERR_UNSUPPORTED, "more SMs than the workspace counts");
-  const Layout layout(a->group, a->head_dim, sms);
-  if (a->workspace_size < static_cast<int64_t>(layout.bytes) ||
-      (reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0) {
-    return reject(RKV_ERR_WORKSPACE, "workspace is too small or not 256-byte aligned");
-  }
-  char* ws = static_cast<char*>(a->workspace);
-  PagedParams p = {};
-  p.query = a->query;
-  p.q_seq = a->query_strides[0];
-  p.q_head = a->query_strides[1];
-  p.query_f32 = a->query_dtype == RKV_DTYPE_F32;
-  p.out = a->output;
-  p.lse = a->lse;
-  p.page_table = a->page_table;
-  p.page_table_stride = a->page_table_stride;
-  p.lengths = a->lengths;
-  p.sequences = static_cast<int>(a->sequences);
-  p.heads = static_cast<int>(a->kv_heads);
-  p.group = static_cast<int>(a->group);
-  p.dim = static_cast<int>(a->head_dim);
-  p.block_shift = a->block_size == 16 ? 4 : a->block_size == 32 ? 5 : 6;
-  p.capacity = static_cast<int>(a->table_blocks * a->block_size);
-  p.pool_pages = static_cast<int>(a->pool_pages);
-  p.window = static_cast<int>(std::min<int64_t>(a->window, kMostPagedTokens));
-  p.scale = static_cast<float>(a->scale);
-  p.status = reinterpret_cast<int*>(ws);
-  p.counters = reinterpret_cast<int*>(ws + kCounterBytes);
-  p.warp_partials = reinterpret_cast<float*>(ws + layout.warp_partials);
-  p.cta_partials = reinterpret_cast<float*>(ws + layout.cta_partials);
-  p.group_partials = reinterpret_cast<float*>(ws + layout.group_partials);
-  const int ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms, tiles)));
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t err = cudaErrorInvalidValue;
-  switch (D) {
-    case 64: err = launch_d<64>(maps, p, ctas, st); break;
-    case 128: err = launch_d<128>(maps, p, ctas, st); break;
-    case 192: err = launch_d<192>(maps, p, ctas, st); break;
-    case 256: err = launch_d<256>(maps, p, ctas, st); break;
-  }
-  if (err != cudaSuccess) {
-    set_last_error(std::string("paged attention launch: ") + cudaGetErrorString(err));
-    return RKV_ERR_CUDA;
-  }
-  return RKV_OK;
-}
-
-}  // extern "C"
+#endif  // RKV_PAGED_CU_

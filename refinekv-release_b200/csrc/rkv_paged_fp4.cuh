@@ -1,0 +1,464 @@
+// paged_kernel over pools of 4 bits.
+//
+// Mathematics.  A channel is code * scale (rkv_fp4.cuh), six significant bits,
+// exact in fp16; so a tile's codes become fp16 operands (one conversion and one
+// product a pair) and the matrix instructions see the very numbers that the pool
+// stands for.  Queries (bf16, 8 bits) are moved by a power of two into fp16's
+// range, and the weights are held in fp16 terms: one for bf16 queries (2^-11,
+// against the output's own 2^-8), two for fp32 queries (2^-22).
+//
+// Tiles hold 64 tokens, so that a page is at most one tile and a page's slab of a KV
+// head is fetched by one bulk copy.  Which channels and tokens a lane holds is
+// chosen so that its codes lie together: the k index of a product and the rows
+// of its result may be taken in any order as long as both operands agree.
+//   scores: lane 4 r + j has a quarter j of the channels of tokens r and r + 8
+//     of 16 (dim 128: 16 bytes of codes and two scales each);
+//   values: lane 4 g + j has an eighth g of the channels of four tokens (dim 128: 8
+//     bytes of codes and one scale each), whose codes are paired by token after the
+//     conversion.  Tokens 2j and 2j + 1 change places for odd j, and with them the
+//     rows of the scores, or the four j of a load would hit the same banks.
+#pragma once
+
+#include "rkv_fp4.cuh"
+#include "rkv_paged.cu"
+
+namespace rkv {
+namespace {
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7},"
+      " {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Kept behind the waits for the copies by being volatile, like them.
+template <int Bytes>
+__device__ __forceinline__ uint32_t lds(uint32_t at) {
+  uint32_t x;
+  if constexpr (Bytes == 1) asm volatile("ld.shared.u8 %0, [%1];" : "=r"(x) : "r"(at));
+  if constexpr (Bytes == 2) asm volatile("ld.shared.u16 %0, [%1];" : "=r"(x) : "r"(at));
+  if constexpr (Bytes == 4) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(at));
+  return x;
+}
+
+// N words from an address that is aligned to the widest load that N allows.
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t at, uint32_t (&x)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(x[i]), "=r"(x[i + 1]), "=r"(x[i + 2]), "=r"(x[i + 3])
+                   : "r"(at + 4 * i));
+    }
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
+                   : "=r"(x[i]), "=r"(x[i + 1])
+                   : "r"(at + 4 * i));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = lds<4>(at + 4 * i);
+  }
+}
+
+__device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {
+  const __half2 y = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+
+__device__ __forceinline__ uint32_t low_twice(uint32_t pair) {
+  return __byte_perm(pair, pair, 0x1010);
+}
+__device__ __forceinline__ uint32_t high_twice(uint32_t pair) {
+  return __byte_perm(pair, pair, 0x3232);
+}
+__device__ __forceinline__ uint32_t lows(uint32_t a, uint32_t b) {
+  return __byte_perm(a, b, 0x5410);
+}
+__device__ __forceinline__ uint32_t highs(uint32_t a, uint32_t b) {
+  return __byte_perm(a, b, 0x7632);
+}
+
+__device__ __forceinline__ float exp2_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Weights and their sums are held 2^15 times as large within a tile and a row's
+// part: fp16 terms of weights down to 2^-29 of the greatest are then normal.
+constexpr float kBoost = 15.f;
+constexpr float kUnboost = 1.f / 32768.f;
+constexpr float kLog2E = 1.44269504088896341f;
+
+template <int Dim, int NT_>
+struct Fp4Pool {
+  static constexpr int D = Dim, NT = NT_, R = kFp4Rows;
+  static constexpr int W = NT == 1 && Dim <= 192 ? 12 : 8;
+  static constexpr int kTile = fp4_slab_bytes(R, Dim);
+  static constexpr bool kFirstInSmem = Dim <= 128;
+  static constexpr int kRow = Dim / 2;      // bytes of a row's codes
+  static constexpr int kScales = Dim / 16;  // and of its scales
+  static constexpr int kWords = Dim / 32;   // words of a lane's part of a key's codes
+  static constexpr int kBytes = Dim / 16;   // bytes of a lane's part of a value's codes
+  static_assert(warp_partial_floats(D, NT) * 4 <= 2 * kTile, "a partial waits in its warp's stage");
+  using Source = Fp4Pages;
+  struct Query {
+    uint32_t frags[D / 16][NT][2];  // fp16, times 2^k
+    float scale[NT][2];             // what the lane's columns are multiplied by
+  };
+  using Logits = float (&)[R / 16][NT][4];
+  using Columns = float (&)[NT][2];
+  using Outputs = float (&)[D / 16][NT][4];
+
+  static __device__ __forceinline__ void prefetch(const Source&) {}
+  static __device__ __forceinline__ int box_bytes(int rows) { return rows * (kRow + kScales); }
+  // A box is a page: its slab in one piece.
+  static __device__ __forceinline__ void fetch(const Source& pages, int which, uint8_t* tile,
+                                               int box, int box_rows, uint64_t* bar, int row,
+                                               int head, int page, uint64_t policy) {
+    const uint8_t* from = which ? pages.values + page * pages.value_page + head * pages.value_head
+                                : pages.keys + page * pages.key_page + head * pages.key_head;
+    const int bytes = box_bytes(box_rows);
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1], %2, [%3], %4;" ::"r"(smem_addr(tile + box * bytes)),
+        "l"(from), "r"(bytes), "r"(smem_addr(bar)), "l"(policy)
+        : "memory");
+  }
+
+  // Word w of the quarter j of a query row: channels j Dim / 4 + 8 w and on.
+  static __device__ __forceinline__ void load_queries(Query& q, const PagedParams& p, int seq,
+                                                      int head, int lane) {
+    const int64_t base = seq * p.q_seq + static_cast<int64_t>(head) * p.group * p.q_head;
+    const float factor = p.scale * (p.key_scale != nullptr ? p.key_scale[head] : 1.f);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int g = nt * 8 + (lane >> 2);
+      const int64_t row = base + min(g, p.group - 1) * p.q_head + (lane & 3) * (Dim / 4);
+      float x[kWords][8];
+      uint32_t most = 0;  // of the finite ones
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) {
+        if (p.query_f32) {
+          const float4* from =
+              reinterpret_cast<const float4*>(static_cast<const float*>(p.query) + row + 8 * w);
+          const float4 a = from[0], b = from[1];
+          const float raw[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[w][i] = bf16_round(raw[i]);
+        } else {
+          const uint4 four = *reinterpret_cast<const uint4*>(
+              static_cast<const __nv_bfloat16*>(p.query) + row + 8 * w);
+          const uint32_t raw[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[w][2 * i] = __uint_as_float(raw[i] << 16);
+            x[w][2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t size = __float_as_uint(x[w][i]) & 0x7fffffffu;
+          if (size < 0x7f800000u) most = max(most, size);
+        }
+      }
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      // 2^k brings the row's greatest into [2^14, 2^15): whatever lies within 2^29
+      // of it keeps all its bits.
+      const int k = min(126, 141 - static_cast<int>(most >> 23));
+      const float up = __int_as_float((127 + k) << 23), down = __int_as_float((127 - k) << 23);
+#pragma unroll
+      for (int w = 0; w < kWords; ++w)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const __half2 pair = __floats2half2_rn(x[w][2 * i] * up, x[w][2 * i + 1] * up);
+          q.frags[2 * w + (i >> 1)][nt][i & 1] =
+              g < p.group ? *reinterpret_cast<const uint32_t*>(&pair) : 0u;
+        }
+#pragma unroll
+      for (int col = 0; col < 2; ++col) {
+        q.scale[nt][col] = factor * __shfl_sync(0xffffffffu, down, 4 * (2 * (lane & 3) + col));
+      }
+    }
+  }
+  static __device__ __forceinline__ float column_scale(const Query& q, const PagedParams&, int nt,
+                                                       int col, int lane) {
+    return q.scale[nt][col];
+  }
+  static __device__ __forceinline__ int swapped(int r) { return r ^ (r >> 1 & 1); }
+  static __device__ __forceinline__ int token_of(int mt, int half, int lane) {
+    return mt * 16 + swapped(lane >> 2) + half * 8;
+  }
+  static __device__ __forceinline__ int channel(int dt, int half, int lane) {
+    return (lane >> 2) * (Dim / 8) + 2 * dt + half;
+  }
+
+  // Rows 16 mt .. of a tile: the address of their first codes and scales.
+  struct Place {
+    uint32_t codes, scales;
+  };
+  static __device__ __forceinline__ Place place_of(uint32_t tile, int mt, int shift) {
+    const int box = mt * 16 >> shift, row = mt * 16 & ((1 << shift) - 1);
+    const uint32_t slab = tile + box * ((kRow + kScales) << shift);
+    return {slab + row * kRow, slab + (kRow << shift) + row * kScales};
+  }
+
+  // The scales of a lane's words of one key row, each twice in a pair.
+  static __device__ __forceinline__ void key_scales(uint32_t at, int j, uint32_t (&s)[kWords]) {
+    if constexpr (kWords % 4 == 0) {
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) {
+        const uint32_t pair = fp4_scales(lds<2>(at + j * (kWords / 2) + 2 * i));
+        s[4 * i] = s[4 * i + 1] = low_twice(pair);
+        s[4 * i + 2] = s[4 * i + 3] = high_twice(pair);
+      }
+    } else {
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) {
+        if (kWords % 2 == 0 && w % 2 == 1) {
+          s[w] = s[w - 1];
+        } else {
+          s[w] = low_twice(fp4_scales(lds<1>(at + ((j * kWords + w) >> 1))));
+        }
+      }
+    }
+  }
+
+  static __device__ __forceinline__ void score(uint32_t tile, const Query& q, Logits acc, int lane,
+                                               const PagedParams& p) {
+    const int j = lane & 3, row = swapped(lane >> 2);
+#pragma unroll
+    for (int mt = 0; mt < R / 16; ++mt) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        acc[mt][nt][0] = acc[mt][nt][1] = acc[mt][nt][2] = acc[mt][nt][3] = 0.f;
+      const Place at = place_of(tile, mt, p.block_shift);
+      uint32_t a[kWords], b[kWords], sa[kWords], sb[kWords];
+      lds_words(at.codes + row * kRow + j * 4 * kWords, a);
+      lds_words(at.codes + (row + 8) * kRow + j * 4 * kWords, b);
+      key_scales(at.scales + row * kScales, j, sa);
+      key_scales(at.scales + (row + 8) * kScales, j, sb);
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) {
+        uint32_t x[4], y[4];
+        fp4_decode(a[w], x);
+        fp4_decode(b[w], y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] = times(x[i], sa[w]);
+          y[i] = times(y[i], sb[w]);
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t frag[4] = {x[2 * half], y[2 * half], x[2 * half + 1], y[2 * half + 1]};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mma_f16(acc[mt][nt], frag, q.frags[2 * w + half][nt][0], q.frags[2 * w + half][nt][1]);
+        }
+      }
+    }
+  }
+
+  // softmax_update with boosted weights; sums are rescaled only where a maximum rose.
+  static __device__ __forceinline__ void softmax(Logits logit, Columns m, Columns l, Outputs o) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float alpha[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int mt = 0; mt < R / 16; ++mt)
+          mx = fmaxf(mx, fmaxf(logit[mt][nt][j], logit[mt][nt][2 + j]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float top = fmaxf(m[nt][j], mx), ref = finite_or_zero(top);
+        alpha[j] = exp2_of((m[nt][j] - ref) * kLog2E);
+        m[nt][j] = top;
+        float sum = 0.f;
+#pragma unroll
+        for (int mt = 0; mt < R / 16; ++mt)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            float& x = logit[mt][nt][2 * half + j];
+            x = exp2_of(fmaf(x - ref, kLog2E, kBoost));
+            sum += x;
+          }
+        l[nt][j] = l[nt][j] * alpha[j] + sum;
+      }
+      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[dt][nt][c] *= alpha[c & 1];
+      }
+    }
+  }
+
+  // A row's part ends: its sums without the boost (exact).
+  static __device__ __forceinline__ void settle(Columns l, Outputs o) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      l[nt][0] *= kUnboost;
+      l[nt][1] *= kUnboost;
+#pragma unroll
+      for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[dt][nt][c] *= kUnboost;
+    }
+  }
+
+  static __device__ __forceinline__ void weigh(uint8_t*, uint32_t tile, Logits weights, Outputs o,
+                                               const Seen& seen, int lane, const PagedParams& p) {
+    if (p.query_f32) {
+      weigh_terms<2>(tile, weights, o, seen, lane, p);
+    } else {
+      weigh_terms<1>(tile, weights, o, seen, lane, p);
+    }
+  }
+
+  // o += V^T p with the weights in fp16 terms.  With two of them (fp32 queries) a tile's
+  // products are summed apart and added by a rounded addition, since the tensor
+  // cores cut their sums off.  Codes are taken kChunk bytes at a time.
+  template <int Terms>
+  static __device__ __forceinline__ void weigh_terms(uint32_t tile, Logits weights, Outputs o,
+                                                     const Seen& seen, int lane,
+                                                     const PagedParams& p) {
+    uint32_t frag[Terms][R / 16][NT][2];
+#pragma unroll
+    for (int term = 0; term < Terms; ++term)
+#pragma unroll
+      for (int mt = 0; mt < R / 16; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            float& a = weights[mt][nt][2 * half];
+            float& b = weights[mt][nt][2 * half + 1];
+            const __half2 part = __floats2half2_rn(a, b);
+            if (term + 1 < Terms) {
+              a -= __low2float(part);
+              b -= __high2float(part);
+            }
+            frag[term][mt][nt][half] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&part));
+          }
+    const int g = lane >> 2, j = lane & 3;
+    const int first = 2 * j + (j & 1), second = 2 * j + 1 - (j & 1);  // swapped(2j), swapped(2j + 1)
+    const bool whole = seen.all(R);
+    // Channels are taken by units of 8 (a word), or 4 where a lane's part is no whole words.
+    constexpr int kUnit = kBytes % 4 == 0 ? 4 : 2;
+    constexpr int kChunk = Terms == 1 && kBytes % 8 == 0 ? 8 : kUnit;
+    constexpr int kUnits = kChunk / kUnit;
+#pragma unroll
+    for (int chunk = 0; chunk < kBytes / kChunk; ++chunk) {
+      float sums[kChunk][NT][4];
+      if (Terms > 1) {
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            sums[i][nt][0] = sums[i][nt][1] = sums[i][nt][2] = sums[i][nt][3] = 0.f;
+      }
+#pragma unroll
+      for (int mt = 0; mt < R / 16; ++mt) {
+        const Place at = place_of(tile, mt, p.block_shift);
+        const int tokens[4] = {first, second, first + 8, second + 8};
+        uint32_t codes[4][kUnits];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const uint32_t from = at.codes + tokens[t] * kRow + g * kBytes + chunk * kChunk;
+          if constexpr (kUnit == 4) {
+            lds_words(from, codes[t]);
+          } else {
+            codes[t][0] = lds<2>(from);
+          }
+        }
+        uint32_t near = 0, far = 0;  // the scales of tokens 0 and 1, and 2 and 3
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+          if (u == 0) {  // two units of a chunk lie in one block of 16 channels
+            const int block = (g * (kBytes / kUnit) + chunk * kUnits) / (kUnit == 4 ? 2 : 4);
+            uint32_t scale[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              scale[t] = lds<1>(at.scales + tokens[t] * kScales + block);
+              // A row that is not visible may hold anything: a scale of zero makes
+              // its channels zero (codes are finite).
+              if (!whole && !seen.row(mt * 16 + tokens[t])) scale[t] = 0;
+            }
+            near = fp4_scales(scale[0] | scale[1] << 8);
+            far = fp4_scales(scale[2] | scale[3] << 8);
+          }
+          uint32_t x[4][4];
+#pragma unroll
+          for (int t = 0; t < 4; t += 4 / kUnit) {
+            if constexpr (kUnit == 4) {
+              fp4_decode(codes[t][u], x[t]);
+            } else {  // two tokens' half words in one
+              uint32_t both[4];
+              fp4_decode(codes[t][0] | codes[t + 1][0] << 16, both);
+              x[t][0] = both[0], x[t][1] = both[1], x[t + 1][0] = both[2], x[t + 1][1] = both[3];
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < kUnit; ++i) {
+            const uint32_t a[4] = {times(lows(x[0][i], x[1][i]), near),
+                                   times(highs(x[0][i], x[1][i]), near),
+                                   times(lows(x[2][i], x[3][i]), far),
+                                   times(highs(x[2][i], x[3][i]), far)};
+            const int k = u * kUnit + i;
+#pragma unroll
+            for (int term = 0; term < Terms; ++term)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                float(&to)[4] = Terms > 1 ? sums[k][nt] : o[chunk * kChunk + k][nt];
+                mma_f16(to, a, frag[term][mt][nt][0], frag[term][mt][nt][1]);
+              }
+          }
+        }
+      }
+      if (Terms > 1) {
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[chunk * kChunk + i][nt][c] += sums[i][nt][c];
+      }
+    }
+  }
+};
+
+// f(pool) for the pool of a head dim.
+template <int NT, typename F>
+auto by_dim(int64_t dim, F&& f) {
+  switch (dim) {
+    case 32: return f(Fp4Pool<32, NT>{});
+    case 64: return f(Fp4Pool<64, NT>{});
+    case 96: return f(Fp4Pool<96, NT>{});
+    case 128: return f(Fp4Pool<128, NT>{});
+    case 160: return f(Fp4Pool<160, NT>{});
+    case 192: return f(Fp4Pool<192, NT>{});
+    case 224: return f(Fp4Pool<224, NT>{});
+    default: return f(Fp4Pool<256, NT>{});
+  }
+}
+
+template <int NT>
+cudaError_t launch_fp4(const Fp4Pages& pages, const PagedParams& p, int ctas, cudaStream_t stream) {
+  return by_dim<NT>(p.dim, [&](auto pool) {
+    return launch_pool<decltype(pool), true>(pages, p, ctas, stream);
+  });
+}
+
+}  // namespace
+}  // namespace rkv

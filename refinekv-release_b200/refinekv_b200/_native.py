@@ -68,6 +68,8 @@ EXPORTS = (
     "rkv_paged_read",
     "rkv_paged_workspace_size",
     "rkv_paged_attention",
+    "rkv_paged_more_workspace_size",
+    "rkv_paged_attention_more",
     "rkv_selftest_wait_timeout",
     "rkv_last_error",
     "rkv_status_string",
@@ -116,6 +118,7 @@ APPEND_ARGS = struct.Struct("=40q")
 APPEND_FP4_ARGS = struct.Struct("=42q")
 READ_ARGS = struct.Struct("=31q")
 PAGED_ARGS = struct.Struct("=27qd")
+PAGED_MORE_ARGS = struct.Struct("=27qd11qd")
 
 _SIGNATURES = {
     "rkv_summarize": (ctypes.c_int, [c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64,
@@ -168,6 +171,8 @@ _SIGNATURES = {
     "rkv_paged_read": (ctypes.c_int, [ctypes.c_char_p, c_ptr]),
     "rkv_paged_workspace_size": (ctypes.c_size_t, [c_i64, c_i64]),
     "rkv_paged_attention": (ctypes.c_int, [ctypes.c_char_p, c_ptr]),
+    "rkv_paged_more_workspace_size": (ctypes.c_size_t, [c_i64, c_i64, c_i64]),
+    "rkv_paged_attention_more": (ctypes.c_int, [ctypes.c_char_p, c_ptr]),
     "rkv_selftest_wait_timeout": (ctypes.c_int, [c_ptr, c_i64, c_ptr]),
     "rkv_last_error": (ctypes.c_char_p, []),
     "rkv_status_string": (ctypes.c_char_p, [ctypes.c_int]),

@@ -24,6 +24,7 @@ own: a call of another shape replaces them in the dict.
 from __future__ import annotations
 
 import functools
+import math
 
 import torch
 
@@ -36,10 +37,11 @@ _BLOCKS = (16, 32, 64)
 
 
 @functools.lru_cache(maxsize=None)
-def _scratch_bytes(index: int, group: int, dim: int) -> int:
-    """``paged_attention``'s workspace size on a device: it follows from the head shape alone."""
+def _scratch_bytes(index: int, group: int, dim: int, dtype: int) -> int:
+    """``paged_attention``'s workspace size on a device: it follows from the head shape and the
+    pools' type alone."""
     with torch.cuda.device(index):
-        return _native.load().rkv_paged_workspace_size(group, dim)
+        return _native.load().rkv_paged_more_workspace_size(group, dim, dtype)
 
 
 def _pools(key_pool, value_pool, layout):
@@ -327,8 +329,11 @@ def paged_read(key_pool: torch.Tensor, value_pool: torch.Tensor, page_table: tor
 
 def paged_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor,
                     page_table: torch.Tensor, lengths: torch.Tensor, *, layout: str = "HND",
-                    scale: float | None = None, window: int | None = None,
-                    return_lse: bool = False, workspace: dict | None = None):
+                    scale: float | None = None, window: int | None = None, prefix: int = 0,
+                    softcap: float | None = None, slopes: torch.Tensor | None = None,
+                    key_scale: torch.Tensor | None = None, value_scale: torch.Tensor | None = None,
+                    weights: torch.Tensor | None = None, return_lse: bool = False,
+                    workspace: dict | None = None):
     """Exact attention of one new token per sequence over its own length of the pool.
 
     ``query``: (sequences, q_heads, head_dim) bf16 or fp32, any strides; query
@@ -337,10 +342,26 @@ def paged_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: tor
     pool (the new one included, once ``paged_append`` has written it); a
     sequence of length 0 (an idle slot) gives a zero row.  ``scale`` defaults
     to head_dim ** -0.5; ``window`` limits each query to the last ``window``
-    tokens.  Rows of a page past a sequence's length, pages past it and pages
-    before its window are never used, whatever they hold.  An fp32 query is
+    tokens, next to which the first ``prefix`` stay visible.  Rows of a page past
+    a sequence's length, pages past it and tokens between its prefix and its window
+    are never used, whatever they hold.  An fp32 query is
     rounded to bf16 first, like every query of this package; its
     probabilities, sums and output stay fp32.
+
+    The logit of token j of a sequence of L is ``c * tanh(scale * q.k / c)`` with
+    ``softcap`` c (without it ``scale * q.k``), plus ``slopes[head] * (j - (L -
+    1))`` with ``slopes``, (q_heads,) fp32: a bias that grows with the distance.
+
+    Pools may hold 4 bits a channel (``fp4_pool``), with the ``key_scale`` and
+    ``value_scale`` that ``paged_append`` was given: the attention is exact over
+    what the pool stands for.
+
+    ``weights``: (sequences, kv_heads, tokens) fp32, contiguous in its last
+    dimension and at least as wide as the page table's row in tokens: to each
+    visible token's entry the softmax weight that it got is added, summed over the
+    query heads of its KV head (what ``paged_evict`` goes by).  A query whose sum is
+    not finite adds nothing.  Takes a second launch and scratch for the logits,
+    4 bytes a query head and token of the page table.
 
     Returns the (sequences, q_heads, head_dim) output in the query's dtype or,
     with ``return_lse``, (output, lse) with the fp32 natural-log sum of the
@@ -352,7 +373,8 @@ def paged_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: tor
     lse) NaN; a negative length sets it and counts as 0.
     One launch; its results repeat bit for bit.
     """
-    pages, heads, block, dim, ks, vs = _pools(key_pool, value_pool, layout)
+    fp4 = key_pool.dtype is torch.uint8
+    pages, heads, block, dim, ks, vs = (_fp4_pools if fp4 else _pools)(key_pool, value_pool, layout)
     device = key_pool.device
     sequences, blocks, table_stride = _table(page_table, device)
     shape, dtype = query.shape, query.dtype
@@ -372,6 +394,10 @@ def paged_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: tor
         raise TypeError("lengths must be int32")
     if window is not None and window < 1:
         raise ValueError("window must be at least 1")
+    if prefix < 0:
+        raise ValueError("prefix must not be negative")
+    if not fp4 and (key_scale is not None or value_scale is not None):
+        raise ValueError("key_scale and value_scale belong to pools of 4 bits")
     scale = dim ** -0.5 if scale is None else float(scale)
     qs = query.stride()
     width = 2 if dtype == torch.bfloat16 else 4
@@ -380,16 +406,70 @@ def paged_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: tor
         qs = query.stride()
     if not lengths.is_contiguous():
         lengths = lengths.contiguous()
+    plain = not (fp4 or softcap is not None or slopes is not None or weights is not None
+                 or (prefix and window is not None))
+    more = ()
+    if not plain:
+        slopes, more = _more(sequences, heads, group, blocks * block, device, prefix, softcap,
+                             slopes, key_scale, value_scale, weights, fp4, workspace)
     out = _buffer(workspace, "paged_output", shape, device, dtype)
-    lse = _buffer(workspace, "paged_lse", shape[:2], device, torch.float32) if return_lse else None
-    scratch = _scratch(workspace, "rkv_paged_scratch", _scratch_bytes(device.index, group, dim),
-                       device)
+    lse = None
+    if return_lse or weights is not None:
+        lse = _buffer(workspace, "paged_lse", shape[:2], device, torch.float32)
+    kind = _native.DTYPE_FP4 if fp4 else _native.DTYPE_BF16
+    scratch = _scratch(workspace, "rkv_paged_scratch",
+                       _scratch_bytes(device.index, group, dim, kind), device)
+    lib = _native.load()
     _native.launch(
-        _native.load().rkv_paged_attention,
-        _native.PAGED_ARGS.pack(
-            query.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
+        lib.rkv_paged_attention if plain else lib.rkv_paged_attention_more,
+        (_native.PAGED_ARGS if plain else _native.PAGED_MORE_ARGS).pack(
+            query.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
             key_pool.data_ptr(), value_pool.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
             scratch.data_ptr(), scratch.numel(), qs[0], qs[1], *ks, *vs, table_stride, sequences,
-            blocks, pages, block, heads, group, dim, _DTYPES[dtype], window or 0, scale),
+            blocks, pages, block, heads, group, dim, _DTYPES[dtype], window or 0, scale, *more),
         device)
+    if weights is not None:
+        mark_written(weights)
     return (out, lse) if return_lse else out
+
+
+def _more(sequences, heads, group, capacity, device, prefix, softcap, slopes, key_scale,
+          value_scale, weights, fp4, workspace):
+    """The checked arguments of ``rkv_paged_attention_more`` behind ``rkv_paged_attention``'s, and
+    the slopes as they must be kept until the launch."""
+    if softcap is None:
+        softcap = 0.0
+    elif not (0 < softcap < math.inf):
+        raise ValueError("softcap must be positive and finite")
+    slopes_ptr = 0
+    if slopes is not None:
+        if slopes.shape != (heads * group,) or slopes.device != device:
+            raise ValueError("slopes must be (q_heads,) on the pools' device")
+        if slopes.dtype is not torch.float32:
+            raise TypeError("slopes must be fp32")
+        slopes = slopes.contiguous()
+        slopes_ptr = slopes.data_ptr()
+    factors = _factors(key_scale, value_scale, heads, device)
+    weights_ptr = scores_ptr = scores_size = tokens = 0
+    strides = (0, 0)
+    if weights is not None:
+        if (weights.ndim != 3 or weights.shape[:2] != (sequences, heads)
+                or weights.shape[2] < capacity or weights.device != device):
+            raise ValueError("weights must be (sequences, kv_heads, tokens) on the pools' device, "
+                             "with at least the page table's tokens")
+        if weights.dtype is not torch.float32:
+            raise TypeError("weights must be fp32")
+        *strides, last = weights.stride()
+        if (last != 1 and weights.shape[2] > 1) or (0 in strides and weights.numel() > 0):
+            raise ValueError("weights must have contiguous rows that do not overlap")
+        count = sequences * heads * group * capacity
+        scores = workspace.get("paged_scores") if workspace is not None else None
+        if scores is None or scores.device != device or scores.numel() < count:
+            scores = torch.empty(max(count, 4), device=device, dtype=torch.float32)
+            if workspace is not None:
+                workspace["paged_scores"] = scores
+        weights_ptr, scores_ptr, scores_size = weights.data_ptr(), scores.data_ptr(), 4 * scores.numel()
+        tokens = weights.shape[2]
+        slopes = (slopes, scores)  # both live until the launch
+    return slopes, (slopes_ptr, *factors, weights_ptr, scores_ptr, scores_size, *strides, tokens,
+                    _native.DTYPE_FP4 if fp4 else _native.DTYPE_BF16, prefix, softcap)
