@@ -698,6 +698,62 @@ RKV_API size_t rkv_paged_more_workspace_size(int64_t group, int64_t head_dim, in
 RKV_API int rkv_paged_attention_more(const rkv_paged_more_args* args, void* stream);
 
 /*
+ * Eviction from a page pool by what weight its tokens got (no reference
+ * counterpart).  For each sequence and KV head with n = lengths[s] > budget rows,
+ * `budget` rows are kept: the `recent` newest, and of the others those whose
+ * weight is greatest (NaN counts least; of equal ones the first).  Kept rows at or
+ * behind row `budget` move to the places of dropped rows before it, the i-th of
+ * the ones to the i-th of the others; the rest stays where it is.  So the rows of
+ * an evicted sequence are in no order of position (and of different tokens in
+ * each KV head), which attention without a window or a bias does not see.
+ *   weights: fp32 rows of weight_width >= table_blocks * block_size tokens by
+ *     element strides [sequence, KV head]: they move along, and those from row
+ *     `budget` to the sequence's end become zero.
+ *   positions: null, or int32 rows of position_width >= table_blocks *
+ *     block_size, which token each row holds: they move along (behind row
+ *     `budget` they are left as they were).  The newest rows are then those of
+ *     the positions above the row's greatest less `recent`; without positions
+ *     they are the last ones.
+ *   lengths_out: (sequences) int32, min(lengths, budget); may be `lengths`.
+ *   pools: as for rkv_paged_read, written in place; page_table as everywhere.
+ * Negative lengths count as 0; one past the page table leaves its sequence as it
+ * is, length included.  Both set RKV_DEVICE_BAD_INPUT in the workspace's status
+ * word, and so does a move from or to a page outside the pool: nothing is read or
+ * written there, and a row that comes from one is NaN.
+ * Two launches.  The workspace follows the rules at the top of this header.
+ */
+typedef struct rkv_evict_args {
+  void* key_pool;
+  void* value_pool;
+  const int32_t* page_table;
+  const int32_t* lengths;
+  int32_t* lengths_out;
+  float* weights;
+  int32_t* positions;
+  void* workspace;
+  int64_t workspace_size;
+  int64_t key_pool_strides[3];
+  int64_t value_pool_strides[3];
+  int64_t weight_strides[2];
+  int64_t position_strides[2];
+  int64_t weight_width;
+  int64_t position_width;
+  int64_t page_table_stride;
+  int64_t sequences;
+  int64_t table_blocks;
+  int64_t pool_pages;
+  int64_t block_size;
+  int64_t kv_heads;
+  int64_t head_dim;
+  int64_t pool_dtype;
+  int64_t budget;
+  int64_t recent;
+} rkv_evict_args;
+RKV_API size_t rkv_paged_evict_workspace_size(int64_t sequences, int64_t kv_heads, int64_t tokens,
+                                              int64_t budget);
+RKV_API int rkv_paged_evict(const rkv_evict_args* args, void* stream);
+
+/*
  * Diagnostic: one bounded device wait on an mbarrier that nothing completes,
  * with a limit of `limit_ns` (0 < limit_ns <= 1e9) instead of the kernels'
  * 1 s; it ORs RKV_DEVICE_TIMEOUT into the device int32 *status and returns,

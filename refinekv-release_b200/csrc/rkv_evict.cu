@@ -1,0 +1,496 @@
+// Eviction from a page pool by what weight its tokens got.
+//
+// Mathematics.  Per sequence and KV head with n > budget rows: a row counts by
+// its weight (NaN least), the `recent` newest before all; the `budget` rows that
+// count most are kept, of equal ones the first.  Kept rows behind the budget
+// move into the places of dropped rows before it, the i-th of the ones into the
+// i-th of the others, so a row moves once at most and nothing that is read is
+// written: sources lie behind the budget, targets before it.
+//
+// Bound: the weights are read once (4 bytes a row) and only the rows that move are
+// touched, 2 x 2 rows of 2 dim bytes (bf16); a step that drops one row a head is
+// latency alone.
+//
+// Two launches.  select_kernel finds the budget-th greatest by four passes of 8
+// bits over the weights as ordered integers, kept in shared memory, and writes the
+// list of moves; a row of a few long sequences is shared by a cluster of CTAs, whose
+// histograms and counts are added through distributed shared memory.  move_kernel
+// copies.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <string>
+
+#include "refinekv_b200.h"
+#include "rkv_device.cuh"
+#include "rkv_fp4.cuh"
+#include "rkv_kernels.h"
+
+namespace rkv {
+void set_last_error(const std::string& message);
+
+namespace {
+
+namespace cg = cooperative_groups;
+
+struct EvictParams {
+  uint8_t* pool[2];                      // keys, values
+  int64_t page[2], head[2], row[2];      // byte strides
+  const int32_t* page_table;
+  int64_t page_table_stride;
+  const int32_t* lengths;
+  int32_t* lengths_out;
+  float* weights;
+  int64_t weight_seq, weight_head;
+  int32_t* positions;
+  int64_t position_seq, position_head;
+  int sequences, heads, dim, block_shift, capacity, pool_pages;
+  int budget, recent;
+  int fp4;
+  int slice;   // rows of a CTA that its shared memory holds; 0: they are read again each time
+  int most;    // entries of a row's list
+  int* status;
+  int* counts;    // (rows): moves
+  int2* moves;    // (rows, most): from, to
+};
+
+constexpr int kSelectThreads = 512, kWarps = kSelectThreads / 32;
+constexpr int kMostCluster = 8;
+constexpr int kSliceBytes = 160 * 1024;
+
+// Weights in their order as unsigned integers: NaN 0, then -inf .. inf; a
+// protected row above all.
+__device__ __forceinline__ uint32_t rank_of(float weight) {
+  const uint32_t bits = __float_as_uint(weight + 0.f);  // -0 as 0
+  if ((bits & 0x7fffffffu) > 0x7f800000u) return 0;
+  return bits ^ (bits >> 31 ? 0xffffffffu : 0x80000000u);
+}
+constexpr uint32_t kProtected = 0xffffffffu;
+
+__global__ void __launch_bounds__(kSelectThreads)
+    select_kernel(const __grid_constant__ EvictParams p) {
+  extern __shared__ uint32_t ranks[];
+  __shared__ unsigned hist[2][256];
+  __shared__ unsigned totals[3];         // of this CTA, for the cluster: equal ones, holes, movers
+  __shared__ int newest;                 // of this CTA
+  __shared__ unsigned warp_counts[2][kWarps];
+  __shared__ uint32_t found;
+  __shared__ unsigned found_rest, found_equal;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int size = cluster.num_blocks(), part = cluster.block_rank();
+  const int row = blockIdx.x / size, seq = row / p.heads, head = row - seq * p.heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const auto meet = [&] {
+    if (size > 1) cluster.sync();
+    else __syncthreads();
+  };
+  pdl_wait();
+  pdl_launch_dependents();
+  const int length = p.lengths[seq];
+  if (length < 0 || length > p.capacity) {
+    if (threadIdx.x == 0 && part == 0 && head == 0) atomicOr(p.status, kStatusBadInput);
+  }
+  if (length <= p.budget || length > p.capacity) {  // the whole cluster
+    if (threadIdx.x == 0 && part == 0) p.counts[row] = 0;
+    return;
+  }
+  const int each = (length + size * kSelectThreads - 1) / (size * kSelectThreads) * kSelectThreads;
+  const int lo = min(length, part * each), hi = min(length, lo + each);
+  float* weights = p.weights + seq * p.weight_seq + head * p.weight_head;
+  const int32_t* positions =
+      p.positions != nullptr ? p.positions + seq * p.position_seq + head * p.position_head : nullptr;
+
+  int last = length - 1;
+  if (positions != nullptr && p.recent > 0) {
+    if (threadIdx.x == 0) newest = INT_MIN;
+    __syncthreads();
+    int mine = INT_MIN;
+    for (int i = lo + threadIdx.x; i < hi; i += kSelectThreads) mine = max(mine, positions[i]);
+    mine = __reduce_max_sync(0xffffffffu, mine);
+    if (lane == 0) atomicMax(&newest, mine);
+    meet();
+    last = INT_MIN;
+    for (int k = 0; k < size; ++k) last = max(last, *cluster.map_shared_rank(&newest, k));
+  }
+  const auto fresh_rank = [&](int i) {
+    // Differences of positions in 64 bits: any two of them.
+    const int64_t age = static_cast<int64_t>(last) - (positions != nullptr ? positions[i] : i);
+    return p.recent > 0 && age < p.recent ? kProtected : rank_of(weights[i]);
+  };
+  const bool held = p.slice > 0;
+  if (held) {
+    for (int i = lo + threadIdx.x; i < hi; i += kSelectThreads) ranks[i - lo] = fresh_rank(i);
+  }
+  const auto rank_at = [&](int i) { return held ? ranks[i - lo] : fresh_rank(i); };
+
+  // The budget-th greatest, from its highest bits down.
+  uint32_t prefix = 0;
+  unsigned want = p.budget, equal = 0;
+  for (int pass = 0; pass < 4; ++pass) {
+    const int shift = 24 - 8 * pass;
+    unsigned* mine = hist[pass & 1];
+    // The other one may still be read by the cluster; this one was two passes ago.
+    for (int b = threadIdx.x; b < 256; b += kSelectThreads) mine[b] = 0;
+    __syncthreads();
+    for (int i = lo + threadIdx.x; i < hi; i += kSelectThreads) {
+      const uint32_t x = rank_at(i);
+      if (pass == 0 || x >> (shift + 8) == prefix) atomicAdd(&mine[x >> shift & 255], 1u);
+    }
+    meet();
+    if (warp == 0) {
+      // Lane 0 has the highest eight bins.
+      unsigned bins[8], sum = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int b = 255 - 8 * lane - k;
+        bins[k] = 0;
+        for (int c = 0; c < size; ++c) bins[k] += *cluster.map_shared_rank(&mine[b], c);
+        sum += bins[k];
+      }
+      unsigned scan = sum;
+#pragma unroll
+      for (int step = 1; step < 32; step <<= 1) {
+        const unsigned other = __shfl_up_sync(0xffffffffu, scan, step);
+        if (lane >= step) scan += other;
+      }
+      const unsigned before = scan - sum;
+      if (before < want && want <= scan) {  // one lane
+        unsigned above = before;
+        bool done = false;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (!done && above + bins[k] >= want) {
+            done = true;
+            found = prefix << 8 | static_cast<uint32_t>(255 - 8 * lane - k);
+            found_rest = want - above;
+            found_equal = bins[k];
+          }
+          if (!done) above += bins[k];
+        }
+      }
+    }
+    __syncthreads();
+    prefix = found;
+    want = found_rest;
+    equal = found_equal;
+  }
+  const uint32_t threshold = prefix;
+  // `want` of the `equal` rows that equal the threshold are kept, the first ones.
+
+  // Counts before this CTA and this warp; a warp's rows are contiguous.
+  const int span = (each / kWarps + 31) / 32 * 32;
+  const int from = min(hi, lo + warp * span), to = min(hi, from + span);
+  // Sums of totals[which] over the CTAs before this one.
+  const auto before_cta = [&](int which) {
+    unsigned sum = 0;
+    for (int c = 0; c < part; ++c) sum += *cluster.map_shared_rank(&totals[which], c);
+    return sum;
+  };
+  unsigned equal_before = 0;
+  if (want < equal) {
+    unsigned mine = 0;
+    for (int i = from + lane; i < to; i += 32) mine += rank_at(i) == threshold;
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    if (lane == 0) warp_counts[0][warp] = mine;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      unsigned sum = 0;
+      for (int w = 0; w < kWarps; ++w) sum += warp_counts[0][w];
+      totals[0] = sum;
+    }
+    meet();
+    equal_before = before_cta(0);
+    for (int w = 0; w < warp; ++w) equal_before += warp_counts[0][w];
+    __syncthreads();
+  }
+  // Walks the warp's rows: visit(i, kept, hole, mover).
+  const auto walk = [&](auto visit) {
+    unsigned seen = equal_before;
+    for (int base = from; base < to; base += 32) {
+      const int i = base + lane;
+      const bool there = i < to;
+      const uint32_t x = there ? rank_at(i) : 0;
+      const bool same = there && x == threshold;
+      const unsigned sames = __ballot_sync(0xffffffffu, same);
+      const unsigned order = seen + __popc(sames & ((1u << lane) - 1));
+      seen += __popc(sames);
+      const bool kept = there && (x > threshold || (same && order < want));
+      visit(i, there, there && !kept && i < p.budget, kept && i >= p.budget);
+    }
+  };
+  unsigned holes = 0, movers = 0;
+  walk([&](int, bool, bool hole, bool mover) {
+    holes += __popc(__ballot_sync(0xffffffffu, hole));
+    movers += __popc(__ballot_sync(0xffffffffu, mover));
+  });
+  if (lane == 0) {
+    warp_counts[0][warp] = holes;
+    warp_counts[1][warp] = movers;
+  }
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    unsigned sum = 0;
+    for (int w = 0; w < kWarps; ++w) sum += warp_counts[threadIdx.x][w];
+    totals[1 + threadIdx.x] = sum;
+  }
+  meet();
+  holes = before_cta(1);
+  movers = before_cta(2);
+  if (threadIdx.x == 0 && part == size - 1) p.counts[row] = static_cast<int>(movers + totals[2]);
+  for (int w = 0; w < warp; ++w) {
+    holes += warp_counts[0][w];
+    movers += warp_counts[1][w];
+  }
+  int2* moves = p.moves + static_cast<int64_t>(row) * p.most;
+  walk([&](int i, bool there, bool hole, bool mover) {
+    const unsigned below = (1u << lane) - 1;
+    const unsigned all_holes = __ballot_sync(0xffffffffu, hole);
+    const unsigned all_movers = __ballot_sync(0xffffffffu, mover);
+    if (mover) moves[movers + __popc(all_movers & below)].x = i;
+    if (hole) moves[holes + __popc(all_holes & below)].y = i;
+    holes += __popc(all_holes);
+    movers += __popc(all_movers);
+    // A dropped row's weight ends with it; a mover's goes along.
+    if (there && i >= p.budget && !mover) weights[i] = 0.f;
+  });
+  if (size > 1) cluster.sync();  // no CTA leaves while another reads its counts
+}
+
+constexpr int kMoveThreads = 256;
+
+// A unit is what a lane copies at once: 16 bytes of a row, or two of its scales'.
+__global__ void __launch_bounds__(kMoveThreads)
+    move_kernel(const __grid_constant__ EvictParams p, unsigned parts) {
+  const int row = static_cast<int>(blockIdx.x / parts);
+  const unsigned part = blockIdx.x - static_cast<unsigned>(row) * parts;
+  const int seq = row / p.heads, head = row - seq * p.heads;
+  const int units = p.fp4 ? p.dim / 16 : p.dim / 8;  // of a key or a value
+  const int wide = p.fp4 ? p.dim / 32 : units;       // of them, 16 bytes each
+  pdl_wait();
+  pdl_launch_dependents();
+  if (part == 0 && head == 0 && threadIdx.x == 0) {
+    const int length = p.lengths[seq];
+    p.lengths_out[seq] = length > p.capacity ? length : min(max(length, 0), p.budget);
+  }
+  const int64_t count = static_cast<int64_t>(p.counts[row]) * 2 * units;
+  const int2* moves = p.moves + static_cast<int64_t>(row) * p.most;
+  const int32_t* table = p.page_table + seq * p.page_table_stride;
+  const int mask = (1 << p.block_shift) - 1;
+  const auto page_of = [&](int token) {
+    const int page = table[token >> p.block_shift];
+    return page >= 0 && page < p.pool_pages ? page : -1;
+  };
+  for (int64_t x = part * kMoveThreads + threadIdx.x; x < count;
+       x += static_cast<int64_t>(parts) * kMoveThreads) {
+    const int move = static_cast<int>(x / (2 * units));
+    const int rest = static_cast<int>(x - static_cast<int64_t>(move) * 2 * units);
+    const int which = rest >= units ? 1 : 0, unit = rest - which * units;
+    const int2 m = moves[move];
+    const int from_page = page_of(m.x), to_page = page_of(m.y);
+    if ((from_page < 0 || to_page < 0) && rest == 0) atomicOr(p.status, kStatusBadInput);
+    const auto place = [&](int page, int token) {
+      const int r = token & mask;
+      uint8_t* slab = p.pool[which] + page * p.page[which] + head * p.head[which];
+      if (unit < wide) return slab + (p.fp4 ? r * (p.dim / 2) : r * p.row[which]) + 16 * unit;
+      return slab + (p.dim / 2 << p.block_shift) + r * (p.dim / 16) + 2 * (unit - wide);
+    };
+    if (to_page >= 0) {
+      uint8_t* to = place(to_page, m.y);
+      if (unit < wide) {
+        // A row whose page is outside the pool is NaN where it goes.
+        uint4 data = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+        if (from_page >= 0) data = *reinterpret_cast<const uint4*>(place(from_page, m.x));
+        *reinterpret_cast<uint4*>(to) = data;
+      } else {
+        uint16_t data = kFp4NanScale << 8 | kFp4NanScale;
+        if (from_page >= 0) data = *reinterpret_cast<const uint16_t*>(place(from_page, m.x));
+        *reinterpret_cast<uint16_t*>(to) = data;
+      }
+    }
+    if (rest == 0) {
+      float* weights = p.weights + seq * p.weight_seq + head * p.weight_head;
+      weights[m.y] = weights[m.x];
+      weights[m.x] = 0.f;
+      if (p.positions != nullptr) {
+        int32_t* positions = p.positions + seq * p.position_seq + head * p.position_head;
+        positions[m.y] = positions[m.x];
+      }
+    }
+  }
+}
+
+int reject(int code, const char* message) {
+  set_last_error(message);
+  return code;
+}
+
+constexpr size_t kEvictHeader = 256;
+
+int64_t list_entries(int64_t capacity, int64_t budget) {
+  return std::max<int64_t>(0, std::min(budget, capacity - budget));
+}
+
+// Bytes of a workspace: the status word, a count a row, a list a row.
+int64_t evict_bytes(int64_t rows, int64_t capacity, int64_t budget, int64_t* lists) {
+  *lists = static_cast<int64_t>(kEvictHeader) + (rows * 4 + 255) / 256 * 256;
+  return *lists + rows * list_entries(capacity, budget) * 8;
+}
+
+template <typename Kernel, typename... Args>
+cudaError_t launch(Kernel kernel, unsigned grid, int threads, size_t smem, int cluster,
+                   cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+}  // namespace
+}  // namespace rkv
+
+extern "C" {
+
+size_t rkv_paged_evict_workspace_size(int64_t sequences, int64_t kv_heads, int64_t tokens,
+                                      int64_t budget) {
+  using namespace rkv;
+  if (sequences < 0 || sequences > kMostSequences || kv_heads < 1 || kv_heads > kMostPagedHeads ||
+      tokens < 0 || tokens > kMostPagedTokens || budget < 1) {
+    return 0;
+  }
+  int64_t lists;
+  return static_cast<size_t>(evict_bytes(sequences * kv_heads, tokens, budget, &lists));
+}
+
+int rkv_paged_evict(const rkv_evict_args* a, void* stream) {
+  using namespace rkv;
+  set_last_error("");
+  if (a == nullptr) return reject(RKV_ERR_INVALID_ARGUMENT, "args is null");
+  if (a->head_dim < 32 || a->head_dim > 256 || a->head_dim % 32 != 0) {
+    return reject(RKV_ERR_UNSUPPORTED, "head_dim must be a multiple of 32 in [32, 256]");
+  }
+  if (a->block_size != 16 && a->block_size != 32 && a->block_size != 64) {
+    return reject(RKV_ERR_UNSUPPORTED, "block_size must be 16, 32 or 64");
+  }
+  if (a->sequences < 0 || a->sequences > kMostSequences || a->kv_heads < 1 ||
+      a->kv_heads > kMostPagedHeads) {
+    return reject(RKV_ERR_UNSUPPORTED, "at most 4096 sequences and 4096 KV heads");
+  }
+  const bool fp4 = a->pool_dtype == RKV_DTYPE_FP4;
+  if (!fp4 && a->pool_dtype != RKV_DTYPE_BF16) {
+    return reject(RKV_ERR_INVALID_ARGUMENT, "pools are bf16 or fp4");
+  }
+  if (a->table_blocks < 0 || a->table_blocks > kMostPagedTokens / a->block_size ||
+      a->page_table_stride < 0 || a->pool_pages < 0 || a->pool_pages > (1LL << 31) - 1) {
+    return reject(RKV_ERR_INVALID_ARGUMENT, "page table or pool sizes are out of range");
+  }
+  if (a->budget < 1 || a->recent < 0 || a->recent > a->budget) {
+    return reject(RKV_ERR_INVALID_ARGUMENT, "budget must be positive and recent at most budget");
+  }
+  const int64_t capacity = a->table_blocks * a->block_size;
+  if (a->weight_width < capacity || (a->positions != nullptr && a->position_width < capacity)) {
+    return reject(RKV_ERR_INVALID_ARGUMENT,
+                  "rows of weights and positions must hold as many tokens as the page table");
+  }
+  if (a->sequences == 0) return RKV_OK;
+  if (!a->key_pool || !a->value_pool || !a->page_table || !a->lengths || !a->lengths_out ||
+      !a->weights) {
+    return reject(RKV_ERR_INVALID_ARGUMENT,
+                  "pools, page_table, lengths, lengths_out and weights must be non-null");
+  }
+  const int width = fp4 ? 1 : 2;
+  uintptr_t bits = reinterpret_cast<uintptr_t>(a->key_pool) | reinterpret_cast<uintptr_t>(a->value_pool);
+  for (int i = 0; i < (fp4 ? 2 : 3); ++i) {
+    bits |= static_cast<uintptr_t>(a->key_pool_strides[i] * width);
+    bits |= static_cast<uintptr_t>(a->value_pool_strides[i] * width);
+  }
+  if (bits & 15u) {
+    return reject(RKV_ERR_ALIGNMENT, "pools and their strides must be multiples of 16 bytes");
+  }
+  if (!aligned_to(4, {a->page_table, a->lengths, a->lengths_out, a->weights, a->positions})) {
+    return reject(RKV_ERR_ALIGNMENT, "page_table, lengths, weights and positions must be aligned to "
+                                     "their elements");
+  }
+  const int64_t rows = a->sequences * a->kv_heads;
+  int64_t lists;
+  if (a->workspace == nullptr ||
+      a->workspace_size < evict_bytes(rows, capacity, a->budget, &lists) ||
+      (reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0) {
+    return reject(RKV_ERR_WORKSPACE, "workspace is missing, too small or not 256-byte aligned");
+  }
+  int sms = 0;
+  const int rc = device_sms(&sms);
+  if (rc != RKV_OK) return rc;
+  EvictParams p = {};
+  p.pool[0] = static_cast<uint8_t*>(a->key_pool);
+  p.pool[1] = static_cast<uint8_t*>(a->value_pool);
+  for (int i = 0; i < 2; ++i) {
+    const int64_t* strides = i ? a->value_pool_strides : a->key_pool_strides;
+    p.page[i] = strides[0] * width;
+    p.head[i] = strides[1] * width;
+    p.row[i] = fp4 ? 0 : strides[2] * width;
+  }
+  p.page_table = a->page_table;
+  p.page_table_stride = a->page_table_stride;
+  p.lengths = a->lengths;
+  p.lengths_out = a->lengths_out;
+  p.weights = a->weights;
+  p.weight_seq = a->weight_strides[0];
+  p.weight_head = a->weight_strides[1];
+  p.positions = a->positions;
+  p.position_seq = a->position_strides[0];
+  p.position_head = a->position_strides[1];
+  p.sequences = static_cast<int>(a->sequences);
+  p.heads = static_cast<int>(a->kv_heads);
+  p.dim = static_cast<int>(a->head_dim);
+  p.block_shift = a->block_size == 16 ? 4 : a->block_size == 32 ? 5 : 6;
+  p.capacity = static_cast<int>(capacity);
+  p.pool_pages = static_cast<int>(a->pool_pages);
+  p.budget = static_cast<int>(std::min<int64_t>(a->budget, kMostPagedTokens));
+  p.recent = static_cast<int>(std::min<int64_t>(a->recent, kMostPagedTokens));
+  p.fp4 = fp4;
+  p.most = static_cast<int>(list_entries(capacity, a->budget));
+  char* ws = static_cast<char*>(a->workspace);
+  p.status = reinterpret_cast<int*>(ws);
+  p.counts = reinterpret_cast<int*>(ws + kEvictHeader);
+  p.moves = reinterpret_cast<int2*>(ws + lists);
+  // A row is shared by as many CTAs as the device has room for, of 4096 tokens at
+  // least, and by eight where its ranks fit in shared memory only so.
+  int size = 1;
+  while (size < kMostCluster && ((rows * size < sms && capacity > 4096 * size) ||
+                                 capacity * 4 > static_cast<int64_t>(kSliceBytes) * size)) {
+    size *= 2;
+  }
+  const int64_t whole = static_cast<int64_t>(size) * kSelectThreads;
+  const int64_t slice = (capacity + whole - 1) / whole * kSelectThreads;
+  p.slice = slice * 4 <= kSliceBytes ? static_cast<int>(slice) : 0;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t err =
+      ensure_smem_limit(reinterpret_cast<const void*>(&select_kernel), kSliceBytes);
+  if (err == cudaSuccess) {
+    err = launch(select_kernel, static_cast<unsigned>(rows * size), kSelectThreads,
+                 static_cast<size_t>(p.slice) * 4, size, st, p);
+  }
+  if (err == cudaSuccess) {
+    const int64_t units = static_cast<int64_t>(p.most) * 2 * (fp4 ? p.dim / 16 : p.dim / 8);
+    const unsigned parts = static_cast<unsigned>(std::max<int64_t>(
+        1, std::min((units + kMoveThreads - 1) / kMoveThreads, (8 * sms + rows - 1) / rows)));
+    err = launch(move_kernel, static_cast<unsigned>(rows * parts), kMoveThreads, 0, 1, st, p, parts);
+  }
+  if (err != cudaSuccess) {
+    set_last_error(std::string("eviction launch: ") + cudaGetErrorString(err));
+    return RKV_ERR_CUDA;
+  }
+  return RKV_OK;
+}
+
+}  // extern "C"

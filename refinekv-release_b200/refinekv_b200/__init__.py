@@ -14,7 +14,8 @@ kernel), ``rotary_table`` / ``apply_rotary`` (rotary positions),
 ``paged_append`` (new tokens into the page pool, rotated on the way; ``fp4_pool`` for one
 of 4 bits), ``paged_read`` (its rows back),
 ``paged_attention`` (dense attention of one new token per sequence, each over
-its own length of the pool) and ``refinekv_b200.parallel`` (KV-head sharding and sequence split
+its own length of the pool), ``paged_evict`` (a sequence down to the tokens that got the
+most weight) and ``refinekv_b200.parallel`` (KV-head sharding and sequence split
 over GPUs).
 
 All compute runs in the CUDA library ``librefinekv_b200.so`` built from
@@ -44,6 +45,7 @@ __all__ = [
     "paged_append",
     "paged_read",
     "paged_attention",
+    "paged_evict",
     "RefineKV",
     "make_visible_static_cache",
 ]
@@ -54,7 +56,8 @@ _HOMES = {
     "summary": ("BlockSummary", "build_summary", "build_summary_batch", "build_summary_into",
                 "attach_page_pool", "page_view", "PageView"),
     "rotary": ("rotary_table", "apply_rotary"),
-    "paged": ("fp4_pool", "paged_append", "paged_read", "paged_attention"),
+    "paged": ("fp4_pool", "paged_append", "paged_read", "paged_attention",
+              "paged_evict"),
     "integrations.transformers": ("RefineKV", "make_visible_static_cache"),
 }
 

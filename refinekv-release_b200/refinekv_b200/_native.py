@@ -70,6 +70,8 @@ EXPORTS = (
     "rkv_paged_attention",
     "rkv_paged_more_workspace_size",
     "rkv_paged_attention_more",
+    "rkv_paged_evict_workspace_size",
+    "rkv_paged_evict",
     "rkv_selftest_wait_timeout",
     "rkv_last_error",
     "rkv_status_string",
@@ -119,6 +121,7 @@ APPEND_FP4_ARGS = struct.Struct("=42q")
 READ_ARGS = struct.Struct("=31q")
 PAGED_ARGS = struct.Struct("=27qd")
 PAGED_MORE_ARGS = struct.Struct("=27qd11qd")
+EVICT_ARGS = struct.Struct("=31q")
 
 _SIGNATURES = {
     "rkv_summarize": (ctypes.c_int, [c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64,
@@ -173,6 +176,8 @@ _SIGNATURES = {
     "rkv_paged_attention": (ctypes.c_int, [ctypes.c_char_p, c_ptr]),
     "rkv_paged_more_workspace_size": (ctypes.c_size_t, [c_i64, c_i64, c_i64]),
     "rkv_paged_attention_more": (ctypes.c_int, [ctypes.c_char_p, c_ptr]),
+    "rkv_paged_evict_workspace_size": (ctypes.c_size_t, [c_i64, c_i64, c_i64, c_i64]),
+    "rkv_paged_evict": (ctypes.c_int, [ctypes.c_char_p, c_ptr]),
     "rkv_selftest_wait_timeout": (ctypes.c_int, [c_ptr, c_i64, c_ptr]),
     "rkv_last_error": (ctypes.c_char_p, []),
     "rkv_status_string": (ctypes.c_char_p, [ctypes.c_int]),

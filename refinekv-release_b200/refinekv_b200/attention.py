@@ -72,7 +72,8 @@ def _buffer(workspace, name, shape, device, dtype, zero=False):
 
 
 #: Workspace entries whose first word is a sticky status that ``device_status`` reports.
-_STATUS_WORDS = ("rkv_decode_scratch", "rkv_paged_scratch", "rkv_append_status")
+_STATUS_WORDS = ("rkv_decode_scratch", "rkv_paged_scratch", "rkv_append_status",
+                 "rkv_evict_scratch")
 
 
 def _scratch(workspace, name, nbytes, device):
@@ -101,8 +102,8 @@ def _scratch(workspace, name, nbytes, device):
 def device_status(workspace: dict) -> int:
     """Sticky device status of a workspace's calls (synchronises); 0 means healthy.
 
-    The union of the status words of ``sparse_attention``, ``paged_attention``
-    and ``paged_append`` calls that were given this workspace.  A call that
+    The union of the status words of ``sparse_attention``, ``paged_attention``,
+    ``paged_append``, ``paged_read`` and ``paged_evict`` calls that were given this workspace.  A call that
     allocates its scratch while a graph is captured (the first with this
     workspace, or one of a wider shape) has the graph clear its word at every replay.
     """

@@ -433,6 +433,24 @@ def paged_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: tor
     return (out, lse) if return_lse else out
 
 
+def _token_rows(name, rows, dtype, sequences, heads, capacity, device):
+    """Checks (sequences, kv_heads, tokens) rows that are written in place."""
+    shape = rows.shape
+    if (len(shape) != 3 or shape[0] != sequences or shape[1] != heads or shape[2] < capacity
+            or rows.device != device):
+        raise ValueError(f"{name} must be (sequences, kv_heads, tokens) on the pools' device, with at "
+                         "least the page table's tokens")
+    if rows.dtype is not dtype:
+        raise TypeError(f"{name} must be {'fp32' if dtype is torch.float32 else 'int32'}")
+    *outer, last = rows.stride()
+    extent, apart = shape[2], last == 1 or shape[2] <= 1
+    for stride, count in sorted(zip(outer, shape)):
+        apart = apart and (count <= 1 or stride >= extent)
+        extent += stride * (count - 1) if count > 1 else 0
+    if not apart:
+        raise ValueError(f"{name} must have contiguous rows that do not overlap")
+
+
 def _more(sequences, heads, group, capacity, device, prefix, softcap, slopes, key_scale,
           value_scale, weights, fp4, workspace):
     """The checked arguments of ``rkv_paged_attention_more`` behind ``rkv_paged_attention``'s, and
@@ -453,15 +471,8 @@ def _more(sequences, heads, group, capacity, device, prefix, softcap, slopes, ke
     weights_ptr = scores_ptr = scores_size = tokens = 0
     strides = (0, 0)
     if weights is not None:
-        if (weights.ndim != 3 or weights.shape[:2] != (sequences, heads)
-                or weights.shape[2] < capacity or weights.device != device):
-            raise ValueError("weights must be (sequences, kv_heads, tokens) on the pools' device, "
-                             "with at least the page table's tokens")
-        if weights.dtype is not torch.float32:
-            raise TypeError("weights must be fp32")
-        *strides, last = weights.stride()
-        if (last != 1 and weights.shape[2] > 1) or (0 in strides and weights.numel() > 0):
-            raise ValueError("weights must have contiguous rows that do not overlap")
+        _token_rows("weights", weights, torch.float32, sequences, heads, capacity, device)
+        strides = weights.stride()[:2]
         count = sequences * heads * group * capacity
         scores = workspace.get("paged_scores") if workspace is not None else None
         if scores is None or scores.device != device or scores.numel() < count:
@@ -473,3 +484,72 @@ def _more(sequences, heads, group, capacity, device, prefix, softcap, slopes, ke
         slopes = (slopes, scores)  # both live until the launch
     return slopes, (slopes_ptr, *factors, weights_ptr, scores_ptr, scores_size, *strides, tokens,
                     _native.DTYPE_FP4 if fp4 else _native.DTYPE_BF16, prefix, softcap)
+
+
+def paged_evict(key_pool: torch.Tensor, value_pool: torch.Tensor, page_table: torch.Tensor,
+                lengths: torch.Tensor, weights: torch.Tensor, budget: int, *, recent: int = 0,
+                positions: torch.Tensor | None = None, layout: str = "HND",
+                workspace: dict | None = None) -> torch.Tensor:
+    """Bring sequences down to ``budget`` tokens a KV head: those that got the most weight stay.
+
+    ``lengths``: (sequences,) int32, the rows each sequence has in the pool (bf16 or
+    4 bits, ``fp4_pool``).  ``weights``: (sequences, kv_heads, tokens) fp32, what
+    ``paged_attention`` adds up.  Of a KV head's rows in a sequence of more than
+    ``budget`` are kept the ``recent`` newest and of the others the ones of
+    greatest weight (of equal ones the first; NaN counts least).  Kept rows at or
+    behind row ``budget`` move into the places of dropped ones before it, keys,
+    values, weights and all, so that the sequence is its first ``budget`` rows
+    again; weights behind it become zero, ready for the next tokens.
+
+    Rows are then in no order of position, and each KV head has its own tokens:
+    ``paged_attention`` does not see that, but a ``window``, ``slopes`` or block
+    summaries no longer fit such a sequence.  ``positions``: (sequences, kv_heads,
+    tokens) int32 says which token each row holds, moves along and decides which
+    rows are newest (those above the greatest less ``recent``); without it they are
+    the last rows, which holds for a first eviction.  A token appended later goes to
+    row ``lengths`` (``paged_append``'s position) but is rotated by its own position
+    (``apply_rotary``).
+
+    Returns the new lengths, ``min(lengths, budget)`` (backed by ``workspace``,
+    reused by the next call).  Pools, weights and positions are written in place;
+    nothing carries a gradient.  A length past the page table leaves its sequence
+    as it is, a negative one counts as 0, and a row from a page outside the pool is
+    NaN where it goes; each sets bit 1 of ``attention.device_status(workspace)``.
+    """
+    fp4 = key_pool.dtype is torch.uint8
+    pages, heads, block, dim, ks, vs = (_fp4_pools if fp4 else _pools)(key_pool, value_pool, layout)
+    device = key_pool.device
+    sequences, blocks, table_stride = _table(page_table, device)
+    if lengths.shape != (sequences,) or lengths.device != device:
+        raise ValueError("lengths must be (sequences,) on the pools' device")
+    if lengths.dtype != torch.int32:
+        raise TypeError("lengths must be int32")
+    if not lengths.is_contiguous():
+        lengths = lengths.contiguous()
+    capacity = blocks * block
+    if budget < 1:
+        raise ValueError("budget must be at least 1")
+    if not 0 <= recent <= budget:
+        raise ValueError("recent must be between 0 and budget")
+    _token_rows("weights", weights, torch.float32, sequences, heads, capacity, device)
+    positions_ptr = positions_width = 0
+    position_strides = (0, 0)
+    if positions is not None:
+        _token_rows("positions", positions, torch.int32, sequences, heads, capacity, device)
+        positions_ptr, positions_width = positions.data_ptr(), positions.shape[2]
+        position_strides = positions.stride()[:2]
+    out = _buffer(workspace, "evict_lengths", (sequences,), device, torch.int32)
+    lib = _native.load()
+    need = lib.rkv_paged_evict_workspace_size(sequences, heads, capacity, budget)
+    scratch = _scratch(workspace, "rkv_evict_scratch", need, device)
+    _native.launch(
+        lib.rkv_paged_evict,
+        _native.EVICT_ARGS.pack(
+            key_pool.data_ptr(), value_pool.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
+            out.data_ptr(), weights.data_ptr(), positions_ptr, scratch.data_ptr(), scratch.numel(),
+            *ks, *vs, *weights.stride()[:2], *position_strides, weights.shape[2], positions_width,
+            table_stride, sequences, blocks, pages, block, heads, dim,
+            _native.DTYPE_FP4 if fp4 else _native.DTYPE_BF16, budget, recent),
+        device)
+    mark_written(key_pool, value_pool, weights, positions)
+    return out
