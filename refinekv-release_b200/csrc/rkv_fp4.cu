@@ -27,27 +27,30 @@ __device__ __forceinline__ float widen(T x) {
   return static_cast<float>(x);
 }
 
-// Where a token's rows are in the pool.
-struct Place {
-  int64_t page;
-  int row;
-  bool keep;  // false: padding, or out of range
-};
-
 __device__ __forceinline__ int64_t position_of(const RowsParams& p, unsigned n) {
   return p.pos_i64 ? static_cast<const int64_t*>(p.positions)[n]
                    : static_cast<const int32_t*>(p.positions)[n];
 }
 
-// `known`: the position is within the rotation table, where there is one.
-__device__ __forceinline__ Place find_place(const RowsParams& p, unsigned n, int64_t pos, bool known,
-                                            bool report) {
-  Place at = {0, 0, pos >= 0};
+// Where a token's rows are in the pool.
+struct Place {
+  int64_t pos;
+  int page, row;
+  bool keep;   // false: padding, or out of range
+  bool known;  // the position is within the rotation table, where there is one
+};
+
+__device__ __forceinline__ Place find_place(const RowsParams& p, unsigned n, bool report) {
+  Place at;
+  at.pos = position_of(p, n);
+  at.known = p.rotary == 0 || (at.pos >= 0 && at.pos < p.table_rows);
+  at.page = at.row = 0;
+  at.keep = at.pos >= 0;
   if (!at.keep) return at;
   const int64_t seq = p.sequence_ids != nullptr ? p.sequence_ids[n] : static_cast<int64_t>(n);
-  const int64_t block = pos >> p.block_shift;
-  at.row = static_cast<int>(pos - (block << p.block_shift));
-  at.keep = known && seq >= 0 && seq < p.sequences && block < p.table_blocks;
+  const int64_t block = at.pos >> p.block_shift;
+  at.row = static_cast<int>(at.pos - (block << p.block_shift));
+  at.keep = at.known && seq >= 0 && seq < p.sequences && block < p.table_blocks;
   if (at.keep) {
     at.page = p.page_table[seq * p.page_table_stride + block];
     at.keep = at.page >= 0 && at.page < p.pool_pages;
@@ -56,34 +59,81 @@ __device__ __forceinline__ Place find_place(const RowsParams& p, unsigned n, int
   return at;
 }
 
-// Sixteen channels' scale; the quotients of 8 of them by it.
-__device__ __forceinline__ uint32_t quotients(float (&y)[8], uint32_t scale) {
-  const float by = fp4_scale_value(scale);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    y[j] = by > 0.f ? __fdiv_rn(y[j], by) : scale == kFp4NanScale ? 0.f : copysignf(0.f, y[j]);
+// A CTA takes every gridDim.x-th token.  Their places hang on three loads in a
+// row, so a thread each finds those of up to kBatch tokens at once, ahead of the
+// rows' own loads.  Returns how many (for the whole CTA).
+constexpr int kBatch = 64;
+
+__device__ __forceinline__ unsigned find_places(const RowsParams& p, Place (&places)[kBatch],
+                                                unsigned first, bool report) {
+  const unsigned left = (static_cast<unsigned>(p.tokens) - first + gridDim.x - 1) / gridDim.x;
+  const unsigned there = min(left, min(static_cast<unsigned>(kBatch), blockDim.x));
+  __syncthreads();  // the batch before is done with
+  if (threadIdx.x < there) {
+    places[threadIdx.x] = find_place(p, first + threadIdx.x * gridDim.x, report);
   }
-  return fp4_encode(y);
+  __syncthreads();
+  return there;
+}
+
+// x / b correctly rounded, r being 1 / b correctly rounded: the first quotient's
+// error x - q b is exact, and corrects it (Markstein 1990, on division by fused
+// multiply-adds).  Ties between two codes must be met exactly (bf16 rows are full of
+// them), which x r alone does not; three instructions instead of a division's ten or
+// so.  Finite numbers whose quotient neither overflows nor is tiny; r = 0 gives 0
+// with the sign of x.
+__device__ __forceinline__ float quotient(float x, float b, float r) {
+  const float q = __fmul_rn(x, r);
+  return __fmaf_rn(-__fmaf_rn(b, q, -x), r, q);  // in these signs -0 stays -0
+}
+
+// The codes of 8 of the 16 channels that share a scale.
+__device__ __forceinline__ uint32_t codes_of(float (&y)[8], uint32_t scale) {
+  const float by = fp4_scale_value(scale), r = by > 0.f ? __frcp_rn(by) : 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) y[j] = quotient(y[j], by, r);
+  const uint32_t codes = fp4_encode(y);
+  return scale == kFp4NanScale ? 0u : codes;
 }
 
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// Eight consecutive channels.
-__device__ __forceinline__ void load8(const __nv_bfloat16* from, float (&x)[8]) {
-  const uint4 four = *reinterpret_cast<const uint4*>(from);
-  const uint32_t words[4] = {four.x, four.y, four.z, four.w};
+// Eight consecutive channels as they lie in memory, and as numbers.
+template <typename T>
+struct Eight;
+template <>
+struct Eight<__nv_bfloat16> {
+  uint4 raw;
+  __device__ void load(const __nv_bfloat16* from) { raw = *reinterpret_cast<const uint4*>(from); }
+  __device__ void widen(float (&x)[8]) const {
+    const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    x[2 * j] = __uint_as_float(words[j] << 16);
-    x[2 * j + 1] = __uint_as_float(words[j] & 0xffff0000u);
+    for (int j = 0; j < 4; ++j) {
+      x[2 * j] = __uint_as_float(words[j] << 16);
+      x[2 * j + 1] = __uint_as_float(words[j] & 0xffff0000u);
+    }
   }
-}
-__device__ __forceinline__ void load8(const float* from, float (&x)[8]) {
+};
+template <>
+struct Eight<float> {
+  float4 raw[2];
+  __device__ void load(const float* from) {
+    raw[0] = *reinterpret_cast<const float4*>(from);
+    raw[1] = *reinterpret_cast<const float4*>(from + 4);
+  }
+  __device__ void widen(float (&x)[8]) const {
 #pragma unroll
-  for (int j = 0; j < 8; j += 4) {
-    const float4 four = *reinterpret_cast<const float4*>(from + j);
-    x[j] = four.x, x[j + 1] = four.y, x[j + 2] = four.z, x[j + 3] = four.w;
+    for (int j = 0; j < 2; ++j) {
+      x[4 * j] = raw[j].x, x[4 * j + 1] = raw[j].y;
+      x[4 * j + 2] = raw[j].z, x[4 * j + 3] = raw[j].w;
+    }
   }
+};
+template <typename T>
+__device__ __forceinline__ void load8(const T* from, float (&x)[8]) {
+  Eight<T> eight;
+  eight.load(from);
+  eight.widen(x);
 }
 __device__ __forceinline__ void store8(__nv_bfloat16* to, const float (&x)[8]) {
   *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]),
@@ -95,17 +145,18 @@ __device__ __forceinline__ void store8(float* to, const float (&x)[8]) {
 }
 
 // A thread takes eight consecutive channels of kHeads heads of a token, and two
-// neighbours share a scale.  A CTA takes the heads of one blockIdx.y and every
-// gridDim.x-th token; the next token's position is requested ahead.  The half
-// layout's partners are read by both threads that need them (the second read
-// is in L1), so that every rotary width of whole pieces goes this way.
+// neighbours share a scale.  A CTA takes the heads of one blockIdx.y; a token's rows
+// are requested while the one before is worked on.  The half layout's partners are
+// read by both threads that need them (the second read is in L1), so that every
+// rotary width of whole pieces goes this way.
 constexpr int kHeads = 2;
 constexpr int kRowThreads = 256;
 
 template <typename T, bool Interleaved>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, sizeof(T) == 2 ? 3 : 2)
     fp4_append_kernel(const __grid_constant__ RowsParams p, const float* __restrict__ key_scale,
                       const float* __restrict__ value_scale) {
+  __shared__ Place places[kBatch];
   const int per_head = p.dim / 8;
   const int stride = blockDim.x / per_head, c = threadIdx.x % per_head;
   const int k_from = p.query.heads, v_from = k_from + p.key.heads, heads = v_from + p.value.heads;
@@ -114,101 +165,118 @@ __global__ void __launch_bounds__(kRowThreads)
   const int gap = second ? -half : half;                                // to the partners
   const int pair = Interleaved ? 4 * c : second ? 8 * c - half : 8 * c;  // the first one's
   int kind[kHeads], own[kHeads];  // 0 query, 1 key, 2 value, -1 nothing
+  const T* in[kHeads];
+  int64_t in_t[kHeads];
 #pragma unroll
   for (int u = 0; u < kHeads; ++u) {
     const int lane_head = threadIdx.x / per_head;
     const int head = (blockIdx.y * kHeads + u) * stride + lane_head;
     kind[u] = lane_head >= stride || head >= heads ? -1 : head < k_from ? 0 : head < v_from ? 1 : 2;
     own[u] = head - (kind[u] <= 0 ? 0 : kind[u] == 1 ? k_from : v_from);
+    const RowStream& s = kind[u] <= 0 ? p.query : kind[u] == 1 ? p.key : p.value;
+    in[u] = static_cast<const T*>(s.in) + own[u] * s.in_h + 8 * c;
+    in_t[u] = s.in_t;
   }
-  pdl_wait();
-  pdl_launch_dependents();
-  const unsigned count = static_cast<unsigned>(p.tokens);
-  int64_t upcoming = position_of(p, blockIdx.x);
-  for (unsigned n = blockIdx.x; n < count; n += gridDim.x) {
-    const int64_t pos = upcoming;
-    float x[kHeads][8], z[kHeads][8];
+  struct Rows {
+    Eight<T> x[kHeads], z[Interleaved ? 1 : kHeads];
+  };
+  const auto request = [&](unsigned n, Rows& rows) {
 #pragma unroll
     for (int u = 0; u < kHeads; ++u) {
       if (kind[u] < 0) continue;
-      const RowStream& s = kind[u] == 0 ? p.query : kind[u] == 1 ? p.key : p.value;
-      const T* from = static_cast<const T*>(s.in) + n * s.in_t + own[u] * s.in_h + 8 * c;
-      load8(from, x[u]);
-      if (!Interleaved && rotary && kind[u] < 2) load8(from + gap, z[u]);
-    }
-    if (n + gridDim.x < count) upcoming = position_of(p, n + gridDim.x);
-    const bool known = p.rotary == 0 || (pos >= 0 && pos < p.table_rows);
-    const Place at = find_place(p, n, pos, known, threadIdx.x == 0 && blockIdx.y == 0);
-    if (rotary) {
-      float cs[8], sn[8];
-      if (known) {
-        const float* table = p.cos_sin + pos * p.table_stride + pair;
-        if constexpr (Interleaved) {
-          const float4 c4 = *reinterpret_cast<const float4*>(table);
-          const float4 s4 = *reinterpret_cast<const float4*>(table + half);
-          cs[0] = c4.x, cs[1] = c4.y, cs[2] = c4.z, cs[3] = c4.w;
-          sn[0] = s4.x, sn[1] = s4.y, sn[2] = s4.z, sn[3] = s4.w;
-        } else {
-          load8(table, cs);
-          load8(table + half, sn);
-        }
-      } else {  // a position outside the table: NaN
-#pragma unroll
-        for (int j = 0; j < 8; ++j) cs[j] = sn[j] = __int_as_float(0x7fc00000);
+      const T* from = in[u] + n * in_t[u];
+      rows.x[u].load(from);
+      if constexpr (!Interleaved) {
+        if (rotary && kind[u] < 2) rows.z[u].load(from + gap);
       }
-      // No fused multiply-add: the codes are those of the formula in fp32.
+    }
+  };
+  pdl_wait();
+  pdl_launch_dependents();
+  const unsigned tokens = static_cast<unsigned>(p.tokens);
+  for (unsigned first = blockIdx.x; first < tokens; first += gridDim.x * min(kBatch, blockDim.x)) {
+    Rows rows, next;
+    request(first, rows);
+    const unsigned there = find_places(p, places, first, blockIdx.y == 0);
+    for (unsigned i = 0; i < there; ++i) {
+      const unsigned n = first + i * gridDim.x;
+      if (i + 1 < there) request(n + gridDim.x, next);
+      const Place at = places[i];
+      float cs[8], sn[8];
+      if (rotary) {
+        if (at.known) {
+          const float* table = p.cos_sin + at.pos * p.table_stride + pair;
+          if constexpr (Interleaved) {
+            const float4 c4 = *reinterpret_cast<const float4*>(table);
+            const float4 s4 = *reinterpret_cast<const float4*>(table + half);
+            cs[0] = c4.x, cs[1] = c4.y, cs[2] = c4.z, cs[3] = c4.w;
+            sn[0] = s4.x, sn[1] = s4.y, sn[2] = s4.z, sn[3] = s4.w;
+          } else {
+            load8(table, cs);
+            load8(table + half, sn);
+          }
+        } else {  // a position outside the table: NaN
+#pragma unroll
+          for (int j = 0; j < 8; ++j) cs[j] = sn[j] = __int_as_float(0x7fc00000);
+        }
+      }
 #pragma unroll
       for (int u = 0; u < kHeads; ++u) {
-        if (kind[u] == 2 || kind[u] < 0) continue;
-        if constexpr (Interleaved) {
+        float x[8];
+        uint32_t most = 0;
+        if (kind[u] >= 0) {
+          rows.x[u].widen(x);
+          if (rotary && kind[u] < 2) {
+            // No fused multiply-add: the codes are those of the formula in fp32.
+            if constexpr (Interleaved) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float a = x[u][2 * j], b = x[u][2 * j + 1];
-            x[u][2 * j] = __fsub_rn(__fmul_rn(a, cs[j]), __fmul_rn(b, sn[j]));
-            x[u][2 * j + 1] = __fadd_rn(__fmul_rn(b, cs[j]), __fmul_rn(a, sn[j]));
+              for (int j = 0; j < 4; ++j) {
+                const float a = x[2 * j], b = x[2 * j + 1];
+                x[2 * j] = __fsub_rn(__fmul_rn(a, cs[j]), __fmul_rn(b, sn[j]));
+                x[2 * j + 1] = __fadd_rn(__fmul_rn(b, cs[j]), __fmul_rn(a, sn[j]));
+              }
+            } else {
+              float z[8];
+              rows.z[u].widen(z);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                // x c - z s is x c + (-z s), rounded the same
+                const float turned = __fmul_rn(z[j], sn[j]);
+                x[j] = __fadd_rn(__fmul_rn(x[j], cs[j]), second ? turned : -turned);
+              }
+            }
           }
-        } else {
+          if (kind[u] == 0) {
+            if (at.pos < 0) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float turned = __fmul_rn(z[u][j], sn[j]);
-            x[u][j] = second ? __fadd_rn(__fmul_rn(x[u][j], cs[j]), turned)
-                             : __fsub_rn(__fmul_rn(x[u][j], cs[j]), turned);
+              for (int j = 0; j < 8; ++j) x[j] = 0.f;
+            }
+            store8(static_cast<T*>(p.query.out) + n * p.query.out_t + own[u] * p.query.out_h + 8 * c,
+                   x);
+          } else {
+            const float* factors = kind[u] == 1 ? key_scale : value_scale;
+            if (factors != nullptr) {
+              const float by = factors[own[u]];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) x[j] = __fdiv_rn(x[j], by);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) most = max(most, magnitude(x[j]));
+          }
+        }
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));  // every lane comes here
+        if (kind[u] > 0 && at.keep) {
+          const uint32_t scale = fp4_scale_of(most);
+          const RowStream& s = kind[u] == 1 ? p.key : p.value;
+          uint8_t* slab = static_cast<uint8_t*>(s.out) + at.page * s.out_b + own[u] * s.out_h;
+          *reinterpret_cast<uint32_t*>(slab + at.row * (p.dim / 2) + 4 * c) = codes_of(x, scale);
+          if (!(c & 1)) {
+            slab[(p.dim / 2 << p.block_shift) + at.row * (p.dim / 16) + c / 2] =
+                static_cast<uint8_t>(scale);
           }
         }
       }
-    }
-#pragma unroll
-    for (int u = 0; u < kHeads; ++u) {
-      if (kind[u] == 0) {
-        if (pos < 0) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[u][j] = 0.f;
-        }
-        store8(static_cast<T*>(p.query.out) + n * p.query.out_t + own[u] * p.query.out_h + 8 * c,
-               x[u]);
-      }
-      uint32_t most = 0;
-      if (kind[u] > 0) {
-        const float* factors = kind[u] == 1 ? key_scale : value_scale;
-        if (factors != nullptr) {
-          const float by = factors[own[u]];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[u][j] = __fdiv_rn(x[u][j], by);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) most = max(most, magnitude(x[u][j]));
-      }
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));  // every lane comes here
-      if (kind[u] > 0 && at.keep) {
-        const uint32_t scale = fp4_scale_of(most);
-        const RowStream& s = kind[u] == 1 ? p.key : p.value;
-        uint8_t* slab = static_cast<uint8_t*>(s.out) + at.page * s.out_b + own[u] * s.out_h;
-        *reinterpret_cast<uint32_t*>(slab + at.row * (p.dim / 2) + 4 * c) = quotients(x[u], scale);
-        if (!(c & 1)) {
-          slab[(p.dim / 2 << p.block_shift) + at.row * (p.dim / 16) + c / 2] =
-              static_cast<uint8_t>(scale);
-        }
-      }
+      if (i + 1 < there) rows = next;
     }
   }
 }
@@ -217,13 +285,15 @@ template <typename T, bool Interleaved>
 cudaError_t launch_append(const RowsParams& p, const float* key_scale, const float* value_scale,
                           cudaStream_t stream) {
   const int heads = p.query.heads + p.key.heads + p.value.heads, per_head = p.dim / 8;
-  const int wanted = std::min(kRowThreads, per_head * ((heads + kHeads - 1) / kHeads));
-  const int threads = (wanted + 31) / 32 * 32;
+  // A token's heads in as few CTAs as hold them, shared out evenly.
+  const int wanted = per_head * ((heads + kHeads - 1) / kHeads);
+  const int ctas = (wanted + kRowThreads - 1) / kRowThreads;
+  const int threads = std::max((wanted / ctas + 31) / 32 * 32, 32);
   const int each = threads / per_head * kHeads, slices = (heads + each - 1) / each;
   int sms = 0;
   if (device_sms(&sms) != RKV_OK) return cudaErrorInvalidDevice;
-  const int64_t resident =
-      std::max<int64_t>(1, static_cast<int64_t>(sms) * std::min(32, 1024 / threads) / slices);
+  const int64_t resident = std::max<int64_t>(
+      1, static_cast<int64_t>(sms) * ((sizeof(T) == 2 ? 3 : 2) * kRowThreads / threads) / slices);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(std::min(p.tokens, resident)), slices);
   cfg.blockDim = dim3(threads);
@@ -242,7 +312,6 @@ __device__ __forceinline__ float turned(const RowsParams& p, const T* row, int d
                                         const float* table, bool interleaved) {
   const float x = widen(row[d]);
   if (d >= p.rotary) return x;
-  if (table == nullptr) return __int_as_float(0x7fc00000);
   const int half = p.rotary / 2;
   const bool second = interleaved ? d & 1 : d >= half;
   const int pair = interleaved ? d >> 1 : second ? d - half : d;
@@ -272,11 +341,9 @@ __global__ void __launch_bounds__(256)
     const RowStream& s = is_key ? p.key : p.value;
     const int own = is_key ? head : head - p.key.heads;
     const T* row = static_cast<const T*>(s.in) + n * s.in_t + own * s.in_h;
-    const int64_t pos = position_of(p, static_cast<unsigned>(n));
-    const bool known = p.rotary == 0 || (pos >= 0 && pos < p.table_rows);
-    const float* table = known && p.rotary > 0 ? p.cos_sin + pos * p.table_stride : nullptr;
-    const Place at = find_place(p, static_cast<unsigned>(n), pos, known, rest == 0);
+    const Place at = find_place(p, static_cast<unsigned>(n), rest == 0);
     if (!at.keep) continue;
+    const float* table = p.rotary > 0 ? p.cos_sin + at.pos * p.table_stride : nullptr;
     const float* factors = is_key ? key_scale : value_scale;
     float y[2][8];
     uint32_t most = 0;
@@ -291,59 +358,102 @@ __global__ void __launch_bounds__(256)
     const uint32_t scale = fp4_scale_of(most);
     uint8_t* slab = static_cast<uint8_t*>(s.out) + at.page * s.out_b + own * s.out_h;
     *reinterpret_cast<uint2*>(slab + at.row * (p.dim / 2) + 8 * block) =
-        make_uint2(quotients(y[0], scale), quotients(y[1], scale));
+        make_uint2(codes_of(y[0], scale), codes_of(y[1], scale));
     slab[(p.dim / 2 << p.block_shift) + at.row * blocks + block] = static_cast<uint8_t>(scale);
   }
 }
 
-// Rows of a pool back as numbers: a thread takes eight channels of a head of a
-// token, keys and values alike.
+// Rows of a pool back as numbers.  A thread takes eight channels of a head of the CTA's
+// tokens, kAhead of them in flight at once.
+constexpr int kAhead = 4;
+
 template <typename Out, bool Fp4>
 __global__ void __launch_bounds__(256)
     read_kernel(const __grid_constant__ RowsParams p, const float* __restrict__ key_scale,
                 const float* __restrict__ value_scale) {
+  __shared__ Place places[kBatch];
+  const int units = p.dim / 8, heads = 2 * p.key.heads;
+  // The thread's unit; blockIdx.y has the rest of a token's.
+  const int all = heads * units, mine = blockIdx.y * blockDim.x + threadIdx.x;
+  const int head = mine / units, unit = mine - head * units;
+  const bool there_is = mine < all, is_key = head < p.key.heads;
+  const RowStream& s = is_key ? p.key : p.value;
+  const int own = is_key ? head : head - p.key.heads;
   pdl_wait();
   pdl_launch_dependents();
-  const int units = p.dim / 8, heads = 2 * p.key.heads;
-  const int64_t count = p.tokens * heads * units;
-  for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < count;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t n = i / (heads * units);
-    const int rest = static_cast<int>(i - n * heads * units);
-    const int head = rest / units, unit = rest - head * units;
-    const bool is_key = head < p.key.heads;
-    const RowStream& s = is_key ? p.key : p.value;
-    const int own = is_key ? head : head - p.key.heads;
-    const int64_t pos = position_of(p, static_cast<unsigned>(n));
-    const Place at = find_place(p, static_cast<unsigned>(n), pos, true, rest == 0);
-    float x[8];
-    if (!at.keep) {
+  const float* factors = is_key ? key_scale : value_scale;
+  const bool scaled = there_is && factors != nullptr;
+  const float factor = scaled ? factors[own] : 1.f;
+  const unsigned tokens = static_cast<unsigned>(p.tokens);
+  for (unsigned first = blockIdx.x; first < tokens; first += gridDim.x * min(kBatch, blockDim.x)) {
+    const unsigned there = find_places(p, places, first, blockIdx.y == 0);
+    if (!there_is) continue;
+    for (unsigned i = 0; i < there; i += kAhead) {
+      uint32_t codes[kAhead], scale[kAhead];
+      Eight<__nv_bfloat16> rows[kAhead];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = pos < 0 ? 0.f : __int_as_float(0x7fc00000);
-    } else if (Fp4) {
-      const uint8_t* slab = static_cast<const uint8_t*>(s.in) + at.page * s.in_b + own * s.in_h;
-      uint32_t pairs[4];
-      fp4_decode(*reinterpret_cast<const uint32_t*>(slab + at.row * (p.dim / 2) + 4 * unit), pairs);
-      const float* factors = is_key ? key_scale : value_scale;
-      const float by =
-          fp4_scale_value(slab[(p.dim / 2 << p.block_shift) + at.row * (p.dim / 16) + unit / 2]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 two = __half22float2(*reinterpret_cast<const __half2*>(&pairs[j]));
-        x[2 * j] = two.x * by;  // exact
-        x[2 * j + 1] = two.y * by;
+      for (int u = 0; u < kAhead; ++u) {
+        if (i + u >= there || !places[i + u].keep) continue;
+        const Place& at = places[i + u];
+        if constexpr (Fp4) {
+          const uint8_t* slab = static_cast<const uint8_t*>(s.in) + at.page * s.in_b + own * s.in_h;
+          codes[u] = *reinterpret_cast<const uint32_t*>(slab + at.row * (p.dim / 2) + 4 * unit);
+          scale[u] = slab[(p.dim / 2 << p.block_shift) + at.row * (p.dim / 16) + unit / 2];
+        } else {
+          rows[u].load(static_cast<const __nv_bfloat16*>(s.in) + at.page * s.in_b +
+                       at.row * s.in_t + own * s.in_h + 8 * unit);
+        }
       }
-      if (factors != nullptr) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] *= factors[own];
+      for (int u = 0; u < kAhead; ++u) {
+        if (i + u >= there) continue;
+        const Place& at = places[i + u];
+        float x[8];
+        if (!at.keep) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = at.pos < 0 ? 0.f : __int_as_float(0x7fc00000);
+        } else if constexpr (Fp4) {
+          uint32_t pairs[4];
+          fp4_decode(codes[u], pairs);
+          const float by = fp4_scale_value(scale[u]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 two = __half22float2(*reinterpret_cast<const __half2*>(&pairs[j]));
+            x[2 * j] = two.x * by;  // exact
+            x[2 * j + 1] = two.y * by;
+          }
+          if (scaled) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] *= factor;
+          }
+        } else {
+          rows[u].widen(x);
+        }
+        const int64_t n = first + (i + u) * gridDim.x;
+        store8(static_cast<Out*>(s.out) + n * s.out_t + own * s.out_h + 8 * unit, x);
       }
-    } else {
-      load8(static_cast<const __nv_bfloat16*>(s.in) + at.page * s.in_b + at.row * s.in_t +
-                own * s.in_h + 8 * unit,
-            x);
     }
-    store8(static_cast<Out*>(s.out) + n * s.out_t + own * s.out_h + 8 * unit, x);
   }
+}
+
+template <typename Out, bool Fp4>
+cudaError_t launch_read(const RowsParams& p, const float* key_scale, const float* value_scale,
+                        cudaStream_t stream) {
+  const int units = 2 * p.key.heads * (p.dim / 8);
+  const int threads = std::min(256, (units + 31) / 32 * 32), slices = (units + threads - 1) / threads;
+  int sms = 0;
+  if (device_sms(&sms) != RKV_OK) return cudaErrorInvalidDevice;
+  const int64_t resident = std::max<int64_t>(1, static_cast<int64_t>(sms) * (2048 / threads) / slices);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min(p.tokens, resident)), slices);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, read_kernel<Out, Fp4>, p, key_scale, value_scale);
 }
 
 template <typename Kernel>
@@ -558,15 +668,12 @@ int rkv_paged_read(const rkv_read_args* a, void* stream) {
   p.value = RowStream{a->value_pool, a->value_out, vs[0], vs[2], vs[1], 0, a->value_out_strides[0],
                       a->value_out_strides[1], heads};
   if (p.tokens == 0) return RKV_OK;
-  const int64_t units = p.tokens * 2 * heads * (p.dim / 8);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const auto read = [&](auto kernel) {
-    return launch_units(kernel, p, units, a->key_scale, a->value_scale, st);
-  };
-  const cudaError_t err = out_width == 4 ? (fp4 ? read(read_kernel<float, true>)
-                                                : read(read_kernel<float, false>))
-                                         : (fp4 ? read(read_kernel<__nv_bfloat16, true>)
-                                                : read(read_kernel<__nv_bfloat16, false>));
+  const auto read = [&](auto launch) { return launch(p, a->key_scale, a->value_scale, st); };
+  const cudaError_t err = out_width == 4 ? (fp4 ? read(launch_read<float, true>)
+                                                : read(launch_read<float, false>))
+                                         : (fp4 ? read(launch_read<__nv_bfloat16, true>)
+                                                : read(launch_read<__nv_bfloat16, false>));
   return launched(err, "read");
 }
 

@@ -23,16 +23,32 @@ __host__ __device__ constexpr int fp4_slab_bytes(int block, int dim) {
 constexpr float kFp4Most = 6.f;  // the largest code
 constexpr uint32_t kFp4NanScale = 0x7f;
 
+// Two codes, byte I of a word, as an fp16 pair.  (An assembler block for each: one with
+// four conversions whose results were not all used gave wrong ones with nvcc 12.9.)
+template <int I>
+__device__ __forceinline__ uint32_t fp4_decode2(uint32_t codes) {
+  uint32_t pair;
+  if constexpr (I == 0)
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\t}" : "=r"(pair) : "r"(codes));
+  if constexpr (I == 1)
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, b;\n\t}" : "=r"(pair) : "r"(codes));
+  if constexpr (I == 2)
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, c;\n\t}" : "=r"(pair) : "r"(codes));
+  if constexpr (I == 3)
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, d;\n\t}" : "=r"(pair) : "r"(codes));
+  return pair;
+}
+
 // Eight codes (a word) as four fp16 pairs, in channel order.
 __device__ __forceinline__ void fp4_decode(uint32_t codes, uint32_t (&pairs)[4]) {
-  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
-      "mov.b32 {a, b, c, d}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
-      : "=r"(pairs[0]), "=r"(pairs[1]), "=r"(pairs[2]), "=r"(pairs[3])
-      : "r"(codes));
+  pairs[0] = fp4_decode2<0>(codes);
+  pairs[1] = fp4_decode2<1>(codes);
+  pairs[2] = fp4_decode2<2>(codes);
+  pairs[3] = fp4_decode2<3>(codes);
 }
 
 // Two scales (the low 16 bits) as an fp16 pair.
@@ -47,18 +63,18 @@ __device__ __forceinline__ float fp4_scale_value(uint32_t scale) {
   return __low2float(*reinterpret_cast<const __half2*>(&pair));
 }
 
-// Eight quotients x / s to the nearest codes, ties to the even one, beyond 6 to 6.
-__device__ __forceinline__ uint32_t fp4_encode(const float (&y)[8]) {
+// Two quotients x / s to the nearest codes, ties to the even one, beyond 6 to 6.
+__device__ __forceinline__ uint32_t fp4_encode2(float first, float second) {
   uint32_t codes;
-  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
-      "mov.b32 %0, {a, b, c, d};\n\t}"
-      : "=r"(codes)
-      : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
+  asm("{\n\t.reg .b8 a;\n\tcvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.u32.u8 %0, a;\n\t}" : "=r"(codes) : "f"(first), "f"(second));
   return codes;
+}
+
+// Eight of them, a word.
+__device__ __forceinline__ uint32_t fp4_encode(const float (&y)[8]) {
+  return __byte_perm(__byte_perm(fp4_encode2(y[0], y[1]), fp4_encode2(y[2], y[3]), 0x0040),
+                     __byte_perm(fp4_encode2(y[4], y[5]), fp4_encode2(y[6], y[7]), 0x0040), 0x5410);
 }
 
 // The scale of 16 channels whose greatest magnitude has the bits `most`: most /
