@@ -62,7 +62,7 @@ __device__ __forceinline__ Place find_place(const RowsParams& p, unsigned n, boo
 // A CTA takes every gridDim.x-th token.  Their places hang on three loads in a
 // row, so a thread each finds those of up to kBatch tokens at once, ahead of the
 // rows' own loads.  Returns how many (for the whole CTA).
-constexpr int kBatch = 64;
+constexpr int kBatch = 32;
 
 __device__ __forceinline__ unsigned find_places(const RowsParams& p, Place (&places)[kBatch],
                                                 unsigned first, bool report) {
@@ -87,6 +87,15 @@ __device__ __forceinline__ float quotient(float x, float b, float r) {
   return __fmaf_rn(-__fmaf_rn(b, q, -x), r, q);  // in these signs -0 stays -0
 }
 
+// The scale of 16 channels whose greatest magnitude is `most`: most / 6 rounded to
+// e4m3, at most 448.  A channel that is infinite or NaN makes it NaN, and with it all
+// 16.
+__device__ __forceinline__ uint32_t scale_of(float most) {
+  uint16_t two;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %1;" : "=h"(two) : "f"(quotient(most, 6.f, 1.f / 6.f)));
+  return most < INFINITY ? two & 0xffu : kFp4NanScale;
+}
+
 // The codes of 8 of the 16 channels that share a scale.
 __device__ __forceinline__ uint32_t codes_of(float (&y)[8], uint32_t scale) {
   const float by = fp4_scale_value(scale), r = by > 0.f ? __frcp_rn(by) : 0.f;
@@ -95,8 +104,6 @@ __device__ __forceinline__ uint32_t codes_of(float (&y)[8], uint32_t scale) {
   const uint32_t codes = fp4_encode(y);
   return scale == kFp4NanScale ? 0u : codes;
 }
-
-__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
 // Eight consecutive channels as they lie in memory, and as numbers.
 template <typename T>
@@ -144,135 +151,184 @@ __device__ __forceinline__ void store8(float* to, const float (&x)[8]) {
   *reinterpret_cast<float4*>(to + 4) = make_float4(x[4], x[5], x[6], x[7]);
 }
 
-// A thread takes eight consecutive channels of kHeads heads of a token, and two
-// neighbours share a scale.  A CTA takes the heads of one blockIdx.y; a token's rows
-// are requested while the one before is worked on.  The half layout's partners are
-// read by both threads that need them (the second read is in L1), so that every
-// rotary width of whole pieces goes this way.
+// The greatest magnitude of eight channels; NaN if one is.
+__device__ __forceinline__ float greatest(const float (&x)[8]) {
+  float most = fabsf(x[0]);
+#pragma unroll
+  for (int j = 1; j < 7; j += 2) {
+    asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(most) : "f"(fabsf(x[j])), "f"(fabsf(x[j + 1])));
+  }
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(fabsf(x[7])));
+  return most;
+}
+
+// A unit of work is two pieces of eight channels of one head: for a rotated
+// half-layout unit c the channels at 8 c and at 8 c + rotary / 2 (the two halves of
+// eight pairs), for an interleaved or copied one the 16 from 16 c.  Pieces 2 i and
+// 2 i + 1 share a scale, wherever in the warp they are, so a warp holds whole heads.
+// A thread keeps its unit of kHeads heads, so the table's row is read once a token;
+// a CTA takes the heads of one blockIdx.y, and a token's rows are requested while
+// the one before is worked on.  Measured (24.5K prompt tokens of 32 + 8 + 8 bf16 heads, D
+// 128, half layout): 116 us, 530 MB; with single pieces, whose partners are read
+// twice, 202 and twice the instructions; with the table's rows read from L2 for each
+// token instead of ahead for a batch 149; one head a thread and 1.5 times the warps 138;
+// two heads and 80 registers, which spill, 158.
 constexpr int kHeads = 2;
-constexpr int kRowThreads = 256;
+constexpr int kRowThreads = 256, kRowCtas = 2;
 
 template <typename T, bool Interleaved>
-__global__ void __launch_bounds__(kRowThreads, sizeof(T) == 2 ? 3 : 2)
+__global__ void __launch_bounds__(kRowThreads, kRowCtas)
     fp4_append_kernel(const __grid_constant__ RowsParams p, const float* __restrict__ key_scale,
                       const float* __restrict__ value_scale) {
   __shared__ Place places[kBatch];
-  const int per_head = p.dim / 8;
-  const int stride = blockDim.x / per_head, c = threadIdx.x % per_head;
+  extern __shared__ float tables[];  // of the batch's tokens
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per_head = p.dim / 16, in_warp = 32 / per_head;
+  const int slot = lane / per_head, c = lane - slot * per_head;
+  const int slots = (blockDim.x >> 5) * in_warp;
   const int k_from = p.query.heads, v_from = k_from + p.key.heads, heads = v_from + p.value.heads;
-  const int half = p.rotary / 2;
-  const bool rotary = 8 * c < p.rotary, second = !Interleaved && 8 * c >= half;
-  const int gap = second ? -half : half;                                // to the partners
-  const int pair = Interleaved ? 4 * c : second ? 8 * c - half : 8 * c;  // the first one's
-  int kind[kHeads], own[kHeads];  // 0 query, 1 key, 2 value, -1 nothing
+  const bool rotary = 16 * c < p.rotary, halves = !Interleaved && rotary;
+  const int first = halves ? 8 * c : 16 * c, gap = halves ? p.rotary / 2 : 8;
+  // The unit's pieces, and where the other one of each scale is.
+  const int piece[2] = {first / 8, (first + gap) / 8};
+  int source[2];
+  bool from_second[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int other = piece[i] ^ 1, h = p.rotary / 16;
+    from_second[i] = halves ? other >= h : i == 0;
+    source[i] = halves ? slot * per_head + (other >= h ? other - h : other) : lane;
+  }
+  int kind[kHeads];  // 0 query, 1 key, 2 value, -1 nothing
   const T* in[kHeads];
+  uint8_t* out[kHeads];  // of a query head, or of a KV head in page 0
   int64_t in_t[kHeads];
+  float factor[kHeads], inverse[kHeads];
 #pragma unroll
   for (int u = 0; u < kHeads; ++u) {
-    const int lane_head = threadIdx.x / per_head;
-    const int head = (blockIdx.y * kHeads + u) * stride + lane_head;
-    kind[u] = lane_head >= stride || head >= heads ? -1 : head < k_from ? 0 : head < v_from ? 1 : 2;
-    own[u] = head - (kind[u] <= 0 ? 0 : kind[u] == 1 ? k_from : v_from);
+    const int head = (blockIdx.y * kHeads + u) * slots + warp * in_warp + slot;
+    kind[u] = slot >= in_warp || head >= heads ? -1 : head < k_from ? 0 : head < v_from ? 1 : 2;
     const RowStream& s = kind[u] <= 0 ? p.query : kind[u] == 1 ? p.key : p.value;
-    in[u] = static_cast<const T*>(s.in) + own[u] * s.in_h + 8 * c;
+    const int own = head - (kind[u] <= 0 ? 0 : kind[u] == 1 ? k_from : v_from);
+    in[u] = static_cast<const T*>(s.in) + own * s.in_h + first;
     in_t[u] = s.in_t;
+    out[u] = kind[u] == 0
+                 ? reinterpret_cast<uint8_t*>(static_cast<T*>(s.out) + own * s.out_h + first)
+                 : static_cast<uint8_t*>(s.out) + own * s.out_h;
+    factor[u] = inverse[u] = 1.f;
   }
   struct Rows {
-    Eight<T> x[kHeads], z[Interleaved ? 1 : kHeads];
+    Eight<T> x[kHeads][2];
   };
   const auto request = [&](unsigned n, Rows& rows) {
 #pragma unroll
     for (int u = 0; u < kHeads; ++u) {
       if (kind[u] < 0) continue;
       const T* from = in[u] + n * in_t[u];
-      rows.x[u].load(from);
-      if constexpr (!Interleaved) {
-        if (rotary && kind[u] < 2) rows.z[u].load(from + gap);
-      }
+      rows.x[u][0].load(from);
+      rows.x[u][1].load(from + gap);
     }
   };
   pdl_wait();
   pdl_launch_dependents();
+  const bool scaled = key_scale != nullptr || value_scale != nullptr;
+  if (scaled) {
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u) {
+      const int head = (blockIdx.y * kHeads + u) * slots + warp * in_warp + slot;
+      if (kind[u] == 1 && key_scale != nullptr) factor[u] = key_scale[head - k_from];
+      if (kind[u] == 2 && value_scale != nullptr) factor[u] = value_scale[head - v_from];
+      inverse[u] = __frcp_rn(factor[u]);
+    }
+  }
   const unsigned tokens = static_cast<unsigned>(p.tokens);
-  for (unsigned first = blockIdx.x; first < tokens; first += gridDim.x * min(kBatch, blockDim.x)) {
+  for (unsigned at_token = blockIdx.x; at_token < tokens;
+       at_token += gridDim.x * min(kBatch, blockDim.x)) {
     Rows rows, next;
-    request(first, rows);
-    const unsigned there = find_places(p, places, first, blockIdx.y == 0);
+    request(at_token, rows);
+    const unsigned there = find_places(p, places, at_token, blockIdx.y == 0);
+    // The batch's rows of the table; a position outside it: NaN.
+    if (p.rotary > 0) {
+      const unsigned quads = p.rotary / 4;
+      for (unsigned x = threadIdx.x; x < there * quads; x += blockDim.x) {
+        const unsigned i = x / quads;
+        const float nan = __int_as_float(0x7fc00000);
+        float4 four = make_float4(nan, nan, nan, nan);
+        if (places[i].known) {
+          four = *reinterpret_cast<const float4*>(p.cos_sin + places[i].pos * p.table_stride +
+                                                  4 * (x - i * quads));
+        }
+        reinterpret_cast<float4*>(tables)[x] = four;
+      }
+      __syncthreads();
+    }
     for (unsigned i = 0; i < there; ++i) {
-      const unsigned n = first + i * gridDim.x;
+      const unsigned n = at_token + i * gridDim.x;
       if (i + 1 < there) request(n + gridDim.x, next);
       const Place at = places[i];
       float cs[8], sn[8];
       if (rotary) {
-        if (at.known) {
-          const float* table = p.cos_sin + at.pos * p.table_stride + pair;
-          if constexpr (Interleaved) {
-            const float4 c4 = *reinterpret_cast<const float4*>(table);
-            const float4 s4 = *reinterpret_cast<const float4*>(table + half);
-            cs[0] = c4.x, cs[1] = c4.y, cs[2] = c4.z, cs[3] = c4.w;
-            sn[0] = s4.x, sn[1] = s4.y, sn[2] = s4.z, sn[3] = s4.w;
-          } else {
-            load8(table, cs);
-            load8(table + half, sn);
-          }
-        } else {  // a position outside the table: NaN
-#pragma unroll
-          for (int j = 0; j < 8; ++j) cs[j] = sn[j] = __int_as_float(0x7fc00000);
-        }
+        const float* table = tables + i * p.rotary + 8 * c;
+        load8(table, cs);
+        load8(table + p.rotary / 2, sn);
       }
 #pragma unroll
       for (int u = 0; u < kHeads; ++u) {
-        float x[8];
-        uint32_t most = 0;
-        if (kind[u] >= 0) {
-          rows.x[u].widen(x);
-          if (rotary && kind[u] < 2) {
-            // No fused multiply-add: the codes are those of the formula in fp32.
+        float x[2][8];
+        rows.x[u][0].widen(x[0]);
+        rows.x[u][1].widen(x[1]);
+        if (rotary && kind[u] < 2) {
+          // No fused multiply-add: the codes are those of the formula in fp32.
+          const auto turn = [](float& a, float& b, float cos, float sin) {
+            const float y = __fsub_rn(__fmul_rn(a, cos), __fmul_rn(b, sin));
+            b = __fadd_rn(__fmul_rn(b, cos), __fmul_rn(a, sin));
+            a = y;
+          };
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
             if constexpr (Interleaved) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float a = x[2 * j], b = x[2 * j + 1];
-                x[2 * j] = __fsub_rn(__fmul_rn(a, cs[j]), __fmul_rn(b, sn[j]));
-                x[2 * j + 1] = __fadd_rn(__fmul_rn(b, cs[j]), __fmul_rn(a, sn[j]));
-              }
+              turn(x[j >> 2][2 * j & 7], x[j >> 2][(2 * j & 7) + 1], cs[j], sn[j]);
             } else {
-              float z[8];
-              rows.z[u].widen(z);
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                // x c - z s is x c + (-z s), rounded the same
-                const float turned = __fmul_rn(z[j], sn[j]);
-                x[j] = __fadd_rn(__fmul_rn(x[j], cs[j]), second ? turned : -turned);
-              }
+              turn(x[0][j], x[1][j], cs[j], sn[j]);
             }
-          }
-          if (kind[u] == 0) {
-            if (at.pos < 0) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) x[j] = 0.f;
-            }
-            store8(static_cast<T*>(p.query.out) + n * p.query.out_t + own[u] * p.query.out_h + 8 * c,
-                   x);
-          } else {
-            const float* factors = kind[u] == 1 ? key_scale : value_scale;
-            if (factors != nullptr) {
-              const float by = factors[own[u]];
-#pragma unroll
-              for (int j = 0; j < 8; ++j) x[j] = __fdiv_rn(x[j], by);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) most = max(most, magnitude(x[j]));
           }
         }
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));  // every lane comes here
+        if (kind[u] == 0) {
+          T* to = reinterpret_cast<T*>(out[u]) + n * p.query.out_t;
+          if (at.pos < 0) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[0][j] = x[1][j] = 0.f;
+          }
+          store8(to, x[0]);
+          store8(to + gap, x[1]);
+        }
+        // Warps of queries alone have no scales to find.
+        if (__all_sync(0xffffffffu, kind[u] <= 0)) continue;
+        if (scaled) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            x[j >> 3][j & 7] = quotient(x[j >> 3][j & 7], factor[u], inverse[u]);
+          }
+        }
+        const float most[2] = {greatest(x[0]), greatest(x[1])};
+        uint32_t scale[2];
+#pragma unroll
+        for (int i2 = 0; i2 < 2; ++i2) {
+          const float p0 = __shfl_sync(0xffffffffu, most[0], source[i2]);
+          const float p1 = __shfl_sync(0xffffffffu, most[1], source[i2]);
+          float both;
+          asm("max.NaN.f32 %0, %1, %2;" : "=f"(both) : "f"(most[i2]), "f"(from_second[i2] ? p1 : p0));
+          scale[i2] = scale_of(both);
+        }
         if (kind[u] > 0 && at.keep) {
-          const uint32_t scale = fp4_scale_of(most);
           const RowStream& s = kind[u] == 1 ? p.key : p.value;
-          uint8_t* slab = static_cast<uint8_t*>(s.out) + at.page * s.out_b + own[u] * s.out_h;
-          *reinterpret_cast<uint32_t*>(slab + at.row * (p.dim / 2) + 4 * c) = codes_of(x, scale);
-          if (!(c & 1)) {
-            slab[(p.dim / 2 << p.block_shift) + at.row * (p.dim / 16) + c / 2] =
-                static_cast<uint8_t>(scale);
+          uint8_t* slab = out[u] + at.page * s.out_b;
+          uint8_t* codes = slab + at.row * (p.dim / 2);
+          uint8_t* scales = slab + (p.dim / 2 << p.block_shift) + at.row * (p.dim / 16);
+#pragma unroll
+          for (int i2 = 0; i2 < 2; ++i2) {
+            *reinterpret_cast<uint32_t*>(codes + 4 * piece[i2]) = codes_of(x[i2], scale[i2]);
+            if (!(piece[i2] & 1)) scales[piece[i2] / 2] = static_cast<uint8_t>(scale[i2]);
           }
         }
       }
@@ -284,19 +340,18 @@ __global__ void __launch_bounds__(kRowThreads, sizeof(T) == 2 ? 3 : 2)
 template <typename T, bool Interleaved>
 cudaError_t launch_append(const RowsParams& p, const float* key_scale, const float* value_scale,
                           cudaStream_t stream) {
-  const int heads = p.query.heads + p.key.heads + p.value.heads, per_head = p.dim / 8;
+  const int heads = p.query.heads + p.key.heads + p.value.heads, in_warp = 32 / (p.dim / 16);
   // A token's heads in as few CTAs as hold them, shared out evenly.
-  const int wanted = per_head * ((heads + kHeads - 1) / kHeads);
-  const int ctas = (wanted + kRowThreads - 1) / kRowThreads;
-  const int threads = std::max((wanted / ctas + 31) / 32 * 32, 32);
-  const int each = threads / per_head * kHeads, slices = (heads + each - 1) / each;
+  const int warps = (heads + kHeads * in_warp - 1) / (kHeads * in_warp), most = kRowThreads / 32;
+  const int ctas = (warps + most - 1) / most, threads = (warps + ctas - 1) / ctas * 32;
   int sms = 0;
   if (device_sms(&sms) != RKV_OK) return cudaErrorInvalidDevice;
   const int64_t resident = std::max<int64_t>(
-      1, static_cast<int64_t>(sms) * ((sizeof(T) == 2 ? 3 : 2) * kRowThreads / threads) / slices);
+      1, static_cast<int64_t>(sms) * (kRowCtas * kRowThreads / threads) / ctas);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min(p.tokens, resident)), slices);
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min(p.tokens, resident)), ctas);
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(kBatch) * p.rotary * 4;  // 32 KB at most
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -346,16 +401,16 @@ __global__ void __launch_bounds__(256)
     const float* table = p.rotary > 0 ? p.cos_sin + at.pos * p.table_stride : nullptr;
     const float* factors = is_key ? key_scale : value_scale;
     float y[2][8];
-    uint32_t most = 0;
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       const int d = 16 * block + j;
       float x = is_key ? turned(p, row, d, table, Interleaved) : widen(row[d]);
       if (factors != nullptr) x = __fdiv_rn(x, factors[own]);
       y[j >> 3][j & 7] = x;
-      most = max(most, magnitude(x));
     }
-    const uint32_t scale = fp4_scale_of(most);
+    float most;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(most) : "f"(greatest(y[0])), "f"(greatest(y[1])));
+    const uint32_t scale = scale_of(most);
     uint8_t* slab = static_cast<uint8_t*>(s.out) + at.page * s.out_b + own * s.out_h;
     *reinterpret_cast<uint2*>(slab + at.row * (p.dim / 2) + 8 * block) =
         make_uint2(codes_of(y[0], scale), codes_of(y[1], scale));
@@ -601,7 +656,7 @@ int rkv_paged_append_fp4(const rkv_append_fp4_args* args, void* stream) {
   if (p.tokens == 0) return RKV_OK;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool inter = a->interleaved != 0;
-  const bool pieces = rows_aligned(16) && (inter ? p.rotary : p.rotary / 2) % 8 == 0 &&
+  const bool pieces = rows_aligned(16) && p.rotary % 16 == 0 &&
                       (p.rotary == 0 || aligned_rows(p.cos_sin, {p.table_stride}, 4, 16));
   if (pieces) {
     const auto append = [&](auto launch) { return launch(p, args->key_scale, args->value_scale, st); };

@@ -20,7 +20,6 @@ __host__ __device__ constexpr int fp4_slab_bytes(int block, int dim) {
   return block * (dim / 2 + dim / 16);
 }
 
-constexpr float kFp4Most = 6.f;  // the largest code
 constexpr uint32_t kFp4NanScale = 0x7f;
 
 // Two codes, byte I of a word, as an fp16 pair.  (An assembler block for each: one with
@@ -75,18 +74,6 @@ __device__ __forceinline__ uint32_t fp4_encode2(float first, float second) {
 __device__ __forceinline__ uint32_t fp4_encode(const float (&y)[8]) {
   return __byte_perm(__byte_perm(fp4_encode2(y[0], y[1]), fp4_encode2(y[2], y[3]), 0x0040),
                      __byte_perm(fp4_encode2(y[4], y[5]), fp4_encode2(y[6], y[7]), 0x0040), 0x5410);
-}
-
-// The scale of 16 channels whose greatest magnitude has the bits `most`: most /
-// 6 rounded to e4m3, at most 448.  A channel that is infinite or NaN makes it
-// NaN, and with it all 16.
-__device__ __forceinline__ uint32_t fp4_scale_of(uint32_t most) {
-  if (most >= 0x7f800000u) return kFp4NanScale;
-  uint16_t two;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %1;"
-      : "=h"(two)
-      : "f"(__fdiv_rn(__uint_as_float(most), kFp4Most)));
-  return two & 0xffu;
 }
 
 }  // namespace rkv

@@ -243,8 +243,6 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Tensor,
             query_strides = query.stride()
         query_strides = query_strides[:2]
         out = _buffer(workspace, "append_query", like, device, dtype)
-        if fp4 and out.data_ptr() == query.data_ptr():  # partners are read by several threads
-            query = query.clone()
         query_ptr, out_ptr, query_heads = query.data_ptr(), out.data_ptr(), like[1]
         out_strides = (query_heads * dim, dim)
     status = 0
