@@ -338,11 +338,11 @@ struct PagedLayout {  // byte offsets into the workspace
   size_t warp_partials, cta_partials, group_partials, bytes;
 };
 
-// Pools of 4 bits: byte strides of a page and a KV head's slab.
+// Pools of 4 bits, keys and values: strides of a page and a KV head's slab in units of
+// 16 bytes.
 struct Fp4Pages {
-  const uint8_t* keys;
-  const uint8_t* values;
-  int64_t key_page, key_head, value_page, value_head;
+  const uint8_t* pool[2];
+  uint32_t page[2], head[2];
 };
 constexpr int kFp4Rows = 64;  // tokens of a tile
 

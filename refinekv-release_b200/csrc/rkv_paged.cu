@@ -70,12 +70,16 @@ constexpr size_t kHeader = 8192;
 constexpr int kPad = 4;
 constexpr int warp_partial_floats(int D, int NT) { return NT * 8 * (D + kPad); }
 constexpr int partial_floats(int D, int NT) { return NT * 8 * (D + 2); }
-// Dynamic shared memory: the stages, the warps' first partials, then the
-// table of the sequences' first tiles.
+// Dynamic shared memory: the stages, the warps' first partials, what else a pool
+// keeps for a warp, then the table of the sequences' first tiles.
 template <typename Pool>
-constexpr size_t table_offset() {
+constexpr size_t scratch_offset() {
   return static_cast<size_t>(Pool::W) *
          (2 * Pool::kTile + (Pool::kFirstInSmem ? warp_partial_floats(Pool::D, Pool::NT) * 4 : 0));
+}
+template <typename Pool>
+constexpr size_t table_offset() {
+  return scratch_offset<Pool>() + static_cast<size_t>(Pool::W) * Pool::kScratch;
 }
 template <typename Pool>
 constexpr size_t paged_smem(int64_t sequences) {
@@ -498,6 +502,7 @@ __global__ void __launch_bounds__(Pool::W * 32, 1)
 
   uint8_t* stage = ring + warp * 2 * kTile;
   const uint32_t k_tile = smem_addr(stage), v_tile = k_tile + kTile;
+  const uint32_t scratch = smem_addr(ring) + scratch_offset<Pool>() + warp * Pool::kScratch;
   // Where partial i of the CTA keeps its o: a warp's last row waits in the
   // warp's own idle stage, an earlier one (cut by the range's start) apart.
   float* firsts = Pool::kFirstInSmem
@@ -511,10 +516,12 @@ __global__ void __launch_bounds__(Pool::W * 32, 1)
   const int page_rows = 1 << p.block_shift;
   const int box_rows = min(R, page_rows), boxes = R / box_rows;
 
-  // Lane i of the first `boxes` lanes looks up the page of the tile's i-th box.
+  // Lane i of the first `boxes` lanes looks up the page of the tile's i-th box (and,
+  // where a box is fetched in pieces, so do the lanes of its other ones).
+  const typename Pool::Lane own(lane, boxes, box_rows);
   auto page_of = [&](const Cursor& c) {
-    if (lane >= boxes) return kNoPage;
-    const int token = tile_token<R, More>(c) + lane * box_rows;
+    if (lane >= boxes * Pool::kPieces) return kNoPage;
+    const int token = tile_token<R, More>(c) + (lane & (boxes - 1)) * box_rows;
     if (token >= c.length) return kNoPage;
     if (token + box_rows <= c.low && !(More && token < c.prefix)) return kNoPage;
     const int page = p.page_table[c.seq * p.page_table_stride + (token >> p.block_shift)];
@@ -526,13 +533,13 @@ __global__ void __launch_bounds__(Pool::W * 32, 1)
   auto issue = [&](int which, const Cursor& c, int page) {
     uint64_t* bar = &bars[warp][which];
     const unsigned used = __ballot_sync(0xffffffffu, page >= 0);
-    if (lane == 0) mbar_expect_tx(bar, __popc(used) * Pool::box_bytes(box_rows));
+    if (lane == 0) mbar_expect_tx(bar, __popc(used) / Pool::kPieces * Pool::box_bytes(box_rows));
     fence_proxy_async();
     __syncwarp();
     if (page >= 0) {
-      const int token = tile_token<R, More>(c) + lane * box_rows;
-      Pool::fetch(source, which, stage + which * kTile, lane, box_rows, bar,
-                  token & (page_rows - 1), c.head, page, policy);
+      const int token = tile_token<R, More>(c) + (lane & (boxes - 1)) * box_rows;
+      Pool::fetch(source, own, which, stage + which * kTile, bar, token & (page_rows - 1), c.head,
+                  page, policy);
     }
   };
 
@@ -560,6 +567,8 @@ __global__ void __launch_bounds__(Pool::W * 32, 1)
     bool bad = __any_sync(0xffffffffu, page == kBadPage), next_bad = false, spoilt = false;
     find_cuts();
     const int count = static_cast<int>(whi - wlo);
+    // Nothing to be done to the logits of a tile that is visible as a whole.
+    const bool bare = More && p.softcap == 0.f && p.slopes == nullptr && p.scores == nullptr;
     int seg_first = cur.tile;  // the segment's first tile of its row
     bool fresh = true, aborted = false;
     const auto again = [&](int which, int parity) { warp_wait(&bars[warp][which], parity); };
@@ -597,8 +606,17 @@ __global__ void __launch_bounds__(Pool::W * 32, 1)
       }
       if (!aborted) {
         float logit[R / 16][NT][4];
-        Pool::score(k_tile, query, logit, lane, p);
-        if constexpr (More) {
+        Pool::score(k_tile, query, logit, scratch, lane, p);
+        if (More && bare && seen.all(R)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const float scale = Pool::column_scale(query, p, nt, c & 1, lane);
+#pragma unroll
+              for (int mt = 0; mt < R / 16; ++mt) logit[mt][nt][c] *= scale;
+            }
+        } else if constexpr (More) {
           shape_logits<Pool>(logit, query, seen, cur, token, lane, p);
         } else {
 #pragma unroll
@@ -623,7 +641,7 @@ __global__ void __launch_bounds__(Pool::W * 32, 1)
           drain_values(j, more, again);
           aborted = true;
         } else {
-          Pool::weigh(stage + kTile, v_tile, logit, o, seen, lane, p);
+          Pool::weigh(stage + kTile, v_tile, logit, o, seen, scratch, lane, p);
           __syncwarp();
           if (more) issue(1, next, page);
         }
@@ -700,7 +718,7 @@ __global__ void __launch_bounds__(Pool::W * 32, 1)
   // written; one that began before it goes to the CTA's slot 0, one that only
   // goes on after it to slot 1.  kLanes threads share the channels of a query.
   constexpr int kLanes = D / 4 < kThreads / G8 ? D / 4 : kThreads / G8;
-  constexpr int kBatch = D > 192 && NT > 1 ? 4 : 8;
+  constexpr int kBatch = Pool::kJoinBatch;
   {
     const int mine = lane < 2 * W ? seg_row[lane] : -1;
     const unsigned used = __ballot_sync(0xffffffffu, mine >= 0);
@@ -780,7 +798,7 @@ __global__ void __launch_bounds__(Pool::W * 32, 1)
       // 21 and 24 parts (16K tokens, seven and six heads) 18.8 and 17.2 against 18.6
       // and 17.0.
       if (kLanes == D / 4 && members >> kBatch) {
-        join<D, kLanes, 20>(members, x % kLanes, m_of, l_of, o_of, put);
+        join<D, kLanes, Pool::kLongBatch>(members, x % kLanes, m_of, l_of, o_of, put);
       } else {
         join<D, kLanes, kBatch>(members, x % kLanes, m_of, l_of, o_of, put);
       }

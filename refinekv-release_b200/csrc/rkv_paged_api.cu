@@ -239,9 +239,17 @@ int rkv_paged_attention_more(const rkv_paged_more_args* args, void* stream) {
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t err;
   if (fp4) {
-    const int64_t *ks = a->key_pool_strides, *vs = a->value_pool_strides;
-    const Fp4Pages pages = {static_cast<const uint8_t*>(a->key_pool),
-                            static_cast<const uint8_t*>(a->value_pool), ks[0], ks[1], vs[0], vs[1]};
+    Fp4Pages pages = {};
+    pages.pool[0] = static_cast<const uint8_t*>(a->key_pool);
+    pages.pool[1] = static_cast<const uint8_t*>(a->value_pool);
+    for (int i = 0; i < 2; ++i) {
+      const int64_t* strides = i ? a->value_pool_strides : a->key_pool_strides;
+      if (strides[0] < 0 || strides[1] < 0 || strides[0] >> 36 != 0 || strides[1] >> 36 != 0) {
+        return reject(RKV_ERR_UNSUPPORTED, "pool strides must lie below 2^36 bytes");
+      }
+      pages.page[i] = static_cast<uint32_t>(strides[0] / 16);
+      pages.head[i] = static_cast<uint32_t>(strides[1] / 16);
+    }
     err = launch_paged_fp4(pages, p, call.ctas, st);
   } else {
     err = launch_paged_more(call.maps, p, call.D, call.ctas, st);

@@ -119,6 +119,8 @@ struct Bf16Pool {
   static constexpr int D = D_, NT = NT_, R = tile_rows(D), W = paged_warps(D);
   static constexpr int kTile = R * D * 2;
   static constexpr bool kFirstInSmem = D <= 128;
+  static constexpr int kScratch = 0;
+  static constexpr int kJoinBatch = D > 192 && NT > 1 ? 4 : 8, kLongBatch = 20;
   using Source = PagedMaps;
   struct Query {
     uint32_t frags[D / 16][NT][2];
@@ -132,10 +134,15 @@ struct Bf16Pool {
     tma_prefetch_desc(&maps.values);
   }
   static __device__ __forceinline__ int box_bytes(int rows) { return rows * D * 2; }
-  static __device__ __forceinline__ void fetch(const Source& maps, int which, uint8_t* tile, int box,
-                                               int box_rows, uint64_t* bar, int row, int head,
+  static constexpr int kPieces = 1;
+  struct Lane {  // the box that a lane fetches
+    int offset;
+    __device__ Lane(int lane, int, int box_rows) : offset(lane * box_rows * 128) {}
+  };
+  static __device__ __forceinline__ void fetch(const Source& maps, const Lane& own, int which,
+                                               uint8_t* tile, uint64_t* bar, int row, int head,
                                                int page, uint64_t policy) {
-    uint8_t* to = tile + box * box_rows * 128;
+    uint8_t* to = tile + own.offset;
     const CUtensorMap* map = which ? &maps.values : &maps.keys;
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
@@ -159,8 +166,8 @@ struct Bf16Pool {
   static __device__ __forceinline__ int channel(int dt, int half, int lane) {
     return dt * 16 + half * 8 + (lane >> 2);
   }
-  static __device__ __forceinline__ void score(uint32_t tile, const Query& q, Logits logit, int lane,
-                                               const PagedParams&) {
+  static __device__ __forceinline__ void score(uint32_t tile, const Query& q, Logits logit, uint32_t,
+                                               int lane, const PagedParams&) {
     score_tile<R, D, NT>(tile, q.frags, logit, lane);
   }
   static __device__ __forceinline__ void softmax(Logits logit, Columns m, Columns l, Outputs o) {
@@ -168,7 +175,8 @@ struct Bf16Pool {
   }
   static __device__ __forceinline__ void settle(Columns, Outputs) {}
   static __device__ __forceinline__ void weigh(uint8_t* tile, uint32_t at, Logits weights, Outputs o,
-                                               const Seen& seen, int lane, const PagedParams& p) {
+                                               const Seen& seen, uint32_t, int lane,
+                                               const PagedParams& p) {
     if (!seen.all(R)) {
       // Rows that are not visible may hold anything: a weight of zero
       // would not silence a NaN, so they are zeroed.

@@ -14,7 +14,7 @@
 //   scores: lane 4 r + j has a quarter j of the channels of tokens r and r + 8
 //     of 16 (dim 128: 16 bytes of codes and two scales each);
 //   values: lane 4 g + j has an eighth g of the channels of four tokens (dim 128: 8
-//     bytes of codes and one scale each), whose codes are paired by token after the
+//     bytes of codes and one scale each), whose codes are paired by token before the
 //     conversion.  Tokens 2j and 2j + 1 change places for odd j, and with them the
 //     rows of the scores, or the four j of a load would hit the same banks.
 #pragma once
@@ -32,6 +32,16 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
       " {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The same from zero.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                              uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7},"
+      " {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 // Kept behind the waits for the copies by being volatile, like them.
@@ -78,23 +88,17 @@ __device__ __forceinline__ uint32_t low_twice(uint32_t pair) {
 __device__ __forceinline__ uint32_t high_twice(uint32_t pair) {
   return __byte_perm(pair, pair, 0x3232);
 }
-__device__ __forceinline__ uint32_t lows(uint32_t a, uint32_t b) {
-  return __byte_perm(a, b, 0x5410);
-}
-__device__ __forceinline__ uint32_t highs(uint32_t a, uint32_t b) {
-  return __byte_perm(a, b, 0x7632);
-}
-
 __device__ __forceinline__ float exp2_of(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
-// Weights and their sums are held 2^15 times as large within a tile and a row's
-// part: fp16 terms of weights down to 2^-29 of the greatest are then normal.
-constexpr float kBoost = 15.f;
-constexpr float kUnboost = 1.f / 32768.f;
+// Weights and their sums are held 2^7 times as large within a tile and a row's part,
+// and up to 2^8 times the reference's: fp16 terms of weights down to 2^-21 of the
+// greatest, or less, are then normal.
+constexpr float kBoost = 7.f, kLag = 8.f;
+constexpr float kUnboost = 1.f / 128.f;
 constexpr float kLog2E = 1.44269504088896341f;
 
 template <int Dim, int NT_>
@@ -103,10 +107,16 @@ struct Fp4Pool {
   static constexpr int W = NT == 1 && Dim <= 192 ? 12 : 8;
   static constexpr int kTile = fp4_slab_bytes(R, Dim);
   static constexpr bool kFirstInSmem = Dim <= 128;
+  // Short batches: the longer ones' registers would spill with 12 warps (128K tokens 53.3
+  // against 49.9 us).
+  static constexpr int kJoinBatch = 4, kLongBatch = 6;
   static constexpr int kRow = Dim / 2;      // bytes of a row's codes
   static constexpr int kScales = Dim / 16;  // and of its scales
   static constexpr int kWords = Dim / 32;   // words of a lane's part of a key's codes
   static constexpr int kBytes = Dim / 16;   // bytes of a lane's part of a value's codes
+  // A lane's logits, and then its weights' terms, of 16 rows each while those are not worked
+  // on: 16 bytes a column tile.
+  static constexpr int kLane = 16 * NT, kScratch = R / 16 * 32 * kLane;
   static_assert(warp_partial_floats(D, NT) * 4 <= 2 * kTile, "a partial waits in its warp's stage");
   using Source = Fp4Pages;
   struct Query {
@@ -119,17 +129,30 @@ struct Fp4Pool {
 
   static __device__ __forceinline__ void prefetch(const Source&) {}
   static __device__ __forceinline__ int box_bytes(int rows) { return rows * (kRow + kScales); }
-  // A box is a page: its slab in one piece.
-  static __device__ __forceinline__ void fetch(const Source& pages, int which, uint8_t* tile,
-                                               int box, int box_rows, uint64_t* bar, int row,
-                                               int head, int page, uint64_t policy) {
-    const uint8_t* from = which ? pages.values + page * pages.value_page + head * pages.value_head
-                                : pages.keys + page * pages.key_page + head * pages.key_head;
-    const int bytes = box_bytes(box_rows);
+  // A box is a page: its slab in two pieces, so that a tile's codes lie together and its
+  // scales behind them, whatever the pages' size.
+  static constexpr int kPieces = 2;
+  struct Lane {  // the piece that a lane fetches: from where in a slab, to where in a tile
+    uint32_t from, to, bytes;
+    __device__ Lane(int lane, int boxes, int box_rows) {
+      const int box = lane & (boxes - 1), codes = box_rows * kRow, scales = box_rows * kScales;
+      const bool second = lane >= boxes;
+      from = second ? codes : 0;
+      to = second ? R * kRow + box * scales : box * codes;
+      bytes = second ? scales : codes;
+    }
+  };
+  static __device__ __forceinline__ void fetch(const Source& pages, const Lane& own, int which,
+                                               uint8_t* tile, uint64_t* bar, int, int head, int page,
+                                               uint64_t policy) {
+    const uint64_t units =
+        static_cast<uint64_t>(static_cast<uint32_t>(page)) * pages.page[which] +
+        static_cast<uint64_t>(static_cast<uint32_t>(head)) * pages.head[which];
     asm volatile(
         "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
-        " [%0], [%1], %2, [%3], %4;" ::"r"(smem_addr(tile + box * bytes)),
-        "l"(from), "r"(bytes), "r"(smem_addr(bar)), "l"(policy)
+        " [%0], [%1], %2, [%3], %4;" ::"r"(smem_addr(tile) + own.to),
+        "l"(pages.pool[which] + own.from + units * 16), "r"(own.bytes), "r"(smem_addr(bar)),
+        "l"(policy)
         : "memory");
   }
 
@@ -201,16 +224,6 @@ struct Fp4Pool {
     return (lane >> 2) * (Dim / 8) + 2 * dt + half;
   }
 
-  // Rows 16 mt .. of a tile: the address of their first codes and scales.
-  struct Place {
-    uint32_t codes, scales;
-  };
-  static __device__ __forceinline__ Place place_of(uint32_t tile, int mt, int shift) {
-    const int box = mt * 16 >> shift, row = mt * 16 & ((1 << shift) - 1);
-    const uint32_t slab = tile + box * ((kRow + kScales) << shift);
-    return {slab + row * kRow, slab + (kRow << shift) + row * kScales};
-  }
-
   // The scales of a lane's words of one key row, each twice in a pair.
   static __device__ __forceinline__ void key_scales(uint32_t at, int j, uint32_t (&s)[kWords]) {
     if constexpr (kWords % 4 == 0) {
@@ -232,20 +245,23 @@ struct Fp4Pool {
     }
   }
 
-  static __device__ __forceinline__ void score(uint32_t tile, const Query& q, Logits acc, int lane,
-                                               const PagedParams& p) {
+  // The rows are taken 16 at a time by loops that are not unrolled: unrolled, a tile is some
+  // 1500 instructions that miss the instruction caches and spill (153 us against 138 for 16
+  // sequences of 32K tokens).  What outlives an iteration waits in shared memory.
+  static __device__ __forceinline__ void score(uint32_t tile, const Query& q, Logits logit,
+                                               uint32_t scratch, int lane, const PagedParams& p) {
     const int j = lane & 3, row = swapped(lane >> 2);
-#pragma unroll
+    uint32_t codes = tile + row * kRow + j * 4 * kWords;
+    uint32_t scales = tile + R * kRow + row * kScales;
+    uint32_t keep = scratch + lane * kLane;
+#pragma unroll 1
     for (int mt = 0; mt < R / 16; ++mt) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        acc[mt][nt][0] = acc[mt][nt][1] = acc[mt][nt][2] = acc[mt][nt][3] = 0.f;
-      const Place at = place_of(tile, mt, p.block_shift);
+      float acc[NT][2][4];  // two sums of products: half as long a chain
       uint32_t a[kWords], b[kWords], sa[kWords], sb[kWords];
-      lds_words(at.codes + row * kRow + j * 4 * kWords, a);
-      lds_words(at.codes + (row + 8) * kRow + j * 4 * kWords, b);
-      key_scales(at.scales + row * kScales, j, sa);
-      key_scales(at.scales + (row + 8) * kScales, j, sb);
+      lds_words(codes, a);
+      lds_words(codes + 8 * kRow, b);
+      key_scales(scales, j, sa);
+      key_scales(scales + 8 * kScales, j, sb);
 #pragma unroll
       for (int w = 0; w < kWords; ++w) {
         uint32_t x[4], y[4];
@@ -260,46 +276,81 @@ struct Fp4Pool {
         for (int half = 0; half < 2; ++half) {
           const uint32_t frag[4] = {x[2 * half], y[2 * half], x[2 * half + 1], y[2 * half + 1]};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            mma_f16(acc[mt][nt], frag, q.frags[2 * w + half][nt][0], q.frags[2 * w + half][nt][1]);
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint32_t(&b)[2] = q.frags[2 * w + half][nt];
+            if (w == 0) {
+              mma_f16_first(acc[nt][half], frag, b[0], b[1]);
+            } else {
+              mma_f16(acc[nt][half], frag, b[0], b[1]);
+            }
+          }
         }
       }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(keep + 16 * nt),
+                     "f"(acc[nt][0][0] + acc[nt][1][0]), "f"(acc[nt][0][1] + acc[nt][1][1]),
+                     "f"(acc[nt][0][2] + acc[nt][1][2]), "f"(acc[nt][0][3] + acc[nt][1][3]));
+      }
+      codes += 16 * kRow;
+      scales += 16 * kScales;
+      keep += 32 * kLane;
     }
+#pragma unroll
+    for (int mt = 0; mt < R / 16; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(logit[mt][nt][0]), "=f"(logit[mt][nt][1]), "=f"(logit[mt][nt][2]),
+                       "=f"(logit[mt][nt][3])
+                     : "r"(scratch + mt * 32 * kLane + lane * kLane + 16 * nt));
+      }
   }
 
-  // softmax_update with boosted weights; sums are rescaled only where a maximum rose.
+  // Online softmax whose reference follows the maximum only when a logit exceeds it by
+  // kLag (in powers of two): a vote a tile instead of six shuffles in a row, and sums
+  // that are seldom rescaled.  Weights are then at most 2^(kLag + kBoost), fp16's
+  // range, and a row's parts join as before: any reference serves.
   static __device__ __forceinline__ void softmax(Logits logit, Columns m, Columns l, Outputs o) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float alpha[2];
+      float mx[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float mx = -INFINITY;
+        mx[j] = fmaxf(logit[0][nt][j], logit[0][nt][2 + j]);
 #pragma unroll
-        for (int mt = 0; mt < R / 16; ++mt)
-          mx = fmaxf(mx, fmaxf(logit[mt][nt][j], logit[mt][nt][2 + j]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        const float top = fmaxf(m[nt][j], mx), ref = finite_or_zero(top);
-        alpha[j] = exp2_of((m[nt][j] - ref) * kLog2E);
-        m[nt][j] = top;
-        float sum = 0.f;
+        for (int mt = 1; mt < R / 16; ++mt)
+          mx[j] = fmaxf(mx[j], fmaxf(logit[mt][nt][j], logit[mt][nt][2 + j]));
+      }
+      if (__any_sync(0xffffffffu, mx[0] > m[nt][0] + kLag / kLog2E ||
+                                      mx[1] > m[nt][1] + kLag / kLog2E)) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 4));
+          mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 8));
+          mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 16));
+          const float top = fmaxf(m[nt][j], mx[j]);
+          const float alpha = exp2_of((m[nt][j] - finite_or_zero(top)) * kLog2E);
+          m[nt][j] = top;
+          l[nt][j] *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < D / 16; ++dt) {
+            o[dt][nt][j] *= alpha;
+            o[dt][nt][2 + j] *= alpha;
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float ref = finite_or_zero(m[nt][j]);
 #pragma unroll
         for (int mt = 0; mt < R / 16; ++mt)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             float& x = logit[mt][nt][2 * half + j];
             x = exp2_of(fmaf(x - ref, kLog2E, kBoost));
-            sum += x;
+            l[nt][j] += x;
           }
-        l[nt][j] = l[nt][j] * alpha[j] + sum;
-      }
-      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) o[dt][nt][c] *= alpha[c & 1];
       }
     }
   }
@@ -317,29 +368,39 @@ struct Fp4Pool {
     }
   }
 
-  static __device__ __forceinline__ void weigh(uint8_t*, uint32_t tile, Logits weights, Outputs o,
-                                               const Seen& seen, int lane, const PagedParams& p) {
+  static __device__ __forceinline__ void weigh(uint8_t* at, uint32_t tile, Logits weights, Outputs o,
+                                               const Seen& seen, uint32_t scratch, int lane,
+                                               const PagedParams& p) {
+    if (!seen.all(R)) {
+      // Rows that are not visible may hold anything: scales of zero make their
+      // channels zero (codes are finite).
+      uint16_t* scales = reinterpret_cast<uint16_t*>(at + R * kRow);
+      for (int i = lane; i < R * kScales / 2; i += 32) {
+        if (!seen.row(i / (kScales / 2))) scales[i] = 0;
+      }
+      __syncwarp();
+    }
     if (p.query_f32) {
-      weigh_terms<2>(tile, weights, o, seen, lane, p);
+      weigh_terms<2>(tile, weights, o, scratch, lane);
     } else {
-      weigh_terms<1>(tile, weights, o, seen, lane, p);
+      weigh_terms<1>(tile, weights, o, scratch, lane);
     }
   }
 
-  // o += V^T p with the weights in fp16 terms.  With two of them (fp32 queries) a tile's
+  // o += V^T p with the weights in fp16 terms.  With two of them (fp32 queries) 16 rows'
   // products are summed apart and added by a rounded addition, since the tensor
   // cores cut their sums off.  Codes are taken kChunk bytes at a time.
   template <int Terms>
   static __device__ __forceinline__ void weigh_terms(uint32_t tile, Logits weights, Outputs o,
-                                                     const Seen& seen, int lane,
-                                                     const PagedParams& p) {
-    uint32_t frag[Terms][R / 16][NT][2];
+                                                     uint32_t scratch, int lane) {
+    const uint32_t kept = scratch + lane * kLane;
 #pragma unroll
-    for (int term = 0; term < Terms; ++term)
+    for (int mt = 0; mt < R / 16; ++mt)
 #pragma unroll
-      for (int mt = 0; mt < R / 16; ++mt)
+      for (int nt = 0; nt < NT; ++nt) {
+        uint32_t frag[2][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int term = 0; term < Terms; ++term)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             float& a = weights[mt][nt][2 * half];
@@ -349,91 +410,92 @@ struct Fp4Pool {
               a -= __low2float(part);
               b -= __high2float(part);
             }
-            frag[term][mt][nt][half] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&part));
+            frag[term][half] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&part));
           }
+        const uint32_t to = kept + mt * 32 * kLane + 16 * nt;
+        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to), "r"(frag[0][0]), "r"(frag[0][1]));
+        if constexpr (Terms > 1) {
+          asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + 8), "r"(frag[1][0]),
+                       "r"(frag[1][1]));
+        }
+      }
     const int g = lane >> 2, j = lane & 3;
     const int first = 2 * j + (j & 1), second = 2 * j + 1 - (j & 1);  // swapped(2j), swapped(2j + 1)
-    const bool whole = seen.all(R);
     // Channels are taken by units of 8 (a word), or 4 where a lane's part is no whole words.
     constexpr int kUnit = kBytes % 4 == 0 ? 4 : 2;
     constexpr int kChunk = Terms == 1 && kBytes % 8 == 0 ? 8 : kUnit;
     constexpr int kUnits = kChunk / kUnit;
+    constexpr uint32_t kLow = 0x0f0f0f0fu;
+    uint32_t codes_at[2] = {tile + first * kRow + g * kBytes, tile + second * kRow + g * kBytes};
+    uint32_t scales_at[2] = {tile + R * kRow + first * kScales, tile + R * kRow + second * kScales};
+    uint32_t from = kept;
+#pragma unroll 1
+    for (int mt = 0; mt < R / 16; ++mt) {
+      uint32_t frag[Terms][NT][2];
 #pragma unroll
-    for (int chunk = 0; chunk < kBytes / kChunk; ++chunk) {
-      float sums[kChunk][NT][4];
-      if (Terms > 1) {
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < kChunk; ++i)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            sums[i][nt][0] = sums[i][nt][1] = sums[i][nt][2] = sums[i][nt][3] = 0.f;
-      }
-#pragma unroll
-      for (int mt = 0; mt < R / 16; ++mt) {
-        const Place at = place_of(tile, mt, p.block_shift);
-        const int tokens[4] = {first, second, first + 8, second + 8};
-        uint32_t codes[4][kUnits];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const uint32_t from = at.codes + tokens[t] * kRow + g * kBytes + chunk * kChunk;
-          if constexpr (kUnit == 4) {
-            lds_words(from, codes[t]);
-          } else {
-            codes[t][0] = lds<2>(from);
-          }
+        for (int term = 0; term < Terms; ++term) {
+          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
+                       : "=r"(frag[term][nt][0]), "=r"(frag[term][nt][1])
+                       : "r"(from + 16 * nt + 8 * term));
         }
-        uint32_t near = 0, far = 0;  // the scales of tokens 0 and 1, and 2 and 3
+#pragma unroll
+      for (int chunk = 0; chunk < kBytes / kChunk; ++chunk) {
+        uint32_t codes[4][kUnits], scale[4];
+        // Two units of a chunk lie in one block of 16 channels.
+        const int block = (g * (kBytes / kUnit) + chunk * kUnits) / (kUnit == 4 ? 2 : 4);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {  // tokens first, second, first + 8, second + 8
+          const uint32_t at = codes_at[t & 1] + (t >> 1) * 8 * kRow + chunk * kChunk;
+          if constexpr (kUnit == 4) {
+            lds_words(at, codes[t]);
+          } else {
+            codes[t][0] = lds<2>(at);
+          }
+          scale[t] = lds<1>(scales_at[t & 1] + block + (t >> 1) * 8 * kScales);
+        }
+        // The scales of tokens 0 and 1, and 2 and 3.
+        const uint32_t near = fp4_scales(__byte_perm(scale[0], scale[1], 0x0040));
+        const uint32_t far = fp4_scales(__byte_perm(scale[2], scale[3], 0x0040));
 #pragma unroll
         for (int u = 0; u < kUnits; ++u) {
-          if (u == 0) {  // two units of a chunk lie in one block of 16 channels
-            const int block = (g * (kBytes / kUnit) + chunk * kUnits) / (kUnit == 4 ? 2 : 4);
-            uint32_t scale[4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              scale[t] = lds<1>(at.scales + tokens[t] * kScales + block);
-              // A row that is not visible may hold anything: a scale of zero makes
-              // its channels zero (codes are finite).
-              if (!whole && !seen.row(mt * 16 + tokens[t])) scale[t] = 0;
-            }
-            near = fp4_scales(scale[0] | scale[1] << 8);
-            far = fp4_scales(scale[2] | scale[3] << 8);
-          }
+          // A byte has two channels of a token; exchanged, one channel of two tokens: the
+          // even channels' and the odd ones' of tokens 0 and 1, and of 2 and 3.
+          const uint32_t mixed[4] = {
+              (codes[0][u] & kLow) | (codes[1][u] << 4 & ~kLow),
+              (codes[0][u] >> 4 & kLow) | (codes[1][u] & ~kLow),
+              (codes[2][u] & kLow) | (codes[3][u] << 4 & ~kLow),
+              (codes[2][u] >> 4 & kLow) | (codes[3][u] & ~kLow)};
           uint32_t x[4][4];
 #pragma unroll
-          for (int t = 0; t < 4; t += 4 / kUnit) {
-            if constexpr (kUnit == 4) {
-              fp4_decode(codes[t][u], x[t]);
-            } else {  // two tokens' half words in one
-              uint32_t both[4];
-              fp4_decode(codes[t][0] | codes[t + 1][0] << 16, both);
-              x[t][0] = both[0], x[t][1] = both[1], x[t + 1][0] = both[2], x[t + 1][1] = both[3];
-            }
-          }
+          for (int t = 0; t < 4; ++t) fp4_decode(mixed[t], x[t]);
 #pragma unroll
           for (int i = 0; i < kUnit; ++i) {
-            const uint32_t a[4] = {times(lows(x[0][i], x[1][i]), near),
-                                   times(highs(x[0][i], x[1][i]), near),
-                                   times(lows(x[2][i], x[3][i]), far),
-                                   times(highs(x[2][i], x[3][i]), far)};
-            const int k = u * kUnit + i;
+            const uint32_t a[4] = {times(x[0][i], near), times(x[1][i], near), times(x[2][i], far),
+                                   times(x[3][i], far)};
+            const int dt = chunk * kChunk + u * kUnit + i;
 #pragma unroll
-            for (int term = 0; term < Terms; ++term)
+            for (int nt = 0; nt < NT; ++nt) {
+              if constexpr (Terms == 1) {
+                mma_f16(o[dt][nt], a, frag[0][nt][0], frag[0][nt][1]);
+              } else {
+                float sum[4];
+                mma_f16_first(sum, a, frag[0][nt][0], frag[0][nt][1]);
+                mma_f16(sum, a, frag[1][nt][0], frag[1][nt][1]);
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                float(&to)[4] = Terms > 1 ? sums[k][nt] : o[chunk * kChunk + k][nt];
-                mma_f16(to, a, frag[term][mt][nt][0], frag[term][mt][nt][1]);
+                for (int c = 0; c < 4; ++c) o[dt][nt][c] += sum[c];
               }
+            }
           }
         }
       }
-      if (Terms > 1) {
 #pragma unroll
-        for (int i = 0; i < kChunk; ++i)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) o[chunk * kChunk + i][nt][c] += sums[i][nt][c];
+      for (int t = 0; t < 2; ++t) {
+        codes_at[t] += 16 * kRow;
+        scales_at[t] += 16 * kScales;
       }
+      from += 32 * kLane;
     }
   }
 };
