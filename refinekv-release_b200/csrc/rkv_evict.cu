@@ -11,11 +11,13 @@
 // touched, 2 x 2 rows of 2 dim bytes (bf16); a step that drops one row a head is
 // latency alone.
 //
-// Two launches.  select_kernel finds the budget-th greatest by four passes of 8
-// bits over the weights as ordered integers, kept in shared memory, and writes the
-// list of moves; a row of a few long sequences is shared by a cluster of CTAs, whose
-// histograms and counts are added through distributed shared memory.  move_kernel
-// copies.
+// Two launches.  select_kernel: a cluster of CTAs for each row (as many as the device has
+// room for); the budget-th greatest is found from the weights as ordered integers, kept
+// in shared memory, eleven bits at a time, until all rows that share the bits found are
+// kept (two passes for weights of many values); the cluster's histograms and counts are
+// added through distributed shared memory, and the moves listed in the workspace.
+// move_kernel makes them with the whole device: in the select kernel's few CTAs a row
+// they took twice as long (161 against 82 us for eight prompts of up to 32K tokens).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -50,13 +52,16 @@ struct EvictParams {
   int slice;   // rows of a CTA that its shared memory holds; 0: they are read again each time
   int most;    // entries of a row's list
   int* status;
-  int* counts;    // (rows): moves
-  int2* moves;    // (rows, most): from, to
+  int* counts;  // (rows): moves
+  int2* moves;  // (rows, most): from, to
 };
 
-constexpr int kSelectThreads = 512, kWarps = kSelectThreads / 32;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMostCluster = 8;
 constexpr int kSliceBytes = 160 * 1024;
+constexpr int kBins = 2048;  // of the widest digit
+static_assert(kBins / kThreads == 4, "a thread reads four bins at once, or two of 1024");
+constexpr int kFlying = 2;   // moves that a lane has in flight
 
 // Weights in their order as unsigned integers: NaN 0, then -inf .. inf; a
 // protected row above all.
@@ -67,12 +72,13 @@ __device__ __forceinline__ uint32_t rank_of(float weight) {
 }
 constexpr uint32_t kProtected = 0xffffffffu;
 
-__global__ void __launch_bounds__(kSelectThreads)
+__global__ void __launch_bounds__(kThreads, 2)
     select_kernel(const __grid_constant__ EvictParams p) {
   extern __shared__ uint32_t ranks[];
-  __shared__ unsigned hist[2][256];
-  __shared__ unsigned totals[3];         // of this CTA, for the cluster: equal ones, holes, movers
-  __shared__ int newest;                 // of this CTA
+  __shared__ __align__(16) unsigned hist[2][kBins];
+  __shared__ unsigned totals[3];  // of this CTA, for the cluster: equal ones, holes, movers
+  __shared__ int newest;          // of this CTA
+  __shared__ unsigned long long least;
   __shared__ unsigned warp_counts[2][kWarps];
   __shared__ uint32_t found;
   __shared__ unsigned found_rest, found_equal;
@@ -87,14 +93,15 @@ __global__ void __launch_bounds__(kSelectThreads)
   pdl_wait();
   pdl_launch_dependents();
   const int length = p.lengths[seq];
-  if (length < 0 || length > p.capacity) {
-    if (threadIdx.x == 0 && part == 0 && head == 0) atomicOr(p.status, kStatusBadInput);
+  if (threadIdx.x == 0 && part == 0 && head == 0) {
+    if (length < 0 || length > p.capacity) atomicOr(p.status, kStatusBadInput);
+    p.lengths_out[seq] = length > p.capacity ? length : min(max(length, 0), p.budget);
   }
   if (length <= p.budget || length > p.capacity) {  // the whole cluster
     if (threadIdx.x == 0 && part == 0) p.counts[row] = 0;
     return;
   }
-  const int each = (length + size * kSelectThreads - 1) / (size * kSelectThreads) * kSelectThreads;
+  const int each = (length + size * kThreads - 1) / (size * kThreads) * kThreads;
   const int lo = min(length, part * each), hi = min(length, lo + each);
   float* weights = p.weights + seq * p.weight_seq + head * p.weight_head;
   const int32_t* positions =
@@ -105,67 +112,138 @@ __global__ void __launch_bounds__(kSelectThreads)
     if (threadIdx.x == 0) newest = INT_MIN;
     __syncthreads();
     int mine = INT_MIN;
-    for (int i = lo + threadIdx.x; i < hi; i += kSelectThreads) mine = max(mine, positions[i]);
+    for (int i = lo + threadIdx.x; i < hi; i += kThreads) mine = max(mine, positions[i]);
     mine = __reduce_max_sync(0xffffffffu, mine);
     if (lane == 0) atomicMax(&newest, mine);
     meet();
-    last = INT_MIN;
-    for (int k = 0; k < size; ++k) last = max(last, *cluster.map_shared_rank(&newest, k));
+    last = lane < size ? *cluster.map_shared_rank(&newest, lane) : INT_MIN;
+    last = __reduce_max_sync(0xffffffffu, last);
   }
   const auto fresh_rank = [&](int i) {
     // Differences of positions in 64 bits: any two of them.
     const int64_t age = static_cast<int64_t>(last) - (positions != nullptr ? positions[i] : i);
     return p.recent > 0 && age < p.recent ? kProtected : rank_of(weights[i]);
   };
+  int2* moves = p.moves + static_cast<int64_t>(row) * p.most;
+  if (length - p.budget == 1) {
+    // One row goes, as in every step of a full cache: the one of least weight, of equal
+    // ones the last (32 sequences of 4097 tokens, 8 KV heads: 8 us against 20 with the
+    // search below).
+    if (threadIdx.x == 0) least = ~0ull;
+    __syncthreads();
+    unsigned long long mine = ~0ull;
+    for (int i = lo + threadIdx.x; i < hi; i += kThreads) {
+      mine = min(mine, static_cast<unsigned long long>(fresh_rank(i)) << 32 |
+                           static_cast<uint32_t>(~i));
+    }
+#pragma unroll
+    for (int step = 16; step > 0; step >>= 1) {
+      mine = min(mine, __shfl_xor_sync(0xffffffffu, mine, step));
+    }
+    if (lane == 0) atomicMin(&least, mine);
+    meet();
+    if (part == 0 && threadIdx.x == 0) {
+      for (int c = 1; c < size; ++c) mine = min(mine, *cluster.map_shared_rank(&least, c));
+      mine = min(mine, least);
+      const int gone = static_cast<int>(~static_cast<uint32_t>(mine));
+      p.counts[row] = gone < p.budget;
+      if (gone < p.budget) moves[0] = make_int2(p.budget, gone);
+      else weights[gone] = 0.f;
+    }
+    if (size > 1) cluster.sync();  // no CTA leaves while another reads its least
+    return;
+  }
+  // Sums over the warps before this one, and over the CTAs before this one.
+  const auto before_warp = [&](int which) {
+    return __reduce_add_sync(0xffffffffu, lane < warp ? warp_counts[which][lane] : 0u);
+  };
+  const auto before_cta = [&](int which) {
+    const unsigned theirs = lane < part ? *cluster.map_shared_rank(&totals[which], lane) : 0u;
+    return __reduce_add_sync(0xffffffffu, theirs);
+  };
+  // A CTA's own total, by its first warp.
+  const auto add_warps = [&](int which, int total) {
+    const unsigned sum =
+        __reduce_add_sync(0xffffffffu, lane < kWarps ? warp_counts[which][lane] : 0u);
+    if (lane == 0) totals[total] = sum;
+  };
   const bool held = p.slice > 0;
   if (held) {
-    for (int i = lo + threadIdx.x; i < hi; i += kSelectThreads) ranks[i - lo] = fresh_rank(i);
+    for (int i = lo + threadIdx.x; i < hi; i += kThreads) ranks[i - lo] = fresh_rank(i);
   }
   const auto rank_at = [&](int i) { return held ? ranks[i - lo] : fresh_rank(i); };
 
-  // The budget-th greatest, from its highest bits down.
+  // The budget-th greatest, from its highest bits down: 11, 11 and 10 of them.
   uint32_t prefix = 0;
   unsigned want = p.budget, equal = 0;
-  for (int pass = 0; pass < 4; ++pass) {
-    const int shift = 24 - 8 * pass;
+  int shift = 32;
+  for (int pass = 0; pass < 3 && (pass == 0 || want < equal); ++pass) {
+    const int above = shift;
+    shift = pass < 2 ? above - 11 : 0;
+    const int bins = 1 << (above - shift);
     unsigned* mine = hist[pass & 1];
     // The other one may still be read by the cluster; this one was two passes ago.
-    for (int b = threadIdx.x; b < 256; b += kSelectThreads) mine[b] = 0;
+    for (int b = threadIdx.x; b < bins; b += kThreads) mine[b] = 0;
     __syncthreads();
-    for (int i = lo + threadIdx.x; i < hi; i += kSelectThreads) {
-      const uint32_t x = rank_at(i);
-      if (pass == 0 || x >> (shift + 8) == prefix) atomicAdd(&mine[x >> shift & 255], 1u);
+#pragma unroll 4
+    for (int base = lo; base < hi; base += kThreads) {  // whole warps
+      const int i = base + threadIdx.x;
+      const uint32_t x = i < hi ? rank_at(i) : 0;
+      const bool counts = i < hi && (pass == 0 || x >> above == prefix);
+      const unsigned bin = x >> shift & (bins - 1);
+      // Equal weights would all add to one place: a warp of one bin adds once.
+      int same;
+      __match_all_sync(0xffffffffu, counts ? bin : kBins, &same);
+      if (!same) {
+        if (counts) atomicAdd(&mine[bin], 1u);
+      } else if (lane == 0 && counts) {
+        atomicAdd(&mine[bin], 32u);
+      }
     }
     meet();
-    if (warp == 0) {
-      // Lane 0 has the highest eight bins.
-      unsigned bins[8], sum = 0;
+    // Thread 0 has the highest bins, four or two each; the CTAs' are all requested at once.
+    const int own_bins = bins / kThreads;
+    const int first = bins - own_bins * (static_cast<int>(threadIdx.x) + 1);
+    unsigned count[4] = {0, 0, 0, 0};
+    uint4 theirs[kMostCluster];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int b = 255 - 8 * lane - k;
-        bins[k] = 0;
-        for (int c = 0; c < size; ++c) bins[k] += *cluster.map_shared_rank(&mine[b], c);
-        sum += bins[k];
+    for (int c = 0; c < kMostCluster; ++c) {
+      theirs[c] = make_uint4(0, 0, 0, 0);
+      if (c >= size) continue;
+      const unsigned* at = cluster.map_shared_rank(mine + first, c);
+      if (own_bins == 4) {
+        theirs[c] = *reinterpret_cast<const uint4*>(at);
+      } else {
+        const uint2 two = *reinterpret_cast<const uint2*>(at);
+        theirs[c].z = two.x, theirs[c].w = two.y;
       }
-      unsigned scan = sum;
+    }
 #pragma unroll
-      for (int step = 1; step < 32; step <<= 1) {
-        const unsigned other = __shfl_up_sync(0xffffffffu, scan, step);
-        if (lane >= step) scan += other;
-      }
-      const unsigned before = scan - sum;
-      if (before < want && want <= scan) {  // one lane
-        unsigned above = before;
-        bool done = false;
+    for (int c = 0; c < kMostCluster; ++c) {
+      count[0] += theirs[c].w, count[1] += theirs[c].z;
+      count[2] += theirs[c].y, count[3] += theirs[c].x;
+    }
+    const unsigned sum = count[0] + count[1] + count[2] + count[3];
+    unsigned scan = sum;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (!done && above + bins[k] >= want) {
-            done = true;
-            found = prefix << 8 | static_cast<uint32_t>(255 - 8 * lane - k);
-            found_rest = want - above;
-            found_equal = bins[k];
-          }
-          if (!done) above += bins[k];
+    for (int step = 1; step < 32; step <<= 1) {
+      const unsigned other = __shfl_up_sync(0xffffffffu, scan, step);
+      if (lane >= step) scan += other;
+    }
+    if (lane == 31) warp_counts[0][warp] = scan;
+    __syncthreads();
+    unsigned before = scan - sum + before_warp(0);
+    if (before < want && want <= before + sum) {  // one thread
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (before < want && want <= before + count[k]) {
+          found = (pass == 0 ? 0 : prefix << (above - shift)) |
+                  static_cast<uint32_t>(bins - 1 - static_cast<int>(threadIdx.x) * own_bins - k);
+          found_rest = want - before;
+          found_equal = count[k];
+          before = want;  // done
+        } else if (before < want) {
+          before += count[k];
         }
       }
     }
@@ -174,146 +252,180 @@ __global__ void __launch_bounds__(kSelectThreads)
     want = found_rest;
     equal = found_equal;
   }
-  const uint32_t threshold = prefix;
-  // `want` of the `equal` rows that equal the threshold are kept, the first ones.
+  // Rows above the prefix are kept, and of the `equal` ones with it the first `want`.
 
   // Counts before this CTA and this warp; a warp's rows are contiguous.
   const int span = (each / kWarps + 31) / 32 * 32;
   const int from = min(hi, lo + warp * span), to = min(hi, from + span);
-  // Sums of totals[which] over the CTAs before this one.
-  const auto before_cta = [&](int which) {
-    unsigned sum = 0;
-    for (int c = 0; c < part; ++c) sum += *cluster.map_shared_rank(&totals[which], c);
-    return sum;
-  };
   unsigned equal_before = 0;
   if (want < equal) {
     unsigned mine = 0;
-    for (int i = from + lane; i < to; i += 32) mine += rank_at(i) == threshold;
+    for (int i = from + lane; i < to; i += 32) mine += rank_at(i) >> shift == prefix;
     mine = __reduce_add_sync(0xffffffffu, mine);
     if (lane == 0) warp_counts[0][warp] = mine;
     __syncthreads();
-    if (threadIdx.x == 0) {
-      unsigned sum = 0;
-      for (int w = 0; w < kWarps; ++w) sum += warp_counts[0][w];
-      totals[0] = sum;
-    }
+    if (warp == 0) add_warps(0, 0);
     meet();
-    equal_before = before_cta(0);
-    for (int w = 0; w < warp; ++w) equal_before += warp_counts[0][w];
+    equal_before = before_cta(0) + before_warp(0);
     __syncthreads();
   }
-  // Walks the warp's rows: visit(i, kept, hole, mover).
+  // Walks the warp's rows: visit(i, there, hole, mover).
   const auto walk = [&](auto visit) {
     unsigned seen = equal_before;
     for (int base = from; base < to; base += 32) {
       const int i = base + lane;
       const bool there = i < to;
-      const uint32_t x = there ? rank_at(i) : 0;
-      const bool same = there && x == threshold;
+      const uint32_t x = there ? rank_at(i) >> shift : 0;
+      const bool same = there && x == prefix;
       const unsigned sames = __ballot_sync(0xffffffffu, same);
       const unsigned order = seen + __popc(sames & ((1u << lane) - 1));
       seen += __popc(sames);
-      const bool kept = there && (x > threshold || (same && order < want));
+      const bool kept = there && (x > prefix || (same && order < want));
       visit(i, there, there && !kept && i < p.budget, kept && i >= p.budget);
     }
   };
+  // The first walk leaves a word of holes and one of movers for each 32 rows, in place of
+  // the ranks it has read (whose first two of 32 they replace).
   unsigned holes = 0, movers = 0;
-  walk([&](int, bool, bool hole, bool mover) {
-    holes += __popc(__ballot_sync(0xffffffffu, hole));
-    movers += __popc(__ballot_sync(0xffffffffu, mover));
+  walk([&](int i, bool, bool hole, bool mover) {
+    const unsigned all_holes = __ballot_sync(0xffffffffu, hole);
+    const unsigned all_movers = __ballot_sync(0xffffffffu, mover);
+    holes += __popc(all_holes);
+    movers += __popc(all_movers);
+    if (held && lane < 2) ranks[i - lo] = lane == 0 ? all_holes : all_movers;
   });
   if (lane == 0) {
     warp_counts[0][warp] = holes;
     warp_counts[1][warp] = movers;
   }
   __syncthreads();
-  if (threadIdx.x < 2) {
-    unsigned sum = 0;
-    for (int w = 0; w < kWarps; ++w) sum += warp_counts[threadIdx.x][w];
-    totals[1 + threadIdx.x] = sum;
-  }
+  if (warp < 2) add_warps(warp, 1 + warp);
   meet();
   holes = before_cta(1);
   movers = before_cta(2);
   if (threadIdx.x == 0 && part == size - 1) p.counts[row] = static_cast<int>(movers + totals[2]);
-  for (int w = 0; w < warp; ++w) {
-    holes += warp_counts[0][w];
-    movers += warp_counts[1][w];
+  holes += before_warp(0);
+  movers += before_warp(1);
+  // A dropped row's weight ends with it; a mover's goes along.
+  if (held) {
+    // A lane takes the words of 32 rows and lists their bits.
+    for (int base = from; base < to; base += 1024) {
+      const int at = base + 32 * lane;
+      unsigned hole = at < to ? ranks[at - lo] : 0, mover = at < to ? ranks[at - lo + 1] : 0;
+      // How many of each the lanes before have: both counts, below 2^16, in one word.
+      const unsigned own = __popc(hole) | __popc(mover) << 16;
+      unsigned scan = own;
+#pragma unroll
+      for (int step = 1; step < 32; step <<= 1) {
+        const unsigned other = __shfl_up_sync(0xffffffffu, scan, step);
+        if (lane >= step) scan += other;
+      }
+      const unsigned total = __shfl_sync(0xffffffffu, scan, 31);
+      unsigned hole_at = holes + (scan - own & 0xffffu), mover_at = movers + (scan - own >> 16);
+      for (; hole != 0; hole &= hole - 1) moves[hole_at++].y = at + __ffs(hole) - 1;
+      for (; mover != 0; mover &= mover - 1) moves[mover_at++].x = at + __ffs(mover) - 1;
+      holes += total & 0xffffu;
+      movers += total >> 16;
+    }
+    for (int base = max(from, p.budget / 32 * 32); base < to; base += 32) {
+      const int i = base + lane;
+      if (i < to && i >= p.budget && !(ranks[base - lo + 1] >> lane & 1)) weights[i] = 0.f;
+    }
+  } else {
+    walk([&](int i, bool there, bool hole, bool mover) {
+      const unsigned below = (1u << lane) - 1;
+      const unsigned all_holes = __ballot_sync(0xffffffffu, hole);
+      const unsigned all_movers = __ballot_sync(0xffffffffu, mover);
+      if (mover) moves[movers + __popc(all_movers & below)].x = i;
+      if (hole) moves[holes + __popc(all_holes & below)].y = i;
+      holes += __popc(all_holes);
+      movers += __popc(all_movers);
+      if (there && i >= p.budget && !mover) weights[i] = 0.f;
+    });
   }
-  int2* moves = p.moves + static_cast<int64_t>(row) * p.most;
-  walk([&](int i, bool there, bool hole, bool mover) {
-    const unsigned below = (1u << lane) - 1;
-    const unsigned all_holes = __ballot_sync(0xffffffffu, hole);
-    const unsigned all_movers = __ballot_sync(0xffffffffu, mover);
-    if (mover) moves[movers + __popc(all_movers & below)].x = i;
-    if (hole) moves[holes + __popc(all_holes & below)].y = i;
-    holes += __popc(all_holes);
-    movers += __popc(all_movers);
-    // A dropped row's weight ends with it; a mover's goes along.
-    if (there && i >= p.budget && !mover) weights[i] = 0.f;
-  });
   if (size > 1) cluster.sync();  // no CTA leaves while another reads its counts
 }
 
+// A unit is what a lane copies at once: 16 bytes of a row, or two of its scales'.  A warp
+// takes as many moves as it has lanes for, kFlying times.
 constexpr int kMoveThreads = 256;
 
-// A unit is what a lane copies at once: 16 bytes of a row, or two of its scales'.
-__global__ void __launch_bounds__(kMoveThreads)
+__global__ void __launch_bounds__(kMoveThreads, 6)
     move_kernel(const __grid_constant__ EvictParams p, unsigned parts) {
   const int row = static_cast<int>(blockIdx.x / parts);
-  const unsigned part = blockIdx.x - static_cast<unsigned>(row) * parts;
+  const int part = static_cast<int>(blockIdx.x - static_cast<unsigned>(row) * parts);
   const int seq = row / p.heads, head = row - seq * p.heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int units = p.fp4 ? p.dim / 16 : p.dim / 8;  // of a key or a value
   const int wide = p.fp4 ? p.dim / 32 : units;       // of them, 16 bytes each
+  const int all = 2 * units, per = all <= 32 ? 32 / all : 1;
+  const int slot = all <= 32 ? lane / all : 0, mine = all <= 32 ? lane - slot * all : lane;
+  const int stride = static_cast<int>(parts) * (kMoveThreads / 32) * per;
   pdl_wait();
   pdl_launch_dependents();
-  if (part == 0 && head == 0 && threadIdx.x == 0) {
-    const int length = p.lengths[seq];
-    p.lengths_out[seq] = length > p.capacity ? length : min(max(length, 0), p.budget);
-  }
-  const int64_t count = static_cast<int64_t>(p.counts[row]) * 2 * units;
+  if (slot >= per) return;
+  const int count = p.counts[row];
   const int2* moves = p.moves + static_cast<int64_t>(row) * p.most;
+  float* weights = p.weights + seq * p.weight_seq + head * p.weight_head;
+  int32_t* positions =
+      p.positions != nullptr ? p.positions + seq * p.position_seq + head * p.position_head : nullptr;
   const int32_t* table = p.page_table + seq * p.page_table_stride;
   const int mask = (1 << p.block_shift) - 1;
   const auto page_of = [&](int token) {
     const int page = table[token >> p.block_shift];
     return page >= 0 && page < p.pool_pages ? page : -1;
   };
-  for (int64_t x = part * kMoveThreads + threadIdx.x; x < count;
-       x += static_cast<int64_t>(parts) * kMoveThreads) {
-    const int move = static_cast<int>(x / (2 * units));
-    const int rest = static_cast<int>(x - static_cast<int64_t>(move) * 2 * units);
-    const int which = rest >= units ? 1 : 0, unit = rest - which * units;
-    const int2 m = moves[move];
-    const int from_page = page_of(m.x), to_page = page_of(m.y);
-    if ((from_page < 0 || to_page < 0) && rest == 0) atomicOr(p.status, kStatusBadInput);
-    const auto place = [&](int page, int token) {
-      const int r = token & mask;
-      uint8_t* slab = p.pool[which] + page * p.page[which] + head * p.head[which];
-      if (unit < wide) return slab + (p.fp4 ? r * (p.dim / 2) : r * p.row[which]) + 16 * unit;
-      return slab + (p.dim / 2 << p.block_shift) + r * (p.dim / 16) + 2 * (unit - wide);
-    };
-    if (to_page >= 0) {
-      uint8_t* to = place(to_page, m.y);
-      if (unit < wide) {
-        // A row whose page is outside the pool is NaN where it goes.
-        uint4 data = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
-        if (from_page >= 0) data = *reinterpret_cast<const uint4*>(place(from_page, m.x));
-        *reinterpret_cast<uint4*>(to) = data;
-      } else {
-        uint16_t data = kFp4NanScale << 8 | kFp4NanScale;
-        if (from_page >= 0) data = *reinterpret_cast<const uint16_t*>(place(from_page, m.x));
-        *reinterpret_cast<uint16_t*>(to) = data;
+  for (int base = (part * (kMoveThreads / 32) + warp) * per + slot; base < count;
+       base += stride * kFlying) {
+    int2 move[kFlying], page[kFlying];
+#pragma unroll
+    for (int f = 0; f < kFlying; ++f) {
+      const int at = base + f * stride;
+      move[f] = at < count ? __ldcg(&moves[at]) : make_int2(-1, -1);
+    }
+#pragma unroll
+    for (int f = 0; f < kFlying; ++f) {
+      page[f] = make_int2(-1, -1);
+      if (move[f].x >= 0) page[f] = make_int2(page_of(move[f].x), page_of(move[f].y));
+      if (move[f].x >= 0 && (page[f].x < 0 || page[f].y < 0) && mine == 0) {
+        atomicOr(p.status, kStatusBadInput);
       }
     }
-    if (rest == 0) {
-      float* weights = p.weights + seq * p.weight_seq + head * p.weight_head;
-      weights[m.y] = weights[m.x];
-      weights[m.x] = 0.f;
-      if (p.positions != nullptr) {
-        int32_t* positions = p.positions + seq * p.position_seq + head * p.position_head;
-        positions[m.y] = positions[m.x];
+    for (int u = mine; u < all; u += 32) {
+      const int which = u >= units ? 1 : 0, unit = u - which * units;
+      const bool is_wide = unit < wide;
+      const auto place = [&](int in_page, int token) {
+        const int r = token & mask;
+        uint8_t* slab = p.pool[which] + in_page * p.page[which] + head * p.head[which];
+        if (is_wide) return slab + (p.fp4 ? r * (p.dim / 2) : r * p.row[which]) + 16 * unit;
+        return slab + (p.dim / 2 << p.block_shift) + r * (p.dim / 16) + 2 * (unit - wide);
+      };
+      // A row whose page is outside the pool is NaN where it goes.
+      uint4 data[kFlying];
+#pragma unroll
+      for (int f = 0; f < kFlying; ++f) {
+        const uint32_t nan = is_wide ? 0x7fc07fc0u : kFp4NanScale << 8 | kFp4NanScale;
+        data[f] = make_uint4(nan, nan, nan, nan);
+        if (page[f].x < 0) continue;
+        const uint8_t* source = place(page[f].x, move[f].x);
+        if (is_wide) data[f] = *reinterpret_cast<const uint4*>(source);
+        else data[f].x = *reinterpret_cast<const uint16_t*>(source);
+      }
+#pragma unroll
+      for (int f = 0; f < kFlying; ++f) {
+        if (page[f].y < 0) continue;
+        uint8_t* target = place(page[f].y, move[f].y);
+        if (is_wide) *reinterpret_cast<uint4*>(target) = data[f];
+        else *reinterpret_cast<uint16_t*>(target) = static_cast<uint16_t>(data[f].x);
+      }
+    }
+    if (mine == 0) {
+#pragma unroll
+      for (int f = 0; f < kFlying; ++f) {
+        if (move[f].x < 0) continue;
+        weights[move[f].y] = weights[move[f].x];
+        weights[move[f].x] = 0.f;
+        if (positions != nullptr) positions[move[f].y] = positions[move[f].x];
       }
     }
   }
@@ -416,6 +528,9 @@ int rkv_paged_evict(const rkv_evict_args* a, void* stream) {
   if (bits & 15u) {
     return reject(RKV_ERR_ALIGNMENT, "pools and their strides must be multiples of 16 bytes");
   }
+  if (a->lengths == a->lengths_out) {
+    return reject(RKV_ERR_INVALID_ARGUMENT, "lengths_out must not be lengths");
+  }
   if (!aligned_to(4, {a->page_table, a->lengths, a->lengths_out, a->weights, a->positions})) {
     return reject(RKV_ERR_ALIGNMENT, "page_table, lengths, weights and positions must be aligned to "
                                      "their elements");
@@ -470,20 +585,20 @@ int rkv_paged_evict(const rkv_evict_args* a, void* stream) {
                                  capacity * 4 > static_cast<int64_t>(kSliceBytes) * size)) {
     size *= 2;
   }
-  const int64_t whole = static_cast<int64_t>(size) * kSelectThreads;
-  const int64_t slice = (capacity + whole - 1) / whole * kSelectThreads;
+  const int64_t whole = static_cast<int64_t>(size) * kThreads;
+  const int64_t slice = (capacity + whole - 1) / whole * kThreads;
   p.slice = slice * 4 <= kSliceBytes ? static_cast<int>(slice) : 0;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t err =
-      ensure_smem_limit(reinterpret_cast<const void*>(&select_kernel), kSliceBytes);
+  cudaError_t err = ensure_smem_limit(reinterpret_cast<const void*>(&select_kernel), kSliceBytes);
   if (err == cudaSuccess) {
-    err = launch(select_kernel, static_cast<unsigned>(rows * size), kSelectThreads,
+    err = launch(select_kernel, static_cast<unsigned>(rows * size), kThreads,
                  static_cast<size_t>(p.slice) * 4, size, st, p);
   }
-  if (err == cudaSuccess) {
-    const int64_t units = static_cast<int64_t>(p.most) * 2 * (fp4 ? p.dim / 16 : p.dim / 8);
+  if (err == cudaSuccess && p.most > 0) {
+    // More CTAs than are resident at once: rows that move nothing leave theirs idle.
+    const int64_t lanes = static_cast<int64_t>(p.most) * 2 * (fp4 ? p.dim / 16 : p.dim / 8);
     const unsigned parts = static_cast<unsigned>(std::max<int64_t>(
-        1, std::min((units + kMoveThreads - 1) / kMoveThreads, (8 * sms + rows - 1) / rows)));
+        1, std::min((lanes + kMoveThreads - 1) / kMoveThreads, (16 * sms + rows - 1) / rows)));
     err = launch(move_kernel, static_cast<unsigned>(rows * parts), kMoveThreads, 0, 1, st, p, parts);
   }
   if (err != cudaSuccess) {

@@ -341,6 +341,27 @@ struct Seen {
   __device__ bool all(int rows) const { return high == rows && (low == 0 || prefix >= rows); }
 };
 
+// The logits of a tile that is visible as a whole, for the weights' sums.
+template <typename Pool>
+__device__ __forceinline__ void keep_scores(const float (&logit)[Pool::R / 16][Pool::NT][4],
+                                            const Cursor& cur, int token, int lane,
+                                            const PagedParams& p) {
+#pragma unroll
+  for (int nt = 0; nt < Pool::NT; ++nt)
+#pragma unroll
+    for (int col = 0; col < 2; ++col) {
+      const int g = nt * 8 + 2 * (lane & 3) + col;
+      if (g >= p.group) continue;
+      float* keep = p.scores + (static_cast<int64_t>(cur.seq * p.heads + cur.head) * p.group + g) *
+                                   p.capacity + token;
+#pragma unroll
+      for (int mt = 0; mt < Pool::R / 16; ++mt)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+          keep[Pool::token_of(mt, half, lane)] = logit[mt][nt][2 * half + col];
+    }
+}
+
 // A tile's products to logits: scaled, capped, biased by distance, -inf where the
 // row is not visible; and kept for the weights' sums where these are wanted.
 //   x = c tanh(scale q.k / c) + slope (j - (L - 1))
@@ -568,7 +589,8 @@ __global__ void __launch_bounds__(Pool::W * 32, 1)
     find_cuts();
     const int count = static_cast<int>(whi - wlo);
     // Nothing to be done to the logits of a tile that is visible as a whole.
-    const bool bare = More && p.softcap == 0.f && p.slopes == nullptr && p.scores == nullptr;
+    const bool bare = More && p.softcap == 0.f && p.slopes == nullptr &&
+                      (Pool::kBareScores || p.scores == nullptr);
     int seg_first = cur.tile;  // the segment's first tile of its row
     bool fresh = true, aborted = false;
     const auto again = [&](int which, int parity) { warp_wait(&bars[warp][which], parity); };
@@ -616,6 +638,9 @@ __global__ void __launch_bounds__(Pool::W * 32, 1)
 #pragma unroll
               for (int mt = 0; mt < R / 16; ++mt) logit[mt][nt][c] *= scale;
             }
+          if constexpr (Pool::kBareScores) {
+            if (p.scores != nullptr) keep_scores<Pool>(logit, cur, token, lane, p);
+          }
         } else if constexpr (More) {
           shape_logits<Pool>(logit, query, seen, cur, token, lane, p);
         } else {

@@ -110,6 +110,8 @@ struct Fp4Pool {
   // Short batches: the longer ones' registers would spill with 12 warps (128K tokens 53.3
   // against 49.9 us).
   static constexpr int kJoinBatch = 4, kLongBatch = 6;
+  // Kept scores apart from shape_logits: 128K tokens 57 us against 64.
+  static constexpr bool kBareScores = true;
   static constexpr int kRow = Dim / 2;      // bytes of a row's codes
   static constexpr int kScales = Dim / 16;  // and of its scales
   static constexpr int kWords = Dim / 32;   // words of a lane's part of a key's codes

@@ -440,6 +440,8 @@ def _token_rows(name, rows, dtype, sequences, heads, capacity, device):
                          "least the page table's tokens")
     if rows.dtype is not dtype:
         raise TypeError(f"{name} must be {'fp32' if dtype is torch.float32 else 'int32'}")
+    if rows.is_contiguous():
+        return
     *outer, last = rows.stride()
     extent, apart = shape[2], last == 1 or shape[2] <= 1
     for stride, count in sorted(zip(outer, shape)):
@@ -482,6 +484,11 @@ def _more(sequences, heads, group, capacity, device, prefix, softcap, slopes, ke
         slopes = (slopes, scores)  # both live until the launch
     return slopes, (slopes_ptr, *factors, weights_ptr, scores_ptr, scores_size, *strides, tokens,
                     _native.DTYPE_FP4 if fp4 else _native.DTYPE_BF16, prefix, softcap)
+
+
+@functools.lru_cache(maxsize=None)
+def _evict_bytes(sequences: int, heads: int, capacity: int, budget: int) -> int:
+    return _native.load().rkv_paged_evict_workspace_size(sequences, heads, capacity, budget)
 
 
 def paged_evict(key_pool: torch.Tensor, value_pool: torch.Tensor, page_table: torch.Tensor,
@@ -537,11 +544,13 @@ def paged_evict(key_pool: torch.Tensor, value_pool: torch.Tensor, page_table: to
         positions_ptr, positions_width = positions.data_ptr(), positions.shape[2]
         position_strides = positions.stride()[:2]
     out = _buffer(workspace, "evict_lengths", (sequences,), device, torch.int32)
-    lib = _native.load()
-    need = lib.rkv_paged_evict_workspace_size(sequences, heads, capacity, budget)
-    scratch = _scratch(workspace, "rkv_evict_scratch", need, device)
+    if sequences and out.data_ptr() == lengths.data_ptr():  # the last call's answer
+        out = torch.empty_like(out)
+        workspace["evict_lengths"] = out
+    scratch = _scratch(workspace, "rkv_evict_scratch",
+                       _evict_bytes(sequences, heads, capacity, budget), device)
     _native.launch(
-        lib.rkv_paged_evict,
+        _native.load().rkv_paged_evict,
         _native.EVICT_ARGS.pack(
             key_pool.data_ptr(), value_pool.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
             out.data_ptr(), weights.data_ptr(), positions_ptr, scratch.data_ptr(), scratch.numel(),

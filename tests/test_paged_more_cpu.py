@@ -65,7 +65,7 @@ def _evict_args(**kw):
              "sequences table_blocks pages block kv_heads dim pool_dtype budget recent").split()
     base = dict.fromkeys(names, 0)
     slab = 16 * 36
-    base.update(key_pool=16, value_pool=16, page_table=16, lengths=16, lengths_out=16, weights=16,
+    base.update(key_pool=16, value_pool=16, page_table=16, lengths=16, lengths_out=32, weights=16,
                 workspace=256, workspace_size=1 << 20, kp0=2 * slab, kp1=slab, vp0=2 * slab, vp1=slab,
                 ws0=128, ws1=64, width=64, table_stride=4, sequences=2, table_blocks=4, pages=8,
                 block=16, kv_heads=2, dim=64, pool_dtype=2, budget=32, recent=4)
@@ -83,6 +83,7 @@ def _evict_args(**kw):
     (dict(width=63), 1, b"weights"),
     (dict(positions=16, position_width=63), 1, b"positions"),
     (dict(lengths_out=0), 1, b"non-null"),
+    (dict(lengths_out=16), 1, b"lengths_out"),
     (dict(key_pool=8), 3, b"16 bytes"),
     (dict(pool_dtype=0, kp2=36), 3, b"16 bytes"),
     (dict(weights=18), 3, b"aligned"),
