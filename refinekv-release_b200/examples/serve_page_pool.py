@@ -1,6 +1,7 @@
 """Serve prompts of different lengths from one page pool, dense and refined layers together.
 
     python refinekv-release_b200/examples/serve_page_pool.py [--prompts 700,95,1301] [--new 32]
+        [--bits 4] [--budget 512 --recent 64]
 
 A small random-weight decoder (attention layers only) runs the serving path a
 host engine would: every layer keeps its keys and values in a pool of 32-token
@@ -15,6 +16,12 @@ grow:
 * a refined layer reads the same pool through ``attach_page_pool``: the prompt's
   block summaries, built from the prompt's keys and values, decide which pages
   are read (``sparse_attention``); the generated tokens are its suffix.
+
+With ``--bits 4`` the dense layers hold their keys and values in 4 bits (``fp4_pool``).
+With ``--budget`` every layer is dense and keeps that many tokens of a sequence:
+the attention adds up what weight each got, and each step drops the least
+(``paged_evict``).  Rows then change places, so a token's row in the pool and its
+position part ways: the keys are rotated by the position and appended at the row.
 """
 
 from __future__ import annotations
@@ -60,10 +67,18 @@ class Decoder:
 
 
 class Server:
-    """``positions``: rows of the rotation table, by default as many as the longest request has."""
+    """``positions``: rows of the rotation table, by default as many as the longest request has.
+    ``bits``: 16 or 4, of the dense layers' pools.  ``budget``: tokens that a sequence keeps in each
+    layer, its ``recent`` newest always (all of them without one)."""
 
-    def __init__(self, model: Decoder, prompts, new_tokens: int, config=None, positions=None):
+    def __init__(self, model: Decoder, prompts, new_tokens: int, config=None, positions=None,
+                 bits=16, budget=None, recent=16):
+        if bits not in (4, 16):
+            raise ValueError("bits: a pool holds 16 or 4 a channel")
+        if budget is not None and model.dense < model.layers:
+            raise ValueError("budget: refined layers keep their whole prompt")
         self.m, self.new, self.config = model, new_tokens, config or rkv.RefineKVConfig()
+        self.budget, self.recent = budget, recent
         dev = model.embed.device
         self.n = len(prompts)
         longest = max(map(len, prompts)) + new_tokens
@@ -77,8 +92,13 @@ class Server:
         for i, count in enumerate(need):
             self.table[i, :count], free = free[:count], free[count:]
         shape = (sum(need) + 1, model.hk, BLOCK, model.dim)
-        self.pools = [tuple(torch.zeros(shape, device=dev, dtype=torch.bfloat16) for _ in "kv")
-                      for _ in range(model.layers)]
+
+        def pool(layer):
+            if bits == 4 and layer < model.dense:
+                return rkv.fp4_pool(*shape, device=dev)
+            return torch.zeros(shape, device=dev, dtype=torch.bfloat16)
+
+        self.pools = [(pool(layer), pool(layer)) for layer in range(model.layers)]
         self.workspaces = [{} for _ in range(model.layers)]
         last = [self._prefill(i, prompt.to(dev)) for i, prompt in enumerate(prompts)]
         self._summarise()
@@ -87,6 +107,15 @@ class Server:
         self.tokens = torch.stack(last)
         self.lengths = torch.tensor([len(p) for p in prompts], device=dev, dtype=torch.int32)
         self.suffix = torch.zeros((), device=dev, dtype=torch.int32)
+        if budget is not None:
+            # The rows that each sequence has in the pool, what weight their tokens got and
+            # which tokens they are.
+            tokens = self.table.shape[1] * BLOCK
+            self.rows = self.lengths.clone()
+            shape = (self.n, model.hk, tokens)
+            self.weights = [torch.zeros(shape, device=dev) for _ in range(model.layers)]
+            self.held = [torch.arange(tokens, device=dev, dtype=torch.int32).expand(shape).clone()
+                         for _ in range(model.layers)]
 
     def _prefill(self, slot, prompt):
         m, length = self.m, len(prompt)
@@ -128,7 +157,9 @@ class Server:
         for layer in range(m.layers):
             q, k, v = m.project(layer, x)
             ws = self.workspaces[layer]
-            if layer < m.dense:
+            if self.budget is not None:
+                y = self._attend_within_budget(layer, q, k, v, ws)
+            elif layer < m.dense:
                 q = rkv.paged_append(k, v, *self.pools[layer], self.table, self.lengths, query=q,
                                      cos_sin=self.cos_sin, workspace=ws)
                 y = rkv.paged_attention(q, *self.pools[layer], self.table, grown, workspace=ws)
@@ -142,9 +173,25 @@ class Server:
             x = x + y.reshape(self.n, -1) @ m.out[layer]
         logits = m.logits(x)
         self.tokens.copy_(logits.argmax(-1))
+        if self.budget is not None:
+            self.rows.copy_(torch.clamp(self.rows + 1, max=self.budget))
         self.lengths.copy_(grown)
         self.suffix.copy_(seen)
         return logits
+
+    def _attend_within_budget(self, layer, q, k, v, ws):
+        """The layer's attention over what it has kept, after which it keeps ``budget`` rows."""
+        pools, weights, held = self.pools[layer], self.weights[layer], self.held[layer]
+        q, k = rkv.apply_rotary(q, k, self.lengths, self.cos_sin)
+        rkv.paged_append(k, v, *pools, self.table, self.rows, workspace=ws)
+        at = (self.n, self.m.hk, 1)
+        held.scatter_(2, self.rows.long().view(-1, 1, 1).expand(at),
+                      self.lengths.view(-1, 1, 1).expand(at))
+        grown = self.rows + 1
+        y = rkv.paged_attention(q, *pools, self.table, grown, weights=weights, workspace=ws)
+        rkv.paged_evict(*pools, self.table, grown, weights, self.budget, recent=self.recent,
+                        positions=held, workspace=ws)
+        return y
 
     def generate(self):
         """(sequences, new tokens) greedy tokens and the logits after each of them."""
@@ -166,12 +213,15 @@ def main():
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     ap.add_argument("--prompts", default="700,95,1301", help="prompt lengths")
     ap.add_argument("--new", type=int, default=32, help="tokens to generate for each")
+    ap.add_argument("--bits", type=int, default=16, choices=(4, 16), help="of the dense layers' pools")
+    ap.add_argument("--budget", type=int, help="tokens that a sequence keeps (every layer dense)")
+    ap.add_argument("--recent", type=int, default=16, help="of them, the newest that always stay")
     args = ap.parse_args()
-    model = Decoder()
+    model = Decoder(dense=1 if args.budget is None else 2)
     gen = torch.Generator().manual_seed(1)
     prompts = [torch.randint(0, model.embed.shape[0], (int(n),), generator=gen)
                for n in args.prompts.split(",")]
-    server = Server(model, prompts, args.new)
+    server = Server(model, prompts, args.new, bits=args.bits, budget=args.budget, recent=args.recent)
     start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
     start.record()
     tokens, _ = server.generate()
