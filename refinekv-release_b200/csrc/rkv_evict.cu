@@ -366,66 +366,64 @@ __global__ void __launch_bounds__(kMoveThreads, 6)
   if (slot >= per) return;
   const int count = p.counts[row];
   const int2* moves = p.moves + static_cast<int64_t>(row) * p.most;
-  float* weights = p.weights + seq * p.weight_seq + head * p.weight_head;
-  int32_t* positions =
-      p.positions != nullptr ? p.positions + seq * p.position_seq + head * p.position_head : nullptr;
   const int32_t* table = p.page_table + seq * p.page_table_stride;
   const int mask = (1 << p.block_shift) - 1;
   const auto page_of = [&](int token) {
     const int page = table[token >> p.block_shift];
     return page >= 0 && page < p.pool_pages ? page : -1;
   };
-  for (int base = (part * (kMoveThreads / 32) + warp) * per + slot; base < count;
-       base += stride * kFlying) {
-    int2 move[kFlying], page[kFlying];
-#pragma unroll
-    for (int f = 0; f < kFlying; ++f) {
-      const int at = base + f * stride;
-      move[f] = at < count ? __ldcg(&moves[at]) : make_int2(-1, -1);
-    }
-#pragma unroll
-    for (int f = 0; f < kFlying; ++f) {
-      page[f] = make_int2(-1, -1);
-      if (move[f].x >= 0) page[f] = make_int2(page_of(move[f].x), page_of(move[f].y));
-      if (move[f].x >= 0 && (page[f].x < 0 || page[f].y < 0) && mine == 0) {
-        atomicOr(p.status, kStatusBadInput);
-      }
-    }
-    for (int u = mine; u < all; u += 32) {
-      const int which = u >= units ? 1 : 0, unit = u - which * units;
-      const bool is_wide = unit < wide;
-      const auto place = [&](int in_page, int token) {
-        const int r = token & mask;
-        uint8_t* slab = p.pool[which] + in_page * p.page[which] + head * p.head[which];
-        if (is_wide) return slab + (p.fp4 ? r * (p.dim / 2) : r * p.row[which]) + 16 * unit;
-        return slab + (p.dim / 2 << p.block_shift) + r * (p.dim / 16) + 2 * (unit - wide);
-      };
-      // A row whose page is outside the pool is NaN where it goes.
+  for (int u = mine; u < all; u += 32) {
+    // Where the lane's unit is, but for the page and the row.
+    const int which = u >= units ? 1 : 0, unit = u - which * units;
+    const bool is_wide = unit < wide;
+    uint8_t* unit_base =
+        p.pool[which] + head * p.head[which] +
+        (is_wide ? 16 * unit : (p.dim / 2 << p.block_shift) + 2 * (unit - wide));
+    const int64_t page_bytes = p.page[which];
+    const int64_t row_bytes = !p.fp4 ? p.row[which] : is_wide ? p.dim / 2 : p.dim / 16;
+    // A row whose page is outside the pool is NaN where it goes.
+    const uint32_t nan = is_wide ? 0x7fc07fc0u : kFp4NanScale << 8 | kFp4NanScale;
+    for (int base = (part * (kMoveThreads / 32) + warp) * per + slot; base < count;
+         base += stride * kFlying) {
+      int2 move[kFlying];
+      uint8_t* target[kFlying];
       uint4 data[kFlying];
 #pragma unroll
       for (int f = 0; f < kFlying; ++f) {
-        const uint32_t nan = is_wide ? 0x7fc07fc0u : kFp4NanScale << 8 | kFp4NanScale;
+        const int at = base + f * stride;
+        move[f] = at < count ? __ldcg(&moves[at]) : make_int2(-1, -1);
+      }
+#pragma unroll
+      for (int f = 0; f < kFlying; ++f) {
+        target[f] = nullptr;
+        if (move[f].x < 0) continue;
+        const int from = page_of(move[f].x), to = page_of(move[f].y);
+        if ((from < 0 || to < 0) && u == 0) atomicOr(p.status, kStatusBadInput);
+        if (to >= 0) target[f] = unit_base + to * page_bytes + (move[f].y & mask) * row_bytes;
         data[f] = make_uint4(nan, nan, nan, nan);
-        if (page[f].x < 0) continue;
-        const uint8_t* source = place(page[f].x, move[f].x);
+        if (from < 0) continue;
+        const uint8_t* source = unit_base + from * page_bytes + (move[f].x & mask) * row_bytes;
         if (is_wide) data[f] = *reinterpret_cast<const uint4*>(source);
         else data[f].x = *reinterpret_cast<const uint16_t*>(source);
       }
 #pragma unroll
       for (int f = 0; f < kFlying; ++f) {
-        if (page[f].y < 0) continue;
-        uint8_t* target = place(page[f].y, move[f].y);
-        if (is_wide) *reinterpret_cast<uint4*>(target) = data[f];
-        else *reinterpret_cast<uint16_t*>(target) = static_cast<uint16_t>(data[f].x);
+        if (target[f] == nullptr) continue;
+        if (is_wide) *reinterpret_cast<uint4*>(target[f]) = data[f];
+        else *reinterpret_cast<uint16_t*>(target[f]) = static_cast<uint16_t>(data[f].x);
       }
-    }
-    if (mine == 0) {
+      if (u == 0) {
+        float* weights = p.weights + seq * p.weight_seq + head * p.weight_head;
 #pragma unroll
-      for (int f = 0; f < kFlying; ++f) {
-        if (move[f].x < 0) continue;
-        weights[move[f].y] = weights[move[f].x];
-        weights[move[f].x] = 0.f;
-        if (positions != nullptr) positions[move[f].y] = positions[move[f].x];
+        for (int f = 0; f < kFlying; ++f) {
+          if (move[f].x < 0) continue;
+          weights[move[f].y] = weights[move[f].x];
+          weights[move[f].x] = 0.f;
+          if (p.positions != nullptr) {
+            int32_t* positions = p.positions + seq * p.position_seq + head * p.position_head;
+            positions[move[f].y] = positions[move[f].x];
+          }
+        }
       }
     }
   }
