@@ -194,7 +194,8 @@ int rkv_paged_attention_more(const rkv_paged_more_args* args, void* stream) {
     return reject(RKV_ERR_INVALID_ARGUMENT, "scales belong to an fp4 pool");
   }
   const float softcap = static_cast<float>(args->softcap);
-  if (!(softcap >= 0.f) || std::isinf(softcap) || (softcap == 0.f && args->softcap != 0)) {
+  // Below the normal numbers its reciprocal could be infinite.
+  if (!(args->softcap == 0 || std::isnormal(softcap)) || softcap < 0.f) {
     return reject(RKV_ERR_INVALID_ARGUMENT, "softcap must be finite and positive, or 0 for none");
   }
   if (args->prefix < 0) return reject(RKV_ERR_INVALID_ARGUMENT, "prefix must not be negative");

@@ -123,6 +123,8 @@ def _fp4_pools(key_pool, value_pool, layout):
 
 def _factors(key_scale, value_scale, heads, device):
     """The addresses of the KV heads' factors of a pool of 4 bits (0: none)."""
+    if key_scale is None and value_scale is None:
+        return 0, 0
     at = [0, 0]
     for i, factor in enumerate((key_scale, value_scale)):
         if factor is None:
@@ -306,10 +308,13 @@ def paged_read(key_pool: torch.Tensor, value_pool: torch.Tensor, page_table: tor
             raise ValueError("sequence_ids must be (tokens,) on the pools' device")
         if sequence_ids.dtype != torch.int32:
             raise TypeError("sequence_ids must be int32")
-        sequence_ids = sequence_ids.contiguous()
+        if not sequence_ids.is_contiguous():
+            sequence_ids = sequence_ids.contiguous()
         ids = sequence_ids.data_ptr()
-    positions = positions.contiguous()
-    keys, values = torch.empty(2, tokens, heads, dim, device=device, dtype=dtype)
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    keys = torch.empty(tokens, heads, dim, device=device, dtype=dtype)
+    values = torch.empty_like(keys)
     status = 0
     if workspace is not None:
         status = _scratch(workspace, "rkv_append_status", 256, device).data_ptr()

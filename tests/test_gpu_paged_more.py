@@ -221,6 +221,17 @@ def test_pools_of_4_bits_match_the_formula(lengths, hq, hk, dim, block, layout, 
     assert torch.equal(s.call(return_lse=False), out)
 
 
+@pytest.mark.parametrize("dim", range(32, 257, 32))
+@pytest.mark.parametrize("group", [1, 5, 8, 9, 16])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_every_head_dim_and_group_over_4_bits(dim, group, dtype):
+    """Every instance, with pages that are a quarter, a half and the whole of a tile."""
+    for block in (16, 32, 64):
+        s = Served([1000, 1, 64, 0, 129], 2 * group, 2, dim, block, bits=4, dtype=dtype,
+                   seed=dim + group, scaled=True, weights=block == 32)
+        s.check(*s.call())
+
+
 @pytest.mark.parametrize("bits", [4, 16])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_sharp_softmax_scale_and_small_queries(bits, dtype):

@@ -36,6 +36,7 @@ def _more_args(**kw):
     (dict(softcap=-1.0), 1, b"softcap"),
     (dict(softcap=math.nan), 1, b"softcap"),
     (dict(softcap=1e-60), 1, b"softcap"),
+    (dict(softcap=1e-39), 1, b"softcap"),  # not a normal number
     (dict(softcap=1e60), 1, b"softcap"),
     (dict(prefix=-1), 1, b"prefix"),
     (dict(slopes=18), 3, b"slopes"),
