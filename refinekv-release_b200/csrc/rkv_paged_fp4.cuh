@@ -17,6 +17,9 @@
 //     bytes of codes and one scale each), whose codes are paired by token before the
 //     conversion.  Tokens 2j and 2j + 1 change places for odd j, and with them the
 //     rows of the scores, or the four j of a load would hit the same banks.
+//
+// Bound: issue.  16 sequences of 32K tokens (32 + 8 heads, D 128, 604 MB): 141 us, 4.3 TB/s,
+// 1380 warp instructions a tile of 64 tokens; 128K tokens 47.7; 333 tokens 9.5 (latency).
 #pragma once
 
 #include "rkv_fp4.cuh"
@@ -129,6 +132,19 @@ struct Fp4Pool {
   using Columns = float (&)[NT][2];
   using Outputs = float (&)[D / 16][NT][4];
 
+  // Neighbouring ranges on different schedulers (warp w's is w % 4): where there are fewer
+  // tiles than warps, every second range has one, and in order those would share two of
+  // the four (333 tokens: 9.5 us against 10.4).
+  static_assert(W % 4 == 0, "as many warps on every scheduler");
+  static __device__ __forceinline__ int range_of(int warp) {
+    return warp % 4 * (W / 4) + warp / 4;
+  }
+  // A tile takes some 4 us alone on its scheduler, so a row is worth a CTA for every
+  // fourth of its tiles (1000 tokens of 8 heads: 10.7 us against 13.3 with every warp a
+  // tile), but one CTA where each tile has a warp (333 tokens: 9.5 against 10.3).
+  static __device__ __forceinline__ unsigned ctas_of(unsigned tiles, unsigned rows) {
+    return tiles <= W * rows ? 1 : (tiles / rows + 3) / 4;
+  }
   static __device__ __forceinline__ void prefetch(const Source&) {}
   static __device__ __forceinline__ int box_bytes(int rows) { return rows * (kRow + kScales); }
   // A box is a page: its slab in two pieces, so that a tile's codes lie together and its
@@ -248,8 +264,8 @@ struct Fp4Pool {
   }
 
   // The rows are taken 16 at a time by loops that are not unrolled: unrolled, a tile is some
-  // 1500 instructions that miss the instruction caches and spill (153 us against 138 for 16
-  // sequences of 32K tokens).  What outlives an iteration waits in shared memory.
+  // 1500 instructions that miss the instruction caches and spill (then 153 us against 146 for
+  // 16 sequences of 32K tokens).  What outlives an iteration waits in shared memory.
   static __device__ __forceinline__ void score(uint32_t tile, const Query& q, Logits logit,
                                                uint32_t scratch, int lane, const PagedParams& p) {
     const int j = lane & 3, row = swapped(lane >> 2);

@@ -4,7 +4,7 @@
 // Weights: with the logits x_gj of the attention (kept in the call's scratch, fp32)
 // and each query's sum lse_g,  W_j += sum_g e^(x_gj - lse_g)  over the queries g of
 // the KV head, in this order.  Bound: HBM or L2, 4 (G + 2) bytes a token and KV
-// head; the attention writes 4 G of them.
+// head; the attention writes 4 G of them (128K tokens, 8 KV heads, G 4: 6 us, 25 MB).
 #include "rkv_paged_bf16.cuh"
 
 namespace rkv {
