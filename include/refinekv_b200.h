@@ -715,7 +715,8 @@ RKV_API int rkv_paged_attention_more(const rkv_paged_more_args* args, void* stre
  *     the positions above the row's greatest less `recent`; without positions
  *     they are the last ones.
  *   lengths_out: (sequences) int32, min(lengths, budget), apart from `lengths`.
- *   pools: as for rkv_paged_read, written in place; page_table as everywhere.
+ *   pools: as for rkv_paged_read, written in place; page_table as everywhere, but
+ *     no page that rows move into may be another sequence's too.
  * Negative lengths count as 0; one past the page table leaves its sequence as it
  * is, length included.  Both set RKV_DEVICE_BAD_INPUT in the workspace's status
  * word, and so does a move from or to a page outside the pool: nothing is read or

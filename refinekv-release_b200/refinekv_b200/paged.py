@@ -520,8 +520,11 @@ def paged_evict(key_pool: torch.Tensor, value_pool: torch.Tensor, page_table: to
     row ``lengths`` (``paged_append``'s position) but is rotated by its own position
     (``apply_rotary``).
 
+    A sequence's pages must be its own: rows that move into a page which another
+    sequence's table names too would change that sequence, so copy shared pages first.
+
     Returns the new lengths, ``min(lengths, budget)`` (backed by ``workspace``,
-    reused by the next call).  Pools, weights and positions are written in place;
+    reused by the next call that is not given them as ``lengths``).  Pools, weights and positions are written in place;
     nothing carries a gradient.  A length past the page table leaves its sequence
     as it is, a negative one counts as 0, and a row from a page outside the pool is
     NaN where it goes; each sets bit 1 of ``attention.device_status(workspace)``.
@@ -550,8 +553,7 @@ def paged_evict(key_pool: torch.Tensor, value_pool: torch.Tensor, page_table: to
         position_strides = positions.stride()[:2]
     out = _buffer(workspace, "evict_lengths", (sequences,), device, torch.int32)
     if sequences and out.data_ptr() == lengths.data_ptr():  # the last call's answer
-        out = torch.empty_like(out)
-        workspace["evict_lengths"] = out
+        out = _buffer(workspace, "evict_lengths_other", (sequences,), device, torch.int32)
     scratch = _scratch(workspace, "rkv_evict_scratch",
                        _evict_bytes(sequences, heads, capacity, budget), device)
     _native.launch(

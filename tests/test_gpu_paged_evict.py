@@ -189,6 +189,23 @@ def test_the_returned_lengths_may_be_the_next_lengths():
     assert f.check(33, 0, workspace=ws).tolist() == [32, 32, 20]
 
 
+def test_the_buffers_of_returned_lengths_stay():
+    """A captured eviction writes its lengths into the workspace's buffer on every replay, so
+    calls that are given that buffer as their lengths must not have it replaced."""
+    pools = [torch.zeros(2, 1, 16, 64, device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+    table = torch.arange(2, device="cuda", dtype=torch.int32).view(1, 2)
+    weights, ws = torch.rand(1, 1, 32, device="cuda"), {}
+    lengths = torch.tensor([32], device="cuda", dtype=torch.int32)
+    buffers = []
+    for budget in (20, 16, 9, 4):
+        lengths = paged_evict(*pools, table, lengths, weights, budget, workspace=ws)
+        assert lengths.item() == budget
+        buffers.append(lengths.data_ptr())
+    assert buffers[0] == buffers[2] and buffers[1] == buffers[3] and buffers[0] != buffers[1]
+    kept = {t.data_ptr() for name, t in ws.items() if name.startswith("evict_lengths")}
+    assert kept == set(buffers)
+
+
 @pytest.mark.parametrize("bits", [4, 16])
 def test_bad_lengths_and_pages(bits):
     f = Full([100, 100, 100, 100], 2, 32, 32, bits=bits, seed=8)
