@@ -5,7 +5,8 @@
 // product a pair) and the matrix instructions see the very numbers that the pool
 // stands for.  Queries (bf16, 8 bits) are moved by a power of two into fp16's
 // range, and the weights are held in fp16 terms: one for bf16 queries (2^-11,
-// against the output's own 2^-8), two for fp32 queries (2^-22).
+// against the output's own 2^-8), two for fp32 queries (2^-22), however small a weight
+// is against the greatest of its row.
 //
 // Tiles hold 64 tokens, so that a page is at most one tile and a page's slab of a KV
 // head is fetched by one bulk copy.  Which channels and tokens a lane holds is
@@ -18,8 +19,8 @@
 //     conversion.  Tokens 2j and 2j + 1 change places for odd j, and with them the
 //     rows of the scores, or the four j of a load would hit the same banks.
 //
-// Bound: issue.  16 sequences of 32K tokens (32 + 8 heads, D 128, 604 MB): 141 us, 4.3 TB/s,
-// 1380 warp instructions a tile of 64 tokens; 128K tokens 47.7; 333 tokens 9.5 (latency).
+// Bound: issue.  16 sequences of 32K tokens (32 + 8 heads, D 128, 604 MB): 145 us, 4.2 TB/s,
+// 1380 warp instructions a tile of 64 tokens; 128K tokens 48.7; 333 tokens 9.5 (latency).
 #pragma once
 
 #include "rkv_fp4.cuh"
@@ -97,11 +98,17 @@ __device__ __forceinline__ float exp2_of(float x) {
   return y;
 }
 
-// Weights and their sums are held 2^7 times as large within a tile and a row's part,
-// and up to 2^8 times the reference's: fp16 terms of weights down to 2^-21 of the
-// greatest, or less, are then normal.
-constexpr float kBoost = 7.f, kLag = 8.f;
-constexpr float kUnboost = 1.f / 128.f;
+// Weights and their sums are held 2^13 times as large within a tile and a row's part,
+// and up to 2^2 times the reference's: fp16 terms of weights down to 2^-27 of the
+// greatest are then normal.  Smaller ones (below kLeast, fp16's smallest normal number) are
+// held kStep times as large.
+constexpr float kBoost = 13.f, kLag = 2.f;
+constexpr float kUnboost = 1.f / 8192.f;
+constexpr float kLeast = 1.f / 16384.f;
+constexpr float kStep = 16777216.f;
+// The second term of a weight is held 2^11 times as large: the first one's error is at
+// most 2^-11 of the weight, so that both have the same range, and 22 bits down to kLeast.
+constexpr float kFine = 2048.f;
 constexpr float kLog2E = 1.44269504088896341f;
 
 template <int Dim, int NT_>
@@ -398,45 +405,199 @@ struct Fp4Pool {
       }
       __syncwarp();
     }
+    // Weights below kLeast have fewer than 11 bits in fp16, or none, and they count where the
+    // values of the greater ones are zero.  bf16 queries: a tile that has such weights has
+    // them in a second operand, and what is smaller than that one holds goes through by itself
+    // where it can matter.  fp32 queries: all of them go through by themselves.  16
+    // sequences of 32K tokens: 143.5 us without such weights (140.9 if they were not looked
+    // for), 162 to 172 with logits that spread by 3.5 to 7 (standard deviation), 392 by 14.
+    const uint32_t least = least_of(weights);
+    const auto some_below = [&](float bound) {
+      return __any_sync(0xffffffffu, least < __float_as_uint(bound) - 1u);
+    };
+    const bool small = some_below(kLeast);
     if (p.query_f32) {
-      weigh_terms<2>(tile, weights, o, scratch, lane);
+      if (small) weigh_small(tile, weights, o, scratch, lane, kLeast);
+      weigh_terms<2, 1>(tile, weights, o, scratch, lane);
+    } else if (small) {
+      if (some_below(kLeast / kStep) && !negligible(o, p)) {
+        weigh_small(tile, weights, o, scratch, lane, kLeast / kStep);
+      }
+      weigh_terms<1, 2>(tile, weights, o, scratch, lane);
     } else {
-      weigh_terms<1>(tile, weights, o, scratch, lane);
+      weigh_terms<1, 1>(tile, weights, o, scratch, lane);
     }
   }
 
-  // o += V^T p with the weights in fp16 terms.  With two of them (fp32 queries) 16 rows'
-  // products are summed apart and added by a rounded addition, since the tensor
-  // cores cut their sums off.  Codes are taken kChunk bytes at a time.
+  // Whether fp16 may cut off weights below kLeast / kStep, held kStep times as large: each is
+  // off by at most 2^-25 / kStep, so all of a row's change a channel's sum by at most
+  // 2^-12 of its size where the channel has that much of it by now.
+  static __device__ __forceinline__ bool negligible(Outputs o, const PagedParams& p) {
+    float least = INFINITY;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) least = fminf(least, fabsf(o[dt][nt][c]));
+    constexpr float kMost = 2688.f;  // of a value
+    const float lost = static_cast<float>(p.capacity + R) * (kMost / 33554432.f / kStep);
+    return __all_sync(0xffffffffu, least >= lost * 4096.f);
+  }
+
+  // The least of a lane's weights that are not zero (those of rows that are not visible are), as
+  // an integer less 1.
+  static __device__ __forceinline__ uint32_t least_of(Logits weights) {
+    uint32_t least = 0xffffffffu;
+#pragma unroll
+    for (int mt = 0; mt < R / 16; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) least = min(least, __float_as_uint(weights[mt][nt][c]) - 1u);
+    return least;
+  }
+
+  // The fp16 terms of a lane's four weights of 16 rows, as operands.
   template <int Terms>
+  static __device__ __forceinline__ void split(float (&w)[4], uint32_t (*frag)[2]) {
+#pragma unroll
+    for (int term = 0; term < Terms; ++term)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float& a = w[2 * half];
+        float& b = w[2 * half + 1];
+        const __half2 part = __floats2half2_rn(a, b);
+        if (term + 1 < Terms) {
+          a = (a - __low2float(part)) * kFine;
+          b = (b - __high2float(part)) * kFine;
+        }
+        frag[term][half] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&part));
+      }
+  }
+
+  // Weights below `from`, as many times as large as brings the greatest of them to 2^9 or
+  // more, in two terms, and their products added by as little of them; then those that lie
+  // 2^24 and more below that one, if there are any, and so on (five times at most: the
+  // exponential gives nothing below fp32's normal numbers).  The others are left.
+  static __device__ __forceinline__ void weigh_small(uint32_t tile, Logits weights, Outputs o,
+                                                     uint32_t scratch, int lane, const float from) {
+    // They wait in shared memory, as the logits did, until they are done with.
+    const uint32_t kept = scratch + lane * kLane;
+    const auto put = [&](int mt, int nt, const float (&w)[4]) {
+      asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(kept + mt * 32 * kLane + 16 * nt),
+                   "f"(w[0]), "f"(w[1]), "f"(w[2]), "f"(w[3]));
+    };
+    const auto get = [&](int mt, int nt, float (&w)[4]) {
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(w[0]), "=f"(w[1]), "=f"(w[2]), "=f"(w[3])
+                   : "r"(kept + mt * 32 * kLane + 16 * nt));
+    };
+#pragma unroll
+    for (int mt = 0; mt < R / 16; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) put(mt, nt, weights[mt][nt]);
+#pragma unroll 1
+    while (true) {
+      float greatest = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < R / 16; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float w = weights[mt][nt][c];
+            if (w < from) greatest = fmaxf(greatest, w);
+          }
+      const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(greatest));
+      if (most == 0) return;
+      // 2^k brings the greatest into [2^9, 2^10), or as near as a normal number 2^-k allows;
+      // this is 2^-k, found again wherever it is needed: registers are short here.
+      const auto down = [most] {
+        uint32_t again = most;
+        asm volatile("" : "+r"(again));
+        return __int_as_float((127 - min(126, 136 - static_cast<int>(again >> 23))) << 23);
+      };
+      weigh_rows<2, 1, true>(tile, o, lane, down, [&](int mt, uint32_t (&frag)[NT][2][2]) {
+        const float unit = down(), up = 1.f / unit, least = kLeast * unit;  // exact, if subnormal
+        bool some = false;
+        float w[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float all[4];
+          get(mt, nt, all);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const bool now = all[c] < from && all[c] >= least;
+            w[nt][c] = now ? all[c] * up : 0.f;
+            if (now) all[c] = 0.f;
+            some = some || now;
+          }
+          put(mt, nt, all);
+        }
+        if (!__any_sync(0xffffffffu, some)) return false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) split<2>(w[nt], frag[nt]);
+        return true;
+      });
+#pragma unroll
+      for (int mt = 0; mt < R / 16; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) get(mt, nt, weights[mt][nt]);
+    }
+  }
+
+  // o += V^T p, the weights of each of `Sizes` sizes in `Terms` fp16 terms.
+  template <int Terms, int Sizes>
   static __device__ __forceinline__ void weigh_terms(uint32_t tile, Logits weights, Outputs o,
                                                      uint32_t scratch, int lane) {
+    constexpr int kOperands = Terms * Sizes;
+    static_assert(kOperands <= 2, "8 bytes each of a lane's 16");
     const uint32_t kept = scratch + lane * kLane;
 #pragma unroll
     for (int mt = 0; mt < R / 16; ++mt)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        uint32_t frag[2][2];
+        uint32_t frag[kOperands][2];
+        float(&w)[4] = weights[mt][nt];
+        if constexpr (Sizes > 1) {
+          float low[4];
 #pragma unroll
-        for (int term = 0; term < Terms; ++term)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            float& a = weights[mt][nt][2 * half];
-            float& b = weights[mt][nt][2 * half + 1];
-            const __half2 part = __floats2half2_rn(a, b);
-            if (term + 1 < Terms) {
-              a -= __low2float(part);
-              b -= __high2float(part);
-            }
-            frag[term][half] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&part));
+          for (int c = 0; c < 4; ++c) {
+            low[c] = w[c] < kLeast ? w[c] * kStep : 0.f;
+            if (w[c] < kLeast) w[c] = 0.f;  // a NaN stays
           }
+          split<1>(low, &frag[1]);
+        }
+        split<Terms>(w, &frag[0]);
         const uint32_t to = kept + mt * 32 * kLane + 16 * nt;
-        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to), "r"(frag[0][0]), "r"(frag[0][1]));
-        if constexpr (Terms > 1) {
-          asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + 8), "r"(frag[1][0]),
-                       "r"(frag[1][1]));
+#pragma unroll
+        for (int k = 0; k < kOperands; ++k) {
+          asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + 8 * k), "r"(frag[k][0]),
+                       "r"(frag[k][1]));
         }
       }
+    weigh_rows<Terms, Sizes, false>(tile, o, lane, [] { return 1.f; }, [&](int mt, uint32_t (&frag)[NT][kOperands][2]) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < kOperands; ++k) {
+          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
+                       : "=r"(frag[nt][k][0]), "=r"(frag[nt][k][1])
+                       : "r"(kept + mt * 32 * kLane + 16 * nt + 8 * k));
+        }
+      return true;
+    });
+  }
+
+  // o += V^T p (factor() times, where Scaled), 16 rows at a time; load(i, frag) gets the
+  // operands of the i-th 16 weights, or says that there is nothing to add.  With two
+  // terms 16 rows' products are summed apart and added by a rounded addition, since the
+  // tensor cores cut their sums off.  Codes are taken kChunk bytes at a time.
+  template <int Terms, int Sizes, bool Scaled, typename Factor, typename Load>
+  static __device__ __forceinline__ void weigh_rows(uint32_t tile, Outputs o, int lane, Factor factor,
+                                                    Load load) {
+    constexpr int kOperands = Terms * Sizes;
     const int g = lane >> 2, j = lane & 3;
     const int first = 2 * j + (j & 1), second = 2 * j + 1 - (j & 1);  // swapped(2j), swapped(2j + 1)
     // Channels are taken by units of 8 (a word), or 4 where a lane's part is no whole words.
@@ -446,32 +607,26 @@ struct Fp4Pool {
     constexpr uint32_t kLow = 0x0f0f0f0fu;
     uint32_t codes_at[2] = {tile + first * kRow + g * kBytes, tile + second * kRow + g * kBytes};
     uint32_t scales_at[2] = {tile + R * kRow + first * kScales, tile + R * kRow + second * kScales};
-    uint32_t from = kept;
 #pragma unroll 1
     for (int mt = 0; mt < R / 16; ++mt) {
-      uint32_t frag[Terms][NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int term = 0; term < Terms; ++term) {
-          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
-                       : "=r"(frag[term][nt][0]), "=r"(frag[term][nt][1])
-                       : "r"(from + 16 * nt + 8 * term));
-        }
+      const uint32_t codes_16 = mt * 16 * kRow, scales_16 = mt * 16 * kScales;
+      uint32_t frag[NT][kOperands][2];
+      if (!load(mt, frag)) continue;
 #pragma unroll
       for (int chunk = 0; chunk < kBytes / kChunk; ++chunk) {
         uint32_t codes[4][kUnits], scale[4];
+        [[maybe_unused]] const float by = factor();
         // Two units of a chunk lie in one block of 16 channels.
         const int block = (g * (kBytes / kUnit) + chunk * kUnits) / (kUnit == 4 ? 2 : 4);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {  // tokens first, second, first + 8, second + 8
-          const uint32_t at = codes_at[t & 1] + (t >> 1) * 8 * kRow + chunk * kChunk;
+          const uint32_t at = codes_at[t & 1] + codes_16 + (t >> 1) * 8 * kRow + chunk * kChunk;
           if constexpr (kUnit == 4) {
             lds_words(at, codes[t]);
           } else {
             codes[t][0] = lds<2>(at);
           }
-          scale[t] = lds<1>(scales_at[t & 1] + block + (t >> 1) * 8 * kScales);
+          scale[t] = lds<1>(scales_at[t & 1] + scales_16 + block + (t >> 1) * 8 * kScales);
         }
         // The scales of tokens 0 and 1, and 2 and 3.
         const uint32_t near = fp4_scales(__byte_perm(scale[0], scale[1], 0x0040));
@@ -496,24 +651,31 @@ struct Fp4Pool {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               if constexpr (Terms == 1) {
-                mma_f16(o[dt][nt], a, frag[0][nt][0], frag[0][nt][1]);
+                if constexpr (Sizes > 1) {
+                  float sum[4];
+                  mma_f16_first(sum, a, frag[nt][1][0], frag[nt][1][1]);
+#pragma unroll
+                  for (int c = 0; c < 4; ++c) {
+                    o[dt][nt][c] = fmaf(sum[c], 1.f / kStep, o[dt][nt][c]);
+                  }
+                }
+                mma_f16(o[dt][nt], a, frag[nt][0][0], frag[nt][0][1]);
               } else {
                 float sum[4];
-                mma_f16_first(sum, a, frag[0][nt][0], frag[0][nt][1]);
-                mma_f16(sum, a, frag[1][nt][0], frag[1][nt][1]);
+                mma_f16_first(sum, a, frag[nt][1][0], frag[nt][1][1]);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) o[dt][nt][c] += sum[c];
+                for (int c = 0; c < 4; ++c) sum[c] *= 1.f / kFine;
+                mma_f16(sum, a, frag[nt][0][0], frag[nt][0][1]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                  if constexpr (Scaled) o[dt][nt][c] = fmaf(sum[c], by, o[dt][nt][c]);
+                  else o[dt][nt][c] += sum[c];
+                }
               }
             }
           }
         }
       }
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        codes_at[t] += 16 * kRow;
-        scales_at[t] += 16 * kScales;
-      }
-      from += 32 * kLane;
     }
   }
 };
