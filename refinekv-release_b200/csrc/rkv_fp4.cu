@@ -88,6 +88,14 @@ __device__ __forceinline__ float quotient(float x, float b, float r) {
   return __fmaf_rn(-__fmaf_rn(b, q, -x), r, q);  // in these signs -0 stays -0
 }
 
+// Whether `quotient` serves for every x divided by this factor: an overflow gives NaN instead of
+// infinity, and both make 16 channels NaN; where x / factor is so small that its digits are
+// lost, its code is a zero whatever they are.  (By a negative one, 0 would keep its sign.)
+__device__ __forceinline__ bool corrects(float factor) {
+  constexpr float kLimit = 1152921504606846976.f;  // 2^60
+  return factor >= 1.f / kLimit && factor <= kLimit;
+}
+
 // The scale of 16 channels whose greatest magnitude is `most`: most / 6 rounded to
 // e4m3, at most 448.  A channel that is infinite or NaN makes it NaN, and with it all
 // 16.
@@ -239,7 +247,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas)
       const int head = (blockIdx.y * kHeads + u) * slots + warp * in_warp + slot;
       if (kind[u] == 1 && key_scale != nullptr) factor[u] = key_scale[head - k_from];
       if (kind[u] == 2 && value_scale != nullptr) factor[u] = value_scale[head - v_from];
-      inverse[u] = __frcp_rn(factor[u]);
+      inverse[u] = corrects(factor[u]) ? __frcp_rn(factor[u]) : 0.f;
     }
   }
   const unsigned tokens = static_cast<unsigned>(p.tokens);
@@ -306,9 +314,14 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas)
         // Warps of queries alone have no scales to find.
         if (__all_sync(0xffffffffu, kind[u] <= 0)) continue;
         if (scaled) {
+          if (inverse[u] != 0.f) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            x[j >> 3][j & 7] = quotient(x[j >> 3][j & 7], factor[u], inverse[u]);
+            for (int j = 0; j < 16; ++j) {
+              x[j >> 3][j & 7] = quotient(x[j >> 3][j & 7], factor[u], inverse[u]);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[j >> 3][j & 7] = __fdiv_rn(x[j >> 3][j & 7], factor[u]);
           }
         }
         const float most[2] = {greatest(x[0]), greatest(x[1])};
