@@ -77,6 +77,8 @@ class Server:
             raise ValueError("bits: a pool holds 16 or 4 a channel")
         if budget is not None and model.dense < model.layers:
             raise ValueError("budget: refined layers keep their whole prompt")
+        if budget is not None and not (budget >= 1 and 0 <= recent <= budget):
+            raise ValueError("budget: at least one token, and recent at most as many")
         self.m, self.new, self.config = model, new_tokens, config or rkv.RefineKVConfig()
         self.budget, self.recent = budget, recent
         dev = model.embed.device

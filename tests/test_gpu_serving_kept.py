@@ -57,3 +57,10 @@ def test_the_newest_and_the_heaviest_stay(bits, budget, recent):
                 got = dict(zip(left, server.weights[0][i, h, :new].tolist()))
                 assert all(abs(got[t] - worth[t]) <= 2 ** -10 * worth[t] for t in left)
     assert server.healthy()
+
+
+@pytest.mark.parametrize("budget,recent", [(8, 16), (0, 0), (-3, 0), (8, -1), (8, 9)])
+def test_a_budget_that_cannot_be_is_refused_at_once(budget, recent):
+    ex = _example()
+    with pytest.raises(ValueError, match="budget"):
+        ex.Server(ex.Decoder(layers=2, dense=2), _prompts(40), 2, budget=budget, recent=recent)
