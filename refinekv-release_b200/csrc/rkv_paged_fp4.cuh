@@ -19,8 +19,8 @@
 //     conversion.  Tokens 2j and 2j + 1 change places for odd j, and with them the
 //     rows of the scores, or the four j of a load would hit the same banks.
 //
-// Bound: issue.  16 sequences of 32K tokens (32 + 8 heads, D 128, 604 MB): 145 us, 4.2 TB/s,
-// 1380 warp instructions a tile of 64 tokens; 128K tokens 48.7; 333 tokens 9.5 (latency).
+// Bound: issue.  16 sequences of 32K tokens (32 + 8 heads, D 128, 604 MB): 144 us, 4.2 TB/s,
+// 1380 warp instructions a tile of 64 tokens; 128K tokens 48.0; 333 tokens 9.6 (latency).
 #pragma once
 
 #include "rkv_fp4.cuh"
@@ -407,32 +407,59 @@ struct Fp4Pool {
     }
     // Weights below kLeast have fewer than 11 bits in fp16, or none, and they count where the
     // values of the greater ones are zero.  bf16 queries: a tile that has such weights has
-    // them in a second operand, and what is smaller than that one holds goes through by itself
-    // where it can matter.  fp32 queries: all of them go through by themselves.  16
-    // sequences of 32K tokens: 143.5 us without such weights (140.9 if they were not looked
-    // for), 162 to 172 with logits that spread by 3.5 to 7 (standard deviation), 392 by 14.
+    // them in a second operand, kStep times as large.  What the operands cut off of a tile's
+    // weights goes through by itself where it can matter.  16 sequences of 32K tokens: 141
+    // to 144 us where fp16 holds all weights, 162 to 180 with logits that spread by 3.5 to 7
+    // (standard deviation), 235 by 14, 222 with biases of up to 0.84 a token (without any
+    // of this 141, and 176 with the biases).
     const uint32_t least = least_of(weights);
     const auto some_below = [&](float bound) {
       return __any_sync(0xffffffffu, least < __float_as_uint(bound) - 1u);
     };
     const bool small = some_below(kLeast);
-    if (p.query_f32) {
-      if (small) weigh_small(tile, weights, o, scratch, lane, kLeast);
-      weigh_terms<2, 1>(tile, weights, o, scratch, lane);
-    } else if (small) {
-      if (some_below(kLeast / kStep) && !negligible(o, p)) {
-        weigh_small(tile, weights, o, scratch, lane, kLeast / kStep);
-      }
-      weigh_terms<1, 2>(tile, weights, o, scratch, lane);
-    } else {
+    if (!p.query_f32 && !small) {
       weigh_terms<1, 1>(tile, weights, o, scratch, lane);
+      return;
     }
+    // The weights below this are cut off, at 2^-11 of it (2^-22: fp32 queries) at the most.
+    const float bound = p.query_f32 ? kLeast : kLeast / kStep;
+    const bool cut = p.query_f32 ? small : some_below(bound);
+    volatile float held[R / 16][NT][4];
+    if (cut) hold(weights, held);
+    if (p.query_f32) weigh_terms<2, 1>(tile, weights, o, scratch, lane);
+    else weigh_terms<1, 2>(tile, weights, o, scratch, lane);
+    if (!cut || negligible(tile, o, bound / kFine / (p.query_f32 ? kFine : 1.f), lane, p)) return;
+    weigh_rest(tile, held, o, scratch, lane, p, [&](float w) {
+      if (!(w < bound)) return 0.f;
+      const float up = p.query_f32 ? 1.f : kStep;
+      const float rest = w - __half2float(__float2half_rn(w * up)) / up;
+      if (!p.query_f32) return rest;
+      return rest - __half2float(__float2half_rn(rest * kFine)) * (1.f / kFine);
+    });
   }
 
-  // Whether fp16 may cut off weights below kLeast / kStep, held kStep times as large: each is
-  // off by at most 2^-25 / kStep, so all of a row's change a channel's sum by at most
-  // 2^-12 of its size where the channel has that much of it by now.
-  static __device__ __forceinline__ bool negligible(Outputs o, const PagedParams& p) {
+  // Puts a tile's weights aside: local memory, since nothing else has room, and it is seldom
+  // read back.
+  static __device__ __forceinline__ void hold(Logits weights, volatile float (&held)[R / 16][NT][4]) {
+#pragma unroll
+    for (int mt = 0; mt < R / 16; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) held[mt][nt][c] = weights[mt][nt][c];
+  }
+
+  // Whether a tile's weights may be off by this much each: where every channel's sum is by now
+  // so large that all tiles together would change it by less than 2^-16 of its size (2^-21:
+  // fp32 queries).
+  static __device__ __forceinline__ bool negligible(uint32_t tile, Outputs o, float off, int lane,
+                                                    const PagedParams& p) {
+    uint32_t words[D / 32], most = 0;  // the greatest scale
+    lds_words(tile + R * kRow + lane * (D / 8), words);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) most = __vmaxu4(most, words[i]);
+    most = __vmaxu4(most, most >> 16);
+    most = __reduce_max_sync(0xffffffffu, max(most & 0xffu, most >> 8 & 0xffu));
     float least = INFINITY;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -440,9 +467,8 @@ struct Fp4Pool {
       for (int dt = 0; dt < D / 16; ++dt)
 #pragma unroll
         for (int c = 0; c < 4; ++c) least = fminf(least, fabsf(o[dt][nt][c]));
-    constexpr float kMost = 2688.f;  // of a value
-    const float lost = static_cast<float>(p.capacity + R) * (kMost / 33554432.f / kStep);
-    return __all_sync(0xffffffffu, least >= lost * 4096.f);
+    off *= 6.f * fp4_scale_value(most) * static_cast<float>(p.capacity + R);
+    return __all_sync(0xffffffffu, least >= off * (p.query_f32 ? 2097152.f : 65536.f));
   }
 
   // The least of a lane's weights that are not zero (those of rows that are not visible are), as
@@ -476,12 +502,16 @@ struct Fp4Pool {
       }
   }
 
-  // Weights below `from`, as many times as large as brings the greatest of them to 2^9 or
-  // more, in two terms, and their products added by as little of them; then those that lie
-  // 2^24 and more below that one, if there are any, and so on (five times at most: the
-  // exponential gives nothing below fp32's normal numbers).  The others are left.
-  static __device__ __forceinline__ void weigh_small(uint32_t tile, Logits weights, Outputs o,
-                                                     uint32_t scratch, int lane, const float from) {
+  // o += V^T r with the part r = rest(w) of each weight that its operands do not hold, numbers of
+  // any size (the exponential gives nothing below fp32's normal ones): those within 2^28 of
+  // the greatest as many times as large as brings that one to 2^14 or more, in two terms, and
+  // their products added by as little of them; then the ones below these, and so on until
+  // what is left is negligible, five times at most.
+  template <typename Rest>
+  static __device__ __forceinline__ void weigh_rest(uint32_t tile,
+                                                    volatile float (&held)[R / 16][NT][4], Outputs o,
+                                                    uint32_t scratch, int lane, const PagedParams& p,
+                                                    Rest rest) {
     // They wait in shared memory, as the logits did, until they are done with.
     const uint32_t kept = scratch + lane * kLane;
     const auto put = [&](int mt, int nt, const float (&w)[4]) {
@@ -496,28 +526,33 @@ struct Fp4Pool {
 #pragma unroll
     for (int mt = 0; mt < R / 16; ++mt)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) put(mt, nt, weights[mt][nt]);
+      for (int nt = 0; nt < NT; ++nt) {
+        float w[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) w[c] = rest(held[mt][nt][c]);
+        put(mt, nt, w);
+      }
 #pragma unroll 1
-    while (true) {
+    for (int time = 0; time < 5; ++time) {
       float greatest = 0.f;
 #pragma unroll
       for (int mt = 0; mt < R / 16; ++mt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
+          float w[4];
+          get(mt, nt, w);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const float w = weights[mt][nt][c];
-            if (w < from) greatest = fmaxf(greatest, w);
-          }
+          for (int c = 0; c < 4; ++c) greatest = fmaxf(greatest, fabsf(w[c]));
+        }
       const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(greatest));
-      if (most == 0) return;
-      // 2^k brings the greatest into [2^9, 2^10), or as near as a normal number 2^-k allows;
+      // 2^k brings the greatest into [2^14, 2^15), or as near as a normal number 2^-k allows;
       // this is 2^-k, found again wherever it is needed: registers are short here.
       const auto down = [most] {
         uint32_t again = most;
         asm volatile("" : "+r"(again));
-        return __int_as_float((127 - min(126, 136 - static_cast<int>(again >> 23))) << 23);
+        return __int_as_float((127 - min(126, 141 - static_cast<int>(again >> 23))) << 23);
       };
+      if (most == 0 || negligible(tile, o, __uint_as_float(most), lane, p)) return;
       weigh_rows<2, 1, true>(tile, o, lane, down, [&](int mt, uint32_t (&frag)[NT][2][2]) {
         const float unit = down(), up = 1.f / unit, least = kLeast * unit;  // exact, if subnormal
         bool some = false;
@@ -528,7 +563,7 @@ struct Fp4Pool {
           get(mt, nt, all);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const bool now = all[c] < from && all[c] >= least;
+            const bool now = fabsf(all[c]) >= least;
             w[nt][c] = now ? all[c] * up : 0.f;
             if (now) all[c] = 0.f;
             some = some || now;
@@ -540,10 +575,6 @@ struct Fp4Pool {
         for (int nt = 0; nt < NT; ++nt) split<2>(w[nt], frag[nt]);
         return true;
       });
-#pragma unroll
-      for (int mt = 0; mt < R / 16; ++mt)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) get(mt, nt, weights[mt][nt]);
     }
   }
 
