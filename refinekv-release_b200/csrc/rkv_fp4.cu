@@ -9,7 +9,9 @@
 //
 // Bound: HBM on long inputs: a bf16 row of 128 channels is read (256 bytes) and
 // 72 bytes written, or the other way round.  24.5K tokens of 8 KV heads read back into
-// bf16 (128 MB): 33 us, 3.9 TB/s, bound by issue.
+// bf16 (128 MB): 33 us, 3.9 TB/s, bound by latency: loads and the barriers of a batch of
+// tokens (issue 61 %, of 13 cycles between a warp's instructions 3.8 wait for memory and
+// 1.5 at a barrier).  From a bf16 pool (217 MB) 40 us, 5.4 TB/s.
 #include <algorithm>
 #include <string>
 
@@ -198,7 +200,8 @@ __device__ __forceinline__ float greatest(const float (&x)[8]) {
 // 128, half layout): 116 us, 530 MB; with single pieces, whose partners are read
 // twice, 202 and twice the instructions; with the table's rows read from L2 for each
 // token instead of ahead for a batch 149; one head a thread and 1.5 times the warps 138;
-// two heads and 80 registers, which spill, 158.
+// two heads and 80 registers, which spill, 158.  fp32 rows, which spill 32 to 64 bytes: 192.
+// With factors 117 and 195.
 constexpr int kHeads = 2;
 constexpr int kRowThreads = 256, kRowCtas = 2;
 
@@ -404,6 +407,7 @@ __device__ __forceinline__ float turned(const RowsParams& p, const T* row, int d
 
 // Any strides, alignment and rotary width, keys and values only: a thread takes
 // 16 channels of a head of a token, element by element.
+// The same tokens with a rotary width of 24: 413 us (fp32 rows 423).
 template <typename T, bool Interleaved>
 __global__ void __launch_bounds__(256)
     fp4_append_any_kernel(const __grid_constant__ RowsParams p,

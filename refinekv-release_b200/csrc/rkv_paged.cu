@@ -18,9 +18,9 @@
 // cannot follow that); a ragged batch of 43, 270 MB: 52 us.  About 5 us before
 // the stream is up and 4 to 6 for the joins at its end are what short calls
 // consist of: one sequence of 333 tokens takes 8.3 us.  Sixteen queries a KV head
-// of D 192 or 256 spill a little (200 and 292 bytes of stores a thread): 8
-// sequences of 32K tokens, 2 KV heads, D 256: 103 us for 537 MB, against 97 with
-// eight queries; D 192: 82 us for 403 MB, against 72 with four.
+// of D 192 or 256 spill a little (200 and 332 bytes of stores a thread): 8
+// sequences of 32K tokens, 2 KV heads, D 256: 102 us for 537 MB, against 94 with
+// eight queries; D 192: 81 us for 403 MB, against 72 with four.
 //
 // Split.  The tiles of all rows, sequence-major then head, form one list that
 // is cut into equal contiguous ranges, one per CTA, and each CTA's range into
@@ -410,8 +410,9 @@ __device__ __forceinline__ void shape_logits(float (&logit)[Pool::R / 16][Pool::
 
 // The pool says how a tile is fetched, scored and weighed (Bf16Pool, Fp4Pool).
 // More: a cap, a bias, a prefix, factors and the logits for the weights' sums,
-// each looked up in the parameters; without it the kernel is as it was before
-// these (the same results, and the same time).
+// each looked up in the parameters; without it the kernel gives the same results in
+// the same time as before these (D 256 with sixteen queries spills 332 bytes a thread
+// instead of 292: 101.5 us against 101.8).
 template <typename Pool, bool More>
 __global__ void __launch_bounds__(Pool::W * 32, 1)
     paged_kernel(const __grid_constant__ typename Pool::Source source,

@@ -5,8 +5,10 @@
 // product a pair) and the matrix instructions see the very numbers that the pool
 // stands for.  Queries (bf16, 8 bits) are moved by a power of two into fp16's
 // range, and the weights are held in fp16 terms: one for bf16 queries (2^-11,
-// against the output's own 2^-8), two for fp32 queries (2^-22), however small a weight
-// is against the greatest of its row.
+// against the output's own 2^-8: the error against 64 bits is that of a result rounded once,
+// and two would take 170 us instead of 143), two for fp32 queries (2^-22), however small a
+// weight is against the greatest of its row.  A query's channels of less than 2^-29 of its
+// greatest one lose digits.
 //
 // Tiles hold 64 tokens, so that a page is at most one tile and a page's slab of a KV
 // head is fetched by one bulk copy.  Which channels and tokens a lane holds is
@@ -19,8 +21,13 @@
 //     conversion.  Tokens 2j and 2j + 1 change places for odd j, and with them the
 //     rows of the scores, or the four j of a load would hit the same banks.
 //
-// Bound: issue.  16 sequences of 32K tokens (32 + 8 heads, D 128, 604 MB): 144 us, 4.2 TB/s,
-// 1380 warp instructions a tile of 64 tokens; 128K tokens 48.0; 333 tokens 9.6 (latency).
+// Bound: latency, with three warps a scheduler that each go alone through loads, conversions,
+// products, votes and exponentials.  An instruction issues in 61 % of the cycles and 1.06 warps
+// could have; of a warp's 4.75 cycles between two of its instructions 1.3 wait for a result
+// of fixed latency, 0.7 for the other warps, 0.55 for a busy pipe (ALU 50 %, tensor 21 %), 0.2
+// for memory.  16 sequences of 32K tokens (32 + 8 heads, D 128, 604 MB): 141 to 144 us, 4.2
+// TB/s, 1400 warp instructions a tile of 64 tokens; 128K tokens 48.0; 333 tokens 9.6, more than
+// from a bf16 pool (8.2): half of the warps have no tile, and a tile alone takes 4 us.
 #pragma once
 
 #include "rkv_fp4.cuh"
@@ -114,6 +121,9 @@ constexpr float kLog2E = 1.44269504088896341f;
 template <int Dim, int NT_>
 struct Fp4Pool {
   static constexpr int D = Dim, NT = NT_, R = kFp4Rows;
+  // Eight where twelve would spill.  Spilled all the same, bytes of stores a thread: 16 (D 256); with
+  // 9 to 16 queries a KV head 12 (D 160), 154 (192), 560 (224), 748 (256).  8 sequences of 32K
+  // tokens, 2 KV heads of 16 queries: 43 us (D 128), 55, 59 and 80 (D 256; bf16 pool: 102).
   static constexpr int W = NT == 1 && Dim <= 192 ? 12 : 8;
   static constexpr int kTile = fp4_slab_bytes(R, Dim);
   static constexpr bool kFirstInSmem = Dim <= 128;
@@ -409,8 +419,8 @@ struct Fp4Pool {
     // values of the greater ones are zero.  bf16 queries: a tile that has such weights has
     // them in a second operand, kStep times as large.  What the operands cut off of a tile's
     // weights goes through by itself where it can matter.  16 sequences of 32K tokens: 141
-    // to 144 us where fp16 holds all weights, 162 to 180 with logits that spread by 3.5 to 7
-    // (standard deviation), 235 by 14, 222 with biases of up to 0.84 a token (without any
+    // to 144 us where fp16 holds all weights, 165 to 182 with logits that spread by 3.5 to 7
+    // (standard deviation), 255 by 14, 222 with biases of up to 0.84 a token (without any
     // of this 141, and 176 with the biases).
     const uint32_t least = least_of(weights);
     const auto some_below = [&](float bound) {
@@ -450,7 +460,7 @@ struct Fp4Pool {
   }
 
   // Whether a tile's weights may be off by this much each: where every channel's sum is by now
-  // so large that all tiles together would change it by less than 2^-16 of its size (2^-21:
+  // so large that all tiles together would change it by less than 2^-18 of its size (2^-21:
   // fp32 queries).
   static __device__ __forceinline__ bool negligible(uint32_t tile, Outputs o, float off, int lane,
                                                     const PagedParams& p) {
@@ -468,7 +478,7 @@ struct Fp4Pool {
 #pragma unroll
         for (int c = 0; c < 4; ++c) least = fminf(least, fabsf(o[dt][nt][c]));
     off *= 6.f * fp4_scale_value(most) * static_cast<float>(p.capacity + R);
-    return __all_sync(0xffffffffu, least >= off * (p.query_f32 ? 2097152.f : 65536.f));
+    return __all_sync(0xffffffffu, least >= off * (p.query_f32 ? 2097152.f : 262144.f));
   }
 
   // The least of a lane's weights that are not zero (those of rows that are not visible are), as

@@ -113,7 +113,8 @@ class Summary(ctypes.Structure):
     ]
 
 
-#: ``struct rkv_rotary_args``, ``rkv_append_args`` and so on: 8-byte fields only, packed in the header's order (pointers as integers, 0 for null).  Packing costs a tenth of filling a
+#: ``struct rkv_rotary_args``, ``rkv_append_args`` and so on: 8-byte fields only, packed in the
+#: header's order (pointers as integers, 0 for null).  Packing costs a tenth of filling a
 #: ``ctypes.Structure``, which counts in calls whose kernel takes a few microseconds.
 ROTARY_ARGS = struct.Struct("=32q")
 APPEND_ARGS = struct.Struct("=40q")

@@ -168,9 +168,9 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Tensor,
     ``position % block``, rounded once to bf16.  With ``cos_sin`` (see
     ``apply_rotary``) keys are rotated by their positions first, and so is
     ``query`` ((tokens, q_heads, head_dim), the keys' dtype) when given.  Into
-    pools of 4 bits (``fp4_pool``) rows go from fp32 in one rounding too, divided by
-    ``key_scale`` and ``value_scale`` ((kv_heads,) fp32) where these are given; 16
-    channels that hold an infinity or a NaN become NaN.
+    pools of 4 bits (``fp4_pool``) rows go from fp32 in one rounding too, divided in
+    fp32 by ``key_scale`` and ``value_scale`` ((kv_heads,) fp32) where these are given;
+    16 channels that hold an infinity or a NaN, or whose quotients do, become NaN.
 
     Returns the rotated queries (backed by ``workspace``, reused by the next
     call of the same shape), or None without ``query``.  The pools are
@@ -357,14 +357,18 @@ def paged_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: tor
 
     Pools may hold 4 bits a channel (``fp4_pool``), with the ``key_scale`` and
     ``value_scale`` that ``paged_append`` was given: the attention is exact over
-    what the pool stands for.
+    what the pool stands for, but for weights held to 2^-11 of themselves (fp32
+    queries: 2^-22) and channels of a query below 2^-29 of its greatest one, which lose
+    digits.  Rows whose logits spread by many nats (steep ``slopes``) take longer there.
 
     ``weights``: (sequences, kv_heads, tokens) fp32, contiguous in its last
     dimension and at least as wide as the page table's row in tokens: to each
     visible token's entry the softmax weight that it got is added, summed over the
     query heads of its KV head (what ``paged_evict`` goes by).  A query whose sum is
-    not finite adds nothing.  Takes a second launch and scratch for the logits,
-    4 bytes a query head and token of the page table.
+    not finite adds nothing.  Takes a second launch and scratch for the logits, 4
+    bytes a query head and token of the page table's width, however short the
+    sequences are (256 of 128K tokens' width and 32 heads: 4.3 GB); it stays in the
+    ``workspace``.
 
     Returns the (sequences, q_heads, head_dim) output in the query's dtype or,
     with ``return_lse``, (output, lse) with the fp32 natural-log sum of the
@@ -374,7 +378,7 @@ def paged_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: tor
     visible page outside the pool sets bit 1 of
     ``attention.device_status(workspace)`` and makes that sequence's output (and
     lse) NaN; a negative length sets it and counts as 0.
-    One launch; its results repeat bit for bit.
+    One launch (two with ``weights``); its results repeat bit for bit.
     """
     fp4 = key_pool.dtype is torch.uint8
     pages, heads, block, dim, ks, vs = (_fp4_pools if fp4 else _pools)(key_pool, value_pool, layout)
@@ -523,8 +527,11 @@ def paged_evict(key_pool: torch.Tensor, value_pool: torch.Tensor, page_table: to
     A sequence's pages must be its own: rows that move into a page which another
     sequence's table names too would change that sequence, so copy shared pages first.
 
-    Returns the new lengths, ``min(lengths, budget)`` (backed by ``workspace``,
-    reused by the next call that is not given them as ``lengths``).  Pools, weights and positions are written in place;
+    Returns the new lengths, ``min(lengths, budget)`` (backed by ``workspace``, reused
+    by the next call that is not given them as ``lengths``).  The ``workspace`` also
+    keeps the list of moves, 8 bytes a KV head and row that could move, min(budget, the
+    page table's tokens - budget) of them (256 sequences of 128K tokens' width, 8 KV heads,
+    a budget of 64K: 1.1 GB).  Pools, weights and positions are written in place;
     nothing carries a gradient.  A length past the page table leaves its sequence
     as it is, a negative one counts as 0, and a row from a page outside the pool is
     NaN where it goes; each sets bit 1 of ``attention.device_status(workspace)``.
