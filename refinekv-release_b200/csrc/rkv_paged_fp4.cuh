@@ -618,7 +618,7 @@ struct Fp4Pool {
                        "r"(frag[k][1]));
         }
       }
-    weigh_rows<Terms, Sizes, false>(tile, o, lane, [] { return 1.f; }, [&](int mt, uint32_t (&frag)[NT][kOperands][2]) {
+    const auto load = [&](int mt, uint32_t (&frag)[NT][kOperands][2]) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -628,7 +628,8 @@ struct Fp4Pool {
                        : "r"(kept + mt * 32 * kLane + 16 * nt + 8 * k));
         }
       return true;
-    });
+    };
+    weigh_rows<Terms, Sizes, false>(tile, o, lane, [] { return 1.f; }, load);
   }
 
   // o += V^T p (factor() times, where Scaled), 16 rows at a time; load(i, frag) gets the

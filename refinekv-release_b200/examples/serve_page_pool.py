@@ -20,9 +20,10 @@ grow:
 With ``--bits 4`` the dense layers hold their keys and values in 4 bits (``fp4_pool``).
 With ``--budget`` every layer is dense and keeps that many tokens of a sequence:
 the attention of each step adds up what weight each got, and the step drops the least
-(``paged_evict``).  The prompt's own queries are not counted, since its attention is torch's:
-a prompt longer than the budget is cut down by what the first step's query saw.  Rows then change places, so a token's row in the pool and its
-position part ways: the keys are rotated by the position and appended at the row.
+(``paged_evict``).  The prompt's own queries are not counted, since its attention is
+torch's: a prompt longer than the budget is cut down by what the first step's query saw.
+Rows then change places, so a token's row in the pool and its position part ways: the keys
+are rotated by the position and appended at the row.
 """
 
 from __future__ import annotations
